@@ -5,6 +5,7 @@ Outputs (git-ignored, shipped with the source tree to the GPU host):
   netra-kernel_amd/lib/libnetra_engine.so      C-ABI engine runtime
   netra-kernel_amd/lib/libnetra_moe.so         direct entry points (weight prep, no-alloc prefill)
   netra-kernel_amd/lib/libnetra_bridges.so     the reference's per-operation bridge ABIs
+  netra-kernel_amd/lib/libnetra_layers.so      block-FP8 linear layer, expert counts, balance loss
 
 Run: python netra-kernel_amd/build.py  (or __graft_entry__.build()).
 """
@@ -40,6 +41,7 @@ HSACO = LIB / "netra_moe_gfx950.hsaco"
 ENGINE_SO = LIB / "libnetra_engine.so"
 BRIDGE_SO = LIB / "libnetra_moe.so"
 OPS_SO = LIB / "libnetra_bridges.so"
+LAYERS_SO = LIB / "libnetra_layers.so"
 
 
 def _run(cmd: list[str]) -> None:
@@ -98,8 +100,17 @@ def build_op_bridges() -> Path:
     return OPS_SO
 
 
+def build_layers() -> Path:
+    LIB.mkdir(exist_ok=True)
+    tmp = LAYERS_SO.with_suffix(".so.tmp")
+    _run([HIPCC, *DEVICE_FLAGS, "-fPIC", "-shared", "-o", str(tmp),
+          str(CSRC / "layers" / "netra_layers.hip")])
+    tmp.replace(LAYERS_SO)
+    return LAYERS_SO
+
+
 def build_all() -> list[Path]:
-    return [build_hsaco(), build_engine(), build_bridge(), build_op_bridges()]
+    return [build_hsaco(), build_engine(), build_bridge(), build_op_bridges(), build_layers()]
 
 
 if __name__ == "__main__":

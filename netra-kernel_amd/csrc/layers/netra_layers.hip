@@ -1,0 +1,263 @@
+// C entry points of libnetra_layers.so (include/netra_layers.h): argument
+// checks, workspace layout, choice of kernels and launches.
+#include "../../../include/netra_layers.h"
+
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "linear_fp8.hip"
+#include "router_balance.hip"
+
+namespace {
+
+thread_local std::string g_error;
+
+// No exception leaves a C entry point: a message there is no memory for is lost.
+int fail(int code, const char* name, const char* text) noexcept {
+  try {
+    g_error = std::string(name) + ": " + text;
+  } catch (...) {
+    g_error.clear();
+  }
+  return code;
+}
+
+int launched(const char* name) noexcept {
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(static_cast<int>(err), name, hipGetErrorString(err));
+  g_error.clear();
+  return 0;
+}
+
+// Sizes up to 2^21 keep every grid dimension, tile count and scale index inside its type.
+constexpr uint32_t kMaxSize = 1u << 21;
+
+uint32_t up(uint32_t v, uint32_t m) { return (v + m - 1u) / m * m; }
+uint32_t blocks(uint32_t v) { return (v + 127u) / 128u; }
+uint32_t elem(uint32_t type) { return type == NETRA_BF16 ? 2u : 4u; }
+bool aligned(const void* p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// A quantised matrix in the workspace: codes of up(rows, 16) x up(cols, 128), then scales [blocks][up(rows, 16)].
+uint64_t code_bytes(uint32_t rows, uint32_t cols) { return static_cast<uint64_t>(up(rows, 16u)) * up(cols, 128u); }
+uint64_t matrix_bytes(uint32_t rows, uint32_t cols) {
+  return code_bytes(rows, cols) + static_cast<uint64_t>(up(rows, 16u)) * blocks(cols) * 4u;
+}
+
+bool bad_sizes(uint32_t rows, uint32_t n, uint32_t k) {
+  return n == 0 || k == 0 || rows > kMaxSize || n > kMaxSize || k > kMaxSize;
+}
+bool bad_type(uint32_t type) { return type != NETRA_BF16 && type != NETRA_F32; }
+// A matrix's base has to be aligned to its elements.
+bool bad_matrix(const void* p, uint32_t type, uint64_t stride, uint32_t cols) {
+  return !p || bad_type(type) || stride < cols || !aligned(p, elem(type));
+}
+
+void quant_rows(const void* x, uint32_t type, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n,
+                hipStream_t stream) {
+  const dim3 grid((rows + 15u) / 16u, (blocks(n) + 3u) / 4u), block(256);
+  const bool vec = aligned(x, 16) && stride * elem(type) % 16u == 0;
+  const uint32_t sld = up(rows, 16u);
+  if (type == NETRA_BF16) {
+    const uint16_t* p = static_cast<const uint16_t*>(x);
+    if (vec) netra_linear_quant_rows_bf16_vec_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
+    else netra_linear_quant_rows_bf16_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
+  } else {
+    const float* p = static_cast<const float*>(x);
+    if (vec) netra_linear_quant_rows_f32_vec_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
+    else netra_linear_quant_rows_f32_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
+  }
+}
+
+void product(nklin::Product a, hipStream_t stream) {
+  a.vec = aligned(a.out, 8) && a.ldo % 4u == 0;
+  netra_linear_product_direct_gfx950<<<dim3((a.ni + 63u) / 64u, (a.nq + 63u) / 64u), dim3(256), 0, stream>>>(a);
+}
+
+bool bad_workspace(const void* p, uint64_t bytes, uint64_t need) {
+  return bytes < need || (need && (!p || !aligned(p, 16)));
+}
+
+}  // namespace
+
+extern "C" uint64_t netra_linear_packed_bytes(uint32_t n, uint32_t k, uint32_t transpose) {
+  return transpose ? code_bytes(k, n) : code_bytes(n, k);
+}
+
+extern "C" int netra_linear_pack(const uint8_t* w, uint8_t* packed, uint32_t n, uint32_t k, uint32_t transpose,
+                                 hipStream_t stream) {
+  if (!w || !packed || w == packed || !aligned(packed, 16) || bad_sizes(0, n, k))
+    return fail(-1, "netra_linear_pack", "null, aliased or misaligned pointers, or n / k not in 1 .. 2^21");
+  const uint32_t rows = transpose ? k : n, cols = transpose ? n : k;
+  netra_linear_pack_gfx950<<<dim3((rows + 15u) / 16u, (blocks(cols) + 3u) / 4u), dim3(256), 0, stream>>>(
+      w, packed, n, k, transpose ? 1u : 0u);
+  return launched("netra_linear_pack");
+}
+
+extern "C" uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  return matrix_bytes(rows, k);
+}
+extern "C" uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  return matrix_bytes(rows, n);
+}
+extern "C" uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  return 0;
+}
+
+// in [rows, nc] times the packed matrix P [ni, nc] -> out [rows, ni]
+static int times_weights(const char* name, const void* in, uint32_t in_type, uint64_t in_stride, const uint8_t* packed,
+                         const float* scale, uint32_t sp_i, uint32_t sp_b, uint16_t* out, uint64_t out_stride,
+                         uint32_t rows, uint32_t ni, uint32_t nc, void* workspace,
+                         uint64_t workspace_bytes, hipStream_t stream) {
+  if (bad_sizes(rows, ni, nc)) return fail(-1, name, "sizes have to be 1 .. 2^21 (rows may be 0)");
+  if (rows == 0) {
+    g_error.clear();
+    return 0;
+  }
+  if (bad_matrix(in, in_type, in_stride, nc) || bad_matrix(out, NETRA_BF16, out_stride, ni) || !packed ||
+      !aligned(packed, 16) || !scale || !aligned(scale, 4))
+    return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
+  if (bad_workspace(workspace, workspace_bytes, matrix_bytes(rows, nc)))
+    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  uint8_t* q = static_cast<uint8_t*>(workspace);
+  float* s = reinterpret_cast<float*>(q + code_bytes(rows, nc));
+  quant_rows(in, in_type, in_stride, q, s, rows, nc, stream);
+  nklin::Product a{};
+  a.p = packed;
+  a.sp = scale;
+  a.sp_i = sp_i;
+  a.sp_b = sp_b;
+  a.q = q;
+  a.sq = s;
+  a.sq_b = up(rows, 16u);
+  a.out = out;
+  a.ldo = out_stride;
+  a.ni = ni;
+  a.nq = rows;
+  a.kb = blocks(nc);
+  product(a, stream);
+  return launched(name);
+}
+
+extern "C" int netra_linear_forward(const void* x, uint32_t x_type, uint64_t x_stride, const uint8_t* packed,
+                                    const float* scale, uint16_t* y, uint64_t y_stride, uint32_t rows, uint32_t n,
+                                    uint32_t k, void* workspace, uint64_t workspace_bytes,
+                                    hipStream_t stream) {
+  return times_weights("netra_linear_forward", x, x_type, x_stride, packed, scale, blocks(k), 1u, y, y_stride,
+                       rows, n, k, workspace, workspace_bytes, stream);
+}
+
+extern "C" int netra_linear_input_gradient(const void* dy, uint32_t dy_type, uint64_t dy_stride,
+                                           const uint8_t* packed_t, const float* scale, uint16_t* dx, uint64_t dx_stride,
+                                           uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                                           uint64_t workspace_bytes, hipStream_t stream) {
+  return times_weights("netra_linear_input_gradient", dy, dy_type, dy_stride, packed_t, scale, 1u, blocks(k), dx,
+                       dx_stride, rows, k, n, workspace, workspace_bytes, stream);
+}
+
+extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* x,
+                                            uint32_t x_type, uint64_t x_stride, float* dw, uint32_t accumulate,
+                                            uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                                            uint64_t workspace_bytes, hipStream_t stream) {
+  const char* name = "netra_linear_weight_gradient";
+  if (bad_sizes(rows, n, k)) return fail(-1, name, "sizes have to be 1 .. 2^21 (rows may be 0)");
+  if (!dw || !aligned(dw, 4)) return fail(-1, name, "null or misaligned dw");
+  if (rows == 0) {
+    if (!accumulate)
+      netra_linear_zero_gfx950<<<dim3(1024), dim3(256), 0, stream>>>(dw, static_cast<uint64_t>(n) * k);
+    return launched(name);
+  }
+  if (bad_matrix(dy, dy_type, dy_stride, n) || bad_matrix(x, x_type, x_stride, k))
+    return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
+  if (bad_workspace(workspace, workspace_bytes, netra_linear_weight_gradient_workspace(rows, n, k)))
+    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  const nklin::Outer a{dy, dy_stride, dy_type, x, x_stride, x_type, dw, rows, n, k, accumulate ? 1u : 0u};
+  netra_linear_outer_direct_gfx950<<<dim3((k + 63u) / 64u, (n + 63u) / 64u), dim3(256), 0, stream>>>(a);
+  return launched(name);
+}
+
+// ---- router -------------------------------------------------------------------
+
+static bool bad_router(uint32_t tokens, uint32_t slots, uint32_t experts) {
+  return experts == 0 || experts > nkbal::kMaxExperts || static_cast<uint64_t>(tokens) * slots > 0x7fffffffull ||
+         tokens > 0x7fffffffu;
+}
+
+extern "C" uint64_t netra_router_counts_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) { return 0; }
+
+extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, const uint8_t* mask, uint32_t tokens,
+                                   uint32_t slots, uint32_t experts, int32_t* counts, uint32_t accumulate,
+                                   void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  const char* name = "netra_router_counts";
+  if (bad_router(tokens, slots, experts) || slots == 0)
+    return fail(-1, name, "experts have to be 1 .. 1024, slots 1 or more, tokens * slots below 2^31");
+  if (!counts || !aligned(counts, 4) || (tokens && (!ids || !aligned(ids, 4) || ids_stride < slots)))
+    return fail(-1, name, "null or misaligned pointer, or ids' row stride below the slots");
+  if (bad_workspace(workspace, workspace_bytes, netra_router_counts_workspace(tokens, slots, experts)))
+    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  netra_router_counts_gfx950<<<dim3(1), dim3(nkbal::kCountThreads), 0, stream>>>(
+      ids, ids_stride, mask, tokens, slots, experts, counts, accumulate, nullptr, nullptr);
+  return launched(name);
+}
+
+static constexpr uint32_t kBalanceGrid = 1024;
+
+extern "C" uint64_t netra_router_balance_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
+  return 16u + 4u * kBalanceGrid;
+}
+
+extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, uint64_t logits_stride, const float* bias,
+                                    const int32_t* ids, uint64_t ids_stride, uint32_t slots, const uint8_t* mask,
+                                    uint32_t tokens, uint32_t experts, float coefficient, int32_t* counts,
+                                    float* loss, void* grad, uint64_t grad_stride, void* workspace,
+                                    uint64_t workspace_bytes, hipStream_t stream) {
+  const char* name = "netra_router_balance";
+  if (bad_router(tokens, slots, experts))
+    return fail(-1, name, "experts have to be 1 .. 1024, tokens and tokens * slots below 2^31");
+  if (bad_type(logits_type) || !counts || !aligned(counts, 4) || !loss || !aligned(loss, 4) ||
+      (bias && !aligned(bias, 4)))
+    return fail(-1, name, "null or misaligned pointer or unknown type");
+  if (tokens && (bad_matrix(logits, logits_type, logits_stride, experts) ||
+                 (slots && (!ids || !aligned(ids, 4) || ids_stride < slots)) ||
+                 (grad && bad_matrix(grad, logits_type, grad_stride, experts))))
+    return fail(-1, name, "null or misaligned pointer, or row stride below the row");
+  if (bad_workspace(workspace, workspace_bytes, netra_router_balance_workspace(tokens, slots, experts)))
+    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  uint32_t* words = static_cast<uint32_t*>(workspace);
+  netra_router_counts_gfx950<<<dim3(1), dim3(nkbal::kCountThreads), 0, stream>>>(
+      ids, ids_stride, mask, tokens, slots, experts, counts, slots ? 0u : 1u, words, words + 1);
+  nkbal::Balance a{};
+  a.z = logits;
+  a.z_stride = logits_stride;
+  a.bias = bias;
+  a.mask = mask;
+  a.tokens = tokens;
+  a.experts = experts;
+  a.coefficient = coefficient;
+  a.counts = counts;
+  a.valid = words;
+  a.loss = loss;
+  a.grad = grad;
+  a.grad_stride = grad_stride;
+  a.partial = reinterpret_cast<float*>(words + 4);
+  a.arrived = words + 1;
+  uint32_t grid = (tokens + 3u) / 4u;
+  grid = grid < 1u ? 1u : grid > kBalanceGrid ? kBalanceGrid : grid;
+#define NETRA_RUN(NAME, NV) netra_router_balance_##NAME##_v##NV##_gfx950<<<dim3(grid), dim3(256), 0, stream>>>(a)
+#define NETRA_PICK(NAME)                     \
+  if (experts <= 64u) NETRA_RUN(NAME, 1);    \
+  else if (experts <= 128u) NETRA_RUN(NAME, 2); \
+  else if (experts <= 256u) NETRA_RUN(NAME, 4); \
+  else if (experts <= 512u) NETRA_RUN(NAME, 8); \
+  else NETRA_RUN(NAME, 16)
+  if (logits_type == NETRA_BF16) {
+    NETRA_PICK(bf16);
+  } else {
+    NETRA_PICK(f32);
+  }
+#undef NETRA_PICK
+#undef NETRA_RUN
+  return launched(name);
+}
+
+extern "C" const char* netra_layers_last_error(void) { return g_error.c_str(); }

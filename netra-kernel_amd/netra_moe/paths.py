@@ -24,5 +24,9 @@ def ops_bridge_library() -> Path:
     return LIB_DIR / "libnetra_bridges.so"
 
 
+def layers_library() -> Path:
+    return LIB_DIR / "libnetra_layers.so"
+
+
 def header_paths() -> list[Path]:
     return sorted((REPO_ROOT / "include").glob("*.h"))
