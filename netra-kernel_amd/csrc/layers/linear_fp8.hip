@@ -12,7 +12,7 @@
 //   input gradient   P = W^T      Q = dy   s_p = s_w[b, i/128]
 // The weight gradient is a bf16 product over the tokens (no scales).
 #pragma once
-#include "../kernels/moe_numerics.h"
+#include "lds_copy.h"
 
 namespace nklin {
 
@@ -132,14 +132,14 @@ __device__ __forceinline__ void store4(float* out, uint32_t left, bool vec, cons
 struct Product {
   const uint8_t* p;       // tiles of P [ni, contraction]
   const float* sp;        // scale of (i, b) at (i / 128) * sp_i + b * sp_b
-  uint32_t sp_i, sp_b;
+  uint32_t sp_i, sp_b, sp_bytes;
   const uint8_t* q;       // tiles of Q [nq, contraction]
   const float* sq;        // scale of (b, q) at b * sq_b + q
   uint32_t sq_b;
   uint16_t* out;          // bf16 [nq, ni], row stride ldo elements
   uint64_t ldo;
   uint32_t ni, nq, kb;    // kb: 128-blocks of the contraction
-  uint32_t vec;           // rows of out are aligned for four-element stores
+  uint32_t vec;           // rows of out are 16-byte aligned
 };
 
 // The simplest form: a wave computes 32 x 32 of the output, its operands read
@@ -189,6 +189,144 @@ __device__ __forceinline__ void product_direct(const Product& a) {
       if (row >= a.nq || col >= a.ni) continue;
       const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
       store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, a.vec != 0u, v);
+    }
+  }
+}
+
+// The same product with both operands staged through LDS.
+//
+// A workgroup of 8 waves (WP along P, WQ along Q) computes 16 WP NP rows of P by
+// 16 WQ NQ rows of Q. Per 128-block ("step") it needs one tile row of each
+// operand and the scales; they are copied global -> LDS one step ahead, into the
+// stage that the step before has been read from. A step's single barrier, behind
+// each wave's wait for its own copies, both shows the step's data to all waves and
+// tells them that the other stage may be overwritten.
+// Each wave holds its NQ operands of Q for the step and streams its NP operands of
+// P past them: NQ products per operand, each scaled and added by VALU while the
+// matrix core works on the next.
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ>
+struct Tile {
+  static constexpr uint32_t kP = WP * NP, kQ = WQ * NQ;              // 16-row tiles of each operand
+  static constexpr uint32_t kScaleAt = (kP + kQ) * 2048u;            // scales of Q (one 1 KiB copy), then of P
+  static constexpr uint32_t kStage = kScaleAt + 1024u + 256u;
+  static constexpr uint32_t kWaves = WP * WQ;
+  // A row's pitch of the output's staging: 16 bytes over its NP tiles spread the writes over the banks.
+  static constexpr uint32_t kPitch = NP * 32u + 16u;
+  static constexpr uint32_t kOut = kWaves * 16u * NQ * kPitch;
+  static constexpr uint32_t kLds = 2u * kStage > kOut ? 2u * kStage : kOut;
+};
+
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ>
+__device__ __forceinline__ void product_tile(const Product& a) {
+  using L = Tile<WP, WQ, NP, NQ>;
+  static_assert(L::kP % 8u == 0u && NP % 8u == 0u && L::kP <= 16u && L::kQ <= 16u && L::kWaves == 8u, "P's scale blocks, waves");
+  __shared__ __align__(16) uint8_t s_stage[L::kLds];
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u;
+  const uint32_t np = (pt + L::kP - 1u) / L::kP, nq = (qt + L::kQ - 1u) / L::kQ;
+  // The workgroups of an XCD (ids deal to the eight XCDs in turn) take neighbouring
+  // tiles, in bands of 8 along Q, so that they share operands in its L2.
+  const uint32_t total = np * nq, per = (total + 7u) / 8u;
+  const uint32_t item = (blockIdx.x % 8u) * per + blockIdx.x / 8u;
+  if (blockIdx.x / 8u >= per || item >= total) return;
+  const uint32_t band = item / (8u * np), in_band = item - band * 8u * np;
+  const uint32_t height = min(8u, nq - band * 8u);
+  const uint32_t bp = in_band / height, bq = band * 8u + in_band % height;
+  const uint32_t p0 = bp * L::kP, q0 = bq * L::kQ;  // first 16-row tiles
+  const uint32_t wp = wave % WP, wq = wave / WP;
+
+  const u32x4 rp = nklds2::rsrc(a.p + (size_t)p0 * a.kb * 2048u, min(L::kP, pt - p0) * a.kb * 2048u);
+  const u32x4 rq = nklds2::rsrc(a.q + (size_t)q0 * a.kb * 2048u, min(L::kQ, qt - q0) * a.kb * 2048u);
+  const u32x4 rsp = nklds2::rsrc(a.sp, a.sp_bytes);
+  // lanes 0, 1: the scales of P's (up to) two 128-blocks
+  const uint32_t spoff = lane < L::kP / 8u && (p0 / 8u + lane) * 128u < a.ni ? (p0 / 8u + lane) * a.sp_i * 4u : 0x80000000u;
+  const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
+  auto issue = [&](uint32_t b) __attribute__((always_inline)) {
+    const uint32_t st = lds0 + (b & 1u) * L::kStage;
+    constexpr uint32_t kTiles = L::kP + L::kQ;
+#pragma unroll
+    for (uint32_t i = 0; i < kTiles / L::kWaves; ++i) {
+      const uint32_t t = i * L::kWaves + wave;  // P's tiles, then Q's
+      const bool is_p = i < L::kP / L::kWaves;
+      const uint32_t voff = (is_p ? t : t - L::kP) * a.kb * 2048u + lane * 16u;
+      const uint32_t m0 = st + t * 2048u;
+      nklds2::copy16(m0, is_p ? rp : rq, voff, b * 2048u);
+      nklds2::copy16(m0 + 1024u, is_p ? rp : rq, voff + 1024u, b * 2048u);
+    }
+    if (wave == 0u) {
+      // num_records ends with this block's scales; rows past them give zeros
+      const u32x4 rsq = nklds2::rsrc(a.sq + (size_t)b * a.sq_b + q0 * 16u, (a.sq_b - q0 * 16u) * 4u);
+      nklds2::copy16(st + L::kScaleAt, rsq, lane < L::kQ * 4u ? lane * 16u : 0x80000000u, 0u);
+    }
+    if (wave == 1u) nklds2::copy4(st + L::kScaleAt + 1024u, rsp, spoff, b * a.sp_b * 4u);
+  };
+
+  v4f acc[NP][NQ];
+#pragma unroll
+  for (uint32_t i = 0; i < NP; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  issue(0u);
+  for (uint32_t b = 0; b < a.kb; ++b) {
+    nklds2::wait_copies<0>();
+    nklds2::barrier();
+    if (b + 1u < a.kb) issue(b + 1u);
+    const uint8_t* st = s_stage + (b & 1u) * L::kStage;
+    const uint8_t* sp_tiles = st + wp * NP * 2048u;
+    const uint8_t* sq_tiles = st + (L::kP + wq * NQ) * 2048u;
+    const float* scale = reinterpret_cast<const float*>(st + L::kScaleAt);
+    v8i qo[NQ];
+    float s[NQ];
+    const float sp = scale[256u + wp * NP / 8u];
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) {
+      qo[j] = nk::load_tile_operand(sq_tiles + j * 2048u, lane);
+      s[j] = scale[(wq * NQ + j) * 16u + (lane & 15u)] * sp;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) {
+      const v8i po = nk::load_tile_operand(sp_tiles + i * 2048u, lane);
+#pragma unroll
+      for (uint32_t j = 0; j < NQ; ++j) {
+        const v4f d = nk::mfma_e4m3_16x16x128(po, qo[j]);
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) acc[i][j][e] = fmaf(s[j], d[e], acc[i][j][e]);
+      }
+    }
+  }
+
+  // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
+  // whole lines.
+  constexpr uint32_t kPitch = L::kPitch;
+  __syncthreads();
+  uint8_t* mine = s_stage + wave * 16u * NQ * kPitch;
+  const uint32_t c = lane & 15u, r4 = (lane >> 4) * 4u;
+#pragma unroll
+  for (uint32_t j = 0; j < NQ; ++j)
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) {
+      const v4f v = acc[i][j];
+      *reinterpret_cast<uint2*>(mine + (j * 16u + c) * kPitch + (i * 16u + r4) * 2u) =
+          make_uint2(nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
+                     nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16));
+    }
+  // (a wave reads back only what it wrote itself)
+  const uint32_t col0 = (p0 + wp * NP) * 16u, row0 = (q0 + wq * NQ) * 16u;
+  constexpr uint32_t kLanes = NP * 2u;  // lanes of 8 values per row
+  for (uint32_t r = lane / kLanes; r < 16u * NQ; r += 64u / kLanes) {
+    const uint32_t cc = (lane % kLanes) * 8u, row = row0 + r, col = col0 + cc;
+    if (row >= a.nq || col >= a.ni) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kPitch + cc * 2u);
+    uint16_t* o = a.out + (uint64_t)row * a.ldo + col;
+    if (a.vec && col + 8u <= a.ni) {
+      *reinterpret_cast<uint4*>(o) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (uint32_t e = 0; e < 8u; ++e)
+        if (col + e < a.ni) o[e] = (uint16_t)(w[e / 2u] >> (16u * (e & 1u)));
     }
   }
 }
@@ -273,7 +411,7 @@ __device__ __forceinline__ void outer_direct(const Outer& a) {
 
 // Weights: w row-major e4m3 [n, k] -> tiles of w, or of w^T. One wave per tile;
 // bytes past the matrix are zeros.
-__global__ __launch_bounds__(256) void netra_linear_pack_gfx950(const uint8_t* __restrict__ w,
+extern "C" __global__ __launch_bounds__(256) void netra_linear_pack_gfx950(const uint8_t* __restrict__ w,
                                                                 uint8_t* __restrict__ dst, uint32_t n, uint32_t k,
                                                                 uint32_t transpose) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -296,7 +434,7 @@ __global__ __launch_bounds__(256) void netra_linear_pack_gfx950(const uint8_t* _
 }
 
 #define NETRA_QUANT_ROWS(NAME, X, VEC)                                                                       \
-  __global__ __launch_bounds__(256) void netra_linear_quant_rows_##NAME##_gfx950(                            \
+  extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_##NAME##_gfx950(                            \
       const X* x, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld) {          \
     nklin::quant_rows<X, VEC>(x, stride, q, s, rows, n, sld);                                                \
   }
@@ -305,13 +443,17 @@ NETRA_QUANT_ROWS(bf16_vec, uint16_t, true)
 NETRA_QUANT_ROWS(f32, float, false)
 NETRA_QUANT_ROWS(f32_vec, float, true)
 
-__global__ __launch_bounds__(256) void netra_linear_product_direct_gfx950(nklin::Product a) {
+extern "C" __global__ __launch_bounds__(256) void netra_linear_product_direct_gfx950(nklin::Product a) {
   nklin::product_direct(a);
 }
 
-__global__ __launch_bounds__(256) void netra_linear_outer_direct_gfx950(nklin::Outer a) { nklin::outer_direct(a); }
+extern "C" __global__ __launch_bounds__(512) void netra_linear_product_256x256_gfx950(nklin::Product a) {
+  nklin::product_tile<2, 4, 8, 4>(a);
+}
+
+extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_direct_gfx950(nklin::Outer a) { nklin::outer_direct(a); }
 
 // dw of no tokens: zeros.
-__global__ __launch_bounds__(256) void netra_linear_zero_gfx950(float* out, uint64_t n) {
+extern "C" __global__ __launch_bounds__(256) void netra_linear_zero_gfx950(float* out, uint64_t n) {
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256u) out[i] = 0.0f;
 }

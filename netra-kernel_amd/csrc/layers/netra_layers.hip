@@ -70,7 +70,12 @@ void quant_rows(const void* x, uint32_t type, uint64_t stride, uint8_t* q, float
 }
 
 void product(nklin::Product a, hipStream_t stream) {
-  a.vec = aligned(a.out, 8) && a.ldo % 4u == 0;
+  a.vec = aligned(a.out, 16) && a.ldo % 8u == 0;
+  const uint32_t tiles = ((a.ni + 255u) / 256u) * ((a.nq + 255u) / 256u);
+  if (a.nq > 64u) {
+    netra_linear_product_256x256_gfx950<<<dim3((tiles + 7u) / 8u * 8u), dim3(512), 0, stream>>>(a);
+    return;
+  }
   netra_linear_product_direct_gfx950<<<dim3((a.ni + 63u) / 64u, (a.nq + 63u) / 64u), dim3(256), 0, stream>>>(a);
 }
 
@@ -127,6 +132,7 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   a.sp = scale;
   a.sp_i = sp_i;
   a.sp_b = sp_b;
+  a.sp_bytes = blocks(ni) * blocks(nc) * 4u;
   a.q = q;
   a.sq = s;
   a.sq_b = up(rows, 16u);

@@ -172,7 +172,7 @@ __device__ __forceinline__ void balance(const Balance& a) {
 }  // namespace nkbal
 
 // counts (and valid, if not null) of all tokens by one workgroup; clears *arrived if not null.
-__global__ __launch_bounds__(1024) void netra_router_counts_gfx950(const int32_t* ids, uint64_t stride,
+extern "C" __global__ __launch_bounds__(1024) void netra_router_counts_gfx950(const int32_t* ids, uint64_t stride,
                                                                    const uint8_t* mask, uint32_t tokens,
                                                                    uint32_t slots, uint32_t E, int32_t* counts,
                                                                    uint32_t accumulate, uint32_t* valid,
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(1024) void netra_router_counts_gfx950(const int32_t
 }
 
 #define NETRA_BALANCE(NAME, X, NV)                                                                   \
-  __global__ __launch_bounds__(256) void netra_router_balance_##NAME##_v##NV##_gfx950(nkbal::Balance a) { \
+  extern "C" __global__ __launch_bounds__(256) void netra_router_balance_##NAME##_v##NV##_gfx950(nkbal::Balance a) { \
     nkbal::balance<X, NV>(a);                                                                        \
   }
 NETRA_BALANCE(bf16, uint16_t, 1)
