@@ -345,6 +345,8 @@ struct Outer {
   float* dw;        // [n, k]
   uint32_t rows, n, k;
   uint32_t accumulate;
+  uint32_t splits, split_rows;  // tokens per split (a multiple of 64)
+  float* partial;               // [splits, n, k] where splits > 1
 };
 
 // Eight tokens' values of one column as an MFMA operand, zeros past the end.
@@ -407,6 +409,172 @@ __device__ __forceinline__ void outer_direct(const Outer& a) {
   }
 }
 
+// The same product with both operands staged through LDS, for bf16 matrices whose
+// rows are 16-byte aligned and whole 16-byte chunks. Both have the contraction (tokens) as their slow
+// dimension, so their rows are copied as they are and the transposed LDS reads
+// (ds_read_b64_tr_b16: among 16 lanes, lane i gets element i % 4 of the 8 bytes
+// that lanes i / 4 + 0, 4, 8, 12 address) turn 4 tokens x 16 columns into operand
+// rows. A stage holds 64 tokens; a token's row is kept in 32-byte groups (16
+// columns) of which group c sits at c ^ f(t), f(t) = t % 4 + 4 (t / 8 % 2): the 16
+// tokens of one read then meet every bank twice, which is what 512 bytes need.
+// Workgroups, waves and the stage hand-over are product_tile's. Columns past the
+// matrix read the next row and make outputs that are not stored; tokens past the
+// end read zeros.
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ>
+__device__ __forceinline__ void outer_tile(const Outer& a) {
+  constexpr uint32_t kP = WP * NP, kQ = WQ * NQ, kTokens = 64u;
+  constexpr uint32_t kRowP = kP * 32u, kRowQ = kQ * 32u;  // bytes of a token's row
+  constexpr uint32_t kStage = kTokens * (kRowP + kRowQ);
+  static_assert(WP * WQ == 8u && (kRowP == 256u || kRowP == 512u) && (kRowQ == 256u || kRowQ == 512u) &&
+                    NP % 4u == 0u, "copies and swizzle");
+  __shared__ __align__(16) uint8_t s_stage[2u * kStage];
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t np = (a.k + 16u * kP - 1u) / (16u * kP), nq = (a.n + 16u * kQ - 1u) / (16u * kQ);
+  const uint32_t total = np * nq * a.splits, per = (total + 7u) / 8u;
+  const uint32_t item = (blockIdx.x % 8u) * per + blockIdx.x / 8u;
+  if (blockIdx.x / 8u >= per || item >= total) return;
+  const uint32_t split = item / (np * nq), tile = item - split * np * nq;
+  const uint32_t band = tile / (8u * np), in_band = tile - band * 8u * np;
+  const uint32_t height = min(8u, nq - band * 8u);
+  const uint32_t p0 = in_band / height * 16u * kP, q0 = (band * 8u + in_band % height) * 16u * kQ;  // first columns
+  const uint32_t wp = wave % WP, wq = wave / WP;
+  // this split's tokens
+  const uint32_t t0 = split * a.split_rows, t1 = min(a.rows, t0 + a.split_rows);
+
+  // lane's place in a copy of 1 KiB: row r of the 1024 / row bytes, 16-byte chunk
+  auto lane_offset = [&](uint32_t row_bytes, uint64_t stride) __attribute__((always_inline)) {
+    const uint32_t lanes = row_bytes / 16u, r = lane / lanes, chunk = lane % lanes;
+    const uint32_t t = wave * (64u / lanes) + r;  // (rows 16 or 32 further have the same f)
+    const uint32_t f = (t & 3u) | ((t >> 3) & 1u) << 2;
+    return r * (uint32_t)stride * 2u + (chunk ^ (f << 1)) * 16u;
+  };
+  const uint32_t pv = lane_offset(kRowP, a.x_stride), qv = lane_offset(kRowQ, a.dy_stride);
+  const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
+  auto issue = [&](uint32_t t, uint32_t parity) __attribute__((always_inline)) {
+    const uint32_t st = lds0 + parity * kStage;
+    auto rows = [&](const void* m, uint64_t stride, uint32_t c0, uint32_t cols, uint32_t row_bytes, uint32_t v,
+                    uint32_t at) __attribute__((always_inline)) {
+      const uint16_t* base = static_cast<const uint16_t*>(m) + (uint64_t)t * stride + c0;
+      // tokens t .. min(t1, t + 64) - 1, from column c0 (rows are whole 16-byte chunks)
+      const uint32_t n = min(kTokens, t1 - t);
+      const u32x4 r = nklds2::rsrc(base, ((n - 1u) * (uint32_t)stride + (((cols + 7u) & ~7u) - c0)) * 2u);
+      const uint32_t each = 1024u / row_bytes;  // rows per copy
+#pragma unroll
+      for (uint32_t i = 0; i < kTokens / each / 8u; ++i) {
+        const uint32_t row = (i * 8u + wave) * each;
+        nklds2::copy16(at + row * row_bytes, r, v, row * (uint32_t)stride * 2u);
+      }
+    };
+    rows(a.x, a.x_stride, p0, a.k, kRowP, pv, st);
+    rows(a.dy, a.dy_stride, q0, a.n, kRowQ, qv, st + kTokens * kRowP);
+  };
+
+  v4f acc[NP][NQ];
+#pragma unroll
+  for (uint32_t i = 0; i < NP; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t c = lane & 15u, g = lane >> 4;
+  const uint32_t f = (c >> 2) | (g & 1u) << 2;  // of the tokens this lane addresses
+  // operand of column tile `tile` and tokens 32 h ..: tokens 32 h + 8 g .. + 7
+  auto operand = [&](const uint8_t* m, uint32_t row_bytes, uint32_t tile, uint32_t h) __attribute__((always_inline)) {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s* lds_v4s;
+    const uint8_t* at = m + (h * 32u + g * 8u + (c >> 2)) * row_bytes + (tile ^ f) * 32u + (c & 3u) * 8u;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)at);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + 4u * row_bytes));
+    typedef short v8s __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  if (t0 < t1) issue(t0, 0u);
+  uint32_t parity = 0u;
+  for (uint32_t t = t0; t < t1; t += kTokens, parity ^= 1u) {
+    nklds2::wait_copies<0>();
+    nklds2::barrier();
+    if (t + kTokens < t1) issue(t + kTokens, parity ^ 1u);
+    const uint8_t* px = s_stage + parity * kStage;
+    const uint8_t* pq = px + kTokens * kRowP;
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; ++h) {
+      v8bf qo[NQ];
+#pragma unroll
+      for (uint32_t j = 0; j < NQ; ++j) qo[j] = operand(pq, kRowQ, wq * NQ + j, h);
+#pragma unroll
+      for (uint32_t i = 0; i < NP; ++i) {
+        const v8bf po = operand(px, kRowP, wp * NP + i, h);
+#pragma unroll
+        for (uint32_t j = 0; j < NQ; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(po, qo[j], acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+  float* dst = a.splits > 1u ? a.partial + (size_t)split * a.n * a.k : a.dw;
+  const bool add = a.accumulate && a.splits == 1u;
+  const bool vec = a.k % 4u == 0u && reinterpret_cast<uintptr_t>(dst) % 16u == 0u;
+#pragma unroll
+  for (uint32_t j = 0; j < NQ; ++j) {
+    const uint32_t row = q0 + (wq * NQ + j) * 16u + c;
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) {
+      const uint32_t col = p0 + (wp * NP + i) * 16u + g * 4u;
+      if (row >= a.n || col >= a.k) continue;
+      float* o = dst + (uint64_t)row * a.k + col;
+      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (add) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e)
+          if (col + e < a.k) v[e] += o[e];
+      }
+      store4(o, a.k - col, vec, v);
+    }
+  }
+}
+
+// dw = (dw +) the sum of the splits, in split order.
+__device__ __forceinline__ void outer_sum(const Outer& a) {
+  const uint64_t n = (uint64_t)a.n * a.k;
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256u + threadIdx.x) * 4u; i < n; i += (uint64_t)gridDim.x * 1024u) {
+    if (i + 4u <= n && reinterpret_cast<uintptr_t>(a.dw) % 16u == 0u && n % 4u == 0u) {
+      float4 s = *reinterpret_cast<const float4*>(a.partial + i);
+      for (uint32_t k = 1; k < a.splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(a.partial + k * n + i);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+      float4* o = reinterpret_cast<float4*>(a.dw + i);
+      if (a.accumulate) {
+        const float4 v = *o;
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+      *o = s;
+    } else {
+      for (uint64_t j = i; j < min(i + 4u, n); ++j) {
+        float s = a.partial[j];
+        for (uint32_t k = 1; k < a.splits; ++k) s += a.partial[k * n + j];
+        a.dw[j] = a.accumulate ? a.dw[j] + s : s;
+      }
+    }
+  }
+}
+
+// A matrix as bf16 with rows of `pitch` elements (a multiple of 8), for operands
+// that are fp32 or not aligned.
+template <typename X>
+__device__ __forceinline__ void to_bf16(const X* __restrict__ x, uint64_t stride, uint16_t* __restrict__ out,
+                                        uint32_t rows, uint32_t cols, uint32_t pitch) {
+  const uint32_t c = (blockIdx.x * 64u + (threadIdx.x & 63u)) * 8u;
+  if (c >= pitch) return;
+  for (uint32_t r = blockIdx.y * 4u + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4u) {
+    const X* p = x + (uint64_t)r * stride + c;
+    uint32_t w[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e)
+      w[e] = nk::bf16_rne(c + 2u * e < cols ? value(p + 2u * e) : 0.0f) |
+             (uint32_t)nk::bf16_rne(c + 2u * e + 1u < cols ? value(p + 2u * e + 1u) : 0.0f) << 16;
+    *reinterpret_cast<uint4*>(out + (uint64_t)r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 }  // namespace nklin
 
 // Weights: w row-major e4m3 [n, k] -> tiles of w, or of w^T. One wave per tile;
@@ -452,6 +620,28 @@ extern "C" __global__ __launch_bounds__(512) void netra_linear_product_256x256_g
 }
 
 extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_direct_gfx950(nklin::Outer a) { nklin::outer_direct(a); }
+
+extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_256x256_gfx950(nklin::Outer a) {
+  nklin::outer_tile<2, 4, 8, 4>(a);
+}
+extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_128x256_gfx950(nklin::Outer a) {
+  nklin::outer_tile<2, 4, 4, 4>(a);
+}
+extern "C" __global__ __launch_bounds__(512, 4) void netra_linear_outer_128x128_gfx950(nklin::Outer a) {
+  nklin::outer_tile<2, 4, 4, 2>(a);
+}
+extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_sum_gfx950(nklin::Outer a) { nklin::outer_sum(a); }
+
+extern "C" __global__ __launch_bounds__(256) void netra_linear_to_bf16_f32_gfx950(const float* x, uint64_t stride,
+                                                                                  uint16_t* out, uint32_t rows,
+                                                                                  uint32_t cols, uint32_t pitch) {
+  nklin::to_bf16<float>(x, stride, out, rows, cols, pitch);
+}
+extern "C" __global__ __launch_bounds__(256) void netra_linear_to_bf16_bf16_gfx950(const uint16_t* x, uint64_t stride,
+                                                                                   uint16_t* out, uint32_t rows,
+                                                                                   uint32_t cols, uint32_t pitch) {
+  nklin::to_bf16<uint16_t>(x, stride, out, rows, cols, pitch);
+}
 
 // dw of no tokens: zeros.
 extern "C" __global__ __launch_bounds__(256) void netra_linear_zero_gfx950(float* out, uint64_t n) {

@@ -79,6 +79,47 @@ void product(nklin::Product a, hipStream_t stream) {
   netra_linear_product_direct_gfx950<<<dim3((a.ni + 63u) / 64u, (a.nq + 63u) / 64u), dim3(256), 0, stream>>>(a);
 }
 
+// An operand of the weight gradient as it is, or as bf16 with aligned rows in the workspace.
+bool outer_ready(const void* m, uint32_t type, uint64_t stride, uint32_t cols) {
+  return type == NETRA_BF16 && aligned(m, 16) && cols % 8u == 0 && stride % 8u == 0 && stride < (1u << 24);
+}
+void outer_operand(const void*& m, uint32_t& type, uint64_t& stride, uint32_t rows, uint32_t cols, uint8_t*& at,
+                   hipStream_t stream) {
+  if (outer_ready(m, type, stride, cols)) return;
+  const uint32_t pitch = up(cols, 8u);
+  const dim3 grid((pitch + 511u) / 512u, rows < 4u * 4096u ? (rows + 3u) / 4u : 4096u);
+  uint16_t* out = reinterpret_cast<uint16_t*>(at);
+  if (type == NETRA_F32)
+    netra_linear_to_bf16_f32_gfx950<<<grid, dim3(256), 0, stream>>>(static_cast<const float*>(m), stride, out, rows,
+                                                                    cols, pitch);
+  else
+    netra_linear_to_bf16_bf16_gfx950<<<grid, dim3(256), 0, stream>>>(static_cast<const uint16_t*>(m), stride, out,
+                                                                     rows, cols, pitch);
+  at += static_cast<uint64_t>(rows) * pitch * 2u;
+  m = out;
+  type = NETRA_BF16;
+  stride = pitch;
+}
+
+// Tile and split of the weight gradient.
+struct OuterPlan {
+  uint32_t p, q;  // columns of x and of dy per workgroup
+  uint32_t splits, split_rows;
+};
+OuterPlan outer_plan(uint32_t rows, uint32_t n, uint32_t k) {
+  auto tiles = [&](uint32_t p, uint32_t q) { return static_cast<uint64_t>((k + p - 1u) / p) * ((n + q - 1u) / q); };
+  OuterPlan plan{256, 256, 1, 0};
+  if (tiles(256, 256) < 200) plan = {128, 256, 1, 0};
+  if (tiles(128, 256) < 200) plan = {128, 128, 1, 0};
+  const uint64_t t = tiles(plan.p, plan.q);
+  uint32_t splits = t >= 200 ? 1u : static_cast<uint32_t>(256 / t);
+  const uint32_t most = (rows + 255u) / 256u;  // 256 tokens at least
+  splits = splits < 1u ? 1u : splits > most ? most : splits;
+  plan.split_rows = up((rows + splits - 1u) / splits, 64u);
+  plan.splits = (rows + plan.split_rows - 1u) / plan.split_rows;
+  return plan;
+}
+
 bool bad_workspace(const void* p, uint64_t bytes, uint64_t need) {
   return bytes < need || (need && (!p || !aligned(p, 16)));
 }
@@ -106,7 +147,10 @@ extern "C" uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_
   return matrix_bytes(rows, n);
 }
 extern "C" uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
-  return 0;
+  if (rows == 0) return 0;
+  const OuterPlan plan = outer_plan(rows, n, k);
+  return static_cast<uint64_t>(rows) * (up(n, 8u) + static_cast<uint64_t>(up(k, 8u))) * 2u +
+         (plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * n * k : 0u) + 16u;
 }
 
 // in [rows, nc] times the packed matrix P [ni, nc] -> out [rows, ni]
@@ -177,8 +221,33 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
   if (bad_workspace(workspace, workspace_bytes, netra_linear_weight_gradient_workspace(rows, n, k)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  const nklin::Outer a{dy, dy_stride, dy_type, x, x_stride, x_type, dw, rows, n, k, accumulate ? 1u : 0u};
-  netra_linear_outer_direct_gfx950<<<dim3((k + 63u) / 64u, (n + 63u) / 64u), dim3(256), 0, stream>>>(a);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  outer_operand(dy, dy_type, dy_stride, rows, n, at, stream);
+  outer_operand(x, x_type, x_stride, rows, k, at, stream);
+  const OuterPlan plan = outer_plan(rows, n, k);
+  nklin::Outer a{};
+  a.dy = dy;
+  a.dy_stride = dy_stride;
+  a.x = x;
+  a.x_stride = x_stride;
+  a.dw = dw;
+  a.rows = rows;
+  a.n = n;
+  a.k = k;
+  a.accumulate = accumulate ? 1u : 0u;
+  a.splits = plan.splits;
+  a.split_rows = plan.split_rows;
+  a.partial = reinterpret_cast<float*>(at);
+  const uint32_t items = ((k + plan.p - 1u) / plan.p) * ((n + plan.q - 1u) / plan.q) * plan.splits;
+  const dim3 grid((items + 7u) / 8u * 8u), block(512);
+  if (plan.p == 256u) netra_linear_outer_256x256_gfx950<<<grid, block, 0, stream>>>(a);
+  else if (plan.q == 256u) netra_linear_outer_128x256_gfx950<<<grid, block, 0, stream>>>(a);
+  else netra_linear_outer_128x128_gfx950<<<grid, block, 0, stream>>>(a);
+  if (plan.splits > 1u) {
+    const uint64_t quads = (static_cast<uint64_t>(n) * k + 1023u) / 1024u;
+    netra_linear_outer_sum_gfx950<<<dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), 0, stream>>>(
+        a);
+  }
   return launched(name);
 }
 
