@@ -140,86 +140,40 @@ struct Product {
   uint64_t ldo;
   uint32_t ni, nq, kb;    // kb: 128-blocks of the contraction
   uint32_t vec;           // rows of out are 16-byte aligned
+  uint32_t splits, split_blocks;  // 128-blocks per split
+  float* partial;         // [splits, nq, ni rounded up to 4] where splits > 1
 };
-
-// The simplest form: a wave computes 32 x 32 of the output, its operands read
-// straight from memory.
-__device__ __forceinline__ void product_direct(const Product& a) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u;
-  const uint32_t p0 = blockIdx.x * 4u + (wave & 1u) * 2u, q0 = blockIdx.y * 4u + (wave >> 1) * 2u;
-  if (p0 >= pt || q0 >= qt) return;
-  const uint32_t c = lane & 15u, r4 = (lane >> 4) * 4u;
-  v4f acc[2][2];
-#pragma unroll
-  for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-    for (uint32_t j = 0; j < 2u; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t b = 0; b < a.kb; ++b) {
-    v8i po[2], qo[2];
-    float sp[2], sq[2];
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
-      const uint32_t t = min(p0 + i, pt - 1u);
-      po[i] = nk::load_tile_operand(nk::tile_base(a.p, t, b, a.kb), lane);
-      sp[i] = a.sp[(size_t)(t / 8u) * a.sp_i + (size_t)b * a.sp_b];
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < 2u; ++j) {
-      const uint32_t t = min(q0 + j, qt - 1u);
-      qo[j] = nk::load_tile_operand(nk::tile_base(a.q, t, b, a.kb), lane);
-      sq[j] = a.sq[(size_t)b * a.sq_b + t * 16u + c];
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-      for (uint32_t j = 0; j < 2u; ++j) {
-        const v4f d = nk::mfma_e4m3_16x16x128(po[i], qo[j]);
-        const float s = sq[j] * sp[i];
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) acc[i][j][e] = fmaf(s, d[e], acc[i][j][e]);
-      }
-  }
-#pragma unroll
-  for (uint32_t j = 0; j < 2u; ++j) {
-    const uint32_t row = (q0 + j) * 16u + c;
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
-      const uint32_t col = (p0 + i) * 16u + r4;
-      if (row >= a.nq || col >= a.ni) continue;
-      const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, a.vec != 0u, v);
-    }
-  }
-}
 
 // The same product with both operands staged through LDS.
 //
 // A workgroup of 8 waves (WP along P, WQ along Q) computes 16 WP NP rows of P by
 // 16 WQ NQ rows of Q. Per 128-block ("step") it needs one tile row of each
-// operand and the scales; they are copied global -> LDS one step ahead, into the
-// stage that the step before has been read from. A step's single barrier, behind
-// each wave's wait for its own copies, both shows the step's data to all waves and
-// tells them that the other stage may be overwritten.
+// operand and the scales; they are copied global -> LDS, S - 1 steps ahead, into
+// a ring of S stages. A step's single barrier, behind each wave's wait for its own
+// copies of the step, both shows the step's data to all waves and tells them that
+// the stage of the step before may be overwritten.
 // Each wave holds its NQ operands of Q for the step and streams its NP operands of
 // P past them: NQ products per operand, each scaled and added by VALU while the
 // matrix core works on the next.
-template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ>
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 struct Tile {
-  static constexpr uint32_t kP = WP * NP, kQ = WQ * NQ;              // 16-row tiles of each operand
-  static constexpr uint32_t kScaleAt = (kP + kQ) * 2048u;            // scales of Q (one 1 KiB copy), then of P
-  static constexpr uint32_t kStage = kScaleAt + 1024u + 256u;
   static constexpr uint32_t kWaves = WP * WQ;
+  static constexpr uint32_t kP = WP * NP, kQ = WQ * NQ;   // 16-row tiles of each operand
+  static constexpr uint32_t kScaleAt = (kP + kQ) * 2048u; // 16 scales per tile of Q, then 64 words for P's
+  static constexpr uint32_t kStage = kScaleAt + kQ * 64u + 256u;
+  static constexpr uint32_t kCopies = (kP + kQ) * 2u / kWaves + 1u;  // a wave's, per step
   // A row's pitch of the output's staging: 16 bytes over its NP tiles spread the writes over the banks.
   static constexpr uint32_t kPitch = NP * 32u + 16u;
   static constexpr uint32_t kOut = kWaves * 16u * NQ * kPitch;
-  static constexpr uint32_t kLds = 2u * kStage > kOut ? 2u * kStage : kOut;
+  static constexpr uint32_t kLds = S * kStage > kOut ? S * kStage : kOut;
+  static_assert(kWaves == 8u && (NP % 8u == 0u || 8u % NP == 0u) && kP % kWaves == 0u && kQ % kWaves == 0u &&
+                    kP <= 64u * 8u && kQ % 4u == 0u && kQ <= 28u && kLds <= 160u * 1024u,
+                "waves, scale blocks, copies and LDS");
 };
 
-template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ>
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 __device__ __forceinline__ void product_tile(const Product& a) {
-  using L = Tile<WP, WQ, NP, NQ>;
-  static_assert(L::kP % 8u == 0u && NP % 8u == 0u && L::kP <= 16u && L::kQ <= 16u && L::kWaves == 8u, "P's scale blocks, waves");
+  using L = Tile<WP, WQ, NP, NQ, S>;
   __shared__ __align__(16) uint8_t s_stage[L::kLds];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -227,39 +181,41 @@ __device__ __forceinline__ void product_tile(const Product& a) {
   const uint32_t np = (pt + L::kP - 1u) / L::kP, nq = (qt + L::kQ - 1u) / L::kQ;
   // The workgroups of an XCD (ids deal to the eight XCDs in turn) take neighbouring
   // tiles, in bands of 8 along Q, so that they share operands in its L2.
-  const uint32_t total = np * nq, per = (total + 7u) / 8u;
+  const uint32_t total = np * nq * a.splits, per = (total + 7u) / 8u;
   const uint32_t item = (blockIdx.x % 8u) * per + blockIdx.x / 8u;
   if (blockIdx.x / 8u >= per || item >= total) return;
-  const uint32_t band = item / (8u * np), in_band = item - band * 8u * np;
+  const uint32_t split = item / (np * nq), tile = item - split * np * nq;
+  const uint32_t band = tile / (8u * np), in_band = tile - band * 8u * np;
   const uint32_t height = min(8u, nq - band * 8u);
-  const uint32_t bp = in_band / height, bq = band * 8u + in_band % height;
-  const uint32_t p0 = bp * L::kP, q0 = bq * L::kQ;  // first 16-row tiles
+  const uint32_t p0 = in_band / height * L::kP, q0 = (band * 8u + in_band % height) * L::kQ;  // first 16-row tiles
   const uint32_t wp = wave % WP, wq = wave / WP;
+  const uint32_t b0 = split * a.split_blocks, b1 = min(a.kb, b0 + a.split_blocks);  // this split's blocks
 
   const u32x4 rp = nklds2::rsrc(a.p + (size_t)p0 * a.kb * 2048u, min(L::kP, pt - p0) * a.kb * 2048u);
   const u32x4 rq = nklds2::rsrc(a.q + (size_t)q0 * a.kb * 2048u, min(L::kQ, qt - q0) * a.kb * 2048u);
   const u32x4 rsp = nklds2::rsrc(a.sp, a.sp_bytes);
-  // lanes 0, 1: the scales of P's (up to) two 128-blocks
-  const uint32_t spoff = lane < L::kP / 8u && (p0 / 8u + lane) * 128u < a.ni ? (p0 / 8u + lane) * a.sp_i * 4u : 0x80000000u;
+  // A wave copies one 64-word part of the scales: Q's by the first kQ / 4 waves, P's
+  // (lane i: 128-block i of the tile) by the others, all of them alike.
+  const bool q_scales = wave < L::kQ / 4u;
+  const uint32_t spoff =
+      lane * 8u < L::kP && (p0 / 8u + lane) * 128u < a.ni ? (p0 / 8u + lane) * a.sp_i * 4u : 0x80000000u;
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
-  auto issue = [&](uint32_t b) __attribute__((always_inline)) {
-    const uint32_t st = lds0 + (b & 1u) * L::kStage;
-    constexpr uint32_t kTiles = L::kP + L::kQ;
+  auto issue = [&](uint32_t b, uint32_t stage) __attribute__((always_inline)) {
+    const uint32_t st = lds0 + stage * L::kStage;
 #pragma unroll
-    for (uint32_t i = 0; i < kTiles / L::kWaves; ++i) {
+    for (uint32_t i = 0; i < (L::kP + L::kQ) / L::kWaves; ++i) {
       const uint32_t t = i * L::kWaves + wave;  // P's tiles, then Q's
       const bool is_p = i < L::kP / L::kWaves;
       const uint32_t voff = (is_p ? t : t - L::kP) * a.kb * 2048u + lane * 16u;
-      const uint32_t m0 = st + t * 2048u;
-      nklds2::copy16(m0, is_p ? rp : rq, voff, b * 2048u);
-      nklds2::copy16(m0 + 1024u, is_p ? rp : rq, voff + 1024u, b * 2048u);
+      nklds2::copy16(st + t * 2048u, is_p ? rp : rq, voff, b * 2048u);
+      nklds2::copy16(st + t * 2048u + 1024u, is_p ? rp : rq, voff + 1024u, b * 2048u);
     }
-    if (wave == 0u) {
-      // num_records ends with this block's scales; rows past them give zeros
+    if (q_scales) {
       const u32x4 rsq = nklds2::rsrc(a.sq + (size_t)b * a.sq_b + q0 * 16u, (a.sq_b - q0 * 16u) * 4u);
-      nklds2::copy16(st + L::kScaleAt, rsq, lane < L::kQ * 4u ? lane * 16u : 0x80000000u, 0u);
+      nklds2::copy4(st + L::kScaleAt + wave * 256u, rsq, wave * 256u + lane * 4u, 0u);
+    } else {
+      nklds2::copy4(st + L::kScaleAt + L::kQ * 64u, rsp, spoff, b * a.sp_b * 4u);
     }
-    if (wave == 1u) nklds2::copy4(st + L::kScaleAt + 1024u, rsp, spoff, b * a.sp_b * 4u);
   };
 
   v4f acc[NP][NQ];
@@ -268,18 +224,25 @@ __device__ __forceinline__ void product_tile(const Product& a) {
 #pragma unroll
     for (uint32_t j = 0; j < NQ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  issue(0u);
-  for (uint32_t b = 0; b < a.kb; ++b) {
-    nklds2::wait_copies<0>();
+#pragma unroll
+  for (uint32_t i = 0; i + 1u < S; ++i)
+    if (b0 + i < b1) issue(b0 + i, i);
+  uint32_t stage = 0u;
+  for (uint32_t b = b0; b < b1; ++b) {
+    // the copies of the steps behind this one may stay in flight
+    if (S > 2u && b + S - 2u < b1) nklds2::wait_copies<(S - 2u) * L::kCopies>();
+    else nklds2::wait_copies<0>();
     nklds2::barrier();
-    if (b + 1u < a.kb) issue(b + 1u);
-    const uint8_t* st = s_stage + (b & 1u) * L::kStage;
+    const uint32_t before = stage == 0u ? S - 1u : stage - 1u;
+    if (b + S - 1u < b1) issue(b + S - 1u, before);
+    const uint8_t* st = s_stage + stage * L::kStage;
+    stage = stage + 1u == S ? 0u : stage + 1u;
     const uint8_t* sp_tiles = st + wp * NP * 2048u;
     const uint8_t* sq_tiles = st + (L::kP + wq * NQ) * 2048u;
     const float* scale = reinterpret_cast<const float*>(st + L::kScaleAt);
     v8i qo[NQ];
     float s[NQ];
-    const float sp = scale[256u + wp * NP / 8u];
+    const float sp = scale[L::kQ * 16u + wp * NP / 8u];
 #pragma unroll
     for (uint32_t j = 0; j < NQ; ++j) {
       qo[j] = nk::load_tile_operand(sq_tiles + j * 2048u, lane);
@@ -297,28 +260,38 @@ __device__ __forceinline__ void product_tile(const Product& a) {
     }
   }
 
-  // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
-  // whole lines.
-  constexpr uint32_t kPitch = L::kPitch;
-  __syncthreads();
-  uint8_t* mine = s_stage + wave * 16u * NQ * kPitch;
   const uint32_t c = lane & 15u, r4 = (lane >> 4) * 4u;
+  const uint32_t col0 = (p0 + wp * NP) * 16u, row0 = (q0 + wq * NQ) * 16u;
+  if (a.splits > 1u) {  // fp32 partial sums, rows of a.ni rounded up to 4
+    const uint32_t pitch = (a.ni + 3u) & ~3u;
+    float* part = a.partial + (size_t)split * a.nq * pitch;
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < NP; ++i) {
+        const uint32_t row = row0 + j * 16u + c, col = col0 + i * 16u + r4;
+        if (row < a.nq && col < pitch) *reinterpret_cast<v4f*>(part + (size_t)row * pitch + col) = acc[i][j];
+      }
+    return;
+  }
+  // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
+  // whole lines. (A wave reads back only what it wrote itself.)
+  __syncthreads();
+  uint8_t* mine = s_stage + wave * 16u * NQ * L::kPitch;
 #pragma unroll
   for (uint32_t j = 0; j < NQ; ++j)
 #pragma unroll
     for (uint32_t i = 0; i < NP; ++i) {
       const v4f v = acc[i][j];
-      *reinterpret_cast<uint2*>(mine + (j * 16u + c) * kPitch + (i * 16u + r4) * 2u) =
+      *reinterpret_cast<uint2*>(mine + (j * 16u + c) * L::kPitch + (i * 16u + r4) * 2u) =
           make_uint2(nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
                      nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16));
     }
-  // (a wave reads back only what it wrote itself)
-  const uint32_t col0 = (p0 + wp * NP) * 16u, row0 = (q0 + wq * NQ) * 16u;
   constexpr uint32_t kLanes = NP * 2u;  // lanes of 8 values per row
   for (uint32_t r = lane / kLanes; r < 16u * NQ; r += 64u / kLanes) {
     const uint32_t cc = (lane % kLanes) * 8u, row = row0 + r, col = col0 + cc;
     if (row >= a.nq || col >= a.ni) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kPitch + cc * 2u);
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * L::kPitch + cc * 2u);
     uint16_t* o = a.out + (uint64_t)row * a.ldo + col;
     if (a.vec && col + 8u <= a.ni) {
       *reinterpret_cast<uint4*>(o) = v;
@@ -331,86 +304,120 @@ __device__ __forceinline__ void product_tile(const Product& a) {
   }
 }
 
+// out = bf16 of the splits' sum, in split order. One row per blockIdx.y step.
+__device__ __forceinline__ void product_sum(const Product& a) {
+  const uint32_t pitch = (a.ni + 3u) & ~3u, col = (blockIdx.x * 256u + threadIdx.x) * 4u;
+  if (col >= a.ni) return;
+  for (uint32_t row = blockIdx.y; row < a.nq; row += gridDim.y) {
+    v4f s = *reinterpret_cast<const v4f*>(a.partial + (size_t)row * pitch + col);
+    for (uint32_t k = 1; k < a.splits; ++k)
+      s += *reinterpret_cast<const v4f*>(a.partial + ((size_t)k * a.nq + row) * pitch + col);
+    const float v[4] = {s[0], s[1], s[2], s[3]};
+    store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, a.vec != 0u, v);
+  }
+}
+
+// Few rows: a workgroup computes 16 NP columns of the output for all 16 NQ rows,
+// its 8 waves dealing the 128-blocks among them. The weights go from memory to
+// registers (each tile is read by one wave of the launch); the activations are
+// quantised on the way, by every wave for its own blocks, so that a call is one
+// launch: a wave's lanes hold a tile of 16 rows x 128 values exactly as an operand
+// wants it, and the four lanes of a row find its scale with two exchanges.
+template <uint32_t NP, uint32_t NQ, typename X, bool kVec>
+__device__ __forceinline__ void product_stream(const Product& a, const X* __restrict__ x, uint64_t x_stride,
+                                               uint32_t n) {
+  __shared__ v4f s_part[8][NP * NQ][64];
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t pt = (a.ni + 15u) / 16u, p0 = blockIdx.x * NP;
+  const uint32_t c = lane & 15u, g = lane >> 4;
+  v4f acc[NP][NQ];
+#pragma unroll
+  for (uint32_t i = 0; i < NP; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint8_t* pb[NP];
+  const float* spb[NP];
+#pragma unroll
+  for (uint32_t i = 0; i < NP; ++i) {
+    const uint32_t t = min(p0 + i, pt - 1u);  // a tile past the end repeats the last one; not stored
+    pb[i] = nk::tile_base(a.p, t, 0, a.kb);
+    spb[i] = a.sp + (size_t)(t / 8u) * a.sp_i;
+  }
+  v8i po[NP];
+  if (wave < a.kb) {
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) po[i] = nk::load_tile_operand_once(pb[i] + (size_t)wave * 2048u, lane);
+  }
+  for (uint32_t b = wave; b < a.kb; b += 8u) {
+    float sp[NP];
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) sp[i] = spb[i][(size_t)b * a.sp_b];
+    v8i next[NP];
+    const uint32_t bn = min(b + 8u, a.kb - 1u);
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) next[i] = nk::load_tile_operand_once(pb[i] + (size_t)bn * 2048u, lane);
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) {
+      const uint32_t r = j * 16u + c;
+      float v[32];
+      if (r < a.nq) {
+        load32<kVec>(x + (uint64_t)r * x_stride, b * 128u + g * 32u, n, v);
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 32u; ++e) v[e] = 0.0f;
+      }
+      uint32_t code[8];
+      const float sq = quantise32(v, code);
+      v8i qo;
+#pragma unroll
+      for (uint32_t e = 0; e < 8u; ++e) qo[e] = (int)code[e];
+#pragma unroll
+      for (uint32_t i = 0; i < NP; ++i) {
+        const v4f d = nk::mfma_e4m3_16x16x128(po[i], qo);
+        const float s = sq * sp[i];
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) acc[i][j][e] = fmaf(s, d[e], acc[i][j][e]);
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) po[i] = next[i];
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < NP; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) s_part[wave][i * NQ + j][lane] = acc[i][j];
+  __syncthreads();
+  for (uint32_t k = threadIdx.x; k < NP * NQ * 64u; k += 512u) {
+    const uint32_t i = k / 64u / NQ, j = k / 64u % NQ, l = k & 63u;
+    v4f s = s_part[0][i * NQ + j][l];
+#pragma unroll
+    for (uint32_t w = 1; w < 8u; ++w) s += s_part[w][i * NQ + j][l];
+    const uint32_t row = j * 16u + (l & 15u), col = (p0 + i) * 16u + (l >> 4) * 4u;
+    if (row >= a.nq || col >= a.ni) continue;
+    const float v[4] = {s[0], s[1], s[2], s[3]};
+    store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, a.vec != 0u, v);
+  }
+}
+
 // ---- weight gradient ------------------------------------------------------------
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 struct Outer {
-  const void* dy;   // [rows, n]
+  const uint16_t* dy;   // [rows, n]
   uint64_t dy_stride;
-  uint32_t dy_type;
-  const void* x;    // [rows, k]
+  const uint16_t* x;    // [rows, k]
   uint64_t x_stride;
-  uint32_t x_type;
-  float* dw;        // [n, k]
+  float* dw;            // [n, k]
   uint32_t rows, n, k;
   uint32_t accumulate;
   uint32_t splits, split_rows;  // tokens per split (a multiple of 64)
   float* partial;               // [splits, n, k] where splits > 1
 };
 
-// Eight tokens' values of one column as an MFMA operand, zeros past the end.
-__device__ __forceinline__ v8bf column8(const void* m, uint64_t stride, uint32_t type, uint32_t c, uint32_t cols,
-                                        uint32_t t, uint32_t rows) {
-  v8bf v;
-#pragma unroll
-  for (uint32_t j = 0; j < 8u; ++j) {
-    float f = 0.0f;
-    if (c < cols && t + j < rows) {
-      const uint64_t at = (uint64_t)(t + j) * stride + c;
-      f = type == 0u ? value(static_cast<const uint16_t*>(m) + at) : value(static_cast<const float*>(m) + at);
-    }
-    v[j] = __builtin_bit_cast(__bf16, nk::bf16_rne(f));
-  }
-  return v;
-}
-
-// dw[n, k] = sum_t dy[t, n] x[t, k]: a wave computes 32 x 32, the columns read
-// straight from memory.
-__device__ __forceinline__ void outer_direct(const Outer& a) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t k0 = blockIdx.x * 64u + (wave & 1u) * 32u, n0 = blockIdx.y * 64u + (wave >> 1) * 32u;
-  if (k0 >= a.k || n0 >= a.n) return;
-  const uint32_t c = lane & 15u, g = lane >> 4;
-  v4f acc[2][2];
-#pragma unroll
-  for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-    for (uint32_t j = 0; j < 2u; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t t = 0; t < a.rows; t += 32u) {
-    v8bf po[2], qo[2];
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
-      po[i] = column8(a.x, a.x_stride, a.x_type, k0 + i * 16u + c, a.k, t + g * 8u, a.rows);
-      qo[i] = column8(a.dy, a.dy_stride, a.dy_type, n0 + i * 16u + c, a.n, t + g * 8u, a.rows);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-      for (uint32_t j = 0; j < 2u; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(po[i], qo[j], acc[i][j], 0, 0, 0);
-  }
-#pragma unroll
-  for (uint32_t j = 0; j < 2u; ++j) {
-    const uint32_t row = n0 + j * 16u + c;
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
-      const uint32_t col = k0 + i * 16u + g * 4u;
-      if (row >= a.n || col >= a.k) continue;
-      float* o = a.dw + (uint64_t)row * a.k + col;
-      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (a.accumulate) {
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e)
-          if (col + e < a.k) v[e] += o[e];
-      }
-      store4(o, a.k - col, a.k % 4u == 0u && reinterpret_cast<uintptr_t>(a.dw) % 16u == 0u, v);
-    }
-  }
-}
-
-// The same product with both operands staged through LDS, for bf16 matrices whose
-// rows are 16-byte aligned and whole 16-byte chunks. Both have the contraction (tokens) as their slow
+// dw[n, k] = sum_t dy[t, n] x[t, k], both operands staged through LDS, for bf16
+// matrices whose rows are 16-byte aligned and whole 16-byte chunks. Both have the contraction (tokens) as their slow
 // dimension, so their rows are copied as they are and the transposed LDS reads
 // (ds_read_b64_tr_b16: among 16 lanes, lane i gets element i % 4 of the 8 bytes
 // that lanes i / 4 + 0, 4, 8, 12 address) turn 4 tokens x 16 columns into operand
@@ -453,9 +460,9 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
   auto issue = [&](uint32_t t, uint32_t parity) __attribute__((always_inline)) {
     const uint32_t st = lds0 + parity * kStage;
-    auto rows = [&](const void* m, uint64_t stride, uint32_t c0, uint32_t cols, uint32_t row_bytes, uint32_t v,
+    auto rows = [&](const uint16_t* m, uint64_t stride, uint32_t c0, uint32_t cols, uint32_t row_bytes, uint32_t v,
                     uint32_t at) __attribute__((always_inline)) {
-      const uint16_t* base = static_cast<const uint16_t*>(m) + (uint64_t)t * stride + c0;
+      const uint16_t* base = m + (uint64_t)t * stride + c0;
       // tokens t .. min(t1, t + 64) - 1, from column c0 (rows are whole 16-byte chunks)
       const uint32_t n = min(kTokens, t1 - t);
       const u32x4 r = nklds2::rsrc(base, ((n - 1u) * (uint32_t)stride + (((cols + 7u) & ~7u) - c0)) * 2u);
@@ -463,7 +470,7 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
 #pragma unroll
       for (uint32_t i = 0; i < kTokens / each / 8u; ++i) {
         const uint32_t row = (i * 8u + wave) * each;
-        nklds2::copy16(at + row * row_bytes, r, v, row * (uint32_t)stride * 2u);
+        nklds2::copy16(at + row * row_bytes, r, v + row * (uint32_t)stride * 2u, 0u);
       }
     };
     rows(a.x, a.x_stride, p0, a.k, kRowP, pv, st);
@@ -611,15 +618,30 @@ NETRA_QUANT_ROWS(bf16_vec, uint16_t, true)
 NETRA_QUANT_ROWS(f32, float, false)
 NETRA_QUANT_ROWS(f32_vec, float, true)
 
-extern "C" __global__ __launch_bounds__(256) void netra_linear_product_direct_gfx950(nklin::Product a) {
-  nklin::product_direct(a);
-}
-
 extern "C" __global__ __launch_bounds__(512) void netra_linear_product_256x256_gfx950(nklin::Product a) {
-  nklin::product_tile<2, 4, 8, 4>(a);
+  nklin::product_tile<2, 4, 8, 4, 2>(a);
+}
+extern "C" __global__ __launch_bounds__(512) void netra_linear_product_128x128_gfx950(nklin::Product a) {
+  nklin::product_tile<2, 4, 4, 2, 4>(a);
+}
+extern "C" __global__ __launch_bounds__(256) void netra_linear_product_sum_gfx950(nklin::Product a) {
+  nklin::product_sum(a);
 }
 
-extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_direct_gfx950(nklin::Outer a) { nklin::outer_direct(a); }
+#define NETRA_PRODUCT_STREAM(NAME, X, VEC, NP, NQ)                                                           \
+  extern "C" __global__ __launch_bounds__(512) void netra_linear_product_stream_##NAME##_p##NP##q##NQ##_gfx950( \
+      nklin::Product a, const X* x, uint64_t x_stride, uint32_t n) {                                         \
+    nklin::product_stream<NP, NQ, X, VEC>(a, x, x_stride, n);                                                \
+  }
+#define NETRA_PRODUCT_STREAMS(NP, NQ)                        \
+  NETRA_PRODUCT_STREAM(bf16, uint16_t, false, NP, NQ)        \
+  NETRA_PRODUCT_STREAM(bf16_vec, uint16_t, true, NP, NQ)     \
+  NETRA_PRODUCT_STREAM(f32, float, false, NP, NQ)            \
+  NETRA_PRODUCT_STREAM(f32_vec, float, true, NP, NQ)
+NETRA_PRODUCT_STREAMS(1, 1)
+NETRA_PRODUCT_STREAMS(2, 1)
+NETRA_PRODUCT_STREAMS(2, 2)
+NETRA_PRODUCT_STREAMS(2, 4)
 
 extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_256x256_gfx950(nklin::Outer a) {
   nklin::outer_tile<2, 4, 8, 4>(a);

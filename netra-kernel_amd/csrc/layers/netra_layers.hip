@@ -69,23 +69,64 @@ void quant_rows(const void* x, uint32_t type, uint64_t stride, uint8_t* q, float
   }
 }
 
-void product(nklin::Product a, hipStream_t stream) {
-  a.vec = aligned(a.out, 16) && a.ldo % 8u == 0;
-  const uint32_t tiles = ((a.ni + 255u) / 256u) * ((a.nq + 255u) / 256u);
-  if (a.nq > 64u) {
-    netra_linear_product_256x256_gfx950<<<dim3((tiles + 7u) / 8u * 8u), dim3(512), 0, stream>>>(a);
-    return;
-  }
-  netra_linear_product_direct_gfx950<<<dim3((a.ni + 63u) / 64u, (a.nq + 63u) / 64u), dim3(256), 0, stream>>>(a);
+// How a product runs: `stream` (quantising on the way) or tiles of p x q with splits of the contraction.
+struct ProductPlan {
+  bool stream;
+  uint32_t p, q, splits, split_blocks;
+};
+ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc) {
+  if (rows <= 64u) return {true, 0, 0, 1, 0};
+  auto tiles = [&](uint32_t p, uint32_t q) {
+    return static_cast<uint64_t>((ni + p - 1u) / p) * ((rows + q - 1u) / q);
+  };
+  ProductPlan plan{false, 256, 256, 1, blocks(nc)};
+  if (tiles(256, 256) < 200) plan.p = plan.q = 128;
+  const uint64_t t = tiles(plan.p, plan.q);
+  uint32_t splits = t >= 128 ? 1u : static_cast<uint32_t>(256 / t);
+  const uint32_t most = (blocks(nc) + 3u) / 4u;  // 4 blocks at least
+  splits = splits > most ? most : splits;
+  plan.split_blocks = (blocks(nc) + splits - 1u) / splits;
+  plan.splits = (blocks(nc) + plan.split_blocks - 1u) / plan.split_blocks;
+  return plan;
+}
+uint64_t product_workspace(uint32_t rows, uint32_t ni, uint32_t nc) {
+  if (rows == 0) return 0;
+  const ProductPlan plan = product_plan(rows, ni, nc);
+  if (plan.stream) return 0;
+  const uint64_t partial = plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * rows * up(ni, 4u) : 0u;
+  return (matrix_bytes(rows, nc) + 15u) / 16u * 16u + partial;
+}
+
+template <typename X>
+void product_stream(const nklin::Product& a, const X* x, uint64_t stride, uint32_t nc, hipStream_t stream) {
+  const bool vec = aligned(x, 16) && stride * sizeof(X) % 16u == 0;
+  const uint32_t pt = (a.ni + 15u) / 16u, q = (a.nq + 15u) / 16u;
+  const bool wide = q > 1u || pt >= 512u;
+  const dim3 grid(wide ? (pt + 1u) / 2u : pt), block(512);
+#define NETRA_RUN(P, Q)                                                                                               \
+  do {                                                                                                                \
+    if constexpr (sizeof(X) == 2) {                                                                                   \
+      if (vec) netra_linear_product_stream_bf16_vec_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc); \
+      else netra_linear_product_stream_bf16_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);        \
+    } else {                                                                                                          \
+      if (vec) netra_linear_product_stream_f32_vec_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc); \
+      else netra_linear_product_stream_f32_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);         \
+    }                                                                                                                 \
+  } while (0)
+  if (q > 2u) NETRA_RUN(2, 4);
+  else if (q == 2u) NETRA_RUN(2, 2);
+  else if (wide) NETRA_RUN(2, 1);
+  else NETRA_RUN(1, 1);
+#undef NETRA_RUN
 }
 
 // An operand of the weight gradient as it is, or as bf16 with aligned rows in the workspace.
 bool outer_ready(const void* m, uint32_t type, uint64_t stride, uint32_t cols) {
   return type == NETRA_BF16 && aligned(m, 16) && cols % 8u == 0 && stride % 8u == 0 && stride < (1u << 24);
 }
-void outer_operand(const void*& m, uint32_t& type, uint64_t& stride, uint32_t rows, uint32_t cols, uint8_t*& at,
-                   hipStream_t stream) {
-  if (outer_ready(m, type, stride, cols)) return;
+const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, uint32_t rows, uint32_t cols,
+                              uint8_t*& at, hipStream_t stream) {
+  if (outer_ready(m, type, stride, cols)) return static_cast<const uint16_t*>(m);
   const uint32_t pitch = up(cols, 8u);
   const dim3 grid((pitch + 511u) / 512u, rows < 4u * 4096u ? (rows + 3u) / 4u : 4096u);
   uint16_t* out = reinterpret_cast<uint16_t*>(at);
@@ -96,9 +137,8 @@ void outer_operand(const void*& m, uint32_t& type, uint64_t& stride, uint32_t ro
     netra_linear_to_bf16_bf16_gfx950<<<grid, dim3(256), 0, stream>>>(static_cast<const uint16_t*>(m), stride, out,
                                                                      rows, cols, pitch);
   at += static_cast<uint64_t>(rows) * pitch * 2u;
-  m = out;
-  type = NETRA_BF16;
   stride = pitch;
+  return out;
 }
 
 // Tile and split of the weight gradient.
@@ -141,10 +181,10 @@ extern "C" int netra_linear_pack(const uint8_t* w, uint8_t* packed, uint32_t n, 
 }
 
 extern "C" uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
-  return matrix_bytes(rows, k);
+  return product_workspace(rows, n, k);
 }
 extern "C" uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
-  return matrix_bytes(rows, n);
+  return product_workspace(rows, k, n);
 }
 extern "C" uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
   if (rows == 0) return 0;
@@ -166,26 +206,41 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   if (bad_matrix(in, in_type, in_stride, nc) || bad_matrix(out, NETRA_BF16, out_stride, ni) || !packed ||
       !aligned(packed, 16) || !scale || !aligned(scale, 4))
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
-  if (bad_workspace(workspace, workspace_bytes, matrix_bytes(rows, nc)))
+  if (bad_workspace(workspace, workspace_bytes, product_workspace(rows, ni, nc)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  uint8_t* q = static_cast<uint8_t*>(workspace);
-  float* s = reinterpret_cast<float*>(q + code_bytes(rows, nc));
-  quant_rows(in, in_type, in_stride, q, s, rows, nc, stream);
+  const ProductPlan plan = product_plan(rows, ni, nc);
   nklin::Product a{};
   a.p = packed;
   a.sp = scale;
   a.sp_i = sp_i;
   a.sp_b = sp_b;
   a.sp_bytes = blocks(ni) * blocks(nc) * 4u;
-  a.q = q;
-  a.sq = s;
-  a.sq_b = up(rows, 16u);
   a.out = out;
   a.ldo = out_stride;
   a.ni = ni;
   a.nq = rows;
   a.kb = blocks(nc);
-  product(a, stream);
+  a.vec = aligned(out, 16) && out_stride % 8u == 0;
+  a.splits = plan.splits;
+  a.split_blocks = plan.split_blocks;
+  if (plan.stream) {
+    if (in_type == NETRA_BF16) product_stream(a, static_cast<const uint16_t*>(in), in_stride, nc, stream);
+    else product_stream(a, static_cast<const float*>(in), in_stride, nc, stream);
+    return launched(name);
+  }
+  uint8_t* q = static_cast<uint8_t*>(workspace);
+  float* s = reinterpret_cast<float*>(q + code_bytes(rows, nc));
+  quant_rows(in, in_type, in_stride, q, s, rows, nc, stream);
+  a.q = q;
+  a.sq = s;
+  a.sq_b = up(rows, 16u);
+  a.partial = reinterpret_cast<float*>(q + (matrix_bytes(rows, nc) + 15u) / 16u * 16u);
+  const uint32_t items = ((ni + plan.p - 1u) / plan.p) * ((rows + plan.q - 1u) / plan.q) * plan.splits;
+  const dim3 grid((items + 7u) / 8u * 8u), block(512);
+  if (plan.p == 256u) netra_linear_product_256x256_gfx950<<<grid, block, 0, stream>>>(a);
+  else netra_linear_product_128x128_gfx950<<<grid, block, 0, stream>>>(a);
+  if (plan.splits > 1u)
+    netra_linear_product_sum_gfx950<<<dim3((ni + 1023u) / 1024u, rows < 4096u ? rows : 4096u), dim3(256), 0, stream>>>(a);
   return launched(name);
 }
 
@@ -222,13 +277,11 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
   if (bad_workspace(workspace, workspace_bytes, netra_linear_weight_gradient_workspace(rows, n, k)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  outer_operand(dy, dy_type, dy_stride, rows, n, at, stream);
-  outer_operand(x, x_type, x_stride, rows, k, at, stream);
   const OuterPlan plan = outer_plan(rows, n, k);
   nklin::Outer a{};
-  a.dy = dy;
+  a.dy = outer_operand(dy, dy_type, dy_stride, rows, n, at, stream);
   a.dy_stride = dy_stride;
-  a.x = x;
+  a.x = outer_operand(x, x_type, x_stride, rows, k, at, stream);
   a.x_stride = x_stride;
   a.dw = dw;
   a.rows = rows;

@@ -44,7 +44,7 @@ def test_packed_bytes():
 @pytest.mark.parametrize("name", ["netra_linear_forward", "netra_linear_input_gradient"])
 def test_product_refusals(name, change):
     lib = layers.library()
-    a = dict(x=A, xt=0, xs=256, packed=A, scale=A, y=A, ys=128, rows=4, n=128, k=256, ws=A)
+    a = dict(x=A, xt=0, xs=256, packed=A, scale=A, y=A, ys=128, rows=300, n=128, k=256, ws=A)
     back = name != "netra_linear_forward"
     if back:
         a.update(n=256, k=128)
