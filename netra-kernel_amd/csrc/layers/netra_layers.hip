@@ -311,7 +311,29 @@ static bool bad_router(uint32_t tokens, uint32_t slots, uint32_t experts) {
          tokens > 0x7fffffffu;
 }
 
-extern "C" uint64_t netra_router_counts_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) { return 0; }
+// Counting is shared out over workgroups of 256 threads where one would take longer
+// than a second launch; each counts `each` tokens.
+struct CountPlan {
+  uint32_t groups, each;
+};
+static CountPlan count_plan(uint32_t tokens, uint32_t few) {
+  if (tokens <= few) return {0, tokens};
+  const uint32_t groups = (tokens - 1u) / 256u + 1u;
+  CountPlan plan{groups > 64u ? 64u : groups, 0};
+  plan.each = (tokens + plan.groups - 1u) / plan.groups;
+  return plan;
+}
+static constexpr uint32_t kFewCounts = 2048;   // tokens one workgroup counts
+static constexpr uint32_t kFewBalance = 64;    // tokens one workgroup takes through the loss
+static constexpr uint32_t kBalanceGrid = 256;
+
+static uint64_t parts_bytes(const CountPlan& plan, uint32_t experts) {
+  return (4u * static_cast<uint64_t>(plan.groups) * (experts + 1u) + 15u) / 16u * 16u;
+}
+
+extern "C" uint64_t netra_router_counts_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
+  return parts_bytes(count_plan(tokens, kFewCounts), experts);
+}
 
 extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, const uint8_t* mask, uint32_t tokens,
                                    uint32_t slots, uint32_t experts, int32_t* counts, uint32_t accumulate,
@@ -323,15 +345,23 @@ extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, cons
     return fail(-1, name, "null or misaligned pointer, or ids' row stride below the slots");
   if (bad_workspace(workspace, workspace_bytes, netra_router_counts_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  netra_router_counts_gfx950<<<dim3(1), dim3(nkbal::kCountThreads), 0, stream>>>(
-      ids, ids_stride, mask, tokens, slots, experts, counts, accumulate, nullptr, nullptr);
+  const CountPlan plan = count_plan(tokens, kFewCounts);
+  if (plan.groups == 0) {
+    netra_router_counts_gfx950<<<dim3(1), dim3(1024), 0, stream>>>(ids, ids_stride, mask, tokens, slots, experts,
+                                                                   counts, accumulate ? 1u : 0u);
+    return launched(name);
+  }
+  uint32_t* parts = static_cast<uint32_t*>(workspace);
+  netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(256), 0, stream>>>(ids, ids_stride, mask, tokens, slots,
+                                                                               experts, plan.each, parts, nullptr);
+  netra_router_count_sum_gfx950<<<dim3((experts + 15u) / 16u), dim3(256), 0, stream>>>(
+      parts, plan.groups, experts, counts, accumulate ? 1u : 0u);
   return launched(name);
 }
 
-static constexpr uint32_t kBalanceGrid = 1024;
-
 extern "C" uint64_t netra_router_balance_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
-  return 16u + 4u * kBalanceGrid;
+  const CountPlan plan = count_plan(tokens, kFewBalance);
+  return plan.groups ? 16u + 4u * kBalanceGrid + parts_bytes(plan, experts) : 0;
 }
 
 extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, uint64_t logits_stride, const float* bias,
@@ -351,33 +381,48 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     return fail(-1, name, "null or misaligned pointer, or row stride below the row");
   if (bad_workspace(workspace, workspace_bytes, netra_router_balance_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  uint32_t* words = static_cast<uint32_t*>(workspace);
-  netra_router_counts_gfx950<<<dim3(1), dim3(nkbal::kCountThreads), 0, stream>>>(
-      ids, ids_stride, mask, tokens, slots, experts, counts, slots ? 0u : 1u, words, words + 1);
+  const CountPlan plan = count_plan(tokens, kFewBalance);
   nkbal::Balance a{};
   a.z = logits;
   a.z_stride = logits_stride;
   a.bias = bias;
+  a.ids = ids;
+  a.ids_stride = ids_stride;
+  a.slots = slots;
   a.mask = mask;
   a.tokens = tokens;
   a.experts = experts;
   a.coefficient = coefficient;
   a.counts = counts;
-  a.valid = words;
   a.loss = loss;
   a.grad = grad;
   a.grad_stride = grad_stride;
-  a.partial = reinterpret_cast<float*>(words + 4);
-  a.arrived = words + 1;
-  uint32_t grid = (tokens + 3u) / 4u;
-  grid = grid < 1u ? 1u : grid > kBalanceGrid ? kBalanceGrid : grid;
-#define NETRA_RUN(NAME, NV) netra_router_balance_##NAME##_v##NV##_gfx950<<<dim3(grid), dim3(256), 0, stream>>>(a)
-#define NETRA_PICK(NAME)                     \
-  if (experts <= 64u) NETRA_RUN(NAME, 1);    \
-  else if (experts <= 128u) NETRA_RUN(NAME, 2); \
-  else if (experts <= 256u) NETRA_RUN(NAME, 4); \
-  else if (experts <= 512u) NETRA_RUN(NAME, 8); \
-  else NETRA_RUN(NAME, 16)
+  uint32_t grid = 1;
+  if (plan.groups) {
+    uint32_t* words = static_cast<uint32_t*>(workspace);
+    a.arrived = words;
+    a.partial = reinterpret_cast<float*>(words + 4);
+    uint32_t* parts = words + 4 + kBalanceGrid;
+    a.parts = parts;
+    a.groups = plan.groups;
+    netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(256), 0, stream>>>(
+        ids, ids_stride, mask, tokens, slots, experts, plan.each, parts, words);
+    grid = (tokens + 15u) / 16u;
+    grid = grid > kBalanceGrid ? kBalanceGrid : grid;
+  }
+  const uint32_t es = elem(logits_type);
+  const bool vec = experts > 128u && experts % 4u == 0 && aligned(logits, 4u * es) && logits_stride % 4u == 0 &&
+                   (!grad || (aligned(grad, 4u * es) && grad_stride % 4u == 0));
+#define NETRA_RUN(NAME, V) netra_router_balance_##NAME##_v##V##_gfx950<<<dim3(grid), dim3(1024), 0, stream>>>(a)
+#define NETRA_PICK(NAME)                                  \
+  if (experts <= 64u) NETRA_RUN(NAME, 1x1);               \
+  else if (experts <= 128u) NETRA_RUN(NAME, 2x1);         \
+  else if (experts <= 256u && vec) NETRA_RUN(NAME, 4x4);  \
+  else if (experts <= 256u) NETRA_RUN(NAME, 4x1);         \
+  else if (experts <= 512u && vec) NETRA_RUN(NAME, 8x4);  \
+  else if (experts <= 512u) NETRA_RUN(NAME, 8x1);         \
+  else if (vec) NETRA_RUN(NAME, 16x4);                    \
+  else NETRA_RUN(NAME, 16x1)
   if (logits_type == NETRA_BF16) {
     NETRA_PICK(bf16);
   } else {

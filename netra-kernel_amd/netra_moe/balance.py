@@ -19,7 +19,7 @@ from typing import NamedTuple
 
 import torch
 
-from .layers import TYPES, call, check_rows, library, row_stride
+from .layers import TYPES, check_rows, entry, launch, workspace
 
 MAX_EXPERTS = 1024
 
@@ -47,10 +47,10 @@ def _check_counts(name: str, counts: torch.Tensor, experts: int, device: torch.d
                          f"{tuple(counts.shape)} on {counts.device}")
 
 
-def _check_ids(ids: torch.Tensor, tokens: int | None, device: torch.device) -> None:
+def _check_ids(ids: torch.Tensor, tokens: int | None, device: torch.device) -> int:
     if not ids.is_cuda or ids.dim() != 2 or ids.shape[1] < 1:
         raise ValueError("topk_ids: need an int32 [T, slots] GPU tensor")
-    check_rows("topk_ids", ids, (ids.shape[0] if tokens is None else tokens, ids.shape[1]), device, (torch.int32,))
+    return check_rows("topk_ids", ids, (ids.shape[0] if tokens is None else tokens, ids.shape[1]), device, (torch.int32,))
 
 
 def _check_experts(experts: int) -> None:
@@ -64,7 +64,7 @@ def expert_counts(topk_ids: torch.Tensor, experts: int, *, mask: torch.Tensor | 
     0 .. experts - 1 and tokens whose mask is false are not counted. accumulate
     adds to out (the load over several calls)."""
     _check_experts(experts)
-    _check_ids(topk_ids, None, topk_ids.device)
+    stride = _check_ids(topk_ids, None, topk_ids.device)
     device, (tokens, slots) = topk_ids.device, topk_ids.shape
     m = _check_mask(mask, tokens, device)
     if out is None:
@@ -73,10 +73,10 @@ def expert_counts(topk_ids: torch.Tensor, experts: int, *, mask: torch.Tensor | 
         out = torch.empty(experts, dtype=torch.int32, device=device)
     else:
         _check_counts("out", out, experts, device)
-    need = library().netra_router_counts_workspace(tokens, slots, experts)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    call("netra_router_counts", device, topk_ids.data_ptr(), row_stride(topk_ids), m, tokens, slots, experts,
-         out.data_ptr(), int(accumulate), ws.data_ptr(), need)
+    need = entry("netra_router_counts_workspace")(tokens, slots, experts)
+    ws, ws_ptr = workspace(need, device)
+    launch(entry("netra_router_counts"), "netra_router_counts", device, topk_ids.data_ptr(), stride, m, tokens, slots,
+           experts, out.data_ptr(), int(accumulate), ws_ptr, need)
     return out
 
 
@@ -91,7 +91,7 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor | None = None, *, 
         raise ValueError("logits: need a bf16 or fp32 [T, E] GPU tensor")
     device, (tokens, experts) = logits.device, logits.shape
     _check_experts(experts)
-    check_rows("logits", logits, (tokens, experts), device)
+    logits_stride = check_rows("logits", logits, (tokens, experts), device)
     if (topk_ids is None) == (counts is None):
         raise ValueError("balance_loss needs either topk_ids or counts")
     m = _check_mask(mask, tokens, device)
@@ -99,17 +99,17 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor | None = None, *, 
                              or not bias.is_contiguous()):
         raise ValueError(f"bias: need contiguous torch.float32 ({experts},) on {device}")
     if topk_ids is not None:
-        _check_ids(topk_ids, tokens, device)
-        slots, ids, stride = topk_ids.shape[1], topk_ids.data_ptr(), row_stride(topk_ids)
+        stride = _check_ids(topk_ids, tokens, device)
+        slots, ids = topk_ids.shape[1], topk_ids.data_ptr()
         counts = torch.empty(experts, dtype=torch.int32, device=device)
     else:
         _check_counts("counts", counts, experts, device)
         slots, ids, stride = 0, 0, 0
     loss = torch.empty((), dtype=torch.float32, device=device)
     g = torch.empty((tokens, experts), dtype=logits.dtype, device=device) if grad else None
-    need = library().netra_router_balance_workspace(tokens, slots, experts)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    call("netra_router_balance", device, logits.data_ptr(), TYPES[logits.dtype], row_stride(logits),
-         bias.data_ptr() if bias is not None else 0, ids, stride, slots, m, tokens, experts, coefficient,
-         counts.data_ptr(), loss.data_ptr(), g.data_ptr() if grad else 0, experts, ws.data_ptr(), need)
+    need = entry("netra_router_balance_workspace")(tokens, slots, experts)
+    ws, ws_ptr = workspace(need, device)
+    launch(entry("netra_router_balance"), "netra_router_balance", device, logits.data_ptr(), TYPES[logits.dtype],
+           logits_stride, bias.data_ptr() if bias is not None else 0, ids, stride, slots, m, tokens, experts,
+           coefficient, counts.data_ptr(), loss.data_ptr(), g.data_ptr() if grad else 0, experts, ws_ptr, need)
     return BalanceLoss(loss, counts, g)

@@ -28,7 +28,7 @@ import torch
 
 from . import prep
 from . import weights as W
-from .layers import TYPES, call, check_rows, library, row_stride
+from .layers import TYPES, check_rows, entry, launch, workspace
 
 
 class BlockLinear:
@@ -46,13 +46,16 @@ class BlockLinear:
                              f"{tuple(weight_scale.shape)} on {weight_scale.device}")
         self.device = weight.device
         self.scale = weight_scale.contiguous().clone()
+        self._scale_ptr = self.scale.data_ptr()
+        self._entries = {n: (entry(n), entry(n + "_workspace")) for n in (
+            "netra_linear_forward", "netra_linear_input_gradient", "netra_linear_weight_gradient")}
         self.packed = self._pack(weight, 0)
         self.packed_t = self._pack(weight, 1) if gradients else None
 
     def _pack(self, weight: torch.Tensor, transpose: int) -> torch.Tensor:
-        packed = torch.empty(library().netra_linear_packed_bytes(self.N, self.K, transpose), dtype=torch.uint8,
+        packed = torch.empty(entry("netra_linear_packed_bytes")(self.N, self.K, transpose), dtype=torch.uint8,
                              device=self.device)
-        call("netra_linear_pack", self.device, weight.data_ptr(), packed.data_ptr(), self.N, self.K, transpose)
+        launch(entry("netra_linear_pack"), "netra_linear_pack", self.device, weight.data_ptr(), packed.data_ptr(), self.N, self.K, transpose)
         return packed
 
     @classmethod
@@ -79,26 +82,24 @@ class BlockLinear:
         s = prep._scale(tensors, f"{name}.weight_scale_inv", -(-n // 128), -(-k // 128), device)
         return cls(q, s, gradients=gradients)
 
-    def _workspace(self, which: str, rows: int) -> torch.Tensor:
-        need = getattr(library(), f"netra_linear_{which}_workspace")(rows, self.N, self.K)
-        return torch.empty(need, dtype=torch.uint8, device=self.device)
-
     def _times(self, which: str, name: str, x: torch.Tensor, cols: int, out: torch.Tensor | None, out_cols: int,
                packed: torch.Tensor) -> torch.Tensor:
         rows = x.shape[0] if x.dim() == 2 else -1
-        check_rows(name, x, (rows, cols), self.device)
+        x_stride = check_rows(name, x, (rows, cols), self.device)
         if out is None:
-            out = torch.empty((rows, out_cols), dtype=torch.bfloat16, device=self.device)
+            out, out_stride = torch.empty((rows, out_cols), dtype=torch.bfloat16, device=self.device), out_cols
         else:
-            check_rows("out", out, (rows, out_cols), self.device, (torch.bfloat16,))
-        ws = self._workspace(which, rows)
-        call(f"netra_linear_{which}", self.device, x.data_ptr(), TYPES[x.dtype], row_stride(x), packed.data_ptr(),
-             self.scale.data_ptr(), out.data_ptr(), row_stride(out), rows, self.N, self.K, ws.data_ptr(), ws.numel())
+            out_stride = check_rows("out", out, (rows, out_cols), self.device, (torch.bfloat16,))
+        fn, need = self._entries[which]
+        need = need(rows, self.N, self.K)
+        ws, ws_ptr = workspace(need, self.device)
+        launch(fn, which, self.device, x.data_ptr(), TYPES[x.dtype], x_stride, packed.data_ptr(), self._scale_ptr,
+               out.data_ptr(), out_stride, rows, self.N, self.K, ws_ptr, need)
         return out
 
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x bf16 or fp32 [T, K] -> x W^T, bf16 [T, N]."""
-        return self._times("forward", "x", x, self.K, out, self.N, self.packed)
+        return self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
 
     __call__ = forward
 
@@ -106,14 +107,14 @@ class BlockLinear:
         """dy bf16 or fp32 [T, N] -> dy W, bf16 [T, K]."""
         if self.packed_t is None:
             raise ValueError("input_gradient needs a layer built with gradients=True")
-        return self._times("input_gradient", "dy", dy, self.N, out, self.K, self.packed_t)
+        return self._times("netra_linear_input_gradient", "dy", dy, self.N, out, self.K, self.packed_t)
 
     def weight_gradient(self, dy: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = None, *,
                         accumulate: bool = False) -> torch.Tensor:
         """dy [T, N], x [T, K] -> dy^T x fp32 [N, K]; accumulate adds it to out."""
         rows = x.shape[0] if x.dim() == 2 else -1
-        check_rows("x", x, (rows, self.K), self.device)
-        check_rows("dy", dy, (rows, self.N), self.device)
+        x_stride = check_rows("x", x, (rows, self.K), self.device)
+        dy_stride = check_rows("dy", dy, (rows, self.N), self.device)
         if out is None:
             if accumulate:
                 raise ValueError("accumulate needs out")
@@ -121,10 +122,12 @@ class BlockLinear:
         elif tuple(out.shape) != (self.N, self.K) or out.dtype != torch.float32 or not out.is_contiguous() \
                 or out.device != self.device:
             raise ValueError(f"out: need contiguous torch.float32 {(self.N, self.K)} on {self.device}")
-        ws = self._workspace("weight_gradient", rows)
-        call("netra_linear_weight_gradient", self.device, dy.data_ptr(), TYPES[dy.dtype], row_stride(dy), x.data_ptr(),
-             TYPES[x.dtype], row_stride(x), out.data_ptr(), int(accumulate), rows, self.N, self.K, ws.data_ptr(),
-             ws.numel())
+        name = "netra_linear_weight_gradient"
+        fn, need = self._entries[name]
+        need = need(rows, self.N, self.K)
+        ws, ws_ptr = workspace(need, self.device)
+        launch(fn, name, self.device, dy.data_ptr(), TYPES[dy.dtype], dy_stride, x.data_ptr(), TYPES[x.dtype], x_stride,
+               out.data_ptr(), int(accumulate), rows, self.N, self.K, ws_ptr, need)
         return out
 
     def backward(self, dy: torch.Tensor, x: torch.Tensor, dw: torch.Tensor | None = None, *,
