@@ -32,51 +32,102 @@ __device__ __forceinline__ float group_scale(uint32_t amax_bits) {
   return fmaxf(__uint_as_float(amax_bits), nk::kAmaxFloor) * nk::inv_e4m3_max();
 }
 
-// 32 consecutive values of one row from column c (zeros from column n on).
-// kVec: 16-byte loads (base and row stride 16-byte aligned).
-template <bool kVec>
-__device__ __forceinline__ void load32(const uint16_t* row, uint32_t c, uint32_t n, float (&v)[32]) {
-  if (kVec && c + 32u <= n) {
+// 32 consecutive values of a row as they lie in memory: bf16 pairs or fp32.
+template <typename X>
+struct Raw;
+template <>
+struct Raw<uint16_t> {
+  uint32_t w[16];
+};
+template <>
+struct Raw<float> {
+  float w[32];
+};
+
+// 16 bytes from any element address: global loads need no alignment on this target.
+struct __attribute__((packed, aligned(2))) Unaligned16 {
+  uint32_t w[4];
+};
+
+// Values from column c of a row of n (zeros from column n on; nothing past it is read).
+__device__ __forceinline__ void load32(const uint16_t* row, uint32_t c, uint32_t n, Raw<uint16_t>& v) {
+  if (c + 32u <= n) {
 #pragma unroll
     for (uint32_t j = 0; j < 4u; ++j) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + c + 8u * j);
-      v[8 * j + 0] = nk::bf16_lo(u.x); v[8 * j + 1] = nk::bf16_hi(u.x);
-      v[8 * j + 2] = nk::bf16_lo(u.y); v[8 * j + 3] = nk::bf16_hi(u.y);
-      v[8 * j + 4] = nk::bf16_lo(u.z); v[8 * j + 5] = nk::bf16_hi(u.z);
-      v[8 * j + 6] = nk::bf16_lo(u.w); v[8 * j + 7] = nk::bf16_hi(u.w);
+      const Unaligned16 u = *reinterpret_cast<const Unaligned16*>(row + c + 8u * j);
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) v.w[4u * j + i] = u.w[i];
     }
     return;
   }
 #pragma unroll
-  for (uint32_t j = 0; j < 32u; ++j) v[j] = c + j < n ? value(row + c + j) : 0.0f;
+  for (uint32_t j = 0; j < 4u; ++j) {
+    const uint32_t e = c + 8u * j;
+    if (e + 8u <= n) {
+      const Unaligned16 u = *reinterpret_cast<const Unaligned16*>(row + e);
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) v.w[4u * j + i] = u.w[i];
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t lo = e + 2u * i < n ? row[e + 2u * i] : 0u;
+        const uint32_t hi = e + 2u * i + 1u < n ? row[e + 2u * i + 1u] : 0u;
+        v.w[4u * j + i] = lo | hi << 16;
+      }
+    }
+  }
 }
-template <bool kVec>
-__device__ __forceinline__ void load32(const float* row, uint32_t c, uint32_t n, float (&v)[32]) {
-  if (kVec && c + 32u <= n) {
+__device__ __forceinline__ void load32(const float* row, uint32_t c, uint32_t n, Raw<float>& v) {
 #pragma unroll
-    for (uint32_t j = 0; j < 8u; ++j) {
-      const float4 u = *reinterpret_cast<const float4*>(row + c + 4u * j);
-      v[4 * j + 0] = u.x; v[4 * j + 1] = u.y; v[4 * j + 2] = u.z; v[4 * j + 3] = u.w;
+  for (uint32_t j = 0; j < 8u; ++j) {
+    const uint32_t e = c + 4u * j;
+    if (e + 4u <= n) {
+      const Unaligned16 u = *reinterpret_cast<const Unaligned16*>(row + e);
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) v.w[4u * j + i] = __uint_as_float(u.w[i]);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) v.w[4u * j + i] = e + i < n ? row[e + i] : 0.0f;
     }
-    return;
   }
-#pragma unroll
-  for (uint32_t j = 0; j < 32u; ++j) v[j] = c + j < n ? value(row + c + j) : 0.0f;
 }
 
-// The 32 values of each lane as MFMA operand bytes, with the scale of the
-// 128-group that the lanes l, l ^ 16, l ^ 32, l ^ 48 hold together.
-__device__ __forceinline__ float quantise32(const float (&v)[32], uint32_t (&q)[8]) {
+// Largest magnitude's bits (fp32), and value j.
+__device__ __forceinline__ uint32_t amax_bits(const Raw<uint16_t>& v) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (uint32_t j = 0; j < 16u; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v.w[j] & 0x7fff7fffu));
+  return (uint32_t)max(m[0], m[1]) << 16;
+}
+__device__ __forceinline__ uint32_t amax_bits(const Raw<float>& v) {
   uint32_t m = 0u;
 #pragma unroll
-  for (uint32_t j = 0; j < 32u; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+  for (uint32_t j = 0; j < 32u; ++j) m = max(m, __float_as_uint(v.w[j]) & 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ float at(const Raw<uint16_t>& v, uint32_t j) {
+  return j & 1u ? nk::bf16_hi(v.w[j / 2u]) : nk::bf16_lo(v.w[j / 2u]);
+}
+__device__ __forceinline__ float at(const Raw<float>& v, uint32_t j) { return v.w[j]; }
+
+// The 32 values of each lane as MFMA operand bytes, with the scale of the
+// 128-group that the lanes l, l ^ 16, l ^ 32, l ^ 48 hold together. |v / scale| is
+// at most 448 (1 + 4 * 2^-24), which rounds to 448 without the contract's clamp.
+template <typename X>
+__device__ __forceinline__ float quantise32(const Raw<X>& v, uint32_t (&q)[8]) {
+  uint32_t m = amax_bits(v);
+  const auto r16 = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = max((uint32_t)r16[0], (uint32_t)r16[1]);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = max((uint32_t)r32[0], (uint32_t)r32[1]);
   const float scale = group_scale(m);
   const float inv = 1.0f / scale;
 #pragma unroll
-  for (uint32_t j = 0; j < 8u; ++j)
-    q[j] = nk::e4m3x4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+  for (uint32_t j = 0; j < 8u; ++j) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(at(v, 4 * j) * inv, at(v, 4 * j + 1) * inv, 0, false);
+    q[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(at(v, 4 * j + 2) * inv, at(v, 4 * j + 3) * inv, lo, true);
+  }
   return scale;
 }
 
@@ -88,7 +139,7 @@ __device__ __forceinline__ void store_tile(uint8_t* tile, uint32_t lane, const u
 // Rows: x [rows, n] -> tiles of 16 rows x 128 columns, scales s[b, row] with
 // `sld` floats per block (sld = rows rounded up to 16 at least). One wave per tile; rows past
 // the end are zeros.
-template <typename X, bool kVec>
+template <typename X>
 __device__ __forceinline__ void quant_rows(const X* __restrict__ x, uint64_t stride, uint8_t* __restrict__ q,
                                            float* __restrict__ s, uint32_t rows, uint32_t n, uint32_t sld) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -96,13 +147,8 @@ __device__ __forceinline__ void quant_rows(const X* __restrict__ x, uint64_t str
   const uint32_t rt = blockIdx.x, b = blockIdx.y * 4u + wave;
   if (b >= kb) return;
   const uint32_t r = rt * 16u + (lane & 15u), c = b * 128u + (lane >> 4) * 32u;
-  float v[32];
-  if (r < rows) {
-    load32<kVec>(x + (uint64_t)r * stride, c, n, v);
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 32u; ++j) v[j] = 0.0f;
-  }
+  Raw<X> v = {};
+  if (r < rows) load32(x + (uint64_t)r * stride, c, n, v);
   uint32_t code[8];
   const float scale = quantise32(v, code);
   store_tile(q + ((size_t)rt * kb + b) * 2048u, lane, code);
@@ -166,8 +212,8 @@ struct Tile {
   static constexpr uint32_t kPitch = NP * 32u + 16u;
   static constexpr uint32_t kOut = kWaves * 16u * NQ * kPitch;
   static constexpr uint32_t kLds = S * kStage > kOut ? S * kStage : kOut;
-  static_assert(kWaves == 8u && (NP % 8u == 0u || 8u % NP == 0u) && kP % kWaves == 0u && kQ % kWaves == 0u &&
-                    kP <= 64u * 8u && kQ % 4u == 0u && kQ <= 28u && kLds <= 160u * 1024u,
+  static_assert(kWaves == 8u && (NP % 8u == 0u || 8u % NP == 0u) && kP % 4u == 0u && kQ % 4u == 0u && kQ <= 28u &&
+                    kLds <= 160u * 1024u,
                 "waves, scale blocks, copies and LDS");
 };
 
@@ -191,31 +237,45 @@ __device__ __forceinline__ void product_tile(const Product& a) {
   const uint32_t wp = wave % WP, wq = wave / WP;
   const uint32_t b0 = split * a.split_blocks, b1 = min(a.kb, b0 + a.split_blocks);  // this split's blocks
 
-  const u32x4 rp = nklds2::rsrc(a.p + (size_t)p0 * a.kb * 2048u, min(L::kP, pt - p0) * a.kb * 2048u);
-  const u32x4 rq = nklds2::rsrc(a.q + (size_t)q0 * a.kb * 2048u, min(L::kQ, qt - q0) * a.kb * 2048u);
-  const u32x4 rsp = nklds2::rsrc(a.sp, a.sp_bytes);
+  const uint32_t np_here = min(L::kP, pt - p0), nq_here = min(L::kQ, qt - q0);
+  const u32x4 rp = nklds2::rsrc(a.p + (size_t)p0 * a.kb * 2048u, np_here * a.kb * 2048u);
+  const u32x4 rq = nklds2::rsrc(a.q + (size_t)q0 * a.kb * 2048u, nq_here * a.kb * 2048u);
   // A wave copies one 64-word part of the scales: Q's by the first kQ / 4 waves, P's
   // (lane i: 128-block i of the tile) by the others, all of them alike.
   const bool q_scales = wave < L::kQ / 4u;
-  const uint32_t spoff =
-      lane * 8u < L::kP && (p0 / 8u + lane) * 128u < a.ni ? (p0 / 8u + lane) * a.sp_i * 4u : 0x80000000u;
+  const uint32_t sq_first = (q0 + wave * 4u) * 16u;
+  const uint64_t s_base = (uint64_t)(q_scales ? a.sq + sq_first : a.sp);
+  const uint32_t s_bytes = q_scales ? (sq_first < a.sq_b ? (a.sq_b - sq_first) * 4u : 0u) : a.sp_bytes;
+  const uint32_t s_step = (q_scales ? a.sq_b : a.sp_b) * 4u, s_less = q_scales ? 0u : s_step;  // bytes per block
+  const uint32_t s_at = q_scales ? wave * 256u : L::kQ * 64u;
+  const uint32_t s_voff = q_scales ? lane * 4u
+                          : lane * 8u < L::kP && (p0 / 8u + lane) * 128u < a.ni ? (p0 / 8u + lane) * a.sp_i * 4u
+                                                                                 : 0x80000000u;
+  const uint32_t voff = lane * 16u;
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
-  auto issue = [&](uint32_t b, uint32_t stage) __attribute__((always_inline)) {
+  // Copy i of a wave's kCopies for block b. A tile past the matrix repeats its last
+  // one (its outputs are not stored); behind the split's last block a copy reads
+  // nothing (an empty range) and leaves zeros that nobody looks at, so that a step's
+  // code has no branch and always the same copies in flight.
+  auto issue_part = [&](uint32_t b, uint32_t stage, uint32_t i) __attribute__((always_inline)) {
     const uint32_t st = lds0 + stage * L::kStage;
-#pragma unroll
-    for (uint32_t i = 0; i < (L::kP + L::kQ) / L::kWaves; ++i) {
-      const uint32_t t = i * L::kWaves + wave;  // P's tiles, then Q's
-      const bool is_p = i < L::kP / L::kWaves;
-      const uint32_t voff = (is_p ? t : t - L::kP) * a.kb * 2048u + lane * 16u;
-      nklds2::copy16(st + t * 2048u, is_p ? rp : rq, voff, b * 2048u);
-      nklds2::copy16(st + t * 2048u + 1024u, is_p ? rp : rq, voff + 1024u, b * 2048u);
-    }
-    if (q_scales) {
-      const u32x4 rsq = nklds2::rsrc(a.sq + (size_t)b * a.sq_b + q0 * 16u, (a.sq_b - q0 * 16u) * 4u);
-      nklds2::copy4(st + L::kScaleAt + wave * 256u, rsq, wave * 256u + lane * 4u, 0u);
+    const bool live = b < b1;
+    if (i + 1u < L::kCopies) {
+      const uint32_t k = i * L::kWaves + wave;  // P's half tiles, then Q's
+      const bool is_p = i * L::kWaves < 2u * L::kP;
+      const uint32_t t = is_p ? min(k >> 1, np_here - 1u) : min((k >> 1) - L::kP, nq_here - 1u);
+      u32x4 r = is_p ? rp : rq;
+      r.z = live ? r.z : 0u;
+      nklds2::copy16(st + k * 1024u, r, voff, live ? (t * a.kb + b) * 2048u + (k & 1u) * 1024u : 0u);
     } else {
-      nklds2::copy4(st + L::kScaleAt + L::kQ * 64u, rsp, spoff, b * a.sp_b * 4u);
+      const uint32_t bytes = s_bytes - b * s_less;
+      const u32x4 r = nklds2::rsrc((const void*)(s_base + (uint64_t)b * s_step), live ? bytes : 0u);
+      nklds2::copy4(st + L::kScaleAt + s_at, r, s_voff, 0u);
     }
+  };
+  auto issue = [&](uint32_t b, uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < L::kCopies; ++i) issue_part(b, stage, i);
   };
 
   v4f acc[NP][NQ];
@@ -225,38 +285,44 @@ __device__ __forceinline__ void product_tile(const Product& a) {
     for (uint32_t j = 0; j < NQ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-  for (uint32_t i = 0; i + 1u < S; ++i)
-    if (b0 + i < b1) issue(b0 + i, i);
+  for (uint32_t i = 0; i + 1u < S; ++i) issue(b0 + i, i);
   uint32_t stage = 0u;
   for (uint32_t b = b0; b < b1; ++b) {
-    // the copies of the steps behind this one may stay in flight
-    if (S > 2u && b + S - 2u < b1) nklds2::wait_copies<(S - 2u) * L::kCopies>();
-    else nklds2::wait_copies<0>();
+    nklds2::wait_copies<(S - 2u) * L::kCopies>();  // the copies of the steps behind this one may stay in flight
     nklds2::barrier();
     const uint32_t before = stage == 0u ? S - 1u : stage - 1u;
-    if (b + S - 1u < b1) issue(b + S - 1u, before);
     const uint8_t* st = s_stage + stage * L::kStage;
     stage = stage + 1u == S ? 0u : stage + 1u;
     const uint8_t* sp_tiles = st + wp * NP * 2048u;
     const uint8_t* sq_tiles = st + (L::kP + wq * NQ) * 2048u;
     const float* scale = reinterpret_cast<const float*>(st + L::kScaleAt);
-    v8i qo[NQ];
+    v8i qo[NQ], po[2];
     float s[NQ];
+    po[0] = nk::load_tile_operand(sp_tiles, lane);
     const float sp = scale[L::kQ * 16u + wp * NP / 8u];
 #pragma unroll
     for (uint32_t j = 0; j < NQ; ++j) {
       qo[j] = nk::load_tile_operand(sq_tiles + j * 2048u, lane);
       s[j] = scale[(wq * NQ + j) * 16u + (lane & 15u)] * sp;
     }
+    v4f d[2][NQ];
 #pragma unroll
-    for (uint32_t i = 0; i < NP; ++i) {
-      const v8i po = nk::load_tile_operand(sp_tiles + i * 2048u, lane);
+    for (uint32_t i = 0; i <= NP; ++i) {
+      if (i + 1u < NP) po[(i + 1u) & 1u] = nk::load_tile_operand(sp_tiles + (i + 1u) * 2048u, lane);
 #pragma unroll
       for (uint32_t j = 0; j < NQ; ++j) {
-        const v4f d = nk::mfma_e4m3_16x16x128(po, qo[j]);
+        if (i < NP) d[i & 1u][j] = nk::mfma_e4m3_16x16x128(po[i & 1u], qo[j]);
+        if (i > 0u) {
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) acc[i][j][e] = fmaf(s[j], d[e], acc[i][j][e]);
+          for (uint32_t e = 0; e < 4u; ++e)
+            acc[i - 1u][j][e] = fmaf(s[j], d[(i - 1u) & 1u][j][e], acc[i - 1u][j][e]);
+        }
       }
+      // the copies of a later step, spread over this one's products
+#pragma unroll
+      for (uint32_t k = i * L::kCopies / (NP + 1u); k < (i + 1u) * L::kCopies / (NP + 1u); ++k)
+        issue_part(b + S - 1u, before, k);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -276,6 +342,7 @@ __device__ __forceinline__ void product_tile(const Product& a) {
   }
   // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
   // whole lines. (A wave reads back only what it wrote itself.)
+  nklds2::wait_copies<0>();
   __syncthreads();
   uint8_t* mine = s_stage + wave * 16u * NQ * L::kPitch;
 #pragma unroll
@@ -318,18 +385,20 @@ __device__ __forceinline__ void product_sum(const Product& a) {
 }
 
 // Few rows: a workgroup computes 16 NP columns of the output for all 16 NQ rows,
-// its 8 waves dealing the 128-blocks among them. The weights go from memory to
-// registers (each tile is read by one wave of the launch); the activations are
-// quantised on the way, by every wave for its own blocks, so that a call is one
-// launch: a wave's lanes hold a tile of 16 rows x 128 values exactly as an operand
-// wants it, and the four lanes of a row find its scale with two exchanges.
-template <uint32_t NP, uint32_t NQ, typename X, bool kVec>
+// its 8 waves dealing the 128-blocks among them and adding up in LDS, in wave
+// order. The weights go from memory to registers (each tile is read by one wave of
+// the launch), one block ahead. Where kFused, the activations are quantised on the
+// way, by every wave for its own blocks, so that a call is one launch: a wave's
+// lanes hold a tile of 16 rows x 128 values exactly as an operand wants it, and the
+// four lanes of a row find its scale with two exchanges. Else their tiles come from
+// a.q.
+template <uint32_t NP, uint32_t NQ, bool kFused, typename X>
 __device__ __forceinline__ void product_stream(const Product& a, const X* __restrict__ x, uint64_t x_stride,
                                                uint32_t n) {
   __shared__ v4f s_part[8][NP * NQ][64];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t pt = (a.ni + 15u) / 16u, p0 = blockIdx.x * NP;
+  const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u, p0 = blockIdx.x * NP;
   const uint32_t c = lane & 15u, g = lane >> 4;
   v4f acc[NP][NQ];
 #pragma unroll
@@ -353,29 +422,36 @@ __device__ __forceinline__ void product_stream(const Product& a, const X* __rest
     float sp[NP];
 #pragma unroll
     for (uint32_t i = 0; i < NP; ++i) sp[i] = spb[i][(size_t)b * a.sp_b];
+    Raw<X> raw[kFused ? NQ : 1u];
+    v8i qo[NQ];
+    float sq[NQ];
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j) {
+      if constexpr (kFused) {
+        raw[j] = {};
+        if (j * 16u + c < a.nq) load32(x + (uint64_t)(j * 16u + c) * x_stride, b * 128u + g * 32u, n, raw[j]);
+      } else {
+        const uint32_t t = min(j, qt - 1u);
+        qo[j] = nk::load_tile_operand(nk::tile_base(a.q, t, b, a.kb), lane);
+        sq[j] = a.sq[(size_t)b * a.sq_b + t * 16u + c];
+      }
+    }
     v8i next[NP];
     const uint32_t bn = min(b + 8u, a.kb - 1u);
 #pragma unroll
     for (uint32_t i = 0; i < NP; ++i) next[i] = nk::load_tile_operand_once(pb[i] + (size_t)bn * 2048u, lane);
 #pragma unroll
     for (uint32_t j = 0; j < NQ; ++j) {
-      const uint32_t r = j * 16u + c;
-      float v[32];
-      if (r < a.nq) {
-        load32<kVec>(x + (uint64_t)r * x_stride, b * 128u + g * 32u, n, v);
-      } else {
+      if constexpr (kFused) {
+        uint32_t code[8];
+        sq[j] = quantise32(raw[j], code);
 #pragma unroll
-        for (uint32_t e = 0; e < 32u; ++e) v[e] = 0.0f;
+        for (uint32_t e = 0; e < 8u; ++e) qo[j][e] = (int)code[e];
       }
-      uint32_t code[8];
-      const float sq = quantise32(v, code);
-      v8i qo;
-#pragma unroll
-      for (uint32_t e = 0; e < 8u; ++e) qo[e] = (int)code[e];
 #pragma unroll
       for (uint32_t i = 0; i < NP; ++i) {
-        const v4f d = nk::mfma_e4m3_16x16x128(po[i], qo);
-        const float s = sq * sp[i];
+        const v4f d = nk::mfma_e4m3_16x16x128(po[i], qo[j]);
+        const float s = sq[j] * sp[i];
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) acc[i][j][e] = fmaf(s, d[e], acc[i][j][e]);
       }
@@ -405,10 +481,12 @@ __device__ __forceinline__ void product_stream(const Product& a, const X* __rest
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 struct Outer {
-  const uint16_t* dy;   // [rows, n]
+  const uint16_t* dy;   // [rows, n] in rows of dy_cols readable elements (an even number)
   uint64_t dy_stride;
+  uint32_t dy_cols;
   const uint16_t* x;    // [rows, k]
   uint64_t x_stride;
+  uint32_t x_cols;
   float* dw;            // [n, k]
   uint32_t rows, n, k;
   uint32_t accumulate;
@@ -417,7 +495,8 @@ struct Outer {
 };
 
 // dw[n, k] = sum_t dy[t, n] x[t, k], both operands staged through LDS, for bf16
-// matrices whose rows are 16-byte aligned and whole 16-byte chunks. Both have the contraction (tokens) as their slow
+// matrices whose rows are whole dwords (a copy's range ends with the last row, and
+// ends are checked per dword). Both have the contraction (tokens) as their slow
 // dimension, so their rows are copied as they are and the transposed LDS reads
 // (ds_read_b64_tr_b16: among 16 lanes, lane i gets element i % 4 of the 8 bytes
 // that lanes i / 4 + 0, 4, 8, 12 address) turn 4 tokens x 16 columns into operand
@@ -463,9 +542,9 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
     auto rows = [&](const uint16_t* m, uint64_t stride, uint32_t c0, uint32_t cols, uint32_t row_bytes, uint32_t v,
                     uint32_t at) __attribute__((always_inline)) {
       const uint16_t* base = m + (uint64_t)t * stride + c0;
-      // tokens t .. min(t1, t + 64) - 1, from column c0 (rows are whole 16-byte chunks)
+      // tokens t .. min(t1, t + 64) - 1, from column c0
       const uint32_t n = min(kTokens, t1 - t);
-      const u32x4 r = nklds2::rsrc(base, ((n - 1u) * (uint32_t)stride + (((cols + 7u) & ~7u) - c0)) * 2u);
+      const u32x4 r = nklds2::rsrc(base, ((n - 1u) * (uint32_t)stride + (cols - c0)) * 2u);
       const uint32_t each = 1024u / row_bytes;  // rows per copy
 #pragma unroll
       for (uint32_t i = 0; i < kTokens / each / 8u; ++i) {
@@ -473,8 +552,8 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
         nklds2::copy16(at + row * row_bytes, r, v + row * (uint32_t)stride * 2u, 0u);
       }
     };
-    rows(a.x, a.x_stride, p0, a.k, kRowP, pv, st);
-    rows(a.dy, a.dy_stride, q0, a.n, kRowQ, qv, st + kTokens * kRowP);
+    rows(a.x, a.x_stride, p0, a.x_cols, kRowP, pv, st);
+    rows(a.dy, a.dy_stride, q0, a.dy_cols, kRowQ, qv, st + kTokens * kRowP);
   };
 
   v4f acc[NP][NQ];
@@ -608,40 +687,47 @@ extern "C" __global__ __launch_bounds__(256) void netra_linear_pack_gfx950(const
   nklin::store_tile(dst + ((size_t)blockIdx.x * cb + b) * 2048u, lane, code);
 }
 
-#define NETRA_QUANT_ROWS(NAME, X, VEC)                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_##NAME##_gfx950(                            \
-      const X* x, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld) {          \
-    nklin::quant_rows<X, VEC>(x, stride, q, s, rows, n, sld);                                                \
-  }
-NETRA_QUANT_ROWS(bf16, uint16_t, false)
-NETRA_QUANT_ROWS(bf16_vec, uint16_t, true)
-NETRA_QUANT_ROWS(f32, float, false)
-NETRA_QUANT_ROWS(f32_vec, float, true)
+extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_bf16_gfx950(
+    const uint16_t* x, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld) {
+  nklin::quant_rows(x, stride, q, s, rows, n, sld);
+}
+extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_f32_gfx950(
+    const float* x, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld) {
+  nklin::quant_rows(x, stride, q, s, rows, n, sld);
+}
 
-extern "C" __global__ __launch_bounds__(512) void netra_linear_product_256x256_gfx950(nklin::Product a) {
-  nklin::product_tile<2, 4, 8, 4, 2>(a);
-}
-extern "C" __global__ __launch_bounds__(512) void netra_linear_product_128x128_gfx950(nklin::Product a) {
-  nklin::product_tile<2, 4, 4, 2, 4>(a);
-}
+#define NETRA_PRODUCT_TILE(P, Q, ...)                                                                             \
+  extern "C" __global__ __launch_bounds__(512) void netra_linear_product_##P##x##Q##_gfx950(nklin::Product a) {    \
+    nklin::product_tile<__VA_ARGS__>(a);                                                                          \
+  }
+NETRA_PRODUCT_TILE(256, 256, 2, 4, 8, 4, 2)
+NETRA_PRODUCT_TILE(256, 128, 2, 4, 8, 2, 3)
+NETRA_PRODUCT_TILE(128, 128, 2, 4, 4, 2, 4)
+NETRA_PRODUCT_TILE(128, 64, 4, 2, 2, 2, 4)
+NETRA_PRODUCT_TILE(64, 64, 4, 2, 1, 2, 4)
 extern "C" __global__ __launch_bounds__(256) void netra_linear_product_sum_gfx950(nklin::Product a) {
   nklin::product_sum(a);
 }
 
-#define NETRA_PRODUCT_STREAM(NAME, X, VEC, NP, NQ)                                                           \
-  extern "C" __global__ __launch_bounds__(512) void netra_linear_product_stream_##NAME##_p##NP##q##NQ##_gfx950( \
+#define NETRA_PRODUCT_FUSED(NAME, X, NP, NQ)                                                                 \
+  extern "C" __global__ __launch_bounds__(512) void netra_linear_product_fused_##NAME##_p##NP##q##NQ##_gfx950( \
       nklin::Product a, const X* x, uint64_t x_stride, uint32_t n) {                                         \
-    nklin::product_stream<NP, NQ, X, VEC>(a, x, x_stride, n);                                                \
+    nklin::product_stream<NP, NQ, true, X>(a, x, x_stride, n);                                               \
   }
-#define NETRA_PRODUCT_STREAMS(NP, NQ)                        \
-  NETRA_PRODUCT_STREAM(bf16, uint16_t, false, NP, NQ)        \
-  NETRA_PRODUCT_STREAM(bf16_vec, uint16_t, true, NP, NQ)     \
-  NETRA_PRODUCT_STREAM(f32, float, false, NP, NQ)            \
-  NETRA_PRODUCT_STREAM(f32_vec, float, true, NP, NQ)
-NETRA_PRODUCT_STREAMS(1, 1)
-NETRA_PRODUCT_STREAMS(2, 1)
-NETRA_PRODUCT_STREAMS(2, 2)
-NETRA_PRODUCT_STREAMS(2, 4)
+#define NETRA_PRODUCTS_FUSED(NP, NQ)           \
+  NETRA_PRODUCT_FUSED(bf16, uint16_t, NP, NQ)  \
+  NETRA_PRODUCT_FUSED(f32, float, NP, NQ)
+NETRA_PRODUCTS_FUSED(1, 1)
+NETRA_PRODUCTS_FUSED(2, 1)
+NETRA_PRODUCTS_FUSED(1, 2)
+NETRA_PRODUCTS_FUSED(2, 2)
+NETRA_PRODUCTS_FUSED(1, 4)
+#define NETRA_PRODUCT_STREAM(NP, NQ)                                                                                  \
+  extern "C" __global__ __launch_bounds__(512) void netra_linear_product_stream_p##NP##q##NQ##_gfx950(nklin::Product a) { \
+    nklin::product_stream<NP, NQ, false, uint16_t>(a, nullptr, 0, 0);                                                 \
+  }
+NETRA_PRODUCT_STREAM(1, 4)
+NETRA_PRODUCT_STREAM(2, 4)
 
 extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_256x256_gfx950(nklin::Outer a) {
   nklin::outer_tile<2, 4, 8, 4>(a);

@@ -56,65 +56,93 @@ bool bad_matrix(const void* p, uint32_t type, uint64_t stride, uint32_t cols) {
 void quant_rows(const void* x, uint32_t type, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n,
                 hipStream_t stream) {
   const dim3 grid((rows + 15u) / 16u, (blocks(n) + 3u) / 4u), block(256);
-  const bool vec = aligned(x, 16) && stride * elem(type) % 16u == 0;
   const uint32_t sld = up(rows, 16u);
-  if (type == NETRA_BF16) {
-    const uint16_t* p = static_cast<const uint16_t*>(x);
-    if (vec) netra_linear_quant_rows_bf16_vec_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
-    else netra_linear_quant_rows_bf16_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
-  } else {
-    const float* p = static_cast<const float*>(x);
-    if (vec) netra_linear_quant_rows_f32_vec_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
-    else netra_linear_quant_rows_f32_gfx950<<<grid, block, 0, stream>>>(p, stride, q, s, rows, n, sld);
-  }
+  if (type == NETRA_BF16)
+    netra_linear_quant_rows_bf16_gfx950<<<grid, block, 0, stream>>>(static_cast<const uint16_t*>(x), stride, q, s, rows,
+                                                                    n, sld);
+  else
+    netra_linear_quant_rows_f32_gfx950<<<grid, block, 0, stream>>>(static_cast<const float*>(x), stride, q, s, rows, n,
+                                                                   sld);
 }
 
-// How a product runs: `stream` (quantising on the way) or tiles of p x q with splits of the contraction.
+// How a product runs: the streaming kernel, quantising on the way (kFused) or not
+// (kStream), or tiles of p x q with splits of the contraction.
+enum Form { kFused, kStream, kTiles };
 struct ProductPlan {
-  bool stream;
+  Form form;
   uint32_t p, q, splits, split_blocks;
 };
-ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc) {
-  if (rows <= 64u) return {true, 0, 0, 1, 0};
-  auto tiles = [&](uint32_t p, uint32_t q) {
-    return static_cast<uint64_t>((ni + p - 1u) / p) * ((rows + q - 1u) / q);
+
+// Tiles: time = rounds of workgroups over the 256 CUs x steps x the step's time, which
+// hardly depends on how many CUs work (us a step, 1 to 32 rounds: 256x256 1.95, 256x128
+// 1.18, 128x128 0.78, 128x64 0.58, 64x64 0.56 with two workgroups per CU). Splits add a
+// launch and the partial sums' way out and in. Measured as whole calls, best and next
+// tile: T 333, N 1024, K 2048 64x64 11.6 us, 128x64 14.3; T 1001, N 1500, K 1111 128x64
+// 15.3, 64x64 17.1; T 2048, N 2048, K 2048 128x128 21.2, 256x128 26.7; T 2048, N 4096,
+// K 4096 256x128 46.0, 128x128 56.0; T 4096, N 4096, K 2048 256x256 46.1, 256x128 55.5;
+// T 128, N 8192, K 8192 128x128 in four splits 24.9, in two 32.3, 64x64 in two 26.0.
+ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
+  struct Shape {
+    uint32_t p, q, at_once;
+    double step_us;
   };
-  ProductPlan plan{false, 256, 256, 1, blocks(nc)};
-  if (tiles(256, 256) < 200) plan.p = plan.q = 128;
-  const uint64_t t = tiles(plan.p, plan.q);
-  uint32_t splits = t >= 128 ? 1u : static_cast<uint32_t>(256 / t);
-  const uint32_t most = (blocks(nc) + 3u) / 4u;  // 4 blocks at least
-  splits = splits > most ? most : splits;
-  plan.split_blocks = (blocks(nc) + splits - 1u) / splits;
-  plan.splits = (blocks(nc) + plan.split_blocks - 1u) / plan.split_blocks;
-  return plan;
+  static const Shape shapes[] = {
+      {256, 256, 256, 1.95}, {256, 128, 256, 1.18}, {128, 128, 256, 0.78}, {128, 64, 256, 0.58}, {64, 64, 512, 0.56}};
+  const uint32_t kb = blocks(nc);
+  ProductPlan best{kTiles, 256, 256, 1, kb};
+  double best_us = 1e30;
+  for (const Shape& s : shapes) {
+    const uint64_t tiles = static_cast<uint64_t>((ni + s.p - 1u) / s.p) * ((rows + s.q - 1u) / s.q);
+    for (uint32_t splits = 1; splits <= 8u && splits <= (kb + 3u) / 4u; splits *= 2u) {
+      if (splits > 1u && tiles * splits > 2u * s.at_once) break;
+      const uint32_t each = (kb + splits - 1u) / splits, n = (kb + each - 1u) / each;
+      const double rounds = static_cast<double>((tiles * n + s.at_once - 1u) / s.at_once);
+      double us = rounds * each * s.step_us;
+      if (n > 1u) us += 3.0 + static_cast<double>(rows) * ni * (8.0 * n) / 5e6;  // 5 TB/s
+      if (us < best_us) {
+        best_us = us;
+        best = {kTiles, s.p, s.q, n, each};
+      }
+    }
+  }
+  return best;
+}
+
+ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc) {
+  if (rows > 64u) return product_tiles(rows, ni, nc);
+  // Quantising on the way saves a launch (10.7 us -> 6.7 at one row) and costs every
+  // workgroup the quantisation of its waves' blocks: 16-row tiles x blocks per wave x
+  // workgroups per CU, of which seven cost what the launch does (T 48, N 4096, K 2048, six:
+  // 10.3 us against 10.7; T 64, eight: 11.7 against 10.8; T 32, N 8192, K 8192, sixteen: 23.5
+  // against 17.5).
+  const uint32_t pt = (ni + 15u) / 16u, q = (rows + 15u) / 16u;
+  const uint32_t groups = pt >= 512u ? (pt + 1u) / 2u : pt;
+  const uint64_t cost = static_cast<uint64_t>((groups + 255u) / 256u) * q * ((blocks(nc) + 7u) / 8u);
+  return {q == 1u || cost < 8u ? kFused : kStream, 0, 0, 1, 0};
 }
 uint64_t product_workspace(uint32_t rows, uint32_t ni, uint32_t nc) {
   if (rows == 0) return 0;
   const ProductPlan plan = product_plan(rows, ni, nc);
-  if (plan.stream) return 0;
+  if (plan.form == kFused) return 0;
   const uint64_t partial = plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * rows * up(ni, 4u) : 0u;
   return (matrix_bytes(rows, nc) + 15u) / 16u * 16u + partial;
 }
 
 template <typename X>
-void product_stream(const nklin::Product& a, const X* x, uint64_t stride, uint32_t nc, hipStream_t stream) {
-  const bool vec = aligned(x, 16) && stride * sizeof(X) % 16u == 0;
+void product_fused(const nklin::Product& a, const X* x, uint64_t stride, uint32_t nc, hipStream_t stream) {
   const uint32_t pt = (a.ni + 15u) / 16u, q = (a.nq + 15u) / 16u;
-  const bool wide = q > 1u || pt >= 512u;
+  // two tiles of columns per workgroup halve the quantisation (T 16, N 8192, K 8192: 21.7 us -> 16.2)
+  const bool wide = q <= 2u && pt >= 512u;
   const dim3 grid(wide ? (pt + 1u) / 2u : pt), block(512);
-#define NETRA_RUN(P, Q)                                                                                               \
-  do {                                                                                                                \
-    if constexpr (sizeof(X) == 2) {                                                                                   \
-      if (vec) netra_linear_product_stream_bf16_vec_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc); \
-      else netra_linear_product_stream_bf16_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);        \
-    } else {                                                                                                          \
-      if (vec) netra_linear_product_stream_f32_vec_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc); \
-      else netra_linear_product_stream_f32_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);         \
-    }                                                                                                                 \
+#define NETRA_RUN(P, Q)                                                                                          \
+  do {                                                                                                           \
+    if constexpr (sizeof(X) == 2)                                                                                \
+      netra_linear_product_fused_bf16_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);         \
+    else netra_linear_product_fused_f32_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);       \
   } while (0)
-  if (q > 2u) NETRA_RUN(2, 4);
-  else if (q == 2u) NETRA_RUN(2, 2);
+  if (q > 2u) NETRA_RUN(1, 4);
+  else if (q == 2u && wide) NETRA_RUN(2, 2);
+  else if (q == 2u) NETRA_RUN(1, 2);
   else if (wide) NETRA_RUN(2, 1);
   else NETRA_RUN(1, 1);
 #undef NETRA_RUN
@@ -122,9 +150,12 @@ void product_stream(const nklin::Product& a, const X* x, uint64_t stride, uint32
 
 // An operand of the weight gradient as it is, or as bf16 with aligned rows in the workspace.
 bool outer_ready(const void* m, uint32_t type, uint64_t stride, uint32_t cols) {
-  return type == NETRA_BF16 && aligned(m, 16) && cols % 8u == 0 && stride % 8u == 0 && stride < (1u << 24);
+  return type == NETRA_BF16 && aligned(m, 4) && cols % 2u == 0 && stride % 2u == 0 && stride < (1u << 24);
 }
-const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, uint32_t rows, uint32_t cols,
+uint64_t outer_bytes(const void* m, uint32_t type, uint64_t stride, uint32_t rows, uint32_t cols) {
+  return outer_ready(m, type, stride, cols) ? 0 : static_cast<uint64_t>(rows) * up(cols, 8u) * 2u;
+}
+const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, uint32_t rows, uint32_t& cols,
                               uint8_t*& at, hipStream_t stream) {
   if (outer_ready(m, type, stride, cols)) return static_cast<const uint16_t*>(m);
   const uint32_t pitch = up(cols, 8u);
@@ -137,27 +168,45 @@ const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, ui
     netra_linear_to_bf16_bf16_gfx950<<<grid, dim3(256), 0, stream>>>(static_cast<const uint16_t*>(m), stride, out,
                                                                      rows, cols, pitch);
   at += static_cast<uint64_t>(rows) * pitch * 2u;
-  stride = pitch;
+  stride = cols = pitch;
   return out;
 }
 
-// Tile and split of the weight gradient.
+// Tile and split of the weight gradient, chosen as product_tiles' (steps of 64 tokens: 256x256
+// 1.65 us, 128x256 1.0, 128x128 0.63 alone on a CU, 1.13 where two share it). As whole calls,
+// best and next: T 333, N 1024, K 2048 128x128 8.5 us, 128x256 12.0; T 4096, N 4096, K 2048
+// 128x256 69, 128x128 76; T 4096, N 1024, K 1024 128x128 in four splits 22.3, in two 27.8; T 8192,
+// N 4096, K 4096 256x256 229, 128x256 276.
 struct OuterPlan {
   uint32_t p, q;  // columns of x and of dy per workgroup
   uint32_t splits, split_rows;
 };
 OuterPlan outer_plan(uint32_t rows, uint32_t n, uint32_t k) {
-  auto tiles = [&](uint32_t p, uint32_t q) { return static_cast<uint64_t>((k + p - 1u) / p) * ((n + q - 1u) / q); };
-  OuterPlan plan{256, 256, 1, 0};
-  if (tiles(256, 256) < 200) plan = {128, 256, 1, 0};
-  if (tiles(128, 256) < 200) plan = {128, 128, 1, 0};
-  const uint64_t t = tiles(plan.p, plan.q);
-  uint32_t splits = t >= 200 ? 1u : static_cast<uint32_t>(256 / t);
-  const uint32_t most = (rows + 255u) / 256u;  // 256 tokens at least
-  splits = splits < 1u ? 1u : splits > most ? most : splits;
-  plan.split_rows = up((rows + splits - 1u) / splits, 64u);
-  plan.splits = (rows + plan.split_rows - 1u) / plan.split_rows;
-  return plan;
+  struct Shape {
+    uint32_t p, q;
+    double step_us;
+  };
+  static const Shape shapes[] = {{256, 256, 1.65}, {128, 256, 1.0}, {128, 128, 0.63}};
+  const uint32_t steps = (rows + 63u) / 64u;
+  OuterPlan best{256, 256, 1, up(rows, 64u)};
+  double best_us = 1e30;
+  for (const Shape& s : shapes) {
+    const uint64_t tiles = static_cast<uint64_t>((k + s.p - 1u) / s.p) * ((n + s.q - 1u) / s.q);
+    for (uint32_t splits = 1; splits <= 16u && splits <= (steps + 3u) / 4u; splits *= 2u) {
+      if (splits > 1u && tiles * splits > 512u) break;
+      const uint32_t each = (steps + splits - 1u) / splits, count = (steps + each - 1u) / each;
+      const uint64_t items = tiles * count;
+      const double rounds = s.p + s.q == 256u && items > 256u ? (items + 511u) / 512u * 1.8
+                                                              : static_cast<double>((items + 255u) / 256u);
+      double us = rounds * each * s.step_us;
+      if (count > 1u) us += 3.0 + static_cast<double>(n) * k * 4.0 * (2.0 * count + 1.0) / 6e6;  // 6 TB/s
+      if (us < best_us) {
+        best_us = us;
+        best = {s.p, s.q, count, each * 64u};
+      }
+    }
+  }
+  return best;
 }
 
 bool bad_workspace(const void* p, uint64_t bytes, uint64_t need) {
@@ -186,11 +235,13 @@ extern "C" uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, ui
 extern "C" uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
   return product_workspace(rows, k, n);
 }
-extern "C" uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+static uint64_t partial_bytes(const OuterPlan& plan, uint32_t n, uint32_t k) {
+  return plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * n * k : 0;
+}
+extern "C" uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t in_place) {
   if (rows == 0) return 0;
-  const OuterPlan plan = outer_plan(rows, n, k);
-  return static_cast<uint64_t>(rows) * (up(n, 8u) + static_cast<uint64_t>(up(k, 8u))) * 2u +
-         (plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * n * k : 0u) + 16u;
+  return partial_bytes(outer_plan(rows, n, k), n, k) +
+         (in_place ? 0 : static_cast<uint64_t>(rows) * (static_cast<uint64_t>(up(n, 8u)) + up(k, 8u)) * 2u);
 }
 
 // in [rows, nc] times the packed matrix P [ni, nc] -> out [rows, ni]
@@ -223,9 +274,9 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   a.vec = aligned(out, 16) && out_stride % 8u == 0;
   a.splits = plan.splits;
   a.split_blocks = plan.split_blocks;
-  if (plan.stream) {
-    if (in_type == NETRA_BF16) product_stream(a, static_cast<const uint16_t*>(in), in_stride, nc, stream);
-    else product_stream(a, static_cast<const float*>(in), in_stride, nc, stream);
+  if (plan.form == kFused) {
+    if (in_type == NETRA_BF16) product_fused(a, static_cast<const uint16_t*>(in), in_stride, nc, stream);
+    else product_fused(a, static_cast<const float*>(in), in_stride, nc, stream);
     return launched(name);
   }
   uint8_t* q = static_cast<uint8_t*>(workspace);
@@ -234,11 +285,22 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   a.q = q;
   a.sq = s;
   a.sq_b = up(rows, 16u);
+  if (plan.form == kStream) {
+    const uint32_t pt = (ni + 15u) / 16u;
+    const bool wide = pt >= 512u;  // the activations are read half as often (T 64, N 8192, K 8192: 24.1 us -> 20.3)
+    const dim3 grid(wide ? (pt + 1u) / 2u : pt), block(512);
+    if (wide) netra_linear_product_stream_p2q4_gfx950<<<grid, block, 0, stream>>>(a);
+    else netra_linear_product_stream_p1q4_gfx950<<<grid, block, 0, stream>>>(a);
+    return launched(name);
+  }
   a.partial = reinterpret_cast<float*>(q + (matrix_bytes(rows, nc) + 15u) / 16u * 16u);
   const uint32_t items = ((ni + plan.p - 1u) / plan.p) * ((rows + plan.q - 1u) / plan.q) * plan.splits;
   const dim3 grid((items + 7u) / 8u * 8u), block(512);
-  if (plan.p == 256u) netra_linear_product_256x256_gfx950<<<grid, block, 0, stream>>>(a);
-  else netra_linear_product_128x128_gfx950<<<grid, block, 0, stream>>>(a);
+  if (plan.p == 256u && plan.q == 256u) netra_linear_product_256x256_gfx950<<<grid, block, 0, stream>>>(a);
+  else if (plan.p == 256u) netra_linear_product_256x128_gfx950<<<grid, block, 0, stream>>>(a);
+  else if (plan.q == 128u) netra_linear_product_128x128_gfx950<<<grid, block, 0, stream>>>(a);
+  else if (plan.p == 128u) netra_linear_product_128x64_gfx950<<<grid, block, 0, stream>>>(a);
+  else netra_linear_product_64x64_gfx950<<<grid, block, 0, stream>>>(a);
   if (plan.splits > 1u)
     netra_linear_product_sum_gfx950<<<dim3((ni + 1023u) / 1024u, rows < 4096u ? rows : 4096u), dim3(256), 0, stream>>>(a);
   return launched(name);
@@ -274,14 +336,18 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
   }
   if (bad_matrix(dy, dy_type, dy_stride, n) || bad_matrix(x, x_type, x_stride, k))
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
-  if (bad_workspace(workspace, workspace_bytes, netra_linear_weight_gradient_workspace(rows, n, k)))
+  const OuterPlan plan = outer_plan(rows, n, k);
+  if (bad_workspace(workspace, workspace_bytes,
+                    outer_bytes(dy, dy_type, dy_stride, rows, n) + outer_bytes(x, x_type, x_stride, rows, k) +
+                        partial_bytes(plan, n, k)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  const OuterPlan plan = outer_plan(rows, n, k);
   nklin::Outer a{};
-  a.dy = outer_operand(dy, dy_type, dy_stride, rows, n, at, stream);
+  a.dy_cols = n;
+  a.x_cols = k;
+  a.dy = outer_operand(dy, dy_type, dy_stride, rows, a.dy_cols, at, stream);
   a.dy_stride = dy_stride;
-  a.x = outer_operand(x, x_type, x_stride, rows, k, at, stream);
+  a.x = outer_operand(x, x_type, x_stride, rows, a.x_cols, at, stream);
   a.x_stride = x_stride;
   a.dw = dw;
   a.rows = rows;

@@ -31,6 +31,11 @@ from . import weights as W
 from .layers import TYPES, check_rows, entry, launch, workspace
 
 
+def _in_place(m: torch.Tensor, stride: int) -> bool:
+    """Whether the weight gradient reads this operand as it is (else through a bf16 copy in the workspace)."""
+    return m.dtype == torch.bfloat16 and not (m.shape[1] | stride) & 1 and not m.data_ptr() & 3 and stride < 1 << 24
+
+
 class BlockLinear:
     def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, *, gradients: bool = False):
         """weight: e4m3 (torch.float8_e4m3fn, or its codes as uint8) [N, K] on the
@@ -124,7 +129,7 @@ class BlockLinear:
             raise ValueError(f"out: need contiguous torch.float32 {(self.N, self.K)} on {self.device}")
         name = "netra_linear_weight_gradient"
         fn, need = self._entries[name]
-        need = need(rows, self.N, self.K)
+        need = need(rows, self.N, self.K, _in_place(x, x_stride) and _in_place(dy, dy_stride))
         ws, ws_ptr = workspace(need, self.device)
         launch(fn, name, self.device, dy.data_ptr(), TYPES[dy.dtype], dy_stride, x.data_ptr(), TYPES[x.dtype], x_stride,
                out.data_ptr(), int(accumulate), rows, self.N, self.K, ws_ptr, need)

@@ -62,11 +62,10 @@ def test_product_refusals(name, change):
                                     dict(ws=0), dict(ws=A + 8), dict(short=1)])
 def test_weight_gradient_refusals(change):
     lib = layers.library()
-    a = dict(g=A, gt=0, gs=128, x=A, xt=0, xs=256, dw=A, rows=300, n=128, k=256, ws=A, short=0)
-    need = lib.netra_linear_weight_gradient_workspace(300, 128, 256)
+    # (fp32: both operands go through the workspace)
+    a = dict(g=A, gt=1, gs=128, x=A, xt=1, xs=256, dw=A, rows=300, n=128, k=256, ws=A, short=0)
+    need = lib.netra_linear_weight_gradient_workspace(300, 128, 256, 0)
     a.update(change)
-    if not need and {"ws", "short"} & set(change):
-        pytest.skip("needs no workspace at this size")
     refused("netra_linear_weight_gradient", a["g"], a["gt"], a["gs"], a["x"], a["xt"], a["xs"], a["dw"], 0, a["rows"],
             a["n"], a["k"], a["ws"], need - a["short"], None)
 
