@@ -155,23 +155,31 @@ __device__ __forceinline__ void quant_rows(const X* __restrict__ x, uint64_t str
   if (lane < 16u) s[(size_t)b * sld + r] = scale;
 }
 
-__device__ __forceinline__ void store4(uint16_t* out, uint32_t left, bool vec, const float (&v)[4]) {
-  if (vec && left >= 4u) {
-    *reinterpret_cast<uint2*>(out) = make_uint2(nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
-                                                nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16));
+// Stores at any element address, `left` values at most.
+__device__ __forceinline__ void store4(uint16_t* out, uint32_t left, const float (&v)[4]) {
+  struct __attribute__((packed, aligned(2))) Pair {
+    uint32_t w[2];
+  };
+  const Pair p = {{nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
+                   nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16)}};
+  if (left >= 4u) {
+    *reinterpret_cast<Pair*>(out) = p;
     return;
   }
 #pragma unroll
-  for (uint32_t j = 0; j < 4u; ++j)
-    if (j < left) out[j] = nk::bf16_rne(v[j]);
+  for (uint32_t j = 0; j < 3u; ++j)
+    if (j < left) out[j] = (uint16_t)(p.w[j / 2u] >> (16u * (j & 1u)));
 }
-__device__ __forceinline__ void store4(float* out, uint32_t left, bool vec, const float (&v)[4]) {
-  if (vec && left >= 4u) {
-    *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+__device__ __forceinline__ void store4(float* out, uint32_t left, const float (&v)[4]) {
+  struct __attribute__((packed, aligned(4))) Quad {
+    float w[4];
+  };
+  if (left >= 4u) {
+    *reinterpret_cast<Quad*>(out) = Quad{{v[0], v[1], v[2], v[3]}};
     return;
   }
 #pragma unroll
-  for (uint32_t j = 0; j < 4u; ++j)
+  for (uint32_t j = 0; j < 3u; ++j)
     if (j < left) out[j] = v[j];
 }
 
@@ -185,7 +193,6 @@ struct Product {
   uint16_t* out;          // bf16 [nq, ni], row stride ldo elements
   uint64_t ldo;
   uint32_t ni, nq, kb;    // kb: 128-blocks of the contraction
-  uint32_t vec;           // rows of out are 16-byte aligned
   uint32_t splits, split_blocks;  // 128-blocks per split
   float* partial;         // [splits, nq, ni rounded up to 4] where splits > 1
 };
@@ -360,13 +367,13 @@ __device__ __forceinline__ void product_tile(const Product& a) {
     if (row >= a.nq || col >= a.ni) continue;
     const uint4 v = *reinterpret_cast<const uint4*>(mine + r * L::kPitch + cc * 2u);
     uint16_t* o = a.out + (uint64_t)row * a.ldo + col;
-    if (a.vec && col + 8u <= a.ni) {
-      *reinterpret_cast<uint4*>(o) = v;
+    const Unaligned16 w = {{v.x, v.y, v.z, v.w}};
+    if (col + 8u <= a.ni) {
+      *reinterpret_cast<Unaligned16*>(o) = w;
     } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (uint32_t e = 0; e < 8u; ++e)
-        if (col + e < a.ni) o[e] = (uint16_t)(w[e / 2u] >> (16u * (e & 1u)));
+        if (col + e < a.ni) o[e] = (uint16_t)(w.w[e / 2u] >> (16u * (e & 1u)));
     }
   }
 }
@@ -380,7 +387,7 @@ __device__ __forceinline__ void product_sum(const Product& a) {
     for (uint32_t k = 1; k < a.splits; ++k)
       s += *reinterpret_cast<const v4f*>(a.partial + ((size_t)k * a.nq + row) * pitch + col);
     const float v[4] = {s[0], s[1], s[2], s[3]};
-    store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, a.vec != 0u, v);
+    store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, v);
   }
 }
 
@@ -472,7 +479,7 @@ __device__ __forceinline__ void product_stream(const Product& a, const X* __rest
     const uint32_t row = j * 16u + (l & 15u), col = (p0 + i) * 16u + (l >> 4) * 4u;
     if (row >= a.nq || col >= a.ni) continue;
     const float v[4] = {s[0], s[1], s[2], s[3]};
-    store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, a.vec != 0u, v);
+    store4(a.out + (uint64_t)row * a.ldo + col, a.ni - col, v);
   }
 }
 
@@ -597,7 +604,6 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
   }
   float* dst = a.splits > 1u ? a.partial + (size_t)split * a.n * a.k : a.dw;
   const bool add = a.accumulate && a.splits == 1u;
-  const bool vec = a.k % 4u == 0u && reinterpret_cast<uintptr_t>(dst) % 16u == 0u;
 #pragma unroll
   for (uint32_t j = 0; j < NQ; ++j) {
     const uint32_t row = q0 + (wq * NQ + j) * 16u + c;
@@ -612,7 +618,7 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
         for (uint32_t e = 0; e < 4u; ++e)
           if (col + e < a.k) v[e] += o[e];
       }
-      store4(o, a.k - col, vec, v);
+      store4(o, a.k - col, v);
     }
   }
 }
@@ -663,28 +669,69 @@ __device__ __forceinline__ void to_bf16(const X* __restrict__ x, uint64_t stride
 
 }  // namespace nklin
 
-// Weights: w row-major e4m3 [n, k] -> tiles of w, or of w^T. One wave per tile;
-// bytes past the matrix are zeros.
+// Weights: w row-major e4m3 [n, k] -> tiles of w. One wave per tile; bytes past the
+// matrix are zeros.
 extern "C" __global__ __launch_bounds__(256) void netra_linear_pack_gfx950(const uint8_t* __restrict__ w,
-                                                                uint8_t* __restrict__ dst, uint32_t n, uint32_t k,
-                                                                uint32_t transpose) {
+                                                                           uint8_t* __restrict__ dst, uint32_t n,
+                                                                           uint32_t k) {
+  struct __attribute__((packed, aligned(1))) Bytes {
+    uint32_t w[8];
+  };
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t rows = transpose ? k : n, cols = transpose ? n : k;
-  const uint32_t cb = (cols + 127u) / 128u, b = blockIdx.y * 4u + wave;
-  if (b >= cb) return;
+  const uint32_t kb = (k + 127u) / 128u, b = blockIdx.y * 4u + wave;
+  if (b >= kb) return;
   const uint32_t r = blockIdx.x * 16u + (lane & 15u), c = b * 128u + (lane >> 4) * 32u;
+  uint32_t code[8] = {};
+  if (r < n) {
+    const uint8_t* at = w + (size_t)r * k + c;
+    if (c + 32u <= k) {
+      const Bytes v = *reinterpret_cast<const Bytes*>(at);
+#pragma unroll
+      for (uint32_t j = 0; j < 8u; ++j) code[j] = v.w[j];
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 32u; ++j)
+        if (c + j < k) code[j / 4u] |= (uint32_t)at[j] << (8u * (j % 4u));
+    }
+  }
+  nklin::store_tile(dst + ((size_t)blockIdx.x * kb + b) * 2048u, lane, code);
+}
+
+// Tiles of w^T: a workgroup turns 128 rows x 64 columns of w through LDS into four
+// tiles (16 columns by 128 rows). An LDS row of 64 bytes is followed by 4, so the
+// four row groups of one read start 32 * 17 words apart and its 16 columns share
+// four banks in each.
+extern "C" __global__ __launch_bounds__(256) void netra_linear_pack_transposed_gfx950(const uint8_t* __restrict__ w,
+                                                                                      uint8_t* __restrict__ dst,
+                                                                                      uint32_t n, uint32_t k) {
+  __shared__ uint32_t rows[128][17];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t nb = (n + 127u) / 128u, c0 = blockIdx.x * 64u, r0 = blockIdx.y * 128u;
+#pragma unroll
+  for (uint32_t i = 0; i < 8u; ++i) {  // 16 lanes of 4 bytes per row
+    const uint32_t r = i * 16u + (threadIdx.x >> 4), c = c0 + (threadIdx.x & 15u) * 4u;
+    uint32_t v = 0u;
+    if (r0 + r < n) {
+      const uint8_t* at = w + (size_t)(r0 + r) * k + c;
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e)
+        if (c + e < k) v |= (uint32_t)at[e] << (8u * e);
+    }
+    rows[r][threadIdx.x & 15u] = v;
+  }
+  __syncthreads();
+  const uint32_t tile = blockIdx.x * 4u + wave;
+  if (tile >= (k + 15u) / 16u) return;
+  const uint32_t c = wave * 16u + (lane & 15u), r = (lane >> 4) * 32u;
   uint32_t code[8];
 #pragma unroll
   for (uint32_t j = 0; j < 8u; ++j) {
     code[j] = 0u;
 #pragma unroll
-    for (uint32_t e = 0; e < 4u; ++e) {
-      const uint32_t cc = c + 4u * j + e;
-      if (r < rows && cc < cols)
-        code[j] |= (uint32_t)(transpose ? w[(size_t)cc * k + r] : w[(size_t)r * k + cc]) << (8u * e);
-    }
+    for (uint32_t e = 0; e < 4u; ++e)
+      code[j] |= ((rows[r + 4u * j + e][c / 4u] >> (8u * (c & 3u))) & 0xffu) << (8u * e);
   }
-  nklin::store_tile(dst + ((size_t)blockIdx.x * cb + b) * 2048u, lane, code);
+  nklin::store_tile(dst + ((size_t)tile * nb + blockIdx.y) * 2048u, lane, code);
 }
 
 extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_bf16_gfx950(

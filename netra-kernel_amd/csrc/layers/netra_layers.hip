@@ -223,9 +223,10 @@ extern "C" int netra_linear_pack(const uint8_t* w, uint8_t* packed, uint32_t n, 
                                  hipStream_t stream) {
   if (!w || !packed || w == packed || !aligned(packed, 16) || bad_sizes(0, n, k))
     return fail(-1, "netra_linear_pack", "null, aliased or misaligned pointers, or n / k not in 1 .. 2^21");
-  const uint32_t rows = transpose ? k : n, cols = transpose ? n : k;
-  netra_linear_pack_gfx950<<<dim3((rows + 15u) / 16u, (blocks(cols) + 3u) / 4u), dim3(256), 0, stream>>>(
-      w, packed, n, k, transpose ? 1u : 0u);
+  if (transpose)
+    netra_linear_pack_transposed_gfx950<<<dim3((k + 63u) / 64u, blocks(n)), dim3(256), 0, stream>>>(w, packed, n, k);
+  else
+    netra_linear_pack_gfx950<<<dim3((n + 15u) / 16u, (blocks(k) + 3u) / 4u), dim3(256), 0, stream>>>(w, packed, n, k);
   return launched("netra_linear_pack");
 }
 
@@ -271,7 +272,6 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   a.ni = ni;
   a.nq = rows;
   a.kb = blocks(nc);
-  a.vec = aligned(out, 16) && out_stride % 8u == 0;
   a.splits = plan.splits;
   a.split_blocks = plan.split_blocks;
   if (plan.form == kFused) {
