@@ -513,14 +513,16 @@ struct Outer {
 // Workgroups, waves and the stage hand-over are product_tile's. Columns past the
 // matrix read the next row and make outputs that are not stored; tokens past the
 // end read zeros.
-template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ>
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 __device__ __forceinline__ void outer_tile(const Outer& a) {
   constexpr uint32_t kP = WP * NP, kQ = WQ * NQ, kTokens = 64u;
   constexpr uint32_t kRowP = kP * 32u, kRowQ = kQ * 32u;  // bytes of a token's row
   constexpr uint32_t kStage = kTokens * (kRowP + kRowQ);
+  constexpr uint32_t kCopies = kStage / 8192u;            // a wave's, per step
   static_assert(WP * WQ == 8u && (kRowP == 256u || kRowP == 512u) && (kRowQ == 256u || kRowQ == 512u) &&
-                    NP % 4u == 0u, "copies and swizzle");
-  __shared__ __align__(16) uint8_t s_stage[2u * kStage];
+                    S * kStage <= 160u * 1024u,
+                "copies, swizzle and LDS");
+  __shared__ __align__(16) uint8_t s_stage[S * kStage];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t np = (a.k + 16u * kP - 1u) / (16u * kP), nq = (a.n + 16u * kQ - 1u) / (16u * kQ);
@@ -544,23 +546,20 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
   };
   const uint32_t pv = lane_offset(kRowP, a.x_stride), qv = lane_offset(kRowQ, a.dy_stride);
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
-  auto issue = [&](uint32_t t, uint32_t parity) __attribute__((always_inline)) {
-    const uint32_t st = lds0 + parity * kStage;
-    auto rows = [&](const uint16_t* m, uint64_t stride, uint32_t c0, uint32_t cols, uint32_t row_bytes, uint32_t v,
-                    uint32_t at) __attribute__((always_inline)) {
-      const uint16_t* base = m + (uint64_t)t * stride + c0;
-      // tokens t .. min(t1, t + 64) - 1, from column c0
-      const uint32_t n = min(kTokens, t1 - t);
-      const u32x4 r = nklds2::rsrc(base, ((n - 1u) * (uint32_t)stride + (cols - c0)) * 2u);
-      const uint32_t each = 1024u / row_bytes;  // rows per copy
-#pragma unroll
-      for (uint32_t i = 0; i < kTokens / each / 8u; ++i) {
-        const uint32_t row = (i * 8u + wave) * each;
-        nklds2::copy16(at + row * row_bytes, r, v + row * (uint32_t)stride * 2u, 0u);
-      }
-    };
-    rows(a.x, a.x_stride, p0, a.x_cols, kRowP, pv, st);
-    rows(a.dy, a.dy_stride, q0, a.dy_cols, kRowQ, qv, st + kTokens * kRowP);
+  // Copy i of a wave's kCopies for tokens t .. min(t1, t + 64) - 1 (x's, then dy's); from
+  // t1 on it reads nothing and leaves zeros, so that a step's code has no branch.
+  auto issue_part = [&](uint32_t t, uint32_t stage, uint32_t i) __attribute__((always_inline)) {
+    constexpr uint32_t kCopiesP = kTokens * kRowP / 8192u;
+    const bool is_p = i < kCopiesP, live = t < t1;
+    const uint32_t row_bytes = is_p ? kRowP : kRowQ, each = 1024u / row_bytes;  // rows per copy
+    const uint32_t row = ((is_p ? i : i - kCopiesP) * 8u + wave) * each;
+    const uint64_t stride = is_p ? a.x_stride : a.dy_stride;
+    const uint32_t c0 = is_p ? p0 : q0, cols = is_p ? a.x_cols : a.dy_cols;
+    const uint32_t n = min(kTokens, t1 - min(t, t1 - 1u));
+    const u32x4 r = nklds2::rsrc((is_p ? a.x : a.dy) + (uint64_t)t * stride + c0,
+                                 live ? ((n - 1u) * (uint32_t)stride + (cols - c0)) * 2u : 0u);
+    nklds2::copy16(lds0 + stage * kStage + (is_p ? 0u : kTokens * kRowP) + row * row_bytes, r, is_p ? pv : qv,
+                   live ? row * (uint32_t)stride * 2u : 0u);
   };
 
   v4f acc[NP][NQ];
@@ -580,26 +579,39 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
     typedef short v8s __attribute__((ext_vector_type(8)));
     return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  if (t0 < t1) issue(t0, 0u);
-  uint32_t parity = 0u;
-  for (uint32_t t = t0; t < t1; t += kTokens, parity ^= 1u) {
-    nklds2::wait_copies<0>();
+#pragma unroll
+  for (uint32_t i = 0; i + 1u < S; ++i)
+#pragma unroll
+    for (uint32_t k = 0; k < kCopies; ++k) issue_part(t0 + i * kTokens, i, k);
+  uint32_t stage = 0u;
+  for (uint32_t t = t0; t < t1; t += kTokens) {
+    nklds2::wait_copies<(S - 2u) * kCopies>();
     nklds2::barrier();
-    if (t + kTokens < t1) issue(t + kTokens, parity ^ 1u);
-    const uint8_t* px = s_stage + parity * kStage;
+    const uint32_t before = stage == 0u ? S - 1u : stage - 1u;
+    const uint8_t* px = s_stage + stage * kStage;
     const uint8_t* pq = px + kTokens * kRowP;
+    stage = stage + 1u == S ? 0u : stage + 1u;
+    v8bf qo[2][NQ], po[2];
+    po[0] = operand(px, kRowP, wp * NP, 0u);
 #pragma unroll
-    for (uint32_t h = 0; h < 2u; ++h) {
-      v8bf qo[NQ];
+    for (uint32_t j = 0; j < NQ; ++j) qo[0][j] = operand(pq, kRowQ, wq * NQ + j, 0u);
+    // tile i of the first 32 tokens, then of the second
 #pragma unroll
-      for (uint32_t j = 0; j < NQ; ++j) qo[j] = operand(pq, kRowQ, wq * NQ + j, h);
+    for (uint32_t i = 0; i < 2u * NP; ++i) {
+      if (i + 1u < 2u * NP) po[(i + 1u) & 1u] = operand(px, kRowP, wp * NP + (i + 1u) % NP, (i + 1u) / NP);
+      if (i == NP - 1u) {
 #pragma unroll
-      for (uint32_t i = 0; i < NP; ++i) {
-        const v8bf po = operand(px, kRowP, wp * NP + i, h);
-#pragma unroll
-        for (uint32_t j = 0; j < NQ; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(po, qo[j], acc[i][j], 0, 0, 0);
+        for (uint32_t j = 0; j < NQ; ++j) qo[1][j] = operand(pq, kRowQ, wq * NQ + j, 1u);
       }
+#pragma unroll
+      for (uint32_t j = 0; j < NQ; ++j)
+        acc[i % NP][j] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(po[i & 1u], qo[i / NP][j], acc[i % NP][j], 0, 0, 0);
+      // the copies of a later step, spread over this one's products
+#pragma unroll
+      for (uint32_t k = i * kCopies / (2u * NP); k < (i + 1u) * kCopies / (2u * NP); ++k)
+        issue_part(t + (S - 1u) * kTokens, before, k);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   float* dst = a.splits > 1u ? a.partial + (size_t)split * a.n * a.k : a.dw;
@@ -777,13 +789,13 @@ NETRA_PRODUCT_STREAM(1, 4)
 NETRA_PRODUCT_STREAM(2, 4)
 
 extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_256x256_gfx950(nklin::Outer a) {
-  nklin::outer_tile<2, 4, 8, 4>(a);
+  nklin::outer_tile<2, 4, 8, 4, 2>(a);
 }
 extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_128x256_gfx950(nklin::Outer a) {
-  nklin::outer_tile<2, 4, 4, 4>(a);
+  nklin::outer_tile<2, 4, 4, 4, 3>(a);
 }
-extern "C" __global__ __launch_bounds__(512, 4) void netra_linear_outer_128x128_gfx950(nklin::Outer a) {
-  nklin::outer_tile<2, 4, 4, 2>(a);
+extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_128x128_gfx950(nklin::Outer a) {
+  nklin::outer_tile<2, 4, 4, 2, 4>(a);
 }
 extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_sum_gfx950(nklin::Outer a) { nklin::outer_sum(a); }
 

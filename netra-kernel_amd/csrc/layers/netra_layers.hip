@@ -173,10 +173,10 @@ const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, ui
 }
 
 // Tile and split of the weight gradient, chosen as product_tiles' (steps of 64 tokens: 256x256
-// 1.65 us, 128x256 1.0, 128x128 0.63 alone on a CU, 1.13 where two share it). As whole calls,
-// best and next: T 333, N 1024, K 2048 128x128 8.5 us, 128x256 12.0; T 4096, N 4096, K 2048
-// 128x256 69, 128x128 76; T 4096, N 1024, K 1024 128x128 in four splits 22.3, in two 27.8; T 8192,
-// N 4096, K 4096 256x256 229, 128x256 276.
+// 1.55 us, 128x256 0.93, 128x128 0.48, one workgroup per CU each). As whole calls, best and
+// next: T 333, N 1024, K 2048 128x128 8.3 us, 128x256 11.8; T 4096, N 4096, K 2048 128x256 64,
+// 128x128 82; T 4096, N 1024, K 1024 128x128 in four splits 21.3, in two 23.9; T 8192, N 4096,
+// K 4096 256x256 231, 128x256 249.
 struct OuterPlan {
   uint32_t p, q;  // columns of x and of dy per workgroup
   uint32_t splits, split_rows;
@@ -186,7 +186,7 @@ OuterPlan outer_plan(uint32_t rows, uint32_t n, uint32_t k) {
     uint32_t p, q;
     double step_us;
   };
-  static const Shape shapes[] = {{256, 256, 1.65}, {128, 256, 1.0}, {128, 128, 0.63}};
+  static const Shape shapes[] = {{256, 256, 1.55}, {128, 256, 0.93}, {128, 128, 0.48}};
   const uint32_t steps = (rows + 63u) / 64u;
   OuterPlan best{256, 256, 1, up(rows, 64u)};
   double best_us = 1e30;
@@ -195,10 +195,7 @@ OuterPlan outer_plan(uint32_t rows, uint32_t n, uint32_t k) {
     for (uint32_t splits = 1; splits <= 16u && splits <= (steps + 3u) / 4u; splits *= 2u) {
       if (splits > 1u && tiles * splits > 512u) break;
       const uint32_t each = (steps + splits - 1u) / splits, count = (steps + each - 1u) / each;
-      const uint64_t items = tiles * count;
-      const double rounds = s.p + s.q == 256u && items > 256u ? (items + 511u) / 512u * 1.8
-                                                              : static_cast<double>((items + 255u) / 256u);
-      double us = rounds * each * s.step_us;
+      double us = static_cast<double>((tiles * count + 255u) / 256u) * each * s.step_us;
       if (count > 1u) us += 3.0 + static_cast<double>(n) * k * 4.0 * (2.0 * count + 1.0) / 6e6;  // 6 TB/s
       if (us < best_us) {
         best_us = us;
