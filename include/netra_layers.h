@@ -59,8 +59,8 @@ int netra_linear_pack(const uint8_t* w, uint8_t* packed, uint32_t n, uint32_t k,
 // Bytes of workspace (16-byte aligned) one call needs. in_place: both operands of
 // the weight gradient are bf16 with n, k and the strides even and 4-byte aligned
 // bases; others are first copied to the workspace as aligned bf16.
-uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k);
-uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k);
+uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t x_type);
+uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t dy_type);
 uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t in_place);
 
 // x [rows, k] -> y bf16 [rows, n]; packed from netra_linear_pack(transpose = 0).

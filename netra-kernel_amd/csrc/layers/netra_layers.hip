@@ -108,7 +108,7 @@ ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
   return best;
 }
 
-ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc) {
+ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc, uint32_t in_type) {
   if (rows > 64u) return product_tiles(rows, ni, nc);
   // Quantising on the way saves a launch (10.7 us -> 6.7 at one row) and costs every
   // workgroup the quantisation of its waves' blocks: 16-row tiles x blocks per wave x
@@ -118,11 +118,11 @@ ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc) {
   const uint32_t pt = (ni + 15u) / 16u, q = (rows + 15u) / 16u;
   const uint32_t groups = pt >= 512u ? (pt + 1u) / 2u : pt;
   const uint64_t cost = static_cast<uint64_t>((groups + 255u) / 256u) * q * ((blocks(nc) + 7u) / 8u);
-  return {q == 1u || cost < 8u ? kFused : kStream, 0, 0, 1, 0};
+  return {q == 1u || (cost < 8u && (q == 2u || in_type == NETRA_BF16)) ? kFused : kStream, 0, 0, 1, 0};
 }
-uint64_t product_workspace(uint32_t rows, uint32_t ni, uint32_t nc) {
+uint64_t product_workspace(uint32_t rows, uint32_t ni, uint32_t nc, uint32_t in_type) {
   if (rows == 0) return 0;
-  const ProductPlan plan = product_plan(rows, ni, nc);
+  const ProductPlan plan = product_plan(rows, ni, nc, in_type);
   if (plan.form == kFused) return 0;
   const uint64_t partial = plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * rows * up(ni, 4u) : 0u;
   return (matrix_bytes(rows, nc) + 15u) / 16u * 16u + partial;
@@ -140,8 +140,9 @@ void product_fused(const nklin::Product& a, const X* x, uint64_t stride, uint32_
       netra_linear_product_fused_bf16_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);         \
     else netra_linear_product_fused_f32_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);       \
   } while (0)
-  if (q > 2u) NETRA_RUN(1, 4);
-  else if (q == 2u && wide) NETRA_RUN(2, 2);
+  if (q > 2u) {
+    if constexpr (sizeof(X) == 2) netra_linear_product_fused_bf16_p1q4_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);
+  } else if (q == 2u && wide) NETRA_RUN(2, 2);
   else if (q == 2u) NETRA_RUN(1, 2);
   else if (wide) NETRA_RUN(2, 1);
   else NETRA_RUN(1, 1);
@@ -227,11 +228,11 @@ extern "C" int netra_linear_pack(const uint8_t* w, uint8_t* packed, uint32_t n, 
   return launched("netra_linear_pack");
 }
 
-extern "C" uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
-  return product_workspace(rows, n, k);
+extern "C" uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t x_type) {
+  return product_workspace(rows, n, k, x_type);
 }
-extern "C" uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k) {
-  return product_workspace(rows, k, n);
+extern "C" uint64_t netra_linear_input_gradient_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t dy_type) {
+  return product_workspace(rows, k, n, dy_type);
 }
 static uint64_t partial_bytes(const OuterPlan& plan, uint32_t n, uint32_t k) {
   return plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * n * k : 0;
@@ -255,9 +256,9 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   if (bad_matrix(in, in_type, in_stride, nc) || bad_matrix(out, NETRA_BF16, out_stride, ni) || !packed ||
       !aligned(packed, 16) || !scale || !aligned(scale, 4))
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
-  if (bad_workspace(workspace, workspace_bytes, product_workspace(rows, ni, nc)))
+  if (bad_workspace(workspace, workspace_bytes, product_workspace(rows, ni, nc, in_type)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  const ProductPlan plan = product_plan(rows, ni, nc);
+  const ProductPlan plan = product_plan(rows, ni, nc, in_type);
   nklin::Product a{};
   a.p = packed;
   a.sp = scale;
@@ -375,14 +376,15 @@ static bool bad_router(uint32_t tokens, uint32_t slots, uint32_t experts) {
 }
 
 // Counting is shared out over workgroups of 256 threads where one would take longer
-// than a second launch; each counts `each` tokens.
+// than a second launch; each counts `each` tokens, one a thread up to `most` workgroups (the loss
+// kernel's workgroups all add up all parts).
 struct CountPlan {
   uint32_t groups, each;
 };
-static CountPlan count_plan(uint32_t tokens, uint32_t few) {
+static CountPlan count_plan(uint32_t tokens, uint32_t few, uint32_t most) {
   if (tokens <= few) return {0, tokens};
   const uint32_t groups = (tokens - 1u) / 256u + 1u;
-  CountPlan plan{groups > 64u ? 64u : groups, 0};
+  CountPlan plan{groups > most ? most : groups, 0};
   plan.each = (tokens + plan.groups - 1u) / plan.groups;
   return plan;
 }
@@ -395,7 +397,7 @@ static uint64_t parts_bytes(const CountPlan& plan, uint32_t experts) {
 }
 
 extern "C" uint64_t netra_router_counts_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
-  return parts_bytes(count_plan(tokens, kFewCounts), experts);
+  return parts_bytes(count_plan(tokens, kFewCounts, 256u), experts);
 }
 
 extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, const uint8_t* mask, uint32_t tokens,
@@ -408,7 +410,7 @@ extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, cons
     return fail(-1, name, "null or misaligned pointer, or ids' row stride below the slots");
   if (bad_workspace(workspace, workspace_bytes, netra_router_counts_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  const CountPlan plan = count_plan(tokens, kFewCounts);
+  const CountPlan plan = count_plan(tokens, kFewCounts, 256u);
   if (plan.groups == 0) {
     netra_router_counts_gfx950<<<dim3(1), dim3(1024), 0, stream>>>(ids, ids_stride, mask, tokens, slots, experts,
                                                                    counts, accumulate ? 1u : 0u);
@@ -423,7 +425,7 @@ extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, cons
 }
 
 extern "C" uint64_t netra_router_balance_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
-  const CountPlan plan = count_plan(tokens, kFewBalance);
+  const CountPlan plan = count_plan(tokens, kFewBalance, 64u);
   return plan.groups ? 16u + 4u * kBalanceGrid + parts_bytes(plan, experts) : 0;
 }
 
@@ -444,7 +446,7 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     return fail(-1, name, "null or misaligned pointer, or row stride below the row");
   if (bad_workspace(workspace, workspace_bytes, netra_router_balance_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  const CountPlan plan = count_plan(tokens, kFewBalance);
+  const CountPlan plan = count_plan(tokens, kFewBalance, 64u);
   nkbal::Balance a{};
   a.z = logits;
   a.z_stride = logits_stride;

@@ -15,7 +15,7 @@ constexpr uint32_t kMaxExperts = 1024;
 
 // Routes of tokens [t0, t1) per expert, and the number of those tokens, into LDS
 // words hist[0 .. E) and hist[E] (cleared here). A thread takes whole tokens and
-// loads eight of a token's ids at a time.
+// loads sixteen of a token's ids at a time (past the slots the last one again).
 __device__ __forceinline__ void histogram(const int32_t* __restrict__ ids, uint64_t stride,
                                           const uint8_t* __restrict__ mask, uint32_t t0, uint32_t t1, uint32_t slots,
                                           uint32_t E, uint32_t* hist) {
@@ -26,12 +26,12 @@ __device__ __forceinline__ void histogram(const int32_t* __restrict__ ids, uint6
     if (mask && !mask[t]) continue;
     ++mine;
     const int32_t* row = ids + (uint64_t)t * stride;
-    for (uint32_t s = 0; s < slots; s += 8u) {
-      uint32_t e[8];
+    for (uint32_t s = 0; s < slots; s += 16u) {
+      uint32_t e[16];
 #pragma unroll
-      for (uint32_t j = 0; j < 8u; ++j) e[j] = (uint32_t)row[min(s + j, slots - 1u)];
+      for (uint32_t j = 0; j < 16u; ++j) e[j] = (uint32_t)row[min(s + j, slots - 1u)];
 #pragma unroll
-      for (uint32_t j = 0; j < 8u; ++j)
+      for (uint32_t j = 0; j < 16u; ++j)
         if (s + j < slots && e[j] < E) atomicAdd(&hist[e[j]], 1u);
     }
   }
@@ -64,6 +64,18 @@ __device__ __forceinline__ float wave_reduce(float v) {
   v = join(__uint_as_float((uint32_t)r16[0]), __uint_as_float((uint32_t)r16[1]));
   const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return join(__uint_as_float((uint32_t)r32[0]), __uint_as_float((uint32_t)r32[1]));
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+#define NETRA_DPP(CTRL) (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false)
+  v += NETRA_DPP(0xB1);
+  v += NETRA_DPP(0x4E);
+  v += NETRA_DPP(0x141);
+  v += NETRA_DPP(0x140);
+#undef NETRA_DPP
+  const auto r16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = (uint32_t)r16[0] + (uint32_t)r16[1];
+  const auto r32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (uint32_t)r32[0] + (uint32_t)r32[1];
 }
 __device__ __forceinline__ float wave_sum(float v) { return wave_reduce<false>(v); }
 __device__ __forceinline__ float wave_max(float v) { return wave_reduce<true>(v); }
@@ -190,17 +202,28 @@ __device__ __forceinline__ void balance(const Balance& a) {
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6;
   const uint32_t E = a.experts;
+  // the wave's first row is on its way while the counts are made
+  const uint32_t step = gridDim.x * waves, first = blockIdx.x * waves + wave;
+  float next[NV];
+  uint32_t live = 1u;
+  if (a.tokens) {
+    const uint32_t t = min(first, a.tokens - 1u);
+    if (a.mask) live = a.mask[t];
+    load_row<X, NV, W>(row_rsrc<X>(a.z, a.z_stride, t, E), E, next);
+  }
   if (a.parts) {
-    for (uint32_t e = threadIdx.x; e <= E; e += blockDim.x) {
-      uint32_t c = 0u;
-      for (uint32_t k = 0; k < a.groups; k += 16u) {  // 16 loads in flight
-        uint32_t v[16];
+    for (uint32_t e = threadIdx.x; e <= E; e += blockDim.x) s_count[e] = 0u;
+    __syncthreads();
+    // an expert's parts by as many threads as have 16 each, their loads in flight together
+    const uint32_t threads = (a.groups + 15u) / 16u;
+    for (uint32_t i = threadIdx.x; i < threads * (E + 1u); i += blockDim.x) {
+      const uint32_t e = i % (E + 1u), k = i / (E + 1u) * 16u;
+      uint32_t v[16], c = 0u;
 #pragma unroll
-        for (uint32_t i = 0; i < 16u; ++i) v[i] = k + i < a.groups ? a.parts[(size_t)(k + i) * (E + 1u) + e] : 0u;
+      for (uint32_t j = 0; j < 16u; ++j) v[j] = a.parts[(size_t)min(k + j, a.groups - 1u) * (E + 1u) + e];
 #pragma unroll
-        for (uint32_t i = 0; i < 16u; ++i) c += v[i];
-      }
-      s_count[e] = c;
+      for (uint32_t j = 0; j < 16u; ++j) c += k + j < a.groups ? v[j] : 0u;
+      if (c) atomicAdd(&s_count[e], c);
     }
     __syncthreads();
   } else {
@@ -222,19 +245,14 @@ __device__ __forceinline__ void balance(const Balance& a) {
     f[j] = (float)c;
     bias[j] = a.bias && e < E ? a.bias[e] : 0.0f;
   }
-#pragma unroll
-  for (uint32_t o = 1; o < 64u; o <<= 1) total += (uint32_t)__shfl_xor((int)total, o);
+  total = wave_total(total);
   const float per = total ? (float)E / (float)total : 0.0f;
 #pragma unroll
   for (uint32_t j = 0; j < NV; ++j) f[j] *= per;
   const uint32_t valid = s_count[E];
   const float scale = valid ? a.coefficient / (float)valid : 0.0f;
   float mine = 0.0f;
-  const uint32_t step = gridDim.x * waves, first = blockIdx.x * waves + wave;
   if (first < a.tokens) {
-    float next[NV];
-    uint32_t live = a.mask ? a.mask[first] : 1u;
-    load_row<X, NV, W>(row_rsrc<X>(a.z, a.z_stride, first, E), E, next);
     for (uint32_t t = first; t < a.tokens; t += step) {
       const uint32_t now = live, ahead = min(t + step, a.tokens - 1u);
       float v[NV];
@@ -311,8 +329,13 @@ extern "C" __global__ __launch_bounds__(256) void netra_router_count_sum_gfx950(
   __shared__ uint32_t s[16][17];
   const uint32_t k = threadIdx.x >> 4, i = threadIdx.x & 15u, e = blockIdx.x * 16u + i;
   uint32_t c = 0u;
-  if (e < E)
-    for (uint32_t g = k; g < groups; g += 16u) c += parts[(size_t)g * (E + 1u) + e];
+  if (e < E) {
+    uint32_t v[16];  // groups <= 256
+#pragma unroll
+    for (uint32_t j = 0; j < 16u; ++j) v[j] = parts[(size_t)min(k + 16u * j, groups - 1u) * (E + 1u) + e];
+#pragma unroll
+    for (uint32_t j = 0; j < 16u; ++j) c += k + 16u * j < groups ? v[j] : 0u;
+  }
   s[k][i] = c;
   __syncthreads();
   if (k != 0u || e >= E) return;

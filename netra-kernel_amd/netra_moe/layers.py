@@ -14,8 +14,8 @@ P, U32, U64, F32 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_f
 SIGNATURES = {
     "netra_linear_packed_bytes": (U64, [U32] * 3),
     "netra_linear_pack": (ctypes.c_int, [P, P, U32, U32, U32, P]),
-    "netra_linear_forward_workspace": (U64, [U32] * 3),
-    "netra_linear_input_gradient_workspace": (U64, [U32] * 3),
+    "netra_linear_forward_workspace": (U64, [U32] * 4),
+    "netra_linear_input_gradient_workspace": (U64, [U32] * 4),
     "netra_linear_weight_gradient_workspace": (U64, [U32] * 4),
     "netra_linear_forward": (ctypes.c_int, [P, U32, U64, P, P, P, U64, U32, U32, U32, P, U64, P]),
     "netra_linear_input_gradient": (ctypes.c_int, [P, U32, U64, P, P, P, U64, U32, U32, U32, P, U64, P]),

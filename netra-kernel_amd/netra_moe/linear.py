@@ -96,9 +96,10 @@ class BlockLinear:
         else:
             out_stride = check_rows("out", out, (rows, out_cols), self.device, (torch.bfloat16,))
         fn, need = self._entries[which]
-        need = need(rows, self.N, self.K)
+        kind = TYPES[x.dtype]
+        need = need(rows, self.N, self.K, kind)
         ws, ws_ptr = workspace(need, self.device)
-        launch(fn, which, self.device, x.data_ptr(), TYPES[x.dtype], x_stride, packed.data_ptr(), self._scale_ptr,
+        launch(fn, which, self.device, x.data_ptr(), kind, x_stride, packed.data_ptr(), self._scale_ptr,
                out.data_ptr(), out_stride, rows, self.N, self.K, ws_ptr, need)
         return out
 

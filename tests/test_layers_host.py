@@ -48,7 +48,7 @@ def test_product_refusals(name, change):
     back = name != "netra_linear_forward"
     if back:
         a.update(n=256, k=128)
-    need = getattr(lib, name + "_workspace")(a["rows"], a["n"], a["k"])
+    need = getattr(lib, name + "_workspace")(a["rows"], a["n"], a["k"], a["xt"])
     a["wb"] = need
     a.update(change)
     if a["wb"] == -1:
