@@ -333,6 +333,7 @@ __device__ __forceinline__ void product_tile(const Product& a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  nklds2::wait_copies<0>();
 
   const uint32_t c = lane & 15u, r4 = (lane >> 4) * 4u;
   const uint32_t col0 = (p0 + wp * NP) * 16u, row0 = (q0 + wq * NQ) * 16u;
@@ -350,7 +351,6 @@ __device__ __forceinline__ void product_tile(const Product& a) {
   }
   // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
   // whole lines. (A wave reads back only what it wrote itself.)
-  nklds2::wait_copies<0>();
   __syncthreads();
   uint8_t* mine = s_stage + wave * 16u * NQ * L::kPitch;
 #pragma unroll
@@ -633,6 +633,7 @@ __device__ __forceinline__ void outer_tile(const Outer& a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  nklds2::wait_copies<0>();
   float* dst = a.splits > 1u ? a.partial + (size_t)split * a.n * a.k : a.dw;
   const bool add = a.accumulate && a.splits == 1u;
 #pragma unroll

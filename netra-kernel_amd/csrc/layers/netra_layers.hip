@@ -53,6 +53,21 @@ bool bad_matrix(const void* p, uint32_t type, uint64_t stride, uint32_t cols) {
   return !p || bad_type(type) || stride < cols || !aligned(p, elem(type));
 }
 
+// Whether an output shares memory with an input: their byte ranges meet and they are
+// not different columns of rows with one stride.
+struct Span {
+  const void* p;
+  uint64_t stride, row, rows;  // bytes, bytes, count
+};
+bool share(const Span& a, const Span& b) {
+  if (a.rows == 0 || b.rows == 0) return false;
+  const uint64_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+  if (pa + (a.rows - 1u) * a.stride + a.row <= pb || pb + (b.rows - 1u) * b.stride + b.row <= pa) return false;
+  if (a.stride != b.stride) return true;
+  const uint64_t d = pb >= pa ? (pb - pa) % a.stride : (a.stride - (pa - pb) % a.stride) % a.stride;
+  return d < a.row || d + b.row > a.stride;
+}
+
 void quant_rows(const void* x, uint32_t type, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n,
                 hipStream_t stream) {
   const dim3 grid((rows + 15u) / 16u, (blocks(n) + 3u) / 4u), block(256);
@@ -256,6 +271,9 @@ static int times_weights(const char* name, const void* in, uint32_t in_type, uin
   if (bad_matrix(in, in_type, in_stride, nc) || bad_matrix(out, NETRA_BF16, out_stride, ni) || !packed ||
       !aligned(packed, 16) || !scale || !aligned(scale, 4))
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
+  if (share({in, in_stride * elem(in_type), static_cast<uint64_t>(nc) * elem(in_type), rows},
+            {out, out_stride * 2u, static_cast<uint64_t>(ni) * 2u, rows}))
+    return fail(-1, name, "the output shares memory with the input");
   if (bad_workspace(workspace, workspace_bytes, product_workspace(rows, ni, nc, in_type)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
   const ProductPlan plan = product_plan(rows, ni, nc, in_type);
@@ -334,6 +352,11 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
   }
   if (bad_matrix(dy, dy_type, dy_stride, n) || bad_matrix(x, x_type, x_stride, k))
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
+  const uint64_t dw_bytes = static_cast<uint64_t>(n) * k * 4u;
+  const Span out{dw, dw_bytes, dw_bytes, 1};
+  if (share({dy, dy_stride * elem(dy_type), static_cast<uint64_t>(n) * elem(dy_type), rows}, out) ||
+      share({x, x_stride * elem(x_type), static_cast<uint64_t>(k) * elem(x_type), rows}, out))
+    return fail(-1, name, "dw shares memory with an input");
   const OuterPlan plan = outer_plan(rows, n, k);
   if (bad_workspace(workspace, workspace_bytes,
                     outer_bytes(dy, dy_type, dy_stride, rows, n) + outer_bytes(x, x_type, x_stride, rows, k) +
@@ -444,6 +467,10 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
                  (slots && (!ids || !aligned(ids, 4) || ids_stride < slots)) ||
                  (grad && bad_matrix(grad, logits_type, grad_stride, experts))))
     return fail(-1, name, "null or misaligned pointer, or row stride below the row");
+  const uint64_t row = static_cast<uint64_t>(experts) * elem(logits_type);
+  if (grad && share({logits, logits_stride * elem(logits_type), row, tokens},
+                    {grad, grad_stride * elem(logits_type), row, tokens}))
+    return fail(-1, name, "grad shares memory with logits");
   if (bad_workspace(workspace, workspace_bytes, netra_router_balance_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
   const CountPlan plan = count_plan(tokens, kFewBalance, 64u);

@@ -253,3 +253,18 @@ def test_refusals():
         BlockLinear(q.to(DEV), s.t().contiguous().to(DEV))
     with pytest.raises(ValueError):
         BlockLinear(q, s)
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused():
+    lin, w = layer(128, 128, seed=30, gradients=True)
+    buf = torch.zeros(40, 300, dtype=BF16, device=DEV)
+    x = C.activations(40, 128, seed=31)
+    buf[:, :128] = x.to(DEV)
+    for out in (buf[:, :128], buf[:, 127:255]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            lin.forward(buf[:, :128], out)
+    lin.forward(buf[:, :128], buf[:, 128:256])  # other columns of the same rows
+    C.assert_within(buf[:, 128:256], *C.product(C.quantised(x, 1), w))
+    dw = torch.zeros(128, 128, device=DEV)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        lin.weight_gradient(dw[:40], x.to(DEV), dw)

@@ -12,7 +12,8 @@ from netra_moe import layers, paths
 
 pytestmark = pytest.mark.skipif(not paths.layers_library().is_file(), reason="library not built")
 
-A = 0x100000  # an aligned address that is never followed
+A = 0x100000000000  # aligned addresses, far apart, that are never followed
+B, D = 2 * A, 3 * A
 
 
 def refused(name, *args):
@@ -39,12 +40,12 @@ def test_packed_bytes():
 
 @pytest.mark.parametrize("change", [
     dict(x=0), dict(x=A + 1), dict(xt=2), dict(xs=255), dict(packed=0), dict(packed=A + 8), dict(scale=0),
-    dict(scale=A + 2), dict(y=0), dict(y=A + 1), dict(ys=127), dict(n=0), dict(k=0), dict(rows=(1 << 21) + 1),
+    dict(scale=A + 2), dict(y=0), dict(y=B + 1), dict(ys=127), dict(y=A + 256), dict(y=A + 512 * 299 + 510), dict(y=A - 2), dict(n=0), dict(k=0), dict(rows=(1 << 21) + 1),
     dict(n=(1 << 21) + 1), dict(ws=0), dict(ws=A + 4), dict(wb=0), dict(wb=-1)])
 @pytest.mark.parametrize("name", ["netra_linear_forward", "netra_linear_input_gradient"])
 def test_product_refusals(name, change):
     lib = layers.library()
-    a = dict(x=A, xt=0, xs=256, packed=A, scale=A, y=A, ys=128, rows=300, n=128, k=256, ws=A)
+    a = dict(x=A, xt=0, xs=256, packed=A, scale=A, y=B, ys=128, rows=300, n=128, k=256, ws=A)
     back = name != "netra_linear_forward"
     if back:
         a.update(n=256, k=128)
@@ -58,12 +59,12 @@ def test_product_refusals(name, change):
 
 
 @pytest.mark.parametrize("change", [dict(g=0), dict(gt=2), dict(gs=127), dict(x=0), dict(x=A + 1), dict(xt=9), dict(xs=255),
-                                    dict(dw=0), dict(dw=A + 2), dict(n=0), dict(k=0), dict(rows=(1 << 21) + 1),
+                                    dict(dw=0), dict(dw=D + 2), dict(dw=A), dict(dw=B - 4), dict(dw=B + 300 * 1024 - 4), dict(n=0), dict(k=0), dict(rows=(1 << 21) + 1),
                                     dict(ws=0), dict(ws=A + 8), dict(short=1)])
 def test_weight_gradient_refusals(change):
     lib = layers.library()
     # (fp32: both operands go through the workspace)
-    a = dict(g=A, gt=1, gs=128, x=A, xt=1, xs=256, dw=A, rows=300, n=128, k=256, ws=A, short=0)
+    a = dict(g=A, gt=1, gs=128, x=B, xt=1, xs=256, dw=D, rows=300, n=128, k=256, ws=A, short=0)
     need = lib.netra_linear_weight_gradient_workspace(300, 128, 256, 0)
     a.update(change)
     refused("netra_linear_weight_gradient", a["g"], a["gt"], a["gs"], a["x"], a["xt"], a["xs"], a["dw"], 0, a["rows"],
@@ -94,10 +95,10 @@ def test_counts_refusals(change):
 
 @pytest.mark.parametrize("change", [dict(z=0), dict(z=A + 1), dict(zt=2), dict(zs=15), dict(bias=A + 1), dict(ids=0),
                                     dict(ids=A + 2), dict(st=1), dict(E=0), dict(E=1025), dict(T=1 << 31),
-                                    dict(counts=0), dict(counts=A + 2), dict(loss=0), dict(loss=A + 1), dict(g=A + 1),
+                                    dict(counts=0), dict(counts=A + 2), dict(loss=0), dict(loss=A + 1), dict(g=B + 1), dict(g=A), dict(g=A + 2), dict(zs=40, gs=40, g=A + 24),
                                     dict(gs=15), dict(ws=0), dict(ws=A + 4), dict(short=1)])
 def test_balance_refusals(change):
-    a = dict(z=A, zt=0, zs=16, bias=None, ids=A, st=2, T=4000, slots=2, E=16, counts=A, loss=A, g=A, gs=16, ws=A, short=0)
+    a = dict(z=A, zt=0, zs=16, bias=None, ids=A, st=2, T=4000, slots=2, E=16, counts=A, loss=A, g=B, gs=16, ws=A, short=0)
     a.update(change)
     need = layers.library().netra_router_balance_workspace(4000, 2, 16)
     refused("netra_router_balance", a["z"], a["zt"], a["zs"], a["bias"], a["ids"], a["st"], a["slots"], None, a["T"],
