@@ -82,6 +82,13 @@ int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, uint64_t dy_s
                                  uint32_t rows, uint32_t n, uint32_t k, void* workspace,
                                  uint64_t workspace_bytes, hipStream_t stream);
 
+// Both gradients in one call (dx and dw must not share memory either).
+uint64_t netra_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t dy_type, uint32_t in_place);
+int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* x, uint32_t x_type,
+                          uint64_t x_stride, const uint8_t* packed_t, const float* scale, uint16_t* dx,
+                          uint64_t dx_stride, float* dw, uint32_t accumulate, uint32_t rows, uint32_t n, uint32_t k,
+                          void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+
 // counts[e] = number of routes (t, s) with ids[t, s] == e over the tokens whose
 // mask byte is nonzero (mask null: all). ids is i32 [tokens, slots] with a row
 // stride in elements; ids outside 0 .. experts - 1 (the shared expert's slot,

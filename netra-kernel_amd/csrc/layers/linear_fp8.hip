@@ -225,9 +225,8 @@ struct Tile {
 };
 
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
-__device__ __forceinline__ void product_tile(const Product& a) {
+__device__ __forceinline__ void product_tile(const Product& a, uint32_t group, uint8_t* s_stage) {
   using L = Tile<WP, WQ, NP, NQ, S>;
-  __shared__ __align__(16) uint8_t s_stage[L::kLds];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u;
@@ -236,8 +235,8 @@ __device__ __forceinline__ void product_tile(const Product& a) {
   // tiles, in bands of 4 along Q, so that they share operands in its L2 (T 4096, N 4096,
   // K 2048: 43.4 us, in bands of 8 45.0, of 16 45.9).
   const uint32_t total = np * nq * a.splits, per = (total + 7u) / 8u;
-  const uint32_t item = (blockIdx.x % 8u) * per + blockIdx.x / 8u;
-  if (blockIdx.x / 8u >= per || item >= total) return;
+  const uint32_t item = (group % 8u) * per + group / 8u;
+  if (group / 8u >= per || item >= total) return;
   const uint32_t split = item / (np * nq), tile = item - split * np * nq;
   const uint32_t band = tile / (4u * np), in_band = tile - band * 4u * np;
   const uint32_t height = min(4u, nq - band * 4u);
@@ -533,21 +532,24 @@ struct Outer {
 // matrix read the next row and make outputs that are not stored; tokens past the
 // end read zeros.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
-__device__ __forceinline__ void outer_tile(const Outer& a) {
+constexpr uint32_t outer_lds() {
+  return S * 64u * 32u * (WP * NP + WQ * NQ);
+}
+template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
+__device__ __forceinline__ void outer_tile(const Outer& a, uint32_t group, uint8_t* s_stage) {
   constexpr uint32_t kP = WP * NP, kQ = WQ * NQ, kTokens = 64u;
   constexpr uint32_t kRowP = kP * 32u, kRowQ = kQ * 32u;  // bytes of a token's row
   constexpr uint32_t kStage = kTokens * (kRowP + kRowQ);
   constexpr uint32_t kCopies = kStage / 8192u;            // a wave's, per step
   static_assert(WP * WQ == 8u && (kRowP == 256u || kRowP == 512u) && (kRowQ == 256u || kRowQ == 512u) &&
-                    S * kStage <= 160u * 1024u,
+                    S * kStage == outer_lds<WP, WQ, NP, NQ, S>() && S * kStage <= 160u * 1024u,
                 "copies, swizzle and LDS");
-  __shared__ __align__(16) uint8_t s_stage[S * kStage];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t np = (a.k + 16u * kP - 1u) / (16u * kP), nq = (a.n + 16u * kQ - 1u) / (16u * kQ);
   const uint32_t total = np * nq * a.splits, per = (total + 7u) / 8u;
-  const uint32_t item = (blockIdx.x % 8u) * per + blockIdx.x / 8u;
-  if (blockIdx.x / 8u >= per || item >= total) return;
+  const uint32_t item = (group % 8u) * per + group / 8u;
+  if (group / 8u >= per || item >= total) return;
   const uint32_t split = item / (np * nq), tile = item - split * np * nq;
   const uint32_t band = tile / (8u * np), in_band = tile - band * 8u * np;
   const uint32_t height = min(8u, nq - band * 8u);
@@ -777,7 +779,8 @@ extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_f32_gf
 
 #define NETRA_PRODUCT_TILE(P, Q, ...)                                                                             \
   extern "C" __global__ __launch_bounds__(512) void netra_linear_product_##P##x##Q##_gfx950(nklin::Product a) {    \
-    nklin::product_tile<__VA_ARGS__>(a);                                                                          \
+    __shared__ __align__(16) uint8_t lds[nklin::Tile<__VA_ARGS__>::kLds];                                         \
+    nklin::product_tile<__VA_ARGS__>(a, blockIdx.x, lds);                                                         \
   }
 NETRA_PRODUCT_TILE(256, 256, 2, 4, 8, 4, 2)
 NETRA_PRODUCT_TILE(256, 128, 2, 4, 8, 2, 3)
@@ -808,14 +811,23 @@ NETRA_PRODUCT_FUSED(bf16, uint16_t, 1, 4)  // (fp32 rows of four tiles do not fi
 NETRA_PRODUCT_STREAM(1, 4)
 NETRA_PRODUCT_STREAM(2, 4)
 
-extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_256x256_gfx950(nklin::Outer a) {
-  nklin::outer_tile<2, 4, 8, 4, 2>(a);
-}
-extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_128x256_gfx950(nklin::Outer a) {
-  nklin::outer_tile<2, 4, 4, 4, 3>(a);
-}
-extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_128x128_gfx950(nklin::Outer a) {
-  nklin::outer_tile<2, 4, 4, 2, 4>(a);
+#define NETRA_OUTER_TILE(P, Q, ...)                                                                                \
+  extern "C" __global__ __launch_bounds__(512) void netra_linear_outer_##P##x##Q##_gfx950(nklin::Outer a) {        \
+    __shared__ __align__(16) uint8_t lds[nklin::outer_lds<__VA_ARGS__>()];                                         \
+    nklin::outer_tile<__VA_ARGS__>(a, blockIdx.x, lds);                                                           \
+  }
+NETRA_OUTER_TILE(256, 256, 2, 4, 8, 4, 2)
+NETRA_OUTER_TILE(128, 256, 2, 4, 4, 4, 3)
+NETRA_OUTER_TILE(128, 128, 2, 4, 4, 2, 4)
+// Both products of a small backward pass in one launch, the weight gradient's
+// workgroups (the first `outer`, a multiple of 8) with their longer way first: neither
+// fills the chip, and a launch is saved.
+extern "C" __global__ __launch_bounds__(512) void netra_linear_backward_small_gfx950(nklin::Product a, nklin::Outer b,
+                                                                                     uint32_t outer) {
+  constexpr uint32_t kP = nklin::Tile<4, 2, 1, 2, 4>::kLds, kO = nklin::outer_lds<2, 4, 4, 2, 4>();
+  __shared__ __align__(16) uint8_t lds[kP > kO ? kP : kO];
+  if (blockIdx.x < outer) nklin::outer_tile<2, 4, 4, 2, 4>(b, blockIdx.x, lds);
+  else nklin::product_tile<4, 2, 1, 2, 4>(a, blockIdx.x - outer, lds);
 }
 extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_sum_gfx950(nklin::Outer a) { nklin::outer_sum(a); }
 

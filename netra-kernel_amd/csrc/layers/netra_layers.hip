@@ -88,31 +88,33 @@ struct ProductPlan {
   uint32_t p, q, splits, split_blocks;
 };
 
-// Tiles: time = rounds of workgroups over the 256 CUs x steps x the step's time, which
-// hardly depends on how many CUs work (us a step, 1 to 32 rounds: 256x256 1.95, 256x128
-// 1.18, 128x128 0.78, 128x64 0.58, 64x64 0.56 with two workgroups per CU). Splits add a
-// launch and the partial sums' way out and in. Measured as whole calls, best and next
-// tile: T 333, N 1024, K 2048 64x64 11.6 us, 128x64 14.3; T 1001, N 1500, K 1111 128x64
-// 15.3, 64x64 17.1; T 2048, N 2048, K 2048 128x128 21.2, 256x128 26.7; T 2048, N 4096,
-// K 4096 256x128 46.0, 128x128 56.0; T 4096, N 4096, K 2048 256x256 46.1, 256x128 55.5;
-// T 128, N 8192, K 8192 128x128 in four splits 24.9, in two 32.3, 64x64 in two 26.0.
+// Tiles: time = rounds of workgroups over the 256 CUs x (steps x the step's time + what a
+// workgroup takes besides), the step's time hardly depending on how many CUs work (us a step:
+// 256x256 1.95, 256x128 1.18, 128x128 0.78, 128x64 0.58, 64x64 0.35, or 0.62 where two workgroups
+// share a CU). Splits add a launch and the partial sums' way out and in. Measured as whole calls,
+// best and next: T 333, N 2048, K 1024 128x64 10.8 us, 64x64 10.9, 128x128 12.0; T 700, N 2048, K
+// 2048 128x64 14.4, 64x64 15.8; T 1500, N 1500, K 1500 128x128 18.3, 64x64 20.7; T 1500, N 4096, K
+// 1024 256x128 18.7, 128x128 22.2; T 8192, N 512, K 4096 128x128 41.6, 128x64 51.5; T 3000, N 6000,
+// K 3000 256x128 91, 128x128 96, 256x256 98; T 4096, N 4096, K 2048 256x256 43.4, 256x128 55.5; T
+// 128, N 8192, K 8192 128x128 in four splits 24.9, in two 32.3, 64x64 in two 26.0.
 ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
   struct Shape {
-    uint32_t p, q, at_once;
-    double step_us;
+    uint32_t p, q;
+    double step_us, group_us;
   };
   static const Shape shapes[] = {
-      {256, 256, 256, 1.95}, {256, 128, 256, 1.18}, {128, 128, 256, 0.78}, {128, 64, 256, 0.58}, {64, 64, 512, 0.56}};
+      {256, 256, 1.95, 3.0}, {256, 128, 1.18, 2.0}, {128, 128, 0.78, 1.5}, {128, 64, 0.58, 1.2}, {64, 64, 0.35, 1.0}};
   const uint32_t kb = blocks(nc);
   ProductPlan best{kTiles, 256, 256, 1, kb};
   double best_us = 1e30;
   for (const Shape& s : shapes) {
     const uint64_t tiles = static_cast<uint64_t>((ni + s.p - 1u) / s.p) * ((rows + s.q - 1u) / s.q);
     for (uint32_t splits = 1; splits <= 8u && splits <= (kb + 3u) / 4u; splits *= 2u) {
-      if (splits > 1u && tiles * splits > 2u * s.at_once) break;
+      if (splits > 1u && tiles * splits > 512u) break;
       const uint32_t each = (kb + splits - 1u) / splits, n = (kb + each - 1u) / each;
-      const double rounds = static_cast<double>((tiles * n + s.at_once - 1u) / s.at_once);
-      double us = rounds * each * s.step_us;
+      const bool pairs = s.p * s.q == 64u * 64u && tiles * n > 256u;
+      const double rounds = static_cast<double>(pairs ? (tiles * n + 511u) / 512u : (tiles * n + 255u) / 256u);
+      double us = rounds * (each * (pairs ? 0.62 : s.step_us) + s.group_us);
       if (n > 1u) us += 3.0 + static_cast<double>(rows) * ni * (8.0 * n) / 5e6;  // 5 TB/s
       if (us < best_us) {
         best_us = us;
@@ -258,135 +260,252 @@ extern "C" uint64_t netra_linear_weight_gradient_workspace(uint32_t rows, uint32
          (in_place ? 0 : static_cast<uint64_t>(rows) * (static_cast<uint64_t>(up(n, 8u)) + up(k, 8u)) * 2u);
 }
 
-// in [rows, nc] times the packed matrix P [ni, nc] -> out [rows, ni]
-static int times_weights(const char* name, const void* in, uint32_t in_type, uint64_t in_stride, const uint8_t* packed,
-                         const float* scale, uint32_t sp_i, uint32_t sp_b, uint16_t* out, uint64_t out_stride,
-                         uint32_t rows, uint32_t ni, uint32_t nc, void* workspace,
-                         uint64_t workspace_bytes, hipStream_t stream) {
-  if (bad_sizes(rows, ni, nc)) return fail(-1, name, "sizes have to be 1 .. 2^21 (rows may be 0)");
-  if (rows == 0) {
-    g_error.clear();
-    return 0;
-  }
-  if (bad_matrix(in, in_type, in_stride, nc) || bad_matrix(out, NETRA_BF16, out_stride, ni) || !packed ||
-      !aligned(packed, 16) || !scale || !aligned(scale, 4))
-    return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
-  if (share({in, in_stride * elem(in_type), static_cast<uint64_t>(nc) * elem(in_type), rows},
-            {out, out_stride * 2u, static_cast<uint64_t>(ni) * 2u, rows}))
-    return fail(-1, name, "the output shares memory with the input");
-  if (bad_workspace(workspace, workspace_bytes, product_workspace(rows, ni, nc, in_type)))
-    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  const ProductPlan plan = product_plan(rows, ni, nc, in_type);
-  nklin::Product a{};
-  a.p = packed;
-  a.sp = scale;
-  a.sp_i = sp_i;
-  a.sp_b = sp_b;
-  a.sp_bytes = blocks(ni) * blocks(nc) * 4u;
-  a.out = out;
-  a.ldo = out_stride;
-  a.ni = ni;
-  a.nq = rows;
-  a.kb = blocks(nc);
+// One call of the product: in [rows, nc] times the packed matrix P [ni, nc] -> out [rows, ni].
+struct ProductCall {
+  const char* name;
+  const void* in;
+  uint32_t in_type;
+  uint64_t in_stride;
+  const uint8_t* packed;
+  const float* scale;
+  uint32_t sp_i, sp_b;
+  uint16_t* out;
+  uint64_t out_stride;
+  uint32_t rows, ni, nc;
+};
+
+static int check(const ProductCall& c) {
+  if (bad_matrix(c.in, c.in_type, c.in_stride, c.nc) || bad_matrix(c.out, NETRA_BF16, c.out_stride, c.ni) ||
+      !c.packed || !aligned(c.packed, 16) || !c.scale || !aligned(c.scale, 4))
+    return fail(-1, c.name, "null or misaligned pointer, unknown type, or row stride below the row");
+  if (share({c.in, c.in_stride * elem(c.in_type), static_cast<uint64_t>(c.nc) * elem(c.in_type), c.rows},
+            {c.out, c.out_stride * 2u, static_cast<uint64_t>(c.ni) * 2u, c.rows}))
+    return fail(-1, c.name, "the output shares memory with the input");
+  return 0;
+}
+
+// Everything in front of the tile kernels (which it leaves to the caller: true), or all of the call.
+static bool begin(const ProductCall& c, const ProductPlan& plan, uint8_t* workspace, nklin::Product& a,
+                  hipStream_t stream) {
+  a.p = c.packed;
+  a.sp = c.scale;
+  a.sp_i = c.sp_i;
+  a.sp_b = c.sp_b;
+  a.sp_bytes = blocks(c.ni) * blocks(c.nc) * 4u;
+  a.out = c.out;
+  a.ldo = c.out_stride;
+  a.ni = c.ni;
+  a.nq = c.rows;
+  a.kb = blocks(c.nc);
   a.splits = plan.splits;
   a.split_blocks = plan.split_blocks;
   if (plan.form == kFused) {
-    if (in_type == NETRA_BF16) product_fused(a, static_cast<const uint16_t*>(in), in_stride, nc, stream);
-    else product_fused(a, static_cast<const float*>(in), in_stride, nc, stream);
-    return launched(name);
+    if (c.in_type == NETRA_BF16)
+      product_fused(a, static_cast<const uint16_t*>(c.in), c.in_stride, c.nc, stream);
+    else product_fused(a, static_cast<const float*>(c.in), c.in_stride, c.nc, stream);
+    return false;
   }
-  uint8_t* q = static_cast<uint8_t*>(workspace);
-  float* s = reinterpret_cast<float*>(q + code_bytes(rows, nc));
-  quant_rows(in, in_type, in_stride, q, s, rows, nc, stream);
-  a.q = q;
+  float* s = reinterpret_cast<float*>(workspace + code_bytes(c.rows, c.nc));
+  quant_rows(c.in, c.in_type, c.in_stride, workspace, s, c.rows, c.nc, stream);
+  a.q = workspace;
   a.sq = s;
-  a.sq_b = up(rows, 16u);
+  a.sq_b = up(c.rows, 16u);
   if (plan.form == kStream) {
-    const uint32_t pt = (ni + 15u) / 16u;
+    const uint32_t pt = (c.ni + 15u) / 16u;
     const bool wide = pt >= 512u;  // the activations are read half as often (T 64, N 8192, K 8192: 24.1 us -> 20.3)
     const dim3 grid(wide ? (pt + 1u) / 2u : pt), block(512);
     if (wide) netra_linear_product_stream_p2q4_gfx950<<<grid, block, 0, stream>>>(a);
     else netra_linear_product_stream_p1q4_gfx950<<<grid, block, 0, stream>>>(a);
-    return launched(name);
+    return false;
   }
-  a.partial = reinterpret_cast<float*>(q + (matrix_bytes(rows, nc) + 15u) / 16u * 16u);
-  const uint32_t items = ((ni + plan.p - 1u) / plan.p) * ((rows + plan.q - 1u) / plan.q) * plan.splits;
-  const dim3 grid((items + 7u) / 8u * 8u), block(512);
+  a.partial = reinterpret_cast<float*>(workspace + (matrix_bytes(c.rows, c.nc) + 15u) / 16u * 16u);
+  return true;
+}
+
+static uint32_t groups_of(const nklin::Product& a, const ProductPlan& plan) {
+  const uint32_t items = ((a.ni + plan.p - 1u) / plan.p) * ((a.nq + plan.q - 1u) / plan.q) * plan.splits;
+  return (items + 7u) / 8u * 8u;
+}
+
+static void run_tiles(const nklin::Product& a, const ProductPlan& plan, hipStream_t stream) {
+  const dim3 grid(groups_of(a, plan)), block(512);
   if (plan.p == 256u && plan.q == 256u) netra_linear_product_256x256_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.p == 256u) netra_linear_product_256x128_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.q == 128u) netra_linear_product_128x128_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.p == 128u) netra_linear_product_128x64_gfx950<<<grid, block, 0, stream>>>(a);
   else netra_linear_product_64x64_gfx950<<<grid, block, 0, stream>>>(a);
   if (plan.splits > 1u)
-    netra_linear_product_sum_gfx950<<<dim3((ni + 1023u) / 1024u, rows < 4096u ? rows : 4096u), dim3(256), 0, stream>>>(a);
-  return launched(name);
+    netra_linear_product_sum_gfx950<<<dim3((a.ni + 1023u) / 1024u, a.nq < 4096u ? a.nq : 4096u), dim3(256), 0, stream>>>(
+        a);
+}
+
+static int times_weights(const ProductCall& c, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  if (bad_sizes(c.rows, c.ni, c.nc)) return fail(-1, c.name, "sizes have to be 1 .. 2^21 (rows may be 0)");
+  if (c.rows == 0) {
+    g_error.clear();
+    return 0;
+  }
+  const int rc = check(c);
+  if (rc != 0) return rc;
+  if (bad_workspace(workspace, workspace_bytes, product_workspace(c.rows, c.ni, c.nc, c.in_type)))
+    return fail(-1, c.name, "workspace too small, null or not 16-byte aligned");
+  const ProductPlan plan = product_plan(c.rows, c.ni, c.nc, c.in_type);
+  nklin::Product a{};
+  if (begin(c, plan, static_cast<uint8_t*>(workspace), a, stream)) run_tiles(a, plan, stream);
+  return launched(c.name);
 }
 
 extern "C" int netra_linear_forward(const void* x, uint32_t x_type, uint64_t x_stride, const uint8_t* packed,
                                     const float* scale, uint16_t* y, uint64_t y_stride, uint32_t rows, uint32_t n,
-                                    uint32_t k, void* workspace, uint64_t workspace_bytes,
-                                    hipStream_t stream) {
-  return times_weights("netra_linear_forward", x, x_type, x_stride, packed, scale, blocks(k), 1u, y, y_stride,
-                       rows, n, k, workspace, workspace_bytes, stream);
+                                    uint32_t k, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  return times_weights({"netra_linear_forward", x, x_type, x_stride, packed, scale, blocks(k), 1u, y, y_stride, rows,
+                        n, k},
+                       workspace, workspace_bytes, stream);
 }
 
 extern "C" int netra_linear_input_gradient(const void* dy, uint32_t dy_type, uint64_t dy_stride,
-                                           const uint8_t* packed_t, const float* scale, uint16_t* dx, uint64_t dx_stride,
-                                           uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                                           const uint8_t* packed_t, const float* scale, uint16_t* dx,
+                                           uint64_t dx_stride, uint32_t rows, uint32_t n, uint32_t k, void* workspace,
                                            uint64_t workspace_bytes, hipStream_t stream) {
-  return times_weights("netra_linear_input_gradient", dy, dy_type, dy_stride, packed_t, scale, 1u, blocks(k), dx,
-                       dx_stride, rows, k, n, workspace, workspace_bytes, stream);
+  return times_weights({"netra_linear_input_gradient", dy, dy_type, dy_stride, packed_t, scale, 1u, blocks(k), dx,
+                        dx_stride, rows, k, n},
+                       workspace, workspace_bytes, stream);
+}
+
+// One call of the weight gradient.
+struct OuterCall {
+  const char* name;
+  const void* dy;
+  uint32_t dy_type;
+  uint64_t dy_stride;
+  const void* x;
+  uint32_t x_type;
+  uint64_t x_stride;
+  float* dw;
+  uint32_t accumulate, rows, n, k;
+};
+
+static int check(const OuterCall& c) {
+  if (bad_matrix(c.dy, c.dy_type, c.dy_stride, c.n) || bad_matrix(c.x, c.x_type, c.x_stride, c.k))
+    return fail(-1, c.name, "null or misaligned pointer, unknown type, or row stride below the row");
+  const uint64_t bytes = static_cast<uint64_t>(c.n) * c.k * 4u;
+  const Span out{c.dw, bytes, bytes, 1};
+  if (share({c.dy, c.dy_stride * elem(c.dy_type), static_cast<uint64_t>(c.n) * elem(c.dy_type), c.rows}, out) ||
+      share({c.x, c.x_stride * elem(c.x_type), static_cast<uint64_t>(c.k) * elem(c.x_type), c.rows}, out))
+    return fail(-1, c.name, "dw shares memory with an input");
+  return 0;
+}
+
+static uint64_t outer_workspace(const OuterCall& c, const OuterPlan& plan) {
+  return outer_bytes(c.dy, c.dy_type, c.dy_stride, c.rows, c.n) + outer_bytes(c.x, c.x_type, c.x_stride, c.rows, c.k) +
+         partial_bytes(plan, c.n, c.k);
+}
+
+static void begin(const OuterCall& c, const OuterPlan& plan, uint8_t* workspace, nklin::Outer& a, hipStream_t stream) {
+  a.dy_stride = c.dy_stride;
+  a.dy_cols = c.n;
+  a.dy = outer_operand(c.dy, c.dy_type, a.dy_stride, c.rows, a.dy_cols, workspace, stream);
+  a.x_stride = c.x_stride;
+  a.x_cols = c.k;
+  a.x = outer_operand(c.x, c.x_type, a.x_stride, c.rows, a.x_cols, workspace, stream);
+  a.dw = c.dw;
+  a.rows = c.rows;
+  a.n = c.n;
+  a.k = c.k;
+  a.accumulate = c.accumulate ? 1u : 0u;
+  a.splits = plan.splits;
+  a.split_rows = plan.split_rows;
+  a.partial = reinterpret_cast<float*>(workspace);
+}
+
+static uint32_t groups_of(const nklin::Outer& a, const OuterPlan& plan) {
+  const uint32_t items = ((a.k + plan.p - 1u) / plan.p) * ((a.n + plan.q - 1u) / plan.q) * plan.splits;
+  return (items + 7u) / 8u * 8u;
+}
+
+static void run_tiles(const nklin::Outer& a, const OuterPlan& plan, hipStream_t stream) {
+  const dim3 grid(groups_of(a, plan)), block(512);
+  if (plan.p == 256u) netra_linear_outer_256x256_gfx950<<<grid, block, 0, stream>>>(a);
+  else if (plan.q == 256u) netra_linear_outer_128x256_gfx950<<<grid, block, 0, stream>>>(a);
+  else netra_linear_outer_128x128_gfx950<<<grid, block, 0, stream>>>(a);
+  if (plan.splits > 1u) {
+    const uint64_t quads = (static_cast<uint64_t>(a.n) * a.k + 1023u) / 1024u;
+    netra_linear_outer_sum_gfx950<<<dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), 0, stream>>>(
+        a);
+  }
+}
+
+// Sizes and dw, and the call without tokens: 0 or an error to return, or 1 to go on.
+static int outer_start(const OuterCall& c, hipStream_t stream) {
+  if (bad_sizes(c.rows, c.n, c.k)) return fail(-1, c.name, "sizes have to be 1 .. 2^21 (rows may be 0)");
+  if (!c.dw || !aligned(c.dw, 4)) return fail(-1, c.name, "null or misaligned dw");
+  if (c.rows != 0) return 1;
+  if (!c.accumulate)
+    netra_linear_zero_gfx950<<<dim3(1024), dim3(256), 0, stream>>>(c.dw, static_cast<uint64_t>(c.n) * c.k);
+  return launched(c.name);
 }
 
 extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* x,
                                             uint32_t x_type, uint64_t x_stride, float* dw, uint32_t accumulate,
                                             uint32_t rows, uint32_t n, uint32_t k, void* workspace,
                                             uint64_t workspace_bytes, hipStream_t stream) {
-  const char* name = "netra_linear_weight_gradient";
-  if (bad_sizes(rows, n, k)) return fail(-1, name, "sizes have to be 1 .. 2^21 (rows may be 0)");
-  if (!dw || !aligned(dw, 4)) return fail(-1, name, "null or misaligned dw");
-  if (rows == 0) {
-    if (!accumulate)
-      netra_linear_zero_gfx950<<<dim3(1024), dim3(256), 0, stream>>>(dw, static_cast<uint64_t>(n) * k);
-    return launched(name);
-  }
-  if (bad_matrix(dy, dy_type, dy_stride, n) || bad_matrix(x, x_type, x_stride, k))
-    return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
-  const uint64_t dw_bytes = static_cast<uint64_t>(n) * k * 4u;
-  const Span out{dw, dw_bytes, dw_bytes, 1};
-  if (share({dy, dy_stride * elem(dy_type), static_cast<uint64_t>(n) * elem(dy_type), rows}, out) ||
-      share({x, x_stride * elem(x_type), static_cast<uint64_t>(k) * elem(x_type), rows}, out))
-    return fail(-1, name, "dw shares memory with an input");
+  const OuterCall c{"netra_linear_weight_gradient", dy, dy_type, dy_stride, x, x_type, x_stride, dw, accumulate, rows,
+                    n, k};
+  int rc = outer_start(c, stream);
+  if (rc != 1) return rc;
+  rc = check(c);
+  if (rc != 0) return rc;
   const OuterPlan plan = outer_plan(rows, n, k);
-  if (bad_workspace(workspace, workspace_bytes,
-                    outer_bytes(dy, dy_type, dy_stride, rows, n) + outer_bytes(x, x_type, x_stride, rows, k) +
-                        partial_bytes(plan, n, k)))
-    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  uint8_t* at = static_cast<uint8_t*>(workspace);
+  if (bad_workspace(workspace, workspace_bytes, outer_workspace(c, plan)))
+    return fail(-1, c.name, "workspace too small, null or not 16-byte aligned");
   nklin::Outer a{};
-  a.dy_cols = n;
-  a.x_cols = k;
-  a.dy = outer_operand(dy, dy_type, dy_stride, rows, a.dy_cols, at, stream);
-  a.dy_stride = dy_stride;
-  a.x = outer_operand(x, x_type, x_stride, rows, a.x_cols, at, stream);
-  a.x_stride = x_stride;
-  a.dw = dw;
-  a.rows = rows;
-  a.n = n;
-  a.k = k;
-  a.accumulate = accumulate ? 1u : 0u;
-  a.splits = plan.splits;
-  a.split_rows = plan.split_rows;
-  a.partial = reinterpret_cast<float*>(at);
-  const uint32_t items = ((k + plan.p - 1u) / plan.p) * ((n + plan.q - 1u) / plan.q) * plan.splits;
-  const dim3 grid((items + 7u) / 8u * 8u), block(512);
-  if (plan.p == 256u) netra_linear_outer_256x256_gfx950<<<grid, block, 0, stream>>>(a);
-  else if (plan.q == 256u) netra_linear_outer_128x256_gfx950<<<grid, block, 0, stream>>>(a);
-  else netra_linear_outer_128x128_gfx950<<<grid, block, 0, stream>>>(a);
-  if (plan.splits > 1u) {
-    const uint64_t quads = (static_cast<uint64_t>(n) * k + 1023u) / 1024u;
-    netra_linear_outer_sum_gfx950<<<dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), 0, stream>>>(
-        a);
+  begin(c, plan, static_cast<uint8_t*>(workspace), a, stream);
+  run_tiles(a, plan, stream);
+  return launched(c.name);
+}
+
+extern "C" uint64_t netra_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t dy_type,
+                                                    uint32_t in_place) {
+  return (product_workspace(rows, k, n, dy_type) + 15u) / 16u * 16u +
+         netra_linear_weight_gradient_workspace(rows, n, k, in_place);
+}
+
+extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* x,
+                                     uint32_t x_type, uint64_t x_stride, const uint8_t* packed_t, const float* scale,
+                                     uint16_t* dx, uint64_t dx_stride, float* dw, uint32_t accumulate, uint32_t rows,
+                                     uint32_t n, uint32_t k, void* workspace, uint64_t workspace_bytes,
+                                     hipStream_t stream) {
+  const char* name = "netra_linear_backward";
+  const OuterCall o{name, dy, dy_type, dy_stride, x, x_type, x_stride, dw, accumulate, rows, n, k};
+  const ProductCall p{name, dy, dy_type, dy_stride, packed_t, scale, 1u, blocks(k), dx, dx_stride, rows, k, n};
+  int rc = outer_start(o, stream);
+  if (rc != 1) return rc;
+  if ((rc = check(p)) != 0 || (rc = check(o)) != 0) return rc;
+  const uint64_t dw_bytes = static_cast<uint64_t>(n) * k * 4u;
+  if (share({dx, dx_stride * 2u, static_cast<uint64_t>(k) * 2u, rows}, {dw, dw_bytes, dw_bytes, 1}) ||
+      share({dx, dx_stride * 2u, static_cast<uint64_t>(k) * 2u, rows},
+            {x, x_stride * elem(x_type), static_cast<uint64_t>(k) * elem(x_type), rows}))
+    return fail(-1, name, "dx shares memory with x or dw");
+  ProductPlan product = product_plan(rows, k, n, dy_type);
+  const OuterPlan outer = outer_plan(rows, n, k);
+  const uint64_t first = (product_workspace(rows, k, n, dy_type) + 15u) / 16u * 16u;
+  if (bad_workspace(workspace, workspace_bytes, first + outer_workspace(o, outer)))
+    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  // Small passes run both products in one launch.
+  const bool small = product.form == kTiles && product.p * product.q <= 128u * 64u && product.splits == 1u &&
+                     outer.p * outer.q == 128u * 128u && outer.splits == 1u;
+  if (small) product.p = product.q = 64u;
+  nklin::Product a{};
+  nklin::Outer b{};
+  const bool tiles = begin(p, product, ws, a, stream);
+  begin(o, outer, ws + first, b, stream);
+  if (small) {
+    const uint32_t groups = groups_of(b, outer);
+    netra_linear_backward_small_gfx950<<<dim3(groups + groups_of(a, product)), dim3(512), 0, stream>>>(a, b, groups);
+  } else {
+    if (tiles) run_tiles(a, product, stream);
+    run_tiles(b, outer, stream);
   }
   return launched(name);
 }
@@ -399,8 +518,8 @@ static bool bad_router(uint32_t tokens, uint32_t slots, uint32_t experts) {
 }
 
 // Counting is shared out over workgroups of 256 threads where one would take longer
-// than a second launch; each counts `each` tokens, one a thread up to `most` workgroups (the loss
-// kernel's workgroups all add up all parts).
+// than a second launch; each counts `each` tokens, one a thread while `most` workgroups reach (the
+// loss kernel's workgroups all add up all parts: few of them, with more threads).
 struct CountPlan {
   uint32_t groups, each;
 };
@@ -497,7 +616,7 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     uint32_t* parts = words + 4 + kBalanceGrid;
     a.parts = parts;
     a.groups = plan.groups;
-    netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(256), 0, stream>>>(
+    netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(plan.each > 256u ? 1024 : 256), 0, stream>>>(
         ids, ids_stride, mask, tokens, slots, experts, plan.each, parts, words);
     grid = (tokens + 15u) / 16u;
     grid = grid > kBalanceGrid ? kBalanceGrid : grid;

@@ -310,7 +310,7 @@ extern "C" __global__ __launch_bounds__(1024) void netra_router_counts_gfx950(co
 }
 
 // Partial counts: workgroup g those of its `each` tokens, to parts[g][0 .. E]; clears *arrived.
-extern "C" __global__ __launch_bounds__(256) void netra_router_count_parts_gfx950(const int32_t* ids, uint64_t stride,
+extern "C" __global__ __launch_bounds__(1024) void netra_router_count_parts_gfx950(const int32_t* ids, uint64_t stride,
                                                                                   const uint8_t* mask, uint32_t tokens,
                                                                                   uint32_t slots, uint32_t E,
                                                                                   uint32_t each, uint32_t* parts,
@@ -318,7 +318,7 @@ extern "C" __global__ __launch_bounds__(256) void netra_router_count_parts_gfx95
   __shared__ uint32_t hist[nkbal::kMaxExperts + 1u];
   const uint32_t t0 = min(tokens, blockIdx.x * each);
   nkbal::histogram(ids, stride, mask, t0, min(tokens, t0 + each), slots, E, hist);
-  for (uint32_t e = threadIdx.x; e <= E; e += 256u) parts[(size_t)blockIdx.x * (E + 1u) + e] = hist[e];
+  for (uint32_t e = threadIdx.x; e <= E; e += blockDim.x) parts[(size_t)blockIdx.x * (E + 1u) + e] = hist[e];
   if (arrived && blockIdx.x == 0u && threadIdx.x == 0u) *arrived = 0u;
 }
 

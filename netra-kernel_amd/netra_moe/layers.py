@@ -20,6 +20,8 @@ SIGNATURES = {
     "netra_linear_forward": (ctypes.c_int, [P, U32, U64, P, P, P, U64, U32, U32, U32, P, U64, P]),
     "netra_linear_input_gradient": (ctypes.c_int, [P, U32, U64, P, P, P, U64, U32, U32, U32, P, U64, P]),
     "netra_linear_weight_gradient": (ctypes.c_int, [P, U32, U64, P, U32, U64, P, U32, U32, U32, U32, P, U64, P]),
+    "netra_linear_backward_workspace": (U64, [U32] * 5),
+    "netra_linear_backward": (ctypes.c_int, [P, U32, U64, P, U32, U64, P, P, P, U64, P, U32, U32, U32, U32, P, U64, P]),
     "netra_router_counts_workspace": (U64, [U32] * 3),
     "netra_router_counts": (ctypes.c_int, [P, U64, P, U32, U32, U32, P, U32, P, U64, P]),
     "netra_router_balance_workspace": (U64, [U32] * 3),

@@ -53,7 +53,7 @@ class BlockLinear:
         self.scale = weight_scale.contiguous().clone()
         self._scale_ptr = self.scale.data_ptr()
         self._entries = {n: (entry(n), entry(n + "_workspace")) for n in (
-            "netra_linear_forward", "netra_linear_input_gradient", "netra_linear_weight_gradient")}
+            "netra_linear_forward", "netra_linear_input_gradient", "netra_linear_weight_gradient", "netra_linear_backward")}
         self.packed = self._pack(weight, 0)
         self.packed_t = self._pack(weight, 1) if gradients else None
 
@@ -115,19 +115,23 @@ class BlockLinear:
             raise ValueError("input_gradient needs a layer built with gradients=True")
         return self._times("netra_linear_input_gradient", "dy", dy, self.N, out, self.K, self.packed_t)
 
+    def _weight_out(self, out: torch.Tensor | None, accumulate: bool) -> torch.Tensor:
+        if out is None:
+            if accumulate:
+                raise ValueError("accumulate needs out")
+            return torch.empty((self.N, self.K), dtype=torch.float32, device=self.device)
+        if tuple(out.shape) != (self.N, self.K) or out.dtype != torch.float32 or not out.is_contiguous() \
+                or out.device != self.device:
+            raise ValueError(f"out: need contiguous torch.float32 {(self.N, self.K)} on {self.device}")
+        return out
+
     def weight_gradient(self, dy: torch.Tensor, x: torch.Tensor, out: torch.Tensor | None = None, *,
                         accumulate: bool = False) -> torch.Tensor:
         """dy [T, N], x [T, K] -> dy^T x fp32 [N, K]; accumulate adds it to out."""
         rows = x.shape[0] if x.dim() == 2 else -1
         x_stride = check_rows("x", x, (rows, self.K), self.device)
         dy_stride = check_rows("dy", dy, (rows, self.N), self.device)
-        if out is None:
-            if accumulate:
-                raise ValueError("accumulate needs out")
-            out = torch.empty((self.N, self.K), dtype=torch.float32, device=self.device)
-        elif tuple(out.shape) != (self.N, self.K) or out.dtype != torch.float32 or not out.is_contiguous() \
-                or out.device != self.device:
-            raise ValueError(f"out: need contiguous torch.float32 {(self.N, self.K)} on {self.device}")
+        out = self._weight_out(out, accumulate)
         name = "netra_linear_weight_gradient"
         fn, need = self._entries[name]
         need = need(rows, self.N, self.K, _in_place(x, x_stride) and _in_place(dy, dy_stride))
@@ -138,5 +142,19 @@ class BlockLinear:
 
     def backward(self, dy: torch.Tensor, x: torch.Tensor, dw: torch.Tensor | None = None, *,
                  accumulate: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
-        """Both gradients: (dx, dw)."""
-        return self.input_gradient(dy), self.weight_gradient(dy, x, dw, accumulate=accumulate)
+        """Both gradients: (dx, dw), as input_gradient() and weight_gradient() give them."""
+        if self.packed_t is None:
+            raise ValueError("backward needs a layer built with gradients=True")
+        rows = x.shape[0] if x.dim() == 2 else -1
+        x_stride = check_rows("x", x, (rows, self.K), self.device)
+        dy_stride = check_rows("dy", dy, (rows, self.N), self.device)
+        dw = self._weight_out(dw, accumulate)
+        dx = torch.empty((rows, self.K), dtype=torch.bfloat16, device=self.device)
+        name, kind = "netra_linear_backward", TYPES[dy.dtype]
+        fn, need = self._entries[name]
+        need = need(rows, self.N, self.K, kind, _in_place(x, x_stride) and _in_place(dy, dy_stride))
+        ws, ws_ptr = workspace(need, self.device)
+        launch(fn, name, self.device, dy.data_ptr(), kind, dy_stride, x.data_ptr(), TYPES[x.dtype], x_stride,
+               self.packed_t.data_ptr(), self._scale_ptr, dx.data_ptr(), self.K, dw.data_ptr(), int(accumulate), rows,
+               self.N, self.K, ws_ptr, need)
+        return dx, dw

@@ -268,3 +268,16 @@ def test_outputs_that_share_memory_with_inputs_are_refused():
     dw = torch.zeros(128, 128, device=DEV)
     with pytest.raises(RuntimeError, match="shares memory"):
         lin.weight_gradient(dw[:40], x.to(DEV), dw)
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 64, 64), (40, 256, 512), (65, 300, 200), (100, 1024, 2048), (333, 1024, 1024), (900, 700, 500),
+                                   (2000, 256, 128)])
+def test_backward_is_both_gradients(T, N, K):
+    lin, _ = layer(N, K, seed=32, gradients=True)
+    x, dy = C.activations(T, K, seed=33).to(DEV), C.activations(T, N, seed=34).to(DEV)
+    dx, dw = lin.backward(dy, x)
+    assert torch.equal(dx, lin.input_gradient(dy)) and torch.equal(dw, lin.weight_gradient(dy, x))
+    acc = dw.clone()
+    assert lin.backward(dy, x, acc, accumulate=True)[1] is acc and torch.equal(acc, dw + dw)
+    with pytest.raises(ValueError, match="gradients=True"):
+        layer(N, K, seed=32)[0].backward(dy, x)
