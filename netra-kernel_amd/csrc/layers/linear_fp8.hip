@@ -551,9 +551,9 @@ __device__ __forceinline__ void outer_tile(const Outer& a, uint32_t group, uint8
   const uint32_t item = (group % 8u) * per + group / 8u;
   if (group / 8u >= per || item >= total) return;
   const uint32_t split = item / (np * nq), tile = item - split * np * nq;
-  const uint32_t band = tile / (8u * np), in_band = tile - band * 8u * np;
-  const uint32_t height = min(8u, nq - band * 8u);
-  const uint32_t p0 = in_band / height * 16u * kP, q0 = (band * 8u + in_band % height) * 16u * kQ;  // first columns
+  const uint32_t band = tile / (4u * np), in_band = tile - band * 4u * np;
+  const uint32_t height = min(4u, nq - band * 4u);
+  const uint32_t p0 = in_band / height * 16u * kP, q0 = (band * 4u + in_band % height) * 16u * kQ;  // first columns
   const uint32_t wp = wave % WP, wq = wave / WP;
   // this split's tokens
   const uint32_t t0 = split * a.split_rows, t1 = min(a.rows, t0 + a.split_rows);
@@ -783,7 +783,7 @@ extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_f32_gf
     nklin::product_tile<__VA_ARGS__>(a, blockIdx.x, lds);                                                         \
   }
 NETRA_PRODUCT_TILE(256, 256, 2, 4, 8, 4, 2)
-NETRA_PRODUCT_TILE(256, 128, 2, 4, 8, 2, 3)
+NETRA_PRODUCT_TILE(256, 128, 4, 2, 4, 4, 3)
 NETRA_PRODUCT_TILE(128, 128, 2, 4, 4, 2, 4)
 NETRA_PRODUCT_TILE(128, 64, 4, 2, 2, 2, 4)
 NETRA_PRODUCT_TILE(64, 64, 4, 2, 1, 2, 4)
