@@ -41,6 +41,17 @@ __device__ __forceinline__ void copy16(uint32_t m0, u32x4 r, uint32_t voff, uint
                : "memory");
 }
 
+// Two such copies, the second 1 KiB further on both sides (the offset counts for both): a
+// 2 KiB tile.
+__device__ __forceinline__ void copy_tile(uint32_t m0, u32x4 r, uint32_t voff, uint32_t soff) {
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
+               "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "s"(m0), "v"(voff), "s"(r), "s"(soff)
+               : "memory");
+}
+
 // 4 bytes per lane -> LDS (m0 + 4 * lane); as copy16.
 __device__ __forceinline__ void copy4(uint32_t m0, u32x4 r, uint32_t voff, uint32_t soff) {
   uint32_t saved;

@@ -224,23 +224,84 @@ struct Tile {
                 "waves, scale blocks, copies and LDS");
 };
 
+// The tile of workgroup `group`: split, and first 16-row tiles of P and Q. False: none.
+// The workgroups of an XCD (ids deal to the eight XCDs in turn) take neighbouring
+// tiles, in bands of 4 along Q, so that they share operands in its L2 (T 4096, N 4096,
+// K 2048: 43.4 us, in bands of 8 45.0, of 16 45.9).
+__device__ __forceinline__ bool product_place(const Product& a, uint32_t group, uint32_t tiles_p, uint32_t tiles_q,
+                                              uint32_t& split, uint32_t& p0, uint32_t& q0) {
+  const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u;
+  const uint32_t np = (pt + tiles_p - 1u) / tiles_p, nq = (qt + tiles_q - 1u) / tiles_q;
+  const uint32_t total = np * nq * a.splits, per = (total + 7u) / 8u;
+  const uint32_t item = (group % 8u) * per + group / 8u;
+  if (group / 8u >= per || item >= total) return false;
+  split = item / (np * nq);
+  const uint32_t tile = item - split * np * nq;
+  const uint32_t band = tile / (4u * np), in_band = tile - band * 4u * np;
+  const uint32_t height = min(4u, nq - band * 4u);
+  p0 = in_band / height * tiles_p;
+  q0 = (band * 4u + in_band % height) * tiles_q;
+  return true;
+}
+
+// A wave's NP x NQ tiles from row tile p of P and q of Q to the output, or, of a split, to the
+// partial sums.
+template <typename L, uint32_t NP, uint32_t NQ>
+__device__ __forceinline__ void product_store(const Product& a, const v4f (&acc)[NP][NQ], uint32_t split, uint32_t p,
+                                              uint32_t q, uint8_t* s_stage) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t c = lane & 15u, r4 = (lane >> 4) * 4u;
+  const uint32_t col0 = p * 16u, row0 = q * 16u;
+  if (a.splits > 1u) {  // fp32 partial sums, rows of a.ni rounded up to 4
+    const uint32_t pitch = (a.ni + 3u) & ~3u;
+    float* part = a.partial + (size_t)split * a.nq * pitch;
+#pragma unroll
+    for (uint32_t j = 0; j < NQ; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < NP; ++i) {
+        const uint32_t row = row0 + j * 16u + c, col = col0 + i * 16u + r4;
+        if (row < a.nq && col < pitch) *reinterpret_cast<v4f*>(part + (size_t)row * pitch + col) = acc[i][j];
+      }
+    return;
+  }
+  // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
+  // whole lines. (A wave reads back only what it wrote itself.)
+  __syncthreads();
+  uint8_t* mine = s_stage + wave * 16u * NQ * L::kPitch;
+#pragma unroll
+  for (uint32_t j = 0; j < NQ; ++j)
+#pragma unroll
+    for (uint32_t i = 0; i < NP; ++i) {
+      const v4f v = acc[i][j];
+      *reinterpret_cast<uint2*>(mine + (j * 16u + c) * L::kPitch + (i * 16u + r4) * 2u) =
+          make_uint2(nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
+                     nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16));
+    }
+  constexpr uint32_t kLanes = NP * 2u;  // lanes of 8 values per row
+  for (uint32_t r = lane / kLanes; r < 16u * NQ; r += 64u / kLanes) {
+    const uint32_t cc = (lane % kLanes) * 8u, row = row0 + r, col = col0 + cc;
+    if (row >= a.nq || col >= a.ni) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * L::kPitch + cc * 2u);
+    uint16_t* o = a.out + (uint64_t)row * a.ldo + col;
+    const Unaligned16 w = {{v.x, v.y, v.z, v.w}};
+    if (col + 8u <= a.ni) {
+      *reinterpret_cast<Unaligned16*>(o) = w;
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8u; ++e)
+        if (col + e < a.ni) o[e] = (uint16_t)(w.w[e / 2u] >> (16u * (e & 1u)));
+    }
+  }
+}
+
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, uint8_t* s_stage) {
   using L = Tile<WP, WQ, NP, NQ, S>;
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u;
-  const uint32_t np = (pt + L::kP - 1u) / L::kP, nq = (qt + L::kQ - 1u) / L::kQ;
-  // The workgroups of an XCD (ids deal to the eight XCDs in turn) take neighbouring
-  // tiles, in bands of 4 along Q, so that they share operands in its L2 (T 4096, N 4096,
-  // K 2048: 43.4 us, in bands of 8 45.0, of 16 45.9).
-  const uint32_t total = np * nq * a.splits, per = (total + 7u) / 8u;
-  const uint32_t item = (group % 8u) * per + group / 8u;
-  if (group / 8u >= per || item >= total) return;
-  const uint32_t split = item / (np * nq), tile = item - split * np * nq;
-  const uint32_t band = tile / (4u * np), in_band = tile - band * 4u * np;
-  const uint32_t height = min(4u, nq - band * 4u);
-  const uint32_t p0 = in_band / height * L::kP, q0 = (band * 4u + in_band % height) * L::kQ;  // first 16-row tiles
+  uint32_t split, p0, q0;
+  if (!product_place(a, group, L::kP, L::kQ, split, p0, q0)) return;
   const uint32_t wp = wave % WP, wq = wave / WP;
   const uint32_t b0 = split * a.split_blocks, b1 = min(a.kb, b0 + a.split_blocks);  // this split's blocks
 
@@ -334,48 +395,120 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
   }
   nklds2::wait_copies<0>();
 
-  const uint32_t c = lane & 15u, r4 = (lane >> 4) * 4u;
-  const uint32_t col0 = (p0 + wp * NP) * 16u, row0 = (q0 + wq * NQ) * 16u;
-  if (a.splits > 1u) {  // fp32 partial sums, rows of a.ni rounded up to 4
-    const uint32_t pitch = (a.ni + 3u) & ~3u;
-    float* part = a.partial + (size_t)split * a.nq * pitch;
+  product_store<L, NP, NQ>(a, acc, split, p0 + wp * NP, q0 + wq * NQ, s_stage);
+}
+
+// The product in tiles of 256 x 256, two groups of four waves taking turns: while one
+// group's waves, one on each SIMD, multiply, the other's read their next operands from
+// LDS and issue copies, so that neither an LDS latency nor a copy that waits for its turn
+// holds the matrix cores up. A phase ends with a barrier; group 1 is one phase behind:
+//   phase      2b          2b + 1        2b + 2
+//   group 0    read b      multiply b    read b + 1
+//   group 1    ..          read b        multiply b
+// Group g owns half g of P's rows. Group 0 copies, while it reads block b, its half of P
+// and all of Q for block b + 1, over block b - 1's: Q was last read by group 1 and the half
+// of P by its own products, both a phase ago. Group 1 copies its own half of P, likewise.
+// Copies are waited for at the end of the products of the same block, a phase and a half
+// after they were issued, and needed by group 0 in the next phase (group 1: its own).
+// A step moves 256 KiB through LDS (64 in, 192 to registers: each tile of P feeds four
+// waves, each of Q two), 2048 cycles of it, as long as its products take: both compete.
+// T 8192, N 8192, K 4096 with the quantisation: 256 us (K 8192: 473 us); all waves in step,
+// product_tile's way: 267 (497); without whole-tile copies 261; with the copies spread over
+// both groups' products 274; Q's operands straight from L2 to registers 302. Of the 256,
+// about 60 go with the copies (a copy of this kernel without them, wrong results: 196).
+__device__ __forceinline__ void product_turns(const Product& a, uint32_t index, uint8_t* s_stage) {
+  using L = Tile<2, 4, 8, 4, 2>;
+  constexpr uint32_t kStage = L::kScaleAt + 1024u + 512u;  // Q's scales, then P's for either group
+  static_assert(2u * kStage <= L::kLds, "two stages");
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t g = wave >> 2, w = wave & 3u;  // group, wave in it
+  const uint32_t pt = (a.ni + 15u) / 16u, qt = (a.nq + 15u) / 16u;
+  uint32_t split, p0, q0;
+  if (!product_place(a, index, 16u, 16u, split, p0, q0)) return;
+  const uint32_t b0 = split * a.split_blocks, b1 = min(a.kb, b0 + a.split_blocks);
+  const uint32_t np_here = min(16u, pt - p0), nq_here = min(16u, qt - q0);
+  const u32x4 rp = nklds2::rsrc(a.p + (size_t)p0 * a.kb * 2048u, np_here * a.kb * 2048u);
+  const u32x4 rq = nklds2::rsrc(a.q + (size_t)q0 * a.kb * 2048u, nq_here * a.kb * 2048u);
+  const uint32_t sq_first = (q0 + w * 4u) * 16u;
+  const uint32_t sq_bytes = sq_first < a.sq_b ? (a.sq_b - sq_first) * 4u : 0u;
+  const uint32_t sp_voff = lane < 2u && (p0 / 8u + lane) * 128u < a.ni ? (p0 / 8u + lane) * a.sp_i * 4u : 0x80000000u;
+  const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
+  // This wave's copies for block b (behind the last block: nothing, as product_tile's).
+  auto issue = [&](uint32_t b) __attribute__((always_inline)) {
+    const uint32_t st = lds0 + (b - b0) % 2u * kStage;
+    const bool live = b < b1;
+    auto tile = [&](const u32x4& from, uint32_t have, uint32_t t, uint32_t at) __attribute__((always_inline)) {
+      u32x4 r = from;
+      r.z = live ? r.z : 0u;
+      nklds2::copy_tile(st + at, r, lane * 16u, live ? (min(t, have - 1u) * a.kb + b) * 2048u : 0u);
+    };
 #pragma unroll
-    for (uint32_t j = 0; j < NQ; ++j)
+    for (uint32_t i = 0; i < 2u; ++i) {
+      const uint32_t t = g * 8u + i * 4u + w;
+      tile(rp, np_here, t, t * 2048u);
+    }  // half g of P
+    const u32x4 rsp = nklds2::rsrc(a.sp + (size_t)b * a.sp_b, live ? a.sp_bytes - b * a.sp_b * 4u : 0u);
+    nklds2::copy4(st + L::kScaleAt + 1024u + g * 256u, rsp, sp_voff, 0u);
+    if (g == 0u) {
 #pragma unroll
-      for (uint32_t i = 0; i < NP; ++i) {
-        const uint32_t row = row0 + j * 16u + c, col = col0 + i * 16u + r4;
-        if (row < a.nq && col < pitch) *reinterpret_cast<v4f*>(part + (size_t)row * pitch + col) = acc[i][j];
+      for (uint32_t i = 0; i < 4u; ++i) tile(rq, nq_here, i * 4u + w, 32768u + (i * 4u + w) * 2048u);
+      const u32x4 rsq = nklds2::rsrc(a.sq + (size_t)b * a.sq_b + sq_first, live ? sq_bytes : 0u);
+      nklds2::copy4(st + L::kScaleAt + w * 256u, rsq, lane * 4u, 0u);
+    }
+  };
+
+  v4f acc[8][4];
+#pragma unroll
+  for (uint32_t i = 0; i < 8u; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  issue(b0);
+  nklds2::wait_copies<0>();
+  nklds2::barrier();
+  if (g == 1u) nklds2::barrier();
+  for (uint32_t b = b0; b < b1; ++b) {
+    const uint8_t* st = s_stage + (b - b0) % 2u * kStage;
+    const uint8_t* tp = st + g * 16384u;
+    const float* scale = reinterpret_cast<const float*>(st + L::kScaleAt);
+    // read
+    v8i qo[4], po[3];
+    float s[4];
+    po[0] = nk::load_tile_operand(tp, lane);
+    po[1] = nk::load_tile_operand(tp + 2048u, lane);
+    const float sp = scale[256u + g * 64u + g];
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) {
+      qo[j] = nk::load_tile_operand(st + 32768u + (w * 4u + j) * 2048u, lane);
+      s[j] = scale[(w * 4u + j) * 16u + (lane & 15u)] * sp;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    issue(b + 1u);
+    nklds2::barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    // multiply
+    __builtin_amdgcn_s_setprio(1);
+    v4f d[4];
+#pragma unroll
+    for (uint32_t i = 0; i <= 8u; ++i) {
+      if (i + 2u < 8u) po[(i + 2u) % 3u] = nk::load_tile_operand(tp + (i + 2u) * 2048u, lane);
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j) {
+        if (i > 0u) {
+#pragma unroll
+          for (uint32_t e = 0; e < 4u; ++e) acc[i - 1u][j][e] = fmaf(s[j], d[j][e], acc[i - 1u][j][e]);
+        }
+        if (i < 8u) d[j] = nk::mfma_e4m3_16x16x128(po[i % 3u], qo[j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    return;
-  }
-  // Output: a wave's 16 NQ rows of 16 NP values through LDS, so that a row leaves as
-  // whole lines. (A wave reads back only what it wrote itself.)
-  __syncthreads();
-  uint8_t* mine = s_stage + wave * 16u * NQ * L::kPitch;
-#pragma unroll
-  for (uint32_t j = 0; j < NQ; ++j)
-#pragma unroll
-    for (uint32_t i = 0; i < NP; ++i) {
-      const v4f v = acc[i][j];
-      *reinterpret_cast<uint2*>(mine + (j * 16u + c) * L::kPitch + (i * 16u + r4) * 2u) =
-          make_uint2(nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
-                     nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16));
     }
-  constexpr uint32_t kLanes = NP * 2u;  // lanes of 8 values per row
-  for (uint32_t r = lane / kLanes; r < 16u * NQ; r += 64u / kLanes) {
-    const uint32_t cc = (lane % kLanes) * 8u, row = row0 + r, col = col0 + cc;
-    if (row >= a.nq || col >= a.ni) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * L::kPitch + cc * 2u);
-    uint16_t* o = a.out + (uint64_t)row * a.ldo + col;
-    const Unaligned16 w = {{v.x, v.y, v.z, v.w}};
-    if (col + 8u <= a.ni) {
-      *reinterpret_cast<Unaligned16*>(o) = w;
-    } else {
-#pragma unroll
-      for (uint32_t e = 0; e < 8u; ++e)
-        if (col + e < a.ni) o[e] = (uint16_t)(w.w[e / 2u] >> (16u * (e & 1u)));
-    }
+    __builtin_amdgcn_s_setprio(0);
+    nklds2::wait_copies<0>();
+    nklds2::barrier();
   }
+  if (g == 0u) nklds2::barrier();
+  nklds2::wait_copies<0>();
+  product_store<L, 8u, 4u>(a, acc, split, p0 + g * 8u, q0 + w * 4u, s_stage);
 }
 
 // out = bf16 of the splits' sum, in split order. One row per blockIdx.y step.
@@ -782,7 +915,10 @@ extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_f32_gf
     __shared__ __align__(16) uint8_t lds[nklin::Tile<__VA_ARGS__>::kLds];                                         \
     nklin::product_tile<__VA_ARGS__>(a, blockIdx.x, lds);                                                         \
   }
-NETRA_PRODUCT_TILE(256, 256, 2, 4, 8, 4, 2)
+extern "C" __global__ __launch_bounds__(512) void netra_linear_product_256x256_gfx950(nklin::Product a) {
+  __shared__ __align__(16) uint8_t lds[nklin::Tile<2, 4, 8, 4, 2>::kLds];
+  nklin::product_turns(a, blockIdx.x, lds);
+}
 NETRA_PRODUCT_TILE(256, 128, 4, 2, 4, 4, 3)
 NETRA_PRODUCT_TILE(128, 128, 2, 4, 4, 2, 4)
 NETRA_PRODUCT_TILE(128, 64, 4, 2, 2, 2, 4)
