@@ -25,10 +25,10 @@
 //
 // Matrices of activations are row-major with a row stride in elements (at least
 // the row length; any alignment of the element type). Input types are
-// NETRA_BF16 or NETRA_F32. Outputs must not share memory with inputs (different
-// columns of rows with the same stride do not); overlaps are refused. rows may be 0: forward and input gradient then do
-// nothing, the weight gradient writes zeros (or leaves dw as it is when it
-// accumulates).
+// NETRA_BF16 or NETRA_F32. Outputs must not share memory with inputs; an overlap
+// with an activation matrix is refused (different columns of rows with the same
+// stride do not overlap). rows may be 0: forward and input gradient then do nothing,
+// the weight gradient writes zeros (or leaves dw as it is when it accumulates).
 //
 // The workspace is scratch of one call: its contents before the call do not
 // matter and nothing is kept in it. Calls that may overlap (two streams, two

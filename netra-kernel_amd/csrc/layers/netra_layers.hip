@@ -90,12 +90,12 @@ struct ProductPlan {
 
 // Tiles: time = rounds of workgroups over the 256 CUs x (steps x the step's time + what a
 // workgroup takes besides), the step's time hardly depending on how many CUs work (us a step:
-// 256x256 1.95, 256x128 1.18, 128x128 0.78, 128x64 0.58, 64x64 0.35, or 0.62 where two workgroups
+// 256x256 1.75, 256x128 1.18, 128x128 0.78, 128x64 0.58, 64x64 0.35, or 0.62 where two workgroups
 // share a CU). Splits add a launch and the partial sums' way out and in. Measured as whole calls,
 // best and next: T 333, N 2048, K 1024 128x64 10.8 us, 64x64 10.9, 128x128 12.0; T 700, N 2048, K
 // 2048 128x64 14.4, 64x64 15.8; T 1500, N 1500, K 1500 128x128 18.3, 64x64 20.7; T 1500, N 4096, K
 // 1024 256x128 18.7, 128x128 22.2; T 8192, N 512, K 4096 128x128 41.6, 128x64 51.5; T 3000, N 6000,
-// K 3000 256x128 91, 128x128 96, 256x256 98; T 4096, N 4096, K 2048 256x256 43.4, 256x128 55.5; T
+// K 3000 256x256 89, 256x128 93, 128x128 96; T 4096, N 4096, K 2048 256x256 42.8, 256x128 52.7; T
 // 128, N 8192, K 8192 128x128 in four splits 24.9, in two 32.3, 64x64 in two 26.0.
 ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
   struct Shape {
@@ -103,7 +103,7 @@ ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
     double step_us, group_us;
   };
   static const Shape shapes[] = {
-      {256, 256, 1.95, 3.0}, {256, 128, 1.18, 2.0}, {128, 128, 0.78, 1.5}, {128, 64, 0.58, 1.2}, {64, 64, 0.35, 1.0}};
+      {256, 256, 1.75, 3.0}, {256, 128, 1.18, 2.0}, {128, 128, 0.78, 1.5}, {128, 64, 0.58, 1.2}, {64, 64, 0.35, 1.0}};
   const uint32_t kb = blocks(nc);
   ProductPlan best{kTiles, 256, 256, 1, kb};
   double best_us = 1e30;
@@ -131,7 +131,8 @@ ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc, uint32_t in_ty
   // workgroup the quantisation of its waves' blocks: 16-row tiles x blocks per wave x
   // workgroups per CU, of which seven cost what the launch does (T 48, N 4096, K 2048, six:
   // 10.3 us against 10.7; T 64, eight: 11.7 against 10.8; T 32, N 8192, K 8192, sixteen: 23.5
-  // against 17.5).
+  // against 17.5). One tile of rows always quantises on the way: at worst it costs 3% (T 16, N
+  // 28672, K 8192: 50.5 us, with the launch 49.0), few rows gain most (T 1: 40.2 against 48.6).
   const uint32_t pt = (ni + 15u) / 16u, q = (rows + 15u) / 16u;
   const uint32_t groups = pt >= 512u ? (pt + 1u) / 2u : pt;
   const uint64_t cost = static_cast<uint64_t>((groups + 255u) / 256u) * q * ((blocks(nc) + 7u) / 8u);
