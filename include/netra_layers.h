@@ -111,7 +111,8 @@ int netra_router_counts(const int32_t* ids, uint64_t ids_stride, const uint8_t* 
 // slots != 0: counts are computed from ids as by netra_router_counts and
 // written to `counts`; slots 0 (ids is not looked at): counts is an input (for
 // instance summed over the ranks of a job). grad (type and shape of logits) may be null.
-// counts have to stay below 2^31 in sum; experts <= 1024.
+// counts have to stay below 2^31 in sum; experts <= 1024; row strides of logits and grad
+// below 2^27.
 uint64_t netra_router_balance_workspace(uint32_t tokens, uint32_t slots, uint32_t experts);
 int netra_router_balance(const void* logits, uint32_t logits_type, uint64_t logits_stride, const float* bias,
                          const int32_t* ids, uint64_t ids_stride, uint32_t slots, const uint8_t* mask,

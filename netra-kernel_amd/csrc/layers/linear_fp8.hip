@@ -138,7 +138,9 @@ __device__ __forceinline__ void store_tile(uint8_t* tile, uint32_t lane, const u
 
 // Rows: x [rows, n] -> tiles of 16 rows x 128 columns, scales s[b, row] with
 // `sld` floats per block (sld = rows rounded up to 16 at least). One wave per tile; rows past
-// the end are zeros.
+// the end are zeros. Bound by memory: a tile's loads, 64 bytes a lane, are one wave's whole
+// work, so enough are under way. 8192 x 4096 bf16: 102 MB in and out, 20.7 us, 4.9 TB/s (a
+// large copy: 5.1); 1001 x 1111 fp32 4.9 us, 64 x 2048 bf16 2.5 us (a launch).
 template <typename X>
 __device__ __forceinline__ void quant_rows(const X* __restrict__ x, uint64_t stride, uint8_t* __restrict__ q,
                                            float* __restrict__ s, uint32_t rows, uint32_t n, uint32_t sld) {
@@ -160,8 +162,7 @@ __device__ __forceinline__ void store4(uint16_t* out, uint32_t left, const float
   struct __attribute__((packed, aligned(2))) Pair {
     uint32_t w[2];
   };
-  const Pair p = {{nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
-                   nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16)}};
+  const Pair p = {{nk::bf16x2_hw(v[0], v[1]), nk::bf16x2_hw(v[2], v[3])}};
   if (left >= 4u) {
     *reinterpret_cast<Pair*>(out) = p;
     return;
@@ -207,7 +208,13 @@ struct Product {
 // the stage of the step before may be overwritten.
 // Each wave holds its NQ operands of Q for the step and streams its NP operands of
 // P past them: NQ products per operand, each scaled and added by VALU while the
-// matrix core works on the next.
+// matrix core works on the next. (The scales differ per row of Q, so the sum over blocks
+// cannot stay in the matrix core.) Copies spread over the products: in a burst at the head of
+// a step they hold up the wave that issues them.
+// What bounds it: LDS traffic beside the products. 256x128 at T 4096, N 2048, K 4096: 43 us
+// (1.6 PFLOP/s; the library's product without block scales reaches 2.6 at 8192 x 8192 x
+// 4096); a step moves 176 KiB through LDS, 1408 cycles, for 1024 cycles of products, and takes
+// about 2600. 128x64 at T 1001, N 1500, K 1111: 8.8 us, nine steps and one round.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 struct Tile {
   static constexpr uint32_t kWaves = WP * WQ;
@@ -274,8 +281,7 @@ __device__ __forceinline__ void product_store(const Product& a, const v4f (&acc)
     for (uint32_t i = 0; i < NP; ++i) {
       const v4f v = acc[i][j];
       *reinterpret_cast<uint2*>(mine + (j * 16u + c) * L::kPitch + (i * 16u + r4) * 2u) =
-          make_uint2(nk::bf16_rne(v[0]) | ((uint32_t)nk::bf16_rne(v[1]) << 16),
-                     nk::bf16_rne(v[2]) | ((uint32_t)nk::bf16_rne(v[3]) << 16));
+          make_uint2(nk::bf16x2_hw(v[0], v[1]), nk::bf16x2_hw(v[2], v[3]));
     }
   constexpr uint32_t kLanes = NP * 2u;  // lanes of 8 values per row
   for (uint32_t r = lane / kLanes; r < 16u * NQ; r += 64u / kLanes) {
@@ -511,7 +517,7 @@ __device__ __forceinline__ void product_turns(const Product& a, uint32_t index, 
   product_store<L, 8u, 4u>(a, acc, split, p0 + g * 8u, q0 + w * 4u, s_stage);
 }
 
-// out = bf16 of the splits' sum, in split order. One row per blockIdx.y step.
+// out = bf16 of the splits' sum, in split order. One row per blockIdx.y step. Memory.
 __device__ __forceinline__ void product_sum(const Product& a) {
   const uint32_t pitch = (a.ni + 3u) & ~3u, col = (blockIdx.x * 256u + threadIdx.x) * 4u;
   if (col >= a.ni) return;
@@ -531,7 +537,9 @@ __device__ __forceinline__ void product_sum(const Product& a) {
 // way, by every wave for its own blocks, so that a call is one launch: a wave's
 // lanes hold a tile of 16 rows x 128 values exactly as an operand wants it, and the
 // four lanes of a row find its scale with two exchanges. Else their tiles come from
-// a.q.
+// a.q. Bound by the weights' way from memory, or by a launch's length where they are few:
+// T 1, N 28672, K 8192 (235 MB) 40.2 us, 5.8 TB/s; T 1, N 2048, K 2048 (4 MB, from the last
+// level cache) 4.4 us, T 64, N 4096, K 2048 4.4 us behind 2.5 of quantisation.
 template <uint32_t NP, uint32_t NQ, bool kFused, typename X>
 __device__ __forceinline__ void product_stream(const Product& a, const X* __restrict__ x, uint64_t x_stride,
                                                uint32_t n) {
@@ -663,7 +671,12 @@ struct Outer {
 // tokens of one read then meet every bank twice, which is what 512 bytes need.
 // Workgroups, waves and the stage hand-over are product_tile's. Columns past the
 // matrix read the next row and make outputs that are not stored; tokens past the
-// end read zeros.
+// end read zeros. 128x256 at T 4096, N 4096, K 2048: 61.5 us, 1.12 PFLOP/s (a library
+// product of the same size 79 us, a large one 1.42 PFLOP/s), the matrix cores busy 41% of
+// the cycles: 176 KiB per step through LDS, 1408 cycles, beside 1024 of products. Reading
+// less, by waves of 64 x 128 over one half of a step's tokens each and a sum of the halves
+// at the end (144 KiB per step), takes 62.5 us, and 9.0 us instead of 8.3 at T 333, N 1024, K
+// 2048: the longer wait for a step's first operands costs as much.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 constexpr uint32_t outer_lds() {
   return S * 64u * 32u * (WP * NP + WQ * NQ);
@@ -828,8 +841,8 @@ __device__ __forceinline__ void to_bf16(const X* __restrict__ x, uint64_t stride
     uint32_t w[4];
 #pragma unroll
     for (uint32_t e = 0; e < 4u; ++e)
-      w[e] = nk::bf16_rne(c + 2u * e < cols ? value(p + 2u * e) : 0.0f) |
-             (uint32_t)nk::bf16_rne(c + 2u * e + 1u < cols ? value(p + 2u * e + 1u) : 0.0f) << 16;
+      w[e] = nk::bf16x2_hw(c + 2u * e < cols ? value(p + 2u * e) : 0.0f,
+                           c + 2u * e + 1u < cols ? value(p + 2u * e + 1u) : 0.0f);
     *reinterpret_cast<uint4*>(out + (uint64_t)r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
@@ -957,7 +970,8 @@ NETRA_OUTER_TILE(128, 256, 2, 4, 4, 4, 3)
 NETRA_OUTER_TILE(128, 128, 2, 4, 4, 2, 4)
 // Both products of a small backward pass in one launch, the weight gradient's
 // workgroups (the first `outer`, a multiple of 8) with their longer way first: neither
-// fills the chip, and a launch is saved.
+// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 14.0 us, 12.0 of it this
+// kernel; in two launches 18.1).
 extern "C" __global__ __launch_bounds__(512) void netra_linear_backward_small_gfx950(nklin::Product a, nklin::Outer b,
                                                                                      uint32_t outer) {
   constexpr uint32_t kP = nklin::Tile<4, 2, 1, 2, 4>::kLds, kO = nklin::outer_lds<2, 4, 4, 2, 4>();

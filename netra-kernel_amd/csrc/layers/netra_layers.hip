@@ -587,6 +587,9 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
                  (slots && (!ids || !aligned(ids, 4) || ids_stride < slots)) ||
                  (grad && bad_matrix(grad, logits_type, grad_stride, experts))))
     return fail(-1, name, "null or misaligned pointer, or row stride below the row");
+  // the kernel's offsets inside four rows have 31 bits
+  if (tokens && (logits_stride >= (1u << 27) || (grad && grad_stride >= (1u << 27))))
+    return fail(-1, name, "row strides of logits and grad have to be below 2^27");
   const uint64_t row = static_cast<uint64_t>(experts) * elem(logits_type);
   if (grad && share({logits, logits_stride * elem(logits_type), row, tokens},
                     {grad, grad_stride * elem(logits_type), row, tokens}))
@@ -619,22 +622,17 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     a.groups = plan.groups;
     netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(plan.each > 256u ? 1024 : 256), 0, stream>>>(
         ids, ids_stride, mask, tokens, slots, experts, plan.each, parts, words);
-    grid = (tokens + 15u) / 16u;
+    const uint32_t rows = experts <= 256u ? 64u : 16u;  // per pass of a workgroup
+    grid = (tokens - 1u) / rows + 1u;
     grid = grid > kBalanceGrid ? kBalanceGrid : grid;
   }
-  const uint32_t es = elem(logits_type);
-  const bool vec = experts > 128u && experts % 4u == 0 && aligned(logits, 4u * es) && logits_stride % 4u == 0 &&
-                   (!grad || (aligned(grad, 4u * es) && grad_stride % 4u == 0));
-#define NETRA_RUN(NAME, V) netra_router_balance_##NAME##_v##V##_gfx950<<<dim3(grid), dim3(1024), 0, stream>>>(a)
-#define NETRA_PICK(NAME)                                  \
-  if (experts <= 64u) NETRA_RUN(NAME, 1x1);               \
-  else if (experts <= 128u) NETRA_RUN(NAME, 2x1);         \
-  else if (experts <= 256u && vec) NETRA_RUN(NAME, 4x4);  \
-  else if (experts <= 256u) NETRA_RUN(NAME, 4x1);         \
-  else if (experts <= 512u && vec) NETRA_RUN(NAME, 8x4);  \
-  else if (experts <= 512u) NETRA_RUN(NAME, 8x1);         \
-  else if (vec) NETRA_RUN(NAME, 16x4);                    \
-  else NETRA_RUN(NAME, 16x1)
+#define NETRA_RUN(NAME, F) netra_router_balance_##NAME##_##F##_gfx950<<<dim3(grid), dim3(1024), 0, stream>>>(a)
+#define NETRA_PICK(NAME)                       \
+  if (experts <= 64u) NETRA_RUN(NAME, 16x4);   \
+  else if (experts <= 128u) NETRA_RUN(NAME, 16x8);  \
+  else if (experts <= 256u) NETRA_RUN(NAME, 16x16); \
+  else if (experts <= 512u) NETRA_RUN(NAME, 64x8);  \
+  else NETRA_RUN(NAME, 64x16)
   if (logits_type == NETRA_BF16) {
     NETRA_PICK(bf16);
   } else {

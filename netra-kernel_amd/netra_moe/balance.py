@@ -70,7 +70,7 @@ def expert_counts(topk_ids: torch.Tensor, experts: int, *, mask: torch.Tensor | 
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(experts, dtype=torch.int32, device=device)
+        out = topk_ids.new_empty(experts)
     else:
         _check_counts("out", out, experts, device)
     need = entry("netra_router_counts_workspace")(tokens, slots, experts)
@@ -101,12 +101,12 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor | None = None, *, 
     if topk_ids is not None:
         stride = _check_ids(topk_ids, tokens, device)
         slots, ids = topk_ids.shape[1], topk_ids.data_ptr()
-        counts = torch.empty(experts, dtype=torch.int32, device=device)
+        counts = topk_ids.new_empty(experts)
     else:
         _check_counts("counts", counts, experts, device)
         slots, ids, stride = 0, 0, 0
     loss = torch.empty((), dtype=torch.float32, device=device)
-    g = torch.empty((tokens, experts), dtype=logits.dtype, device=device) if grad else None
+    g = logits.new_empty((tokens, experts)) if grad else None
     need = entry("netra_router_balance_workspace")(tokens, slots, experts)
     ws, ws_ptr = workspace(need, device)
     launch(entry("netra_router_balance"), "netra_router_balance", device, logits.data_ptr(), TYPES[logits.dtype],
