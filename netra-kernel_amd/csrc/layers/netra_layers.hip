@@ -92,11 +92,12 @@ struct ProductPlan {
 // workgroup takes besides), the step's time hardly depending on how many CUs work (us a step:
 // 256x256 1.75, 256x128 1.18, 128x128 0.78, 128x64 0.58, 64x64 0.35, or 0.62 where two workgroups
 // share a CU). Splits add a launch and the partial sums' way out and in. Measured as whole calls,
-// best and next: T 333, N 2048, K 1024 128x64 10.8 us, 64x64 10.9, 128x128 12.0; T 700, N 2048, K
-// 2048 128x64 14.4, 64x64 15.8; T 1500, N 1500, K 1500 128x128 18.3, 64x64 20.7; T 1500, N 4096, K
-// 1024 256x128 18.7, 128x128 22.2; T 8192, N 512, K 4096 128x128 41.6, 128x64 51.5; T 3000, N 6000,
-// K 3000 256x256 89, 256x128 93, 128x128 96; T 4096, N 4096, K 2048 256x256 42.8, 256x128 52.7; T
-// 128, N 8192, K 8192 128x128 in four splits 24.9, in two 32.3, 64x64 in two 26.0.
+// best and next: T 333, N 2048, K 1024 64x64 10.0 us, 128x64 10.7, 128x128 11.0; T 700, N 2048, K
+// 2048 128x64 13.8, 64x64 15.4; T 1500, N 1500, K 1500 128x128 17.3, 64x64 20.4; T 1500, N 4096, K
+// 1024 256x128 16.4, 128x128 20.2; T 8192, N 512, K 4096 128x128 40.7, 256x128 in two splits 48.5;
+// T 3000, N 6000, K 3000 256x256 81.3, 256x128 83.7, 128x128 92.5; T 4096, N 4096, K 2048 256x256
+// 39.8, 256x128 45.9; T 200, N 500, K 8000 64x64 in eight splits 14.6, in two 19.5. The model misses
+// by 7% at T 128, N 8192, K 8192: 128x64 in two splits 25.1, 64x64 26.8.
 ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
   struct Shape {
     uint32_t p, q;
@@ -531,9 +532,18 @@ static CountPlan count_plan(uint32_t tokens, uint32_t few, uint32_t most) {
   plan.each = (tokens + plan.groups - 1u) / plan.groups;
   return plan;
 }
-static constexpr uint32_t kFewCounts = 2048;   // tokens one workgroup counts
-static constexpr uint32_t kFewBalance = 64;    // tokens one workgroup takes through the loss
+// Tokens one workgroup counts (1024 of 9 ids: 7.3 us, in two launches 9.5; 2048: 10.0, 9.5; 3500:
+// 14.2, 9.6).
+static constexpr uint32_t kFewCounts = 2048;
 static constexpr uint32_t kBalanceGrid = 256;
+// One workgroup takes 32768 logits through the loss, 256 tokens at most (128 x 256: 11.7 us, shared
+// out 13.6; 256 x 16: 9.9, 13.6; 512 x 16: 13.3, 13.7; 64 x 512: 11.2, 13.6; 64 x 1024: 16.0, 13.6).
+// More parts than 64 cost their summing up what they gain (32768 x 256 24.1 us with 128, 24.7 with
+// 64; x 500 33.8, 32.3; with 32 27.7, 32.9).
+static CountPlan balance_plan(uint32_t tokens, uint32_t experts) {
+  const uint32_t few = 32768u / (experts ? experts : 1u);
+  return count_plan(tokens, few < 256u ? few : 256u, 64u);
+}
 
 static uint64_t parts_bytes(const CountPlan& plan, uint32_t experts) {
   return (4u * static_cast<uint64_t>(plan.groups) * (experts + 1u) + 15u) / 16u * 16u;
@@ -568,7 +578,7 @@ extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, cons
 }
 
 extern "C" uint64_t netra_router_balance_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
-  const CountPlan plan = count_plan(tokens, kFewBalance, 64u);
+  const CountPlan plan = balance_plan(tokens, experts);
   return plan.groups ? 16u + 4u * kBalanceGrid + parts_bytes(plan, experts) : 0;
 }
 
@@ -596,7 +606,7 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     return fail(-1, name, "grad shares memory with logits");
   if (bad_workspace(workspace, workspace_bytes, netra_router_balance_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
-  const CountPlan plan = count_plan(tokens, kFewBalance, 64u);
+  const CountPlan plan = balance_plan(tokens, experts);
   nkbal::Balance a{};
   a.z = logits;
   a.z_stride = logits_stride;
@@ -622,7 +632,8 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     a.groups = plan.groups;
     netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(plan.each > 256u ? 1024 : 256), 0, stream>>>(
         ids, ids_stride, mask, tokens, slots, experts, plan.each, parts, words);
-    const uint32_t rows = experts <= 256u ? 64u : 16u;  // per pass of a workgroup
+    // Rows per pass of a workgroup. (Workgroups of 512 threads: 32768 x 256 bf16 26.8 us, of 1024 24.6.)
+    const uint32_t rows = experts <= 256u ? 64u : 16u;
     grid = (tokens - 1u) / rows + 1u;
     grid = grid > kBalanceGrid ? kBalanceGrid : grid;
   }

@@ -78,7 +78,9 @@ def test_counts_of_strided_ids():
 
 
 BALANCE = [(1, 1, 1, 0), (1, 16, 2, 0), (2, 64, 4, 1), (16, 16, 2, 0), (17, 65, 3, 0), (64, 256, 8, 1), (300, 128, 4, 1),
-           (1000, 129, 2, 0), (513, 500, 6, 1), (4096, 256, 8, 1), (777, 1024, 8, 0), (2049, 700, 5, 0), (9001, 33, 3, 1)]
+           (1000, 129, 2, 0), (513, 500, 6, 1), (4096, 256, 8, 1), (777, 1024, 8, 0), (2049, 700, 5, 0), (9001, 33, 3, 1),
+           (5, 3, 1, 0), (100, 62, 3, 0), (200, 99, 4, 1), (256, 128, 8, 0), (128, 250, 8, 1), (257, 16, 2, 0),
+           (32, 1024, 8, 1), (33, 1023, 4, 0)]
 
 
 @pytest.mark.parametrize("dt", [BF16, F32])

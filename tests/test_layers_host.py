@@ -96,7 +96,8 @@ def test_counts_refusals(change):
 @pytest.mark.parametrize("change", [dict(z=0), dict(z=A + 1), dict(zt=2), dict(zs=15), dict(bias=A + 1), dict(ids=0),
                                     dict(ids=A + 2), dict(st=1), dict(E=0), dict(E=1025), dict(T=1 << 31),
                                     dict(counts=0), dict(counts=A + 2), dict(loss=0), dict(loss=A + 1), dict(g=B + 1), dict(g=A), dict(g=A + 2), dict(zs=40, gs=40, g=A + 24),
-                                    dict(gs=15), dict(ws=0), dict(ws=A + 4), dict(short=1)])
+                                    dict(gs=15), dict(ws=0), dict(ws=A + 4), dict(short=1),
+                                    dict(zs=1 << 27), dict(gs=1 << 27)])
 def test_balance_refusals(change):
     a = dict(z=A, zt=0, zs=16, bias=None, ids=A, st=2, T=4000, slots=2, E=16, counts=A, loss=A, g=B, gs=16, ws=A, short=0)
     a.update(change)
