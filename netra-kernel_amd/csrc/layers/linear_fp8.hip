@@ -211,10 +211,10 @@ struct Product {
 // matrix core works on the next. (The scales differ per row of Q, so the sum over blocks
 // cannot stay in the matrix core.) Copies spread over the products: in a burst at the head of
 // a step they hold up the wave that issues them.
-// What bounds it: LDS traffic beside the products. 256x128 at T 4096, N 2048, K 4096: 43 us
-// (1.6 PFLOP/s; the library's product without block scales reaches 2.6 at 8192 x 8192 x
+// What bounds it: LDS traffic beside the products. 256x128 at T 4096, N 2048, K 4096: 41 us
+// (1.7 PFLOP/s; the library's product without block scales reaches 2.6 at 8192 x 8192 x
 // 4096); a step moves 176 KiB through LDS, 1408 cycles, for 1024 cycles of products, and takes
-// about 2600. 128x64 at T 1001, N 1500, K 1111: 8.8 us, nine steps and one round.
+// about 2600. 128x64 at T 1001, N 1500, K 1111: 7.6 us, nine steps and one round.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 struct Tile {
   static constexpr uint32_t kWaves = WP * WQ;
@@ -418,10 +418,11 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
 // after they were issued, and needed by group 0 in the next phase (group 1: its own).
 // A step moves 256 KiB through LDS (64 in, 192 to registers: each tile of P feeds four
 // waves, each of Q two), 2048 cycles of it, as long as its products take: both compete.
-// T 8192, N 8192, K 4096 with the quantisation: 256 us (K 8192: 473 us); all waves in step,
-// product_tile's way: 267 (497); without whole-tile copies 261; with the copies spread over
-// both groups' products 274; Q's operands straight from L2 to registers 302. Of the 256,
-// about 60 go with the copies (a copy of this kernel without them, wrong results: 196).
+// T 8192, N 8192, K 4096 with the quantisation: 243 us, 235 here beside 20.7 of it at its best
+// (2.3 PFLOP/s; the library's product without block scales 212 us). All waves in step,
+// product_tile's way, take 4% longer, without whole-tile copies 2%, with the copies spread over
+// both groups' products 7%, with Q's operands straight from L2 to registers 18%. About 60 us go
+// with the copies (timed without them).
 __device__ __forceinline__ void product_turns(const Product& a, uint32_t index, uint8_t* s_stage) {
   using L = Tile<2, 4, 8, 4, 2>;
   constexpr uint32_t kStage = L::kScaleAt + 1024u + 512u;  // Q's scales, then P's for either group
@@ -450,10 +451,10 @@ __device__ __forceinline__ void product_turns(const Product& a, uint32_t index, 
       nklds2::copy_tile(st + at, r, lane * 16u, live ? (min(t, have - 1u) * a.kb + b) * 2048u : 0u);
     };
 #pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
+    for (uint32_t i = 0; i < 2u; ++i) {  // half g of P
       const uint32_t t = g * 8u + i * 4u + w;
       tile(rp, np_here, t, t * 2048u);
-    }  // half g of P
+    }
     const u32x4 rsp = nklds2::rsrc(a.sp + (size_t)b * a.sp_b, live ? a.sp_bytes - b * a.sp_b * 4u : 0u);
     nklds2::copy4(st + L::kScaleAt + 1024u + g * 256u, rsp, sp_voff, 0u);
     if (g == 0u) {
@@ -500,7 +501,7 @@ __device__ __forceinline__ void product_turns(const Product& a, uint32_t index, 
       if (i + 2u < 8u) po[(i + 2u) % 3u] = nk::load_tile_operand(tp + (i + 2u) * 2048u, lane);
 #pragma unroll
       for (uint32_t j = 0; j < 4u; ++j) {
-        if (i > 0u) {
+        if (i > 0u) {  // the tile before, one product of each row behind
 #pragma unroll
           for (uint32_t e = 0; e < 4u; ++e) acc[i - 1u][j][e] = fmaf(s[j], d[j][e], acc[i - 1u][j][e]);
         }
@@ -676,7 +677,9 @@ struct Outer {
 // the cycles: 176 KiB per step through LDS, 1408 cycles, beside 1024 of products. Reading
 // less, by waves of 64 x 128 over one half of a step's tokens each and a sum of the halves
 // at the end (144 KiB per step), takes 62.5 us, and 9.0 us instead of 8.3 at T 333, N 1024, K
-// 2048: the longer wait for a step's first operands costs as much.
+// 2048: the longer wait for a step's first operands costs as much. Two groups of waves in
+// turn, product_turns' way, take 76 us. 256x256 at T 8192, N 4096, K 4096: 230 us, of which
+// its stores, which nothing hides with one workgroup per CU, are 30.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 constexpr uint32_t outer_lds() {
   return S * 64u * 32u * (WP * NP + WQ * NQ);
@@ -970,7 +973,7 @@ NETRA_OUTER_TILE(128, 256, 2, 4, 4, 4, 3)
 NETRA_OUTER_TILE(128, 128, 2, 4, 4, 2, 4)
 // Both products of a small backward pass in one launch, the weight gradient's
 // workgroups (the first `outer`, a multiple of 8) with their longer way first: neither
-// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 14.0 us, 12.0 of it this
+// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 13.9 us, 11.1 of it this
 // kernel; in two launches 18.1).
 extern "C" __global__ __launch_bounds__(512) void netra_linear_backward_small_gfx950(nklin::Product a, nklin::Outer b,
                                                                                      uint32_t outer) {

@@ -231,9 +231,10 @@ struct Balance {
 
 // Counts, then the tokens' rows, 64 / G per wave. With `parts` the counting was
 // shared out over the workgroups of the launch before; without, this launch is
-// one workgroup. Bound by memory at the largest sizes (32768 x 500 fp32: 131 MB, 26.9 us, 4.9
-// TB/s), else by what every workgroup does once: a chain of parts, barriers and the last sum
-// (4096 x 256 bf16: 7.6 us for 4 MB; 16 x 16 in one workgroup 4.0).
+// one workgroup. Bound by memory at the largest sizes (32768 x 500 fp32: 131 MB, 26.2 us, 5.0
+// TB/s), else by the vector units (32768 x 256 bf16: 15.2 us for 34 MB) and by what every
+// workgroup does once: a chain of parts, barriers and the last sum (4096 x 256 bf16: 7.7 us for 4
+// MB; 16 x 16 in one workgroup 3.8).
 template <typename X, uint32_t G, uint32_t NV>
 __device__ __forceinline__ void balance(const Balance& a) {
   __shared__ uint32_t s_count[kMaxExperts + 1u];
