@@ -418,8 +418,8 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
 // after they were issued, and needed by group 0 in the next phase (group 1: its own).
 // A step moves 256 KiB through LDS (64 in, 192 to registers: each tile of P feeds four
 // waves, each of Q two), 2048 cycles of it, as long as its products take: both compete.
-// T 8192, N 8192, K 4096 with the quantisation: 243 us, 235 here beside 20.7 of it at its best
-// (2.3 PFLOP/s; the library's product without block scales 212 us). All waves in step,
+// T 8192, N 8192, K 4096 with the quantisation: 243 us (2.26 PFLOP/s; the library's product
+// without block scales and without the quantisation 212 us). All waves in step,
 // product_tile's way, take 4% longer, without whole-tile copies 2%, with the copies spread over
 // both groups' products 7%, with Q's operands straight from L2 to registers 18%. About 60 us go
 // with the copies (timed without them).
