@@ -221,12 +221,14 @@ struct Tile {
   static constexpr uint32_t kP = WP * NP, kQ = WQ * NQ;   // 16-row tiles of each operand
   static constexpr uint32_t kScaleAt = (kP + kQ) * 2048u; // 16 scales per tile of Q, then 64 words for P's
   static constexpr uint32_t kStage = kScaleAt + kQ * 64u + 256u;
-  static constexpr uint32_t kCopies = (kP + kQ) * 2u / kWaves + 1u;  // a wave's, per step
+  // A wave's copies per step: two for each of its whole tiles, one for a half of the rest, scales.
+  static constexpr uint32_t kTiles = (kP + kQ) / kWaves, kHalves = (kP + kQ) % kWaves * 2u / kWaves;
+  static constexpr uint32_t kCopies = 2u * kTiles + kHalves + 1u;
   // A row's pitch of the output's staging: 16 bytes over its NP tiles spread the writes over the banks.
   static constexpr uint32_t kPitch = NP * 32u + 16u;
   static constexpr uint32_t kOut = kWaves * 16u * NQ * kPitch;
   static constexpr uint32_t kLds = S * kStage > kOut ? S * kStage : kOut;
-  static_assert(kWaves == 8u && (NP % 8u == 0u || 8u % NP == 0u) && kP % 4u == 0u && kQ % 4u == 0u && kQ <= 28u &&
+  static_assert(kWaves == 8u && (NP % 8u == 0u || 8u % NP == 0u) && (kP + kQ) % 4u == 0u && kQ % 4u == 0u && kQ <= 28u &&
                     kLds <= 160u * 1024u,
                 "waves, scale blocks, copies and LDS");
 };
@@ -327,20 +329,27 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
                                                                                  : 0x80000000u;
   const uint32_t voff = lane * 16u;
   const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)nklds2::lds_offset(&s_stage[0]));
-  // Copy i of a wave's kCopies for block b. A tile past the matrix repeats its last
-  // one (its outputs are not stored); behind the split's last block a copy reads
+  // This wave's tiles (of P's, then Q's), and then its half tile where they do not go round.
+  // A tile past the matrix repeats its last one (its outputs are not stored).
+  constexpr uint32_t kOwn = L::kTiles + L::kHalves;
+  uint32_t own[kOwn], first[kOwn];
+#pragma unroll
+  for (uint32_t i = 0; i < kOwn; ++i) {
+    own[i] = L::kWaves * i + (i < L::kTiles ? wave : wave >> 1);
+    first[i] = (own[i] < L::kP ? min(own[i], np_here - 1u) : min(own[i] - L::kP, nq_here - 1u)) * a.kb * 2048u;
+  }
+  // Part i of a wave's copies for block b. Behind the split's last block a copy reads
   // nothing (an empty range) and leaves zeros that nobody looks at, so that a step's
   // code has no branch and always the same copies in flight.
   auto issue_part = [&](uint32_t b, uint32_t stage, uint32_t i) __attribute__((always_inline)) {
     const uint32_t st = lds0 + stage * L::kStage;
     const bool live = b < b1;
-    if (i + 1u < L::kCopies) {
-      const uint32_t k = i * L::kWaves + wave;  // P's half tiles, then Q's
-      const bool is_p = i * L::kWaves < 2u * L::kP;
-      const uint32_t t = is_p ? min(k >> 1, np_here - 1u) : min((k >> 1) - L::kP, nq_here - 1u);
-      u32x4 r = is_p ? rp : rq;
+    if (i < kOwn) {
+      u32x4 r = own[i] < L::kP ? rp : rq;
       r.z = live ? r.z : 0u;
-      nklds2::copy16(st + k * 1024u, r, voff, live ? (t * a.kb + b) * 2048u + (k & 1u) * 1024u : 0u);
+      const uint32_t to = st + own[i] * 2048u, from = live ? first[i] + b * 2048u : 0u, half = (wave & 1u) * 1024u;
+      if (i < L::kTiles) nklds2::copy_tile(to, r, voff, from);
+      else nklds2::copy16(to + half, r, voff, from + half);
     } else {
       const uint32_t bytes = s_bytes - b * s_less;
       const u32x4 r = nklds2::rsrc((const void*)(s_base + (uint64_t)b * s_step), live ? bytes : 0u);
@@ -349,7 +358,7 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
   };
   auto issue = [&](uint32_t b, uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t i = 0; i < L::kCopies; ++i) issue_part(b, stage, i);
+    for (uint32_t i = 0; i <= kOwn; ++i) issue_part(b, stage, i);
   };
 
   v4f acc[NP][NQ];
@@ -394,7 +403,7 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
       }
       // the copies of a later step, spread over this one's products
 #pragma unroll
-      for (uint32_t k = i * L::kCopies / (NP + 1u); k < (i + 1u) * L::kCopies / (NP + 1u); ++k)
+      for (uint32_t k = i * (kOwn + 1u) / (NP + 1u); k < (i + 1u) * (kOwn + 1u) / (NP + 1u); ++k)
         issue_part(b + S - 1u, before, k);
       __builtin_amdgcn_sched_barrier(0);
     }
