@@ -10,6 +10,9 @@ shared expert as id E in the last slot, which is not counted.
     r = balance_loss(logits, topk_ids, coefficient=0.01)
     r.loss, r.counts, r.grad            # grad: with respect to logits, in their type
 
+Nothing is recorded by autograd: r.grad goes to logits.backward(r.grad) of a caller
+whose router torch differentiates.
+
 Over several ranks the loss uses the whole job's counts: sum expert_counts()
 over the ranks and pass the result as counts=.
 """

@@ -17,7 +17,7 @@ BF16, F32 = torch.bfloat16, torch.float32
 SHAPES = [(1, 128, 128), (1, 2048, 2048), (1, 5, 7), (1, 320, 16384), (2, 130, 257), (5, 576, 512), (15, 16, 128),
           (16, 256, 640), (17, 1000, 333), (33, 129, 2048), (48, 64, 100), (64, 512, 2048), (65, 264, 384),
           (100, 2048, 512), (127, 127, 127), (128, 128, 1024), (130, 1, 300), (200, 3, 1000), (256, 256, 256),
-          (257, 513, 1025), (300, 1024, 640), (513, 384, 200), (700, 1030, 520), (1024, 512, 130)]
+          (257, 513, 1025), (300, 1024, 640), (513, 384, 200), (700, 1030, 520), (1024, 512, 130), (40, 7, 1), (90, 1, 1)]
 
 
 def layer(n, k, seed, gradients=False):
@@ -44,6 +44,21 @@ def test_gradients(T, N, K, dt):
     assert dx.dtype == BF16 and dw.dtype == F32
     C.assert_within(dx, *C.product(C.quantised(dy, 1), w.t().contiguous()), "dx")
     C.assert_within(dw, *C.outer(dy, x), "dw")
+
+
+# sizes that take the largest tiles, with ragged last ones
+@pytest.mark.parametrize("T,N,K", [(4095, 4097, 257), (4100, 4000, 100), (1500, 4001, 260)])
+def test_forward_of_many_tiles(T, N, K):
+    lin, w = layer(N, K, seed=T)
+    x = C.activations(T, K, seed=T)
+    C.assert_within(lin.forward(x.to(DEV)), *C.product(C.quantised(x, 1), w))
+
+
+@pytest.mark.parametrize("T,N,K", [(130, 4001, 3999), (70, 4000, 4000), (1300, 2050, 2050)])
+def test_weight_gradient_of_many_tiles(T, N, K):
+    lin, _ = layer(N, K, seed=T)
+    x, dy = C.activations(T, K, seed=T), C.activations(T, N, seed=T + 1, std=1e-3)
+    C.assert_within(lin.weight_gradient(dy.to(DEV), x.to(DEV)), *C.outer(dy, x))
 
 
 def test_weight_gradient_of_mixed_types():
