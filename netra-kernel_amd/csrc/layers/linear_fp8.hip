@@ -786,9 +786,11 @@ __device__ __forceinline__ void outer_tile(const Outer& a, uint32_t group, uint8
       for (uint32_t j = 0; j < NQ; ++j)
         acc[i % NP][j] =
             __builtin_amdgcn_mfma_f32_16x16x32_bf16(po[i & 1u], qo[i / NP][j], acc[i % NP][j], 0, 0, 0);
-      // the copies of a later step, spread over this one's products
+      // the copies of a later step, spread over this one's products (with two stages, where
+      // they are the next step's, over the first half of them)
+      constexpr uint32_t kOver = S == 2u ? NP : 2u * NP;
 #pragma unroll
-      for (uint32_t k = i * kCopies / (2u * NP); k < (i + 1u) * kCopies / (2u * NP); ++k)
+      for (uint32_t k = min(kOver, i) * kCopies / kOver; k < min(kOver, i + 1u) * kCopies / kOver; ++k)
         issue_part(t + (S - 1u) * kTokens, before, k);
       __builtin_amdgcn_sched_barrier(0);
     }
