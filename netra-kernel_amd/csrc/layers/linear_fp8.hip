@@ -20,10 +20,6 @@ using nk::u32x4;
 using nk::v4f;
 using nk::v8i;
 
-// One activation value as fp32.
-__device__ __forceinline__ float value(const uint16_t* p) { return nk::bf16_f32(*p); }
-__device__ __forceinline__ float value(const float* p) { return *p; }
-
 // Scale of a 128-group from the largest magnitude's bits (as an unsigned
 // integer, a NaN's magnitude is above infinity's, so the maximum keeps it). A
 // group with an infinity or NaN gets a NaN scale.
@@ -143,10 +139,10 @@ __device__ __forceinline__ void store_tile(uint8_t* tile, uint32_t lane, const u
 // large copy: 5.1); 1001 x 1111 fp32 4.9 us, 64 x 2048 bf16 2.5 us (a launch).
 template <typename X>
 __device__ __forceinline__ void quant_rows(const X* __restrict__ x, uint64_t stride, uint8_t* __restrict__ q,
-                                           float* __restrict__ s, uint32_t rows, uint32_t n, uint32_t sld) {
+                                           float* __restrict__ s, uint32_t rows, uint32_t n, uint32_t sld,
+                                           uint32_t rt, uint32_t b4) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t kb = (n + 127u) / 128u;
-  const uint32_t rt = blockIdx.x, b = blockIdx.y * 4u + wave;
+  const uint32_t kb = (n + 127u) / 128u, b = b4 * 4u + wave;
   if (b >= kb) return;
   const uint32_t r = rt * 16u + (lane & 15u), c = b * 128u + (lane >> 4) * 32u;
   Raw<X> v = {};
@@ -687,8 +683,10 @@ struct Outer {
 // less, by waves of 64 x 128 over one half of a step's tokens each and a sum of the halves
 // at the end (144 KiB per step), takes 62.5 us, and 9.0 us instead of 8.3 at T 333, N 1024, K
 // 2048: the longer wait for a step's first operands costs as much. Two groups of waves in
-// turn, product_turns' way, take 76 us. 256x256 at T 8192, N 4096, K 4096: 230 us, of which
-// its stores, which nothing hides with one workgroup per CU, are 30.
+// turn, product_turns' way, take 76 us, steps of 32 tokens in six stages 70, operands read two tiles ahead the same
+// 62. 256x256 at T 8192, N 4096, K 4096: 216 us (1.27 PFLOP/s), with its two stages' copies
+// spread over the whole step 230; about 30 are its stores, which nothing hides with one
+// workgroup per CU, and with all copies from lines the cache holds it takes 40 less.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 constexpr uint32_t outer_lds() {
   return S * 64u * 32u * (WP * NP + WQ * NQ);
@@ -843,22 +841,68 @@ __device__ __forceinline__ void outer_sum(const Outer& a) {
   }
 }
 
-// A matrix as bf16 with rows of `pitch` elements (a multiple of 8), for operands
-// that are fp32 or not aligned.
-template <typename X>
-__device__ __forceinline__ void to_bf16(const X* __restrict__ x, uint64_t stride, uint16_t* __restrict__ out,
-                                        uint32_t rows, uint32_t cols, uint32_t pitch) {
-  const uint32_t c = (blockIdx.x * 64u + (threadIdx.x & 63u)) * 8u;
-  if (c >= pitch) return;
-  for (uint32_t r = blockIdx.y * 4u + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4u) {
-    const X* p = x + (uint64_t)r * stride + c;
-    uint32_t w[4];
+// A matrix as bf16 with rows of `pitch` elements (a multiple of 8, zeros behind the columns), for
+// operands that are fp32 or not aligned. Group g of `groups`: four rows and 512 columns at a time.
+struct Copy {
+  const void* m;
+  uint64_t stride;
+  uint16_t* out;
+  uint32_t type, cols, pitch, groups;  // groups: a multiple of pitch / 512 rounded up, or 0
+};
+__device__ __forceinline__ void pack8(const uint16_t* p, uint32_t left, uint32_t (&w)[4]) {
+  if (left >= 8u) {
+    const Unaligned16 u = *reinterpret_cast<const Unaligned16*>(p);
 #pragma unroll
-    for (uint32_t e = 0; e < 4u; ++e)
-      w[e] = nk::bf16x2_hw(c + 2u * e < cols ? value(p + 2u * e) : 0.0f,
-                           c + 2u * e + 1u < cols ? value(p + 2u * e + 1u) : 0.0f);
-    *reinterpret_cast<uint4*>(out + (uint64_t)r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (uint32_t e = 0; e < 4u; ++e) w[e] = u.w[e];
+    return;
   }
+#pragma unroll
+  for (uint32_t e = 0; e < 8u; ++e)
+    if (e < left) w[e / 2u] |= (uint32_t)p[e] << (16u * (e & 1u));
+}
+__device__ __forceinline__ void pack8(const float* p, uint32_t left, uint32_t (&w)[4]) {
+  float v[8] = {};
+  if (left >= 8u) {
+    const Unaligned16 lo = *reinterpret_cast<const Unaligned16*>(p), hi = *reinterpret_cast<const Unaligned16*>(p + 4);
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e) {
+      v[e] = __uint_as_float(lo.w[e]);
+      v[e + 4u] = __uint_as_float(hi.w[e]);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8u; ++e)
+      if (e < left) v[e] = p[e];
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 4u; ++e) w[e] = nk::bf16x2_hw(v[2u * e], v[2u * e + 1u]);
+}
+template <typename X>
+__device__ __forceinline__ void to_bf16(const Copy& a, uint32_t rows, uint32_t g) {
+  const uint32_t across = (a.pitch + 511u) / 512u, c = (g % across * 64u + (threadIdx.x & 63u)) * 8u;
+  if (c >= a.pitch) return;
+  for (uint32_t r = g / across * 4u + (threadIdx.x >> 6); r < rows; r += a.groups / across * 4u) {
+    uint32_t w[4] = {};
+    if (c < a.cols) pack8(static_cast<const X*>(a.m) + (uint64_t)r * a.stride + c, a.cols - c, w);
+    *reinterpret_cast<uint4*>(a.out + (uint64_t)r * a.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ void to_bf16(const Copy& a, uint32_t rows, uint32_t g) {
+  if (a.type == NETRA_F32) to_bf16<float>(a, rows, g);
+  else to_bf16<uint16_t>(a, rows, g);
+}
+
+// What a backward pass needs made of dy and x, in one launch: dy quantised (`quant` workgroups,
+// quant_rows's grid of row tiles first), then the copies.
+template <typename X>
+__device__ __forceinline__ void prepare(const X* dy, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n,
+                                        uint32_t sld, uint32_t quant, const Copy& a, const Copy& b) {
+  uint32_t g = blockIdx.x;
+  const uint32_t tiles = (rows + 15u) / 16u;
+  if (g < quant) return quant_rows(dy, stride, q, s, rows, n, sld, g % tiles, g / tiles);
+  g -= quant;
+  if (g < a.groups) to_bf16(a, rows, g);
+  else to_bf16(b, rows, g - a.groups);
 }
 
 }  // namespace nklin
@@ -930,11 +974,11 @@ extern "C" __global__ __launch_bounds__(256) void netra_linear_pack_transposed_g
 
 extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_bf16_gfx950(
     const uint16_t* x, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld) {
-  nklin::quant_rows(x, stride, q, s, rows, n, sld);
+  nklin::quant_rows(x, stride, q, s, rows, n, sld, blockIdx.x, blockIdx.y);
 }
 extern "C" __global__ __launch_bounds__(256) void netra_linear_quant_rows_f32_gfx950(
     const float* x, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld) {
-  nklin::quant_rows(x, stride, q, s, rows, n, sld);
+  nklin::quant_rows(x, stride, q, s, rows, n, sld, blockIdx.x, blockIdx.y);
 }
 
 #define NETRA_PRODUCT_TILE(P, Q, ...)                                                                             \
@@ -995,16 +1039,14 @@ extern "C" __global__ __launch_bounds__(512) void netra_linear_backward_small_gf
 }
 extern "C" __global__ __launch_bounds__(256) void netra_linear_outer_sum_gfx950(nklin::Outer a) { nklin::outer_sum(a); }
 
-extern "C" __global__ __launch_bounds__(256) void netra_linear_to_bf16_f32_gfx950(const float* x, uint64_t stride,
-                                                                                  uint16_t* out, uint32_t rows,
-                                                                                  uint32_t cols, uint32_t pitch) {
-  nklin::to_bf16<float>(x, stride, out, rows, cols, pitch);
-}
-extern "C" __global__ __launch_bounds__(256) void netra_linear_to_bf16_bf16_gfx950(const uint16_t* x, uint64_t stride,
-                                                                                   uint16_t* out, uint32_t rows,
-                                                                                   uint32_t cols, uint32_t pitch) {
-  nklin::to_bf16<uint16_t>(x, stride, out, rows, cols, pitch);
-}
+#define NETRA_PREPARE(NAME, X)                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void netra_linear_prepare_##NAME##_gfx950(                        \
+      const X* dy, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n, uint32_t sld, uint32_t quant, \
+      nklin::Copy a, nklin::Copy b) {                                                                             \
+    nklin::prepare(dy, stride, q, s, rows, n, sld, quant, a, b);                                                  \
+  }
+NETRA_PREPARE(bf16, uint16_t)
+NETRA_PREPARE(f32, float)
 
 // dw of no tokens: zeros.
 extern "C" __global__ __launch_bounds__(256) void netra_linear_zero_gfx950(float* out, uint64_t n) {

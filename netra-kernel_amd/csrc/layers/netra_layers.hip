@@ -175,18 +175,13 @@ bool outer_ready(const void* m, uint32_t type, uint64_t stride, uint32_t cols) {
 uint64_t outer_bytes(const void* m, uint32_t type, uint64_t stride, uint32_t rows, uint32_t cols) {
   return outer_ready(m, type, stride, cols) ? 0 : static_cast<uint64_t>(rows) * up(cols, 8u) * 2u;
 }
+// Its pointer, and the copy that has to be made of it, if any.
 const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, uint32_t rows, uint32_t& cols,
-                              uint8_t*& at, hipStream_t stream) {
+                              uint8_t*& at, nklin::Copy& copy) {
   if (outer_ready(m, type, stride, cols)) return static_cast<const uint16_t*>(m);
-  const uint32_t pitch = up(cols, 8u);
-  const dim3 grid((pitch + 511u) / 512u, rows < 4u * 4096u ? (rows + 3u) / 4u : 4096u);
+  const uint32_t pitch = up(cols, 8u), down = rows < 4u * 4096u ? (rows + 3u) / 4u : 4096u;
   uint16_t* out = reinterpret_cast<uint16_t*>(at);
-  if (type == NETRA_F32)
-    netra_linear_to_bf16_f32_gfx950<<<grid, dim3(256), 0, stream>>>(static_cast<const float*>(m), stride, out, rows,
-                                                                    cols, pitch);
-  else
-    netra_linear_to_bf16_bf16_gfx950<<<grid, dim3(256), 0, stream>>>(static_cast<const uint16_t*>(m), stride, out,
-                                                                     rows, cols, pitch);
+  copy = {m, stride, out, type, cols, pitch, (pitch + 511u) / 512u * down};
   at += static_cast<uint64_t>(rows) * pitch * 2u;
   stride = cols = pitch;
   return out;
@@ -196,7 +191,7 @@ const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, ui
 // 1.55 us, 128x256 0.93, 128x128 0.48, one workgroup per CU each). As whole calls, best and
 // next: T 333, N 1024, K 2048 128x128 8.3 us, 128x256 11.8; T 4096, N 4096, K 2048 128x256 64,
 // 128x128 82; T 4096, N 1024, K 1024 128x128 in four splits 21.3, in two 23.9; T 8192, N 4096,
-// K 4096 256x256 231, 128x256 249.
+// K 4096 256x256 216, 128x256 249.
 struct OuterPlan {
   uint32_t p, q;  // columns of x and of dy per workgroup
   uint32_t splits, split_rows;
@@ -286,9 +281,7 @@ static int check(const ProductCall& c) {
   return 0;
 }
 
-// Everything in front of the tile kernels (which it leaves to the caller: true), or all of the call.
-static bool begin(const ProductCall& c, const ProductPlan& plan, uint8_t* workspace, nklin::Product& a,
-                  hipStream_t stream) {
+static void set_up(const ProductCall& c, const ProductPlan& plan, uint8_t* workspace, nklin::Product& a) {
   a.p = c.packed;
   a.sp = c.scale;
   a.sp_i = c.sp_i;
@@ -301,27 +294,17 @@ static bool begin(const ProductCall& c, const ProductPlan& plan, uint8_t* worksp
   a.kb = blocks(c.nc);
   a.splits = plan.splits;
   a.split_blocks = plan.split_blocks;
-  if (plan.form == kFused) {
-    if (c.in_type == NETRA_BF16)
-      product_fused(a, static_cast<const uint16_t*>(c.in), c.in_stride, c.nc, stream);
-    else product_fused(a, static_cast<const float*>(c.in), c.in_stride, c.nc, stream);
-    return false;
-  }
-  float* s = reinterpret_cast<float*>(workspace + code_bytes(c.rows, c.nc));
-  quant_rows(c.in, c.in_type, c.in_stride, workspace, s, c.rows, c.nc, stream);
+  if (plan.form == kFused) return;
   a.q = workspace;
-  a.sq = s;
+  a.sq = reinterpret_cast<float*>(workspace + code_bytes(c.rows, c.nc));
   a.sq_b = up(c.rows, 16u);
-  if (plan.form == kStream) {
-    const uint32_t pt = (c.ni + 15u) / 16u;
-    const bool wide = pt >= 512u;  // the activations are read half as often (T 64, N 8192, K 8192: 24.1 us -> 20.3)
-    const dim3 grid(wide ? (pt + 1u) / 2u : pt), block(512);
-    if (wide) netra_linear_product_stream_p2q4_gfx950<<<grid, block, 0, stream>>>(a);
-    else netra_linear_product_stream_p1q4_gfx950<<<grid, block, 0, stream>>>(a);
-    return false;
-  }
   a.partial = reinterpret_cast<float*>(workspace + (matrix_bytes(c.rows, c.nc) + 15u) / 16u * 16u);
-  return true;
+}
+
+static void quantise(const ProductCall& c, const ProductPlan& plan, uint8_t* workspace, hipStream_t stream) {
+  if (plan.form != kFused)
+    quant_rows(c.in, c.in_type, c.in_stride, workspace, reinterpret_cast<float*>(workspace + code_bytes(c.rows, c.nc)),
+               c.rows, c.nc, stream);
 }
 
 static uint32_t groups_of(const nklin::Product& a, const ProductPlan& plan) {
@@ -329,8 +312,22 @@ static uint32_t groups_of(const nklin::Product& a, const ProductPlan& plan) {
   return (items + 7u) / 8u * 8u;
 }
 
-static void run_tiles(const nklin::Product& a, const ProductPlan& plan, hipStream_t stream) {
-  const dim3 grid(groups_of(a, plan)), block(512);
+static void run(const ProductCall& c, const nklin::Product& a, const ProductPlan& plan, hipStream_t stream) {
+  if (plan.form == kFused) {
+    if (c.in_type == NETRA_BF16)
+      return product_fused(a, static_cast<const uint16_t*>(c.in), c.in_stride, c.nc, stream);
+    return product_fused(a, static_cast<const float*>(c.in), c.in_stride, c.nc, stream);
+  }
+  const dim3 block(512);
+  if (plan.form == kStream) {
+    const uint32_t pt = (a.ni + 15u) / 16u;
+    const bool wide = pt >= 512u;  // the activations are read half as often (T 64, N 8192, K 8192: 24.1 us -> 20.3)
+    const dim3 grid(wide ? (pt + 1u) / 2u : pt);
+    if (wide) netra_linear_product_stream_p2q4_gfx950<<<grid, block, 0, stream>>>(a);
+    else netra_linear_product_stream_p1q4_gfx950<<<grid, block, 0, stream>>>(a);
+    return;
+  }
+  const dim3 grid(groups_of(a, plan));
   if (plan.p == 256u && plan.q == 256u) netra_linear_product_256x256_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.p == 256u) netra_linear_product_256x128_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.q == 128u) netra_linear_product_128x128_gfx950<<<grid, block, 0, stream>>>(a);
@@ -353,7 +350,9 @@ static int times_weights(const ProductCall& c, void* workspace, uint64_t workspa
     return fail(-1, c.name, "workspace too small, null or not 16-byte aligned");
   const ProductPlan plan = product_plan(c.rows, c.ni, c.nc, c.in_type);
   nklin::Product a{};
-  if (begin(c, plan, static_cast<uint8_t*>(workspace), a, stream)) run_tiles(a, plan, stream);
+  set_up(c, plan, static_cast<uint8_t*>(workspace), a);
+  quantise(c, plan, static_cast<uint8_t*>(workspace), stream);
+  run(c, a, plan, stream);
   return launched(c.name);
 }
 
@@ -403,13 +402,14 @@ static uint64_t outer_workspace(const OuterCall& c, const OuterPlan& plan) {
          partial_bytes(plan, c.n, c.k);
 }
 
-static void begin(const OuterCall& c, const OuterPlan& plan, uint8_t* workspace, nklin::Outer& a, hipStream_t stream) {
+static void set_up(const OuterCall& c, const OuterPlan& plan, uint8_t* workspace, nklin::Outer& a,
+                   nklin::Copy (&copies)[2]) {
   a.dy_stride = c.dy_stride;
   a.dy_cols = c.n;
-  a.dy = outer_operand(c.dy, c.dy_type, a.dy_stride, c.rows, a.dy_cols, workspace, stream);
+  a.dy = outer_operand(c.dy, c.dy_type, a.dy_stride, c.rows, a.dy_cols, workspace, copies[0]);
   a.x_stride = c.x_stride;
   a.x_cols = c.k;
-  a.x = outer_operand(c.x, c.x_type, a.x_stride, c.rows, a.x_cols, workspace, stream);
+  a.x = outer_operand(c.x, c.x_type, a.x_stride, c.rows, a.x_cols, workspace, copies[1]);
   a.dw = c.dw;
   a.rows = c.rows;
   a.n = c.n;
@@ -420,12 +420,26 @@ static void begin(const OuterCall& c, const OuterPlan& plan, uint8_t* workspace,
   a.partial = reinterpret_cast<float*>(workspace);
 }
 
+// The operands' copies, with dy's quantisation (to `codes`, or null) in the same launch.
+static void prepare(const OuterCall& c, const nklin::Copy (&copies)[2], uint8_t* codes, hipStream_t stream) {
+  const uint32_t quant = codes ? (c.rows + 15u) / 16u * ((blocks(c.n) + 3u) / 4u) : 0u;
+  const dim3 grid(quant + copies[0].groups + copies[1].groups), block(256);
+  float* s = codes ? reinterpret_cast<float*>(codes + code_bytes(c.rows, c.n)) : nullptr;
+  const uint32_t sld = up(c.rows, 16u);
+  if (c.dy_type == NETRA_BF16)
+    netra_linear_prepare_bf16_gfx950<<<grid, block, 0, stream>>>(static_cast<const uint16_t*>(c.dy), c.dy_stride, codes,
+                                                                 s, c.rows, c.n, sld, quant, copies[0], copies[1]);
+  else
+    netra_linear_prepare_f32_gfx950<<<grid, block, 0, stream>>>(static_cast<const float*>(c.dy), c.dy_stride, codes, s,
+                                                                c.rows, c.n, sld, quant, copies[0], copies[1]);
+}
+
 static uint32_t groups_of(const nklin::Outer& a, const OuterPlan& plan) {
   const uint32_t items = ((a.k + plan.p - 1u) / plan.p) * ((a.n + plan.q - 1u) / plan.q) * plan.splits;
   return (items + 7u) / 8u * 8u;
 }
 
-static void run_tiles(const nklin::Outer& a, const OuterPlan& plan, hipStream_t stream) {
+static void run(const nklin::Outer& a, const OuterPlan& plan, hipStream_t stream) {
   const dim3 grid(groups_of(a, plan)), block(512);
   if (plan.p == 256u) netra_linear_outer_256x256_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.q == 256u) netra_linear_outer_128x256_gfx950<<<grid, block, 0, stream>>>(a);
@@ -461,8 +475,10 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
   if (bad_workspace(workspace, workspace_bytes, outer_workspace(c, plan)))
     return fail(-1, c.name, "workspace too small, null or not 16-byte aligned");
   nklin::Outer a{};
-  begin(c, plan, static_cast<uint8_t*>(workspace), a, stream);
-  run_tiles(a, plan, stream);
+  nklin::Copy copies[2] = {};
+  set_up(c, plan, static_cast<uint8_t*>(workspace), a, copies);
+  if (copies[0].groups + copies[1].groups) prepare(c, copies, nullptr, stream);
+  run(a, plan, stream);
   return launched(c.name);
 }
 
@@ -500,14 +516,17 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   if (small) product.p = product.q = 64u;
   nklin::Product a{};
   nklin::Outer b{};
-  const bool tiles = begin(p, product, ws, a, stream);
-  begin(o, outer, ws + first, b, stream);
+  nklin::Copy copies[2] = {};
+  set_up(p, product, ws, a);
+  set_up(o, outer, ws + first, b, copies);
+  if (copies[0].groups + copies[1].groups) prepare(o, copies, product.form == kFused ? nullptr : ws, stream);
+  else quantise(p, product, ws, stream);
   if (small) {
     const uint32_t groups = groups_of(b, outer);
     netra_linear_backward_small_gfx950<<<dim3(groups + groups_of(a, product)), dim3(512), 0, stream>>>(a, b, groups);
   } else {
-    if (tiles) run_tiles(a, product, stream);
-    run_tiles(b, outer, stream);
+    run(p, a, product, stream);
+    run(b, outer, stream);
   }
   return launched(name);
 }
