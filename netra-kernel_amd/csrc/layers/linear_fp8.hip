@@ -1028,8 +1028,8 @@ NETRA_OUTER_TILE(128, 256, 2, 4, 4, 4, 3)
 NETRA_OUTER_TILE(128, 128, 2, 4, 4, 2, 4)
 // Both products of a small backward pass in one launch, the weight gradient's
 // workgroups (the first `outer`, a multiple of 8) with their longer way first: neither
-// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 13.9 us, 11.1 of it this
-// kernel; in two launches 18.1).
+// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 13.3 us, 10.0 of it this
+// kernel; in two launches 16.9).
 extern "C" __global__ __launch_bounds__(512) void netra_linear_backward_small_gfx950(nklin::Product a, nklin::Outer b,
                                                                                      uint32_t outer) {
   constexpr uint32_t kP = nklin::Tile<4, 2, 1, 2, 4>::kLds, kO = nklin::outer_lds<2, 4, 4, 2, 4>();

@@ -439,16 +439,18 @@ static uint32_t groups_of(const nklin::Outer& a, const OuterPlan& plan) {
   return (items + 7u) / 8u * 8u;
 }
 
+static void sum(const nklin::Outer& a, hipStream_t stream) {
+  if (a.splits == 1u) return;
+  const uint64_t quads = (static_cast<uint64_t>(a.n) * a.k + 1023u) / 1024u;
+  netra_linear_outer_sum_gfx950<<<dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), 0, stream>>>(a);
+}
+
 static void run(const nklin::Outer& a, const OuterPlan& plan, hipStream_t stream) {
   const dim3 grid(groups_of(a, plan)), block(512);
   if (plan.p == 256u) netra_linear_outer_256x256_gfx950<<<grid, block, 0, stream>>>(a);
   else if (plan.q == 256u) netra_linear_outer_128x256_gfx950<<<grid, block, 0, stream>>>(a);
   else netra_linear_outer_128x128_gfx950<<<grid, block, 0, stream>>>(a);
-  if (plan.splits > 1u) {
-    const uint64_t quads = (static_cast<uint64_t>(a.n) * a.k + 1023u) / 1024u;
-    netra_linear_outer_sum_gfx950<<<dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), 0, stream>>>(
-        a);
-  }
+  sum(a, stream);
 }
 
 // Sizes and dw, and the call without tokens: 0 or an error to return, or 1 to go on.
@@ -510,9 +512,11 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   if (bad_workspace(workspace, workspace_bytes, first + outer_workspace(o, outer)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  // Small passes run both products in one launch.
+  // Passes of small tiles run both products in one launch (T 333, N 1024, K 2048 13.3 us, in two
+  // 16.9; T 3584, N 360, K 189 16.3, 20.7; T 1200, N 1000, K 1000 18.3, 24.5; T 3000, N 500, K 500
+  // 21.3, 24.1); with larger tiles most lose by it (T 5000, N 600, K 1000 36.6, 33.5).
   const bool small = product.form == kTiles && product.p * product.q <= 128u * 64u && product.splits == 1u &&
-                     outer.p * outer.q == 128u * 128u && outer.splits == 1u;
+                     outer.p * outer.q == 128u * 128u;
   if (small) product.p = product.q = 64u;
   nklin::Product a{};
   nklin::Outer b{};
@@ -524,6 +528,7 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   if (small) {
     const uint32_t groups = groups_of(b, outer);
     netra_linear_backward_small_gfx950<<<dim3(groups + groups_of(a, product)), dim3(512), 0, stream>>>(a, b, groups);
+    sum(b, stream);
   } else {
     run(p, a, product, stream);
     run(b, outer, stream);

@@ -296,3 +296,13 @@ def test_backward_is_both_gradients(T, N, K):
     assert lin.backward(dy, x, acc, accumulate=True)[1] is acc and torch.equal(acc, dw + dw)
     with pytest.raises(ValueError, match="gradients=True"):
         layer(N, K, seed=32)[0].backward(dy, x)
+
+
+@pytest.mark.parametrize("T,N,K", [(3, 40, 60), (40, 255, 130), (200, 129, 250), (2000, 256, 127)])
+@pytest.mark.parametrize("dt,xt", [(F32, BF16), (BF16, F32)])
+def test_backward_of_mixed_types(T, N, K, dt, xt):
+    lin, w = layer(N, K, seed=35, gradients=True)
+    x, dy = C.activations(T, K, seed=36, dtype=xt), C.activations(T, N, seed=37, dtype=dt)
+    dx, dw = lin.backward(dy.to(DEV), x.to(DEV))
+    C.assert_within(dx, *C.product(C.quantised(dy, 1), w.t().contiguous()), "dx")
+    C.assert_within(dw, *C.outer(dy, x), "dw")
