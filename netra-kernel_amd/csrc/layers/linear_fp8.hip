@@ -426,7 +426,8 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
 // T 8192, N 8192, K 4096 with the quantisation: 243 us (2.26 PFLOP/s; the library's product
 // without block scales and without the quantisation 212 us). All waves in step,
 // product_tile's way, take 4% longer, without whole-tile copies 2%, with the copies spread over
-// both groups' products 7%, with Q's operands straight from L2 to registers 18%. About 60 us go
+// both groups' products 7%, with Q's operands straight from L2 to registers 18%. (256x128 in turns is
+// slower, 47.8 us against 41.5 at T 2048, N 4096, K 4096: its phases are 16 products long.) About 60 us go
 // with the copies (timed without them).
 __device__ __forceinline__ void product_turns(const Product& a, uint32_t index, uint8_t* s_stage) {
   using L = Tile<2, 4, 8, 4, 2>;
