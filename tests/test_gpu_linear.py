@@ -306,3 +306,21 @@ def test_backward_of_mixed_types(T, N, K, dt, xt):
     dx, dw = lin.backward(dy.to(DEV), x.to(DEV))
     C.assert_within(dx, *C.product(C.quantised(dy, 1), w.t().contiguous()), "dx")
     C.assert_within(dw, *C.outer(dy, x), "dw")
+
+
+@pytest.mark.parametrize("T,N,K,dt", [(2000, 255, 130, BF16), (300, 129, 250, F32), (30, 40, 61, F32)])
+def test_captured_backward_with_copies_and_splits(T, N, K, dt):
+    lin, _ = layer(N, K, seed=38, gradients=True)
+    x, dy = C.activations(T, K, seed=39, dtype=dt).to(DEV), C.activations(T, N, seed=40, dtype=dt).to(DEV)
+    lin.backward(dy, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, dw = lin.backward(dy, x)
+    for i in range(4):
+        x.copy_(C.activations(T, K, seed=50 + i, dtype=dt))
+        dy.copy_(C.activations(T, N, seed=60 + i, dtype=dt))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((dx, dw), lin.backward(dy, x)):
+            assert torch.equal(a, b)
