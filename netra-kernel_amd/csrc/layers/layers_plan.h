@@ -60,20 +60,26 @@ inline ProductPlan product_tiles(uint32_t rows, uint32_t ni, uint32_t nc) {
 
 inline ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc, bool bf16) {
   if (rows > 64u) return product_tiles(rows, ni, nc);
-  // Quantising on the way saves a launch (10.7 us -> 6.7 at one row) and costs every
-  // workgroup the quantisation of its waves' blocks: 16-row tiles x blocks per wave x
-  // workgroups per CU, of which seven cost what the launch does (T 48, N 4096, K 2048, six:
-  // 10.3 us against 10.7; T 64, eight: 11.7 against 10.8; T 32, N 8192, K 8192, sixteen: 23.5
-  // against 17.5). One tile of rows always quantises on the way: at worst it costs 3% (T 16, N
-  // 28672, K 8192: 50.5 us, with the launch 49.0), few rows gain most (T 1: 40.2 against 48.6).
-  const uint32_t pt = (ni + 15u) / 16u, q = (rows + 15u) / 16u;
-  const uint32_t groups = pt >= 512u ? (pt + 1u) / 2u : pt;
-  const uint64_t cost = static_cast<uint64_t>((groups + 255u) / 256u) * q * ((blocks(nc) + 7u) / 8u);
   // Two tiles of columns per workgroup: fused they halve the quantisation (T 16, N 8192, K 8192:
   // 21.7 us -> 16.2; of more than two tiles of rows they do not fit the registers), else the
   // activations are read half as often (T 64, N 8192, K 8192: 24.1 us -> 20.3).
-  const uint32_t wide = pt >= 512u ? 2u : 1u;
-  if (q == 1u || (cost < 8u && (q == 2u || bf16))) return {kFused, q <= 2u ? wide : 1u, q <= 2u ? q : 4u, 1, 0};
+  const uint32_t pt = (ni + 15u) / 16u, q = (rows + 15u) / 16u, kb = blocks(nc), wide = pt >= 512u ? 2u : 1u;
+  const uint32_t p = q <= 2u ? wide : 1u;  // of a fused workgroup
+  // Quantising on the way saves a launch (10.7 us -> 6.7 at one row) and costs every
+  // workgroup the quantisation of its waves' blocks. One tile of rows always quantises on the
+  // way: at worst it costs 3% (T 16, N 28672, K 8192: 50.5 us, with the launch 49.0), few rows
+  // gain most (T 1: 40.2 against 48.6). Two do up to seven tile-blocks per wave and CU (T 32, N
+  // 8192, K 8192, sixteen: 23.5 against 17.5). With three or four a CU holds one workgroup at a
+  // time, and what pays falls with the rounds that the columns take (us, fused / with the launch):
+  //   one round      T 48, K 1152  9.1 / 10.3    K 2048 11.0 / 10.2    T 64, K 2048 12.1 / 10.4
+  //   N 8192, two    T 64, K 512  10.1 / 10.4    T 48, K 768 11.8 / 10.5    K 2048 20.0 / 10.4
+  //   N 12288        T 64, K 128  10.0 / 10.5    K 256  11.4 / 10.5
+  //   N 16384        T 48, K 128  11.8 / 10.4
+  const uint32_t rounds = ((pt + p - 1u) / p + 255u) / 256u, each = q * ((kb + 7u) / 8u);
+  const uint32_t all = q * (kb < 8u ? kb : (kb + 7u) / 8u * 8u);  // tile-blocks that a workgroup quantises
+  const bool few = q <= 2u ? static_cast<uint64_t>(rounds) * each < 8u
+                           : bf16 && all <= (rounds == 1u ? 48u : rounds == 2u ? 16u : rounds == 3u ? 4u : 0u);
+  if (q == 1u || few) return {kFused, p, q <= 2u ? q : 4u, 1, 0};
   return {kStream, wide, 4, 1, 0};
 }
 

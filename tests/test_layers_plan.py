@@ -73,3 +73,15 @@ def test_every_kernel_form_is_listed():
     assert {f[1:3] for f in F.BF16 if f[0] == "stream"} == streams
     assert {f[1:] for f in F.BF16 if f[0] == "tiles"} == {(*t, s) for t in tiles for s in (1, 2)}
     assert set(F.OUTER) == {(*t, s) for t in outer for s in (1, 2)}
+
+
+def test_quantising_on_the_way_counts_the_workgroups_that_it_launches(plan):
+    """33 to 64 rows are quantised on the way by workgroups of one tile of columns, however many
+    columns there are: 512 of them are two rounds, 1024 four."""
+    for rows, ni, nc in [(64, 8192, 1024), (48, 8192, 2048), (48, 16384, 1024), (40, 8190, 1100), (48, 16384, 128),
+                         (64, 32768, 128)]:
+        assert plan(("product", rows, ni, nc, 1))[0][:3] == ["stream", 2, 4], (rows, ni, nc)
+    for rows, ni, nc in [(48, 4096, 2048), (64, 4096, 1024), (64, 8192, 512), (48, 8192, 128), (64, 12288, 128)]:
+        assert plan(("product", rows, ni, nc, 1))[0][:3] == ["fused", 1, 4], (rows, ni, nc)
+    for rows, ni, nc in [(20, 8192, 1024), (32, 16384, 1024)]:
+        assert plan(("product", rows, ni, nc, 1))[0][:3] == ["fused", 2, 2], (rows, ni, nc)
