@@ -6,6 +6,7 @@
 
 #include <string>
 
+#include "../kernels/launch.h"
 #include "layers_plan.h"
 #include "linear_fp8.hip"
 #include "router_balance.hip"
@@ -26,12 +27,24 @@ int fail(int code, const char* name, const char* text) noexcept {
   return code;
 }
 
-int launched(const char* name) noexcept {
-  const hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return fail(static_cast<int>(err), name, hipGetErrorString(err));
-  g_error.clear();
-  return 0;
-}
+// The launches of one call: behind one that failed there are no more.
+class Launcher {
+ public:
+  explicit Launcher(hipStream_t stream) : stream_(stream) {}
+  template <typename... A>
+  void operator()(void (*kernel)(A...), dim3 grid, dim3 block, typename nk::Same<A>::type... args) noexcept {
+    if (status_ == hipSuccess) status_ = nk::launch_kernel(kernel, grid, block, stream_, args...);
+  }
+  int result(const char* name) noexcept {
+    if (status_ != hipSuccess) return fail(static_cast<int>(status_), name, hipGetErrorString(status_));
+    g_error.clear();
+    return 0;
+  }
+
+ private:
+  hipStream_t stream_;
+  hipError_t status_ = hipSuccess;
+};
 
 uint32_t elem(uint32_t type) { return type == NETRA_BF16 ? 2u : 4u; }
 bool aligned(const void* p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -67,15 +80,14 @@ bool share(const Span& a, const Span& b) {
 }
 
 void quant_rows(const void* x, uint32_t type, uint64_t stride, uint8_t* q, float* s, uint32_t rows, uint32_t n,
-                hipStream_t stream) {
+                Launcher& launch) {
   const dim3 grid((rows + 15u) / 16u, (blocks(n) + 3u) / 4u), block(256);
   const uint32_t sld = up(rows, 16u);
   if (type == NETRA_BF16)
-    netra_linear_quant_rows_bf16_gfx950<<<grid, block, 0, stream>>>(static_cast<const uint16_t*>(x), stride, q, s, rows,
-                                                                    n, sld);
+    launch(netra_linear_quant_rows_bf16_gfx950, grid, block, static_cast<const uint16_t*>(x), stride, q, s, rows, n,
+           sld);
   else
-    netra_linear_quant_rows_f32_gfx950<<<grid, block, 0, stream>>>(static_cast<const float*>(x), stride, q, s, rows, n,
-                                                                   sld);
+    launch(netra_linear_quant_rows_f32_gfx950, grid, block, static_cast<const float*>(x), stride, q, s, rows, n, sld);
 }
 
 uint64_t product_workspace(uint32_t rows, uint32_t ni, uint32_t nc, uint32_t in_type) {
@@ -88,16 +100,16 @@ uint64_t product_workspace(uint32_t rows, uint32_t ni, uint32_t nc, uint32_t in_
 
 template <typename X>
 void product_fused(const nklin::Product& a, const ProductPlan& plan, const X* x, uint64_t stride, uint32_t nc,
-                   hipStream_t stream) {
+                   Launcher& launch) {
   const dim3 grid(((a.ni + 15u) / 16u + plan.p - 1u) / plan.p), block(512);
 #define NETRA_RUN(P, Q)                                                                                          \
   do {                                                                                                           \
     if constexpr (sizeof(X) == 2)                                                                                \
-      netra_linear_product_fused_bf16_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);         \
-    else netra_linear_product_fused_f32_p##P##q##Q##_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);       \
+      launch(netra_linear_product_fused_bf16_p##P##q##Q##_gfx950, grid, block, a, x, stride, nc);                \
+    else launch(netra_linear_product_fused_f32_p##P##q##Q##_gfx950, grid, block, a, x, stride, nc);              \
   } while (0)
   if (plan.q == 4u) {
-    if constexpr (sizeof(X) == 2) netra_linear_product_fused_bf16_p1q4_gfx950<<<grid, block, 0, stream>>>(a, x, stride, nc);
+    if constexpr (sizeof(X) == 2) launch(netra_linear_product_fused_bf16_p1q4_gfx950, grid, block, a, x, stride, nc);
   } else if (plan.q == 2u && plan.p == 2u) NETRA_RUN(2, 2);
   else if (plan.q == 2u) NETRA_RUN(1, 2);
   else if (plan.p == 2u) NETRA_RUN(2, 1);
@@ -138,11 +150,12 @@ extern "C" int netra_linear_pack(const uint8_t* w, uint8_t* packed, uint32_t n, 
                                  hipStream_t stream) {
   if (!w || !packed || w == packed || !aligned(packed, 16) || bad_sizes(0, n, k))
     return fail(-1, "netra_linear_pack", "null, aliased or misaligned pointers, or n / k not in 1 .. 2^21");
+  Launcher launch(stream);
   if (transpose)
-    netra_linear_pack_transposed_gfx950<<<dim3((k + 63u) / 64u, blocks(n)), dim3(256), 0, stream>>>(w, packed, n, k);
+    launch(netra_linear_pack_transposed_gfx950, dim3((k + 63u) / 64u, blocks(n)), dim3(256), w, packed, n, k);
   else
-    netra_linear_pack_gfx950<<<dim3((n + 15u) / 16u, (blocks(k) + 3u) / 4u), dim3(256), 0, stream>>>(w, packed, n, k);
-  return launched("netra_linear_pack");
+    launch(netra_linear_pack_gfx950, dim3((n + 15u) / 16u, (blocks(k) + 3u) / 4u), dim3(256), w, packed, n, k);
+  return launch.result("netra_linear_pack");
 }
 
 extern "C" uint64_t netra_linear_forward_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t x_type) {
@@ -204,10 +217,10 @@ static void set_up(const ProductCall& c, const ProductPlan& plan, uint8_t* works
   a.partial = reinterpret_cast<float*>(workspace + (matrix_bytes(c.rows, c.nc) + 15u) / 16u * 16u);
 }
 
-static void quantise(const ProductCall& c, const ProductPlan& plan, uint8_t* workspace, hipStream_t stream) {
+static void quantise(const ProductCall& c, const ProductPlan& plan, uint8_t* workspace, Launcher& launch) {
   if (plan.form != kFused)
     quant_rows(c.in, c.in_type, c.in_stride, workspace, reinterpret_cast<float*>(workspace + code_bytes(c.rows, c.nc)),
-               c.rows, c.nc, stream);
+               c.rows, c.nc, launch);
 }
 
 static uint32_t groups_of(const nklin::Product& a, const ProductPlan& plan) {
@@ -215,28 +228,28 @@ static uint32_t groups_of(const nklin::Product& a, const ProductPlan& plan) {
   return (items + 7u) / 8u * 8u;
 }
 
-static void run(const ProductCall& c, const nklin::Product& a, const ProductPlan& plan, hipStream_t stream) {
+static void run(const ProductCall& c, const nklin::Product& a, const ProductPlan& plan, Launcher& launch) {
   if (plan.form == kFused) {
     if (c.in_type == NETRA_BF16)
-      return product_fused(a, plan, static_cast<const uint16_t*>(c.in), c.in_stride, c.nc, stream);
-    return product_fused(a, plan, static_cast<const float*>(c.in), c.in_stride, c.nc, stream);
+      return product_fused(a, plan, static_cast<const uint16_t*>(c.in), c.in_stride, c.nc, launch);
+    return product_fused(a, plan, static_cast<const float*>(c.in), c.in_stride, c.nc, launch);
   }
   const dim3 block(512);
   if (plan.form == kStream) {
     const dim3 grid(((a.ni + 15u) / 16u + plan.p - 1u) / plan.p);
-    if (plan.p == 2u) netra_linear_product_stream_p2q4_gfx950<<<grid, block, 0, stream>>>(a);
-    else netra_linear_product_stream_p1q4_gfx950<<<grid, block, 0, stream>>>(a);
+    if (plan.p == 2u) launch(netra_linear_product_stream_p2q4_gfx950, grid, block, a);
+    else launch(netra_linear_product_stream_p1q4_gfx950, grid, block, a);
     return;
   }
   const dim3 grid(groups_of(a, plan));
-  if (plan.p == 256u && plan.q == 256u) netra_linear_product_256x256_gfx950<<<grid, block, 0, stream>>>(a);
-  else if (plan.p == 256u) netra_linear_product_256x128_gfx950<<<grid, block, 0, stream>>>(a);
-  else if (plan.q == 128u) netra_linear_product_128x128_gfx950<<<grid, block, 0, stream>>>(a);
-  else if (plan.p == 128u) netra_linear_product_128x64_gfx950<<<grid, block, 0, stream>>>(a);
-  else netra_linear_product_64x64_gfx950<<<grid, block, 0, stream>>>(a);
+  if (plan.p == 256u && plan.q == 256u) launch(netra_linear_product_256x256_gfx950, grid, block, a);
+  else if (plan.p == 256u) launch(netra_linear_product_256x128_gfx950, grid, block, a);
+  else if (plan.q == 128u) launch(netra_linear_product_128x128_gfx950, grid, block, a);
+  else if (plan.p == 128u) launch(netra_linear_product_128x64_gfx950, grid, block, a);
+  else launch(netra_linear_product_64x64_gfx950, grid, block, a);
   if (plan.splits > 1u)
-    netra_linear_product_sum_gfx950<<<dim3((a.ni + 1023u) / 1024u, a.nq < 4096u ? a.nq : 4096u), dim3(256), 0, stream>>>(
-        a);
+    launch(netra_linear_product_sum_gfx950, dim3((a.ni + 1023u) / 1024u, a.nq < 4096u ? a.nq : 4096u), dim3(256),
+           a);
 }
 
 static int times_weights(const ProductCall& c, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
@@ -252,9 +265,10 @@ static int times_weights(const ProductCall& c, void* workspace, uint64_t workspa
   const ProductPlan plan = product_plan(c.rows, c.ni, c.nc, c.in_type == NETRA_BF16);
   nklin::Product a{};
   set_up(c, plan, static_cast<uint8_t*>(workspace), a);
-  quantise(c, plan, static_cast<uint8_t*>(workspace), stream);
-  run(c, a, plan, stream);
-  return launched(c.name);
+  Launcher launch(stream);
+  quantise(c, plan, static_cast<uint8_t*>(workspace), launch);
+  run(c, a, plan, launch);
+  return launch.result(c.name);
 }
 
 extern "C" int netra_linear_forward(const void* x, uint32_t x_type, uint64_t x_stride, const uint8_t* packed,
@@ -322,17 +336,17 @@ static void set_up(const OuterCall& c, const OuterPlan& plan, uint8_t* workspace
 }
 
 // The operands' copies, with dy's quantisation (to `codes`, or null) in the same launch.
-static void prepare(const OuterCall& c, const nklin::Copy (&copies)[2], uint8_t* codes, hipStream_t stream) {
+static void prepare(const OuterCall& c, const nklin::Copy (&copies)[2], uint8_t* codes, Launcher& launch) {
   const uint32_t quant = codes ? (c.rows + 15u) / 16u * ((blocks(c.n) + 3u) / 4u) : 0u;
   const dim3 grid(quant + copies[0].groups + copies[1].groups), block(256);
   float* s = codes ? reinterpret_cast<float*>(codes + code_bytes(c.rows, c.n)) : nullptr;
   const uint32_t sld = up(c.rows, 16u);
   if (c.dy_type == NETRA_BF16)
-    netra_linear_prepare_bf16_gfx950<<<grid, block, 0, stream>>>(static_cast<const uint16_t*>(c.dy), c.dy_stride, codes,
-                                                                 s, c.rows, c.n, sld, quant, copies[0], copies[1]);
+    launch(netra_linear_prepare_bf16_gfx950, grid, block, static_cast<const uint16_t*>(c.dy), c.dy_stride, codes,
+           s, c.rows, c.n, sld, quant, copies[0], copies[1]);
   else
-    netra_linear_prepare_f32_gfx950<<<grid, block, 0, stream>>>(static_cast<const float*>(c.dy), c.dy_stride, codes, s,
-                                                                c.rows, c.n, sld, quant, copies[0], copies[1]);
+    launch(netra_linear_prepare_f32_gfx950, grid, block, static_cast<const float*>(c.dy), c.dy_stride, codes, s,
+           c.rows, c.n, sld, quant, copies[0], copies[1]);
 }
 
 static uint32_t groups_of(const nklin::Outer& a, const OuterPlan& plan) {
@@ -340,28 +354,28 @@ static uint32_t groups_of(const nklin::Outer& a, const OuterPlan& plan) {
   return (items + 7u) / 8u * 8u;
 }
 
-static void sum(const nklin::Outer& a, hipStream_t stream) {
+static void sum(const nklin::Outer& a, Launcher& launch) {
   if (a.splits == 1u) return;
   const uint64_t quads = (static_cast<uint64_t>(a.n) * a.k + 1023u) / 1024u;
-  netra_linear_outer_sum_gfx950<<<dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), 0, stream>>>(a);
+  launch(netra_linear_outer_sum_gfx950, dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), a);
 }
 
-static void run(const nklin::Outer& a, const OuterPlan& plan, hipStream_t stream) {
+static void run(const nklin::Outer& a, const OuterPlan& plan, Launcher& launch) {
   const dim3 grid(groups_of(a, plan)), block(512);
-  if (plan.p == 256u) netra_linear_outer_256x256_gfx950<<<grid, block, 0, stream>>>(a);
-  else if (plan.q == 256u) netra_linear_outer_128x256_gfx950<<<grid, block, 0, stream>>>(a);
-  else netra_linear_outer_128x128_gfx950<<<grid, block, 0, stream>>>(a);
-  sum(a, stream);
+  if (plan.p == 256u) launch(netra_linear_outer_256x256_gfx950, grid, block, a);
+  else if (plan.q == 256u) launch(netra_linear_outer_128x256_gfx950, grid, block, a);
+  else launch(netra_linear_outer_128x128_gfx950, grid, block, a);
+  sum(a, launch);
 }
 
 // Sizes and dw, and the call without tokens: 0 or an error to return, or 1 to go on.
-static int outer_start(const OuterCall& c, hipStream_t stream) {
+static int outer_start(const OuterCall& c, Launcher& launch) {
   if (bad_sizes(c.rows, c.n, c.k)) return fail(-1, c.name, "sizes have to be 1 .. 2^21 (rows may be 0)");
   if (!c.dw || !aligned(c.dw, 4)) return fail(-1, c.name, "null or misaligned dw");
   if (c.rows != 0) return 1;
   if (!c.accumulate)
-    netra_linear_zero_gfx950<<<dim3(1024), dim3(256), 0, stream>>>(c.dw, static_cast<uint64_t>(c.n) * c.k);
-  return launched(c.name);
+    launch(netra_linear_zero_gfx950, dim3(1024), dim3(256), c.dw, static_cast<uint64_t>(c.n) * c.k);
+  return launch.result(c.name);
 }
 
 extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* x,
@@ -370,7 +384,8 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
                                             uint64_t workspace_bytes, hipStream_t stream) {
   const OuterCall c{"netra_linear_weight_gradient", dy, dy_type, dy_stride, x, x_type, x_stride, dw, accumulate, rows,
                     n, k};
-  int rc = outer_start(c, stream);
+  Launcher launch(stream);
+  int rc = outer_start(c, launch);
   if (rc != 1) return rc;
   rc = check(c);
   if (rc != 0) return rc;
@@ -380,9 +395,9 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
   nklin::Outer a{};
   nklin::Copy copies[2] = {};
   set_up(c, plan, static_cast<uint8_t*>(workspace), a, copies);
-  if (copies[0].groups + copies[1].groups) prepare(c, copies, nullptr, stream);
-  run(a, plan, stream);
-  return launched(c.name);
+  if (copies[0].groups + copies[1].groups) prepare(c, copies, nullptr, launch);
+  run(a, plan, launch);
+  return launch.result(c.name);
 }
 
 extern "C" uint64_t netra_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t dy_type,
@@ -399,7 +414,8 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   const char* name = "netra_linear_backward";
   const OuterCall o{name, dy, dy_type, dy_stride, x, x_type, x_stride, dw, accumulate, rows, n, k};
   const ProductCall p{name, dy, dy_type, dy_stride, packed_t, scale, 1u, blocks(k), dx, dx_stride, rows, k, n};
-  int rc = outer_start(o, stream);
+  Launcher launch(stream);
+  int rc = outer_start(o, launch);
   if (rc != 1) return rc;
   if ((rc = check(p)) != 0 || (rc = check(o)) != 0) return rc;
   const uint64_t dw_bytes = static_cast<uint64_t>(n) * k * 4u;
@@ -420,17 +436,17 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   nklin::Copy copies[2] = {};
   set_up(p, product, ws, a);
   set_up(o, outer, ws + first, b, copies);
-  if (copies[0].groups + copies[1].groups) prepare(o, copies, product.form == kFused ? nullptr : ws, stream);
-  else quantise(p, product, ws, stream);
+  if (copies[0].groups + copies[1].groups) prepare(o, copies, product.form == kFused ? nullptr : ws, launch);
+  else quantise(p, product, ws, launch);
   if (small) {
     const uint32_t groups = groups_of(b, outer);
-    netra_linear_backward_small_gfx950<<<dim3(groups + groups_of(a, product)), dim3(512), 0, stream>>>(a, b, groups);
-    sum(b, stream);
+    launch(netra_linear_backward_small_gfx950, dim3(groups + groups_of(a, product)), dim3(512), a, b, groups);
+    sum(b, launch);
   } else {
-    run(p, a, product, stream);
-    run(b, outer, stream);
+    run(p, a, product, launch);
+    run(b, outer, launch);
   }
-  return launched(name);
+  return launch.result(name);
 }
 
 // ---- router -------------------------------------------------------------------
@@ -459,17 +475,18 @@ extern "C" int netra_router_counts(const int32_t* ids, uint64_t ids_stride, cons
   if (bad_workspace(workspace, workspace_bytes, netra_router_counts_workspace(tokens, slots, experts)))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
   const CountPlan plan = count_plan(tokens, kFewCounts, 256u);
+  Launcher launch(stream);
   if (plan.groups == 0) {
-    netra_router_counts_gfx950<<<dim3(1), dim3(1024), 0, stream>>>(ids, ids_stride, mask, tokens, slots, experts,
-                                                                   counts, accumulate ? 1u : 0u);
-    return launched(name);
+    launch(netra_router_counts_gfx950, dim3(1), dim3(1024), ids, ids_stride, mask, tokens, slots, experts, counts,
+           accumulate ? 1u : 0u);
+    return launch.result(name);
   }
   uint32_t* parts = static_cast<uint32_t*>(workspace);
-  netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(256), 0, stream>>>(ids, ids_stride, mask, tokens, slots,
-                                                                               experts, plan.each, parts, nullptr);
-  netra_router_count_sum_gfx950<<<dim3((experts + 15u) / 16u), dim3(256), 0, stream>>>(
-      parts, plan.groups, experts, counts, accumulate ? 1u : 0u);
-  return launched(name);
+  launch(netra_router_count_parts_gfx950, dim3(plan.groups), dim3(256), ids, ids_stride, mask, tokens, slots,
+         experts, plan.each, parts, nullptr);
+  launch(netra_router_count_sum_gfx950, dim3((experts + 15u) / 16u), dim3(256), parts, plan.groups, experts,
+         counts, accumulate ? 1u : 0u);
+  return launch.result(name);
 }
 
 extern "C" uint64_t netra_router_balance_workspace(uint32_t tokens, uint32_t slots, uint32_t experts) {
@@ -517,6 +534,7 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
   a.loss = loss;
   a.grad = grad;
   a.grad_stride = grad_stride;
+  Launcher launch(stream);
   uint32_t grid = 1;
   if (plan.groups) {
     uint32_t* words = static_cast<uint32_t*>(workspace);
@@ -525,14 +543,14 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
     uint32_t* parts = words + 4 + kBalanceGrid;
     a.parts = parts;
     a.groups = plan.groups;
-    netra_router_count_parts_gfx950<<<dim3(plan.groups), dim3(plan.each > 256u ? 1024 : 256), 0, stream>>>(
-        ids, ids_stride, mask, tokens, slots, experts, plan.each, parts, words);
+    launch(netra_router_count_parts_gfx950, dim3(plan.groups), dim3(plan.each > 256u ? 1024 : 256), ids,
+           ids_stride, mask, tokens, slots, experts, plan.each, parts, words);
     // Rows per pass of a workgroup. (Workgroups of 512 threads: 32768 x 256 bf16 26.8 us, of 1024 24.6.)
     const uint32_t rows = experts <= 256u ? 64u : 16u;
     grid = (tokens - 1u) / rows + 1u;
     grid = grid > kBalanceGrid ? kBalanceGrid : grid;
   }
-#define NETRA_RUN(NAME, F) netra_router_balance_##NAME##_##F##_gfx950<<<dim3(grid), dim3(1024), 0, stream>>>(a)
+#define NETRA_RUN(NAME, F) launch(netra_router_balance_##NAME##_##F##_gfx950, dim3(grid), dim3(1024), a)
 #define NETRA_PICK(NAME)                       \
   if (experts <= 64u) NETRA_RUN(NAME, 16x4);   \
   else if (experts <= 128u) NETRA_RUN(NAME, 16x8);  \
@@ -546,7 +564,7 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
   }
 #undef NETRA_PICK
 #undef NETRA_RUN
-  return launched(name);
+  return launch.result(name);
 }
 
 extern "C" const char* netra_layers_last_error(void) { return g_error.c_str(); }
