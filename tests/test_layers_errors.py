@@ -1,4 +1,4 @@
-"""Errors of HIP calls that the layers library did not make: an error that an
+"""Errors of HIP calls that the layers and weight-prep libraries did not make: an error that an
 earlier call left on the thread is the caller's, and a call that runs is not
 reported as failed for it."""
 import ctypes
@@ -10,6 +10,7 @@ import layers_case as C
 from conftest import gpu_available
 from netra_moe import balance as B
 from netra_moe import layers, paths
+from netra_moe import weights as W
 from netra_moe.linear import BlockLinear
 
 pytestmark = pytest.mark.skipif(not paths.layers_library().is_file(), reason="library not built")
@@ -62,3 +63,21 @@ def test_calls_run_behind_a_stale_error_and_leave_it_to_the_caller():
     want = C.counts(ids, 16)
     assert outs[1].tolist() == want.tolist() == r.counts.tolist()
     assert torch.isfinite(r.loss) and torch.isfinite(r.grad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not gpu_available(), reason="needs a GPU")
+def test_weight_prep_runs_behind_a_stale_error():
+    w = torch.randn(2, 128, 256, device="cuda:0") * 0.02
+    q, s = W.quantize_blocks(w)
+    packed = [W.pack_tiles(q), W.pack_tiles(q, gate_up=True), W.pack_tiles_from_aiter(q)]
+    torch.cuda.synchronize()
+    assert hip("hipSetDevice", 12345) == INVALID_DEVICE
+    try:
+        again = W.quantize_blocks(w)
+        repacked = [W.pack_tiles(q), W.pack_tiles(q, gate_up=True), W.pack_tiles_from_aiter(q)]
+        assert hip("hipPeekAtLastError") == INVALID_DEVICE
+    finally:
+        hip("hipGetLastError")
+    assert torch.equal(again[0], q) and torch.equal(again[1], s)
+    assert all(torch.equal(a, b) for a, b in zip(packed, repacked))
