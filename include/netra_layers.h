@@ -4,8 +4,9 @@
 //
 // Block-FP8 linear layer. W [n, k] is e4m3 with one fp32 scale per 128x128
 // block (scale grid [ceil(n/128), ceil(k/128)], row-major), as a block-FP8
-// checkpoint holds every dense projection; n and k are any positive sizes, the
-// last block of either may be short. Activations are quantised inside the call by the
+// checkpoint holds every dense projection; n, k and the rows go up to 2^21 each
+// (a call whose workgroups do not fit a launch, of outputs beyond the memory, is
+// refused), the last block of n or k may be short. Activations are quantised inside the call by the
 // MoE layer's rule: per 1x128, scale = max(amax, 1e-10) * 0x3b124925, code =
 // e4m3_rne(v * (1 / scale)). A 128-group that holds an infinity or NaN gets the
 // scale NaN, so every output it reaches is NaN. Products are accumulated in

@@ -117,6 +117,22 @@ inline OuterPlan outer_plan(uint32_t rows, uint32_t n, uint32_t k) {
   return best;
 }
 
+// Workgroups that copy an operand of the weight gradient [rows, pitch] to the workspace: a multiple of
+// the 512-column parts of a row, four rows at a time, 2^18 at most (they loop over the rows).
+inline uint32_t copy_groups(uint32_t rows, uint32_t pitch) {
+  const uint32_t across = (pitch + 511u) / 512u, most = across <= 64u ? 4096u : (1u << 18) / across;
+  const uint32_t down = (rows + 3u) / 4u;
+  return across * (down < most ? down : most);
+}
+// Workgroups that quantise [rows, n] in a launch with the copies.
+inline uint32_t quant_groups(uint32_t rows, uint32_t n) { return (rows + 15u) / 16u * ((blocks(n) + 3u) / 4u); }
+// Workgroups of a product [rows, ni] in tiles and of a weight gradient: a multiple of the eight XCDs.
+inline uint64_t tile_groups(uint64_t a, uint32_t p, uint64_t b, uint32_t q, uint32_t splits) {
+  return ((a + p - 1u) / p * ((b + q - 1u) / q) * splits + 7u) / 8u * 8u;
+}
+// A launch's threads in one dimension have 32 bits.
+inline bool launchable(uint64_t groups, uint32_t threads) { return groups * threads < (1ull << 32); }
+
 // Whether a backward pass runs both products in one launch, dx in tiles of 64 x 64 then: passes of
 // small tiles (T 333, N 1024, K 2048 13.3 us, in two 16.9; T 3584, N 360, K 189 16.3, 20.7; T 1200,
 // N 1000, K 1000 18.3, 24.5; T 3000, N 500, K 500 21.3, 24.1); with larger tiles most lose by it (T

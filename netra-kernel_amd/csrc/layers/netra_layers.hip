@@ -128,9 +128,9 @@ uint64_t outer_bytes(const void* m, uint32_t type, uint64_t stride, uint32_t row
 const uint16_t* outer_operand(const void* m, uint32_t type, uint64_t& stride, uint32_t rows, uint32_t& cols,
                               uint8_t*& at, nklin::Copy& copy) {
   if (outer_ready(m, type, stride, cols)) return static_cast<const uint16_t*>(m);
-  const uint32_t pitch = up(cols, 8u), down = rows < 4u * 4096u ? (rows + 3u) / 4u : 4096u;
+  const uint32_t pitch = up(cols, 8u);
   uint16_t* out = reinterpret_cast<uint16_t*>(at);
-  copy = {m, stride, out, type, cols, pitch, (pitch + 511u) / 512u * down};
+  copy = {m, stride, out, type, cols, pitch, copy_groups(rows, pitch)};
   at += static_cast<uint64_t>(rows) * pitch * 2u;
   stride = cols = pitch;
   return out;
@@ -223,9 +223,15 @@ static void quantise(const ProductCall& c, const ProductPlan& plan, uint8_t* wor
                c.rows, c.nc, launch);
 }
 
-static uint32_t groups_of(const nklin::Product& a, const ProductPlan& plan) {
-  const uint32_t items = ((a.ni + plan.p - 1u) / plan.p) * ((a.nq + plan.q - 1u) / plan.q) * plan.splits;
-  return (items + 7u) / 8u * 8u;
+static uint64_t groups_of(const ProductCall& c, const ProductPlan& plan) {
+  return tile_groups(c.ni, plan.p, c.rows, plan.q, plan.splits);
+}
+// Before anything is launched: whether the product's workgroups fit a launch. (Those that do not
+// have outputs larger than the memory.)
+static int check_grid(const ProductCall& c, const ProductPlan& plan) {
+  if (plan.form == kTiles && !launchable(groups_of(c, plan), 512u))
+    return fail(-1, c.name, "more workgroups than one launch takes");
+  return 0;
 }
 
 static void run(const ProductCall& c, const nklin::Product& a, const ProductPlan& plan, Launcher& launch) {
@@ -241,7 +247,7 @@ static void run(const ProductCall& c, const nklin::Product& a, const ProductPlan
     else launch(netra_linear_product_stream_p1q4_gfx950, grid, block, a);
     return;
   }
-  const dim3 grid(groups_of(a, plan));
+  const dim3 grid(static_cast<uint32_t>(groups_of(c, plan)));
   if (plan.p == 256u && plan.q == 256u) launch(netra_linear_product_256x256_gfx950, grid, block, a);
   else if (plan.p == 256u) launch(netra_linear_product_256x128_gfx950, grid, block, a);
   else if (plan.q == 128u) launch(netra_linear_product_128x128_gfx950, grid, block, a);
@@ -263,6 +269,7 @@ static int times_weights(const ProductCall& c, void* workspace, uint64_t workspa
   if (bad_workspace(workspace, workspace_bytes, product_workspace(c.rows, c.ni, c.nc, c.in_type)))
     return fail(-1, c.name, "workspace too small, null or not 16-byte aligned");
   const ProductPlan plan = product_plan(c.rows, c.ni, c.nc, c.in_type == NETRA_BF16);
+  if (check_grid(c, plan) != 0) return -1;
   nklin::Product a{};
   set_up(c, plan, static_cast<uint8_t*>(workspace), a);
   Launcher launch(stream);
@@ -337,7 +344,7 @@ static void set_up(const OuterCall& c, const OuterPlan& plan, uint8_t* workspace
 
 // The operands' copies, with dy's quantisation (to `codes`, or null) in the same launch.
 static void prepare(const OuterCall& c, const nklin::Copy (&copies)[2], uint8_t* codes, Launcher& launch) {
-  const uint32_t quant = codes ? (c.rows + 15u) / 16u * ((blocks(c.n) + 3u) / 4u) : 0u;
+  const uint32_t quant = codes ? quant_groups(c.rows, c.n) : 0u;
   const dim3 grid(quant + copies[0].groups + copies[1].groups), block(256);
   float* s = codes ? reinterpret_cast<float*>(codes + code_bytes(c.rows, c.n)) : nullptr;
   const uint32_t sld = up(c.rows, 16u);
@@ -349,9 +356,15 @@ static void prepare(const OuterCall& c, const nklin::Copy (&copies)[2], uint8_t*
            c.rows, c.n, sld, quant, copies[0], copies[1]);
 }
 
-static uint32_t groups_of(const nklin::Outer& a, const OuterPlan& plan) {
-  const uint32_t items = ((a.k + plan.p - 1u) / plan.p) * ((a.n + plan.q - 1u) / plan.q) * plan.splits;
-  return (items + 7u) / 8u * 8u;
+static uint64_t groups_of(const OuterCall& c, const OuterPlan& plan) {
+  return tile_groups(c.k, plan.p, c.n, plan.q, plan.splits);
+}
+static int check_grid(const OuterCall& c, const OuterPlan& plan) {
+  const uint64_t before = static_cast<uint64_t>(quant_groups(c.rows, c.n)) + copy_groups(c.rows, up(c.n, 8u)) +
+                          copy_groups(c.rows, up(c.k, 8u));
+  if (!launchable(groups_of(c, plan), 512u) || !launchable(before, 256u))
+    return fail(-1, c.name, "more workgroups than one launch takes");
+  return 0;
 }
 
 static void sum(const nklin::Outer& a, Launcher& launch) {
@@ -360,8 +373,8 @@ static void sum(const nklin::Outer& a, Launcher& launch) {
   launch(netra_linear_outer_sum_gfx950, dim3(static_cast<uint32_t>(quads < 2048u ? quads : 2048u)), dim3(256), a);
 }
 
-static void run(const nklin::Outer& a, const OuterPlan& plan, Launcher& launch) {
-  const dim3 grid(groups_of(a, plan)), block(512);
+static void run(const OuterCall& c, const nklin::Outer& a, const OuterPlan& plan, Launcher& launch) {
+  const dim3 grid(static_cast<uint32_t>(groups_of(c, plan))), block(512);
   if (plan.p == 256u) launch(netra_linear_outer_256x256_gfx950, grid, block, a);
   else if (plan.q == 256u) launch(netra_linear_outer_128x256_gfx950, grid, block, a);
   else launch(netra_linear_outer_128x128_gfx950, grid, block, a);
@@ -390,13 +403,14 @@ extern "C" int netra_linear_weight_gradient(const void* dy, uint32_t dy_type, ui
   rc = check(c);
   if (rc != 0) return rc;
   const OuterPlan plan = outer_plan(rows, n, k);
+  if (check_grid(c, plan) != 0) return -1;
   if (bad_workspace(workspace, workspace_bytes, outer_workspace(c, plan)))
     return fail(-1, c.name, "workspace too small, null or not 16-byte aligned");
   nklin::Outer a{};
   nklin::Copy copies[2] = {};
   set_up(c, plan, static_cast<uint8_t*>(workspace), a, copies);
   if (copies[0].groups + copies[1].groups) prepare(c, copies, nullptr, launch);
-  run(a, plan, launch);
+  run(c, a, plan, launch);
   return launch.result(c.name);
 }
 
@@ -431,6 +445,9 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const bool small = backward_in_one(product, outer);
   if (small) product.p = product.q = 64u;
+  if (check_grid(p, product) != 0 || check_grid(o, outer) != 0) return -1;
+  const uint64_t outer_groups = groups_of(o, outer), groups = outer_groups + (small ? groups_of(p, product) : 0u);
+  if (!launchable(groups, 512u)) return fail(-1, name, "more workgroups than one launch takes");
   nklin::Product a{};
   nklin::Outer b{};
   nklin::Copy copies[2] = {};
@@ -439,12 +456,12 @@ extern "C" int netra_linear_backward(const void* dy, uint32_t dy_type, uint64_t 
   if (copies[0].groups + copies[1].groups) prepare(o, copies, product.form == kFused ? nullptr : ws, launch);
   else quantise(p, product, ws, launch);
   if (small) {
-    const uint32_t groups = groups_of(b, outer);
-    launch(netra_linear_backward_small_gfx950, dim3(groups + groups_of(a, product)), dim3(512), a, b, groups);
+    launch(netra_linear_backward_small_gfx950, dim3(static_cast<uint32_t>(groups)), dim3(512), a, b,
+           static_cast<uint32_t>(outer_groups));
     sum(b, launch);
   } else {
     run(p, a, product, launch);
-    run(b, outer, launch);
+    run(o, b, outer, launch);
   }
   return launch.result(name);
 }

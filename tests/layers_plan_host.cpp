@@ -1,6 +1,8 @@
 // Prints the kernels that layers_plan.h picks. stdin, a query a line:
 //   product <rows> <ni> <nc> <bf16>  ->  fused|stream|tiles p q splits blocks per split
 //   outer <rows> <n> <k>             ->  p q splits tokens per split
+//   grids <rows> <n> <k>             ->  workgroups of the quantisation of dy with the copies of dy and x, of
+//                                        y, of dx and of dw (0: not in tiles)
 //   backward <rows> <n> <k> <bf16>   ->  1 where both products run in one launch
 #include <cstdint>
 #include <cstdio>
@@ -15,6 +17,17 @@ int main() {
     if (!std::strcmp(what, "outer")) {
       const nkplan::OuterPlan o = nkplan::outer_plan(a, b, c);
       std::printf("%u %u %u %u\n", o.p, o.q, o.splits, o.split_rows);
+      continue;
+    }
+    if (!std::strcmp(what, "grids")) {
+      using namespace nkplan;
+      auto product = [&](unsigned ni, unsigned nc) -> unsigned long long {
+        const ProductPlan p = product_plan(a, ni, nc, true);
+        return p.form == kTiles ? tile_groups(ni, p.p, a, p.q, p.splits) : 0ull;
+      };
+      const OuterPlan o = outer_plan(a, b, c);
+      std::printf("%llu %llu %llu %llu\n", 0ull + quant_groups(a, b) + copy_groups(a, up(b, 8)) + copy_groups(a, up(c, 8)),
+                  product(b, c), product(c, b), 0ull + tile_groups(c, o.p, b, o.q, o.splits));
       continue;
     }
     if (std::scanf("%u", &d) != 1) return 1;

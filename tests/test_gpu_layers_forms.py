@@ -59,3 +59,14 @@ def test_backward_form(size):
     C.assert_within(dx, *C.product(C.quantised(dy, 1), w.t().contiguous()), "dx")
     C.assert_within(dw, *C.outer(dy, x), "dw")
     assert torch.equal(dx, lin.input_gradient(dy.to(DEV))) and torch.equal(dw, lin.weight_gradient(dy.to(DEV), x.to(DEV)))
+
+
+def test_copies_that_loop_over_the_rows():
+    """Operands too wide for a workgroup per four rows of the copy; whole numbers, so exact."""
+    rows, n, k = 7700, 3, 70001
+    assert (rows + 3) // 4 > (1 << 18) // -(-k // 512)
+    lin = BlockLinear(torch.zeros(n, k, dtype=torch.uint8, device=DEV), torch.ones(1, -(-k // 128), device=DEV))
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randint(-7, 8, (rows, k), generator=g, device=DEV).float()
+    dy = torch.randint(-7, 8, (rows, n), generator=g, device=DEV).float()
+    assert torch.equal(lin.weight_gradient(dy, x).double(), dy.double().t().contiguous() @ x.double())

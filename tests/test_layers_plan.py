@@ -10,6 +10,7 @@ import pytest
 
 import layers_forms as F
 from conftest import REPO
+from netra_moe import layers, paths
 
 LAYERS = REPO / "netra-kernel_amd" / "csrc" / "layers"
 
@@ -85,3 +86,28 @@ def test_quantising_on_the_way_counts_the_workgroups_that_it_launches(plan):
         assert plan(("product", rows, ni, nc, 1))[0][:3] == ["fused", 1, 4], (rows, ni, nc)
     for rows, ni, nc in [(20, 8192, 1024), (32, 16384, 1024)]:
         assert plan(("product", rows, ni, nc, 1))[0][:3] == ["fused", 2, 2], (rows, ni, nc)
+
+
+def test_launches_of_any_size_that_fits_the_memory_fit_their_grids(plan):
+    """Threads of a launch's dimension have 32 bits. x, dy, y, dx and dw with the codes and copies
+    of a backward pass on fp32 in 288 GB: any sizes up to 2^21."""
+    sizes = [1, 17, 65, 333, 1000, 4096, 16384, 1 << 18, (1 << 21) - 1, 1 << 21]
+    fit = [(r, n, k) for r in sizes for n in sizes for k in sizes
+           if 4 * r * (n + k) + 4 * n * k + 3 * r * n + 2 * r * k < 288e9]
+    assert (16384, 1 << 21, 333) in fit and (1, 1 << 21, 16384) in fit
+    for size, (prepare, y, dx, dw) in zip(fit, plan(*(("grids", *s) for s in fit))):
+        assert 0 < prepare * 256 < 1 << 32 and max(y, dx) * 512 < 1 << 31 and 0 < dw * 512 <= 1 << 31, size
+
+
+@pytest.mark.skipif(not paths.layers_library().is_file(), reason="library not built")
+@pytest.mark.parametrize("rows,n,k", [(1 << 21, 1 << 21, 128), (1 << 21, 1 << 21, 1 << 21), (128, 1 << 21, 1 << 21)])
+def test_more_workgroups_than_a_launch_takes_are_refused_before_any_launch(rows, n, k):
+    lib, far = layers.library(), 1 << 44  # addresses that are never followed
+    big = 1 << 60
+    calls = [("netra_linear_weight_gradient", far, 1, n, 3 * far, 1, k, 5 * far, 0, rows, n, k, 16, big, None),
+             ("netra_linear_backward", far, 1, n, 3 * far, 1, k, 16, 16, 5 * far, k, 9 * far, 0, rows, n, k, 16, big, None)]
+    if rows > 128:
+        calls.append(("netra_linear_forward", far, 1, k, 16, 16, 3 * far, n, rows, n, k, 16, big, None))
+    for name, *args in calls:
+        assert getattr(lib, name)(*args) == -1, name
+        assert "more workgroups" in lib.netra_layers_last_error().decode()
