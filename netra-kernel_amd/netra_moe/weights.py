@@ -50,6 +50,20 @@ def bridge_library() -> ctypes.CDLL:
     return _bridge
 
 
+def _launch(name: str, device: torch.device, *args) -> None:
+    """Launch an entry point on the device's current stream, with that device current (a null
+    stream means the current device's)."""
+    lib = bridge_library()
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, stream)
+    if rc != 0:
+        raise RuntimeError(f"{name} failed ({rc}): {lib.netra_moe_last_error().decode()}")
+
+
 def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """fp32 [G, N, K] on the GPU -> (e4m3 bytes [G, N, K], fp32 scales [G, N/128, K/128])."""
     if w.dim() != 3 or w.dtype != torch.float32 or not w.is_cuda or not w.is_contiguous():
@@ -59,11 +73,7 @@ def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError("N and K must be multiples of 128")
     q = torch.empty((g, n, k), dtype=torch.uint8, device=w.device)
     s = torch.empty((g, n // 128, k // 128), dtype=torch.float32, device=w.device)
-    stream = torch.cuda.current_stream(w.device).cuda_stream
-    lib = bridge_library()
-    rc = lib.netra_moe_quant_blocks(w.data_ptr(), q.data_ptr(), s.data_ptr(), g, n, k, stream)
-    if rc != 0:
-        raise RuntimeError(f"netra_moe_quant_blocks failed ({rc}): {lib.netra_moe_last_error().decode()}")
+    _launch("netra_moe_quant_blocks", w.device, w.data_ptr(), q.data_ptr(), s.data_ptr(), g, n, k)
     return q, s
 
 
@@ -76,11 +86,8 @@ def pack_tiles(q: torch.Tensor, gate_up: bool = False) -> torch.Tensor:
     if n % (32 if gate_up else 16) or k % 128:
         raise ValueError("N must be a multiple of 16 (32 for W13) and K of 128")
     out = torch.empty_like(q)
-    lib = bridge_library()
-    fn = lib.netra_moe_pack_tiles_gate_up if gate_up else lib.netra_moe_pack_tiles
-    rc = fn(q.data_ptr(), out.data_ptr(), g, n, k, torch.cuda.current_stream(q.device).cuda_stream)
-    if rc != 0:
-        raise RuntimeError(f"weight packing failed ({rc}): {lib.netra_moe_last_error().decode()}")
+    name = "netra_moe_pack_tiles_gate_up" if gate_up else "netra_moe_pack_tiles"
+    _launch(name, q.device, q.data_ptr(), out.data_ptr(), g, n, k)
     return out
 
 
@@ -94,11 +101,8 @@ def pack_tiles_from_aiter(q: torch.Tensor, gate_up: bool = False) -> torch.Tenso
     if n % (32 if gate_up else 16) or k % 128:
         raise ValueError("N must be a multiple of 16 (32 for W13) and K of 128")
     out = torch.empty_like(q)
-    lib = bridge_library()
-    fn = lib.netra_moe_pack_tiles_gate_up_from_aiter if gate_up else lib.netra_moe_pack_tiles_from_aiter
-    rc = fn(q.data_ptr(), out.data_ptr(), g, n, k, torch.cuda.current_stream(q.device).cuda_stream)
-    if rc != 0:
-        raise RuntimeError(f"weight packing failed ({rc}): {lib.netra_moe_last_error().decode()}")
+    name = "netra_moe_pack_tiles_gate_up_from_aiter" if gate_up else "netra_moe_pack_tiles_from_aiter"
+    _launch(name, q.device, q.data_ptr(), out.data_ptr(), g, n, k)
     return out
 
 
@@ -115,15 +119,12 @@ def aiter_shuffle_host(q: np.ndarray) -> np.ndarray:
 
 def device_copy(src: torch.Tensor, dst: torch.Tensor) -> None:
     """Byte copy src -> dst (same size, GPU, 16-byte multiple) by the library's
-    plain streaming kernel, on the current stream."""
+    plain streaming kernel, on the current stream of src's device."""
     n = src.numel() * src.element_size()
     if not (src.is_cuda and dst.is_cuda and src.is_contiguous() and dst.is_contiguous()) or \
             n != dst.numel() * dst.element_size():
         raise ValueError("device_copy needs two contiguous GPU tensors of the same byte size")
-    lib = bridge_library()
-    rc = lib.netra_moe_copy(src.data_ptr(), dst.data_ptr(), n, torch.cuda.current_stream(src.device).cuda_stream)
-    if rc != 0:
-        raise RuntimeError(f"netra_moe_copy failed ({rc}): {lib.netra_moe_last_error().decode()}")
+    _launch("netra_moe_copy", src.device, src.data_ptr(), dst.data_ptr(), n)
 
 
 def gu_order(nt: int) -> np.ndarray:
