@@ -70,3 +70,14 @@ def test_copies_that_loop_over_the_rows():
     x = torch.randint(-7, 8, (rows, k), generator=g, device=DEV).float()
     dy = torch.randint(-7, 8, (rows, n), generator=g, device=DEV).float()
     assert torch.equal(lin.weight_gradient(dy, x).double(), dy.double().t().contiguous() @ x.double())
+
+
+@pytest.mark.parametrize("direction", ["forward", "input_gradient"])
+@pytest.mark.parametrize("dt,form,size", PRODUCTS, ids=lambda v: "-".join(map(str, v)) if isinstance(v, tuple) else None)
+def test_a_row_has_the_same_bits_wherever_it_stands(dt, form, size, direction):
+    rows, ni, nc = size
+    lin, _ = layer(*((ni, nc) if direction == "forward" else (nc, ni)), seed=3, gradients=direction != "forward")
+    x = C.activations(rows, nc, seed=4, dtype=dt).to(DEV)
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(5)).to(DEV)
+    call = getattr(lin, direction)
+    assert torch.equal(call(x[order]), call(x)[order])
