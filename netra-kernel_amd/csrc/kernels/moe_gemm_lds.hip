@@ -37,7 +37,7 @@
 #pragma once
 #include <type_traits>
 
-#include "moe_numerics.h"
+#include "lds_copy.h"
 
 #define NK_KERNEL extern "C" __global__
 
@@ -59,10 +59,6 @@ constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kCopiesPerWave = 7;            // per step: A tile (2) + gate tile (2) + up tile (2) [+ tail share (1)]
 constexpr uint32_t kFar = 0x80000000u;            // an offset past the activation range (T * H < 2^31): zeros
 
-__device__ __forceinline__ uint32_t lds_offset(const void* p) {
-  return (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)p;
-}
-
 // Raw buffer descriptor (base, num_records bytes, raw dword format) in SGPRs.
 __device__ __forceinline__ u32x4 rsrc(const void* base, uint32_t bytes) {
   const uint64_t a = (uint64_t)base;
@@ -74,25 +70,6 @@ __device__ __forceinline__ u32x4 rsrc(const void* base, uint32_t bytes) {
   return r;
 }
 
-// 16 bytes per lane, global (rsrc + voff + soff) -> LDS (m0 + 16 * lane).
-// Offsets at or past num_records read as zeros without a memory access.
-// The compiler's hazard recognizer does not look inside inline assembly, so
-// the s_nop 4 supplies the five wait states a vector-memory instruction needs
-// after a VALU write (v_readfirstlane, v_readlane, carry outputs) of an SGPR
-// it reads (resource, offset), which also covers the M0 write before an
-// LDS-destination load. The compiler treats m0 as a reserved register and
-// does not honour it in a clobber list, so the copy saves m0 and puts it back
-// (the LDS address is taken from m0 when the load issues): any value the
-// compiler keeps in m0 survives the copy.
-__device__ __forceinline__ void copy16(uint32_t m0, u32x4 r, uint32_t voff, uint32_t soff) {
-  uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
-               "s_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "s"(m0), "v"(voff), "s"(r), "s"(soff)
-               : "memory");
-}
-
 // copy16 with a non-temporal load, for weights that one item of a launch reads.
 __device__ __forceinline__ void copy16_once(uint32_t m0, u32x4 r, uint32_t voff, uint32_t soff) {
   uint32_t saved;
@@ -102,25 +79,6 @@ __device__ __forceinline__ void copy16_once(uint32_t m0, u32x4 r, uint32_t voff,
                : "s"(m0), "v"(voff), "s"(r), "s"(soff)
                : "memory");
 }
-
-// 4 bytes per lane, global (rsrc + voff + soff) -> LDS (m0 + 4 * lane); as copy16.
-__device__ __forceinline__ void copy4(uint32_t m0, u32x4 r, uint32_t voff, uint32_t soff) {
-  uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dword %2, %3, %4 offen lds\n\t"
-               "s_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "s"(m0), "v"(voff), "s"(r), "s"(soff)
-               : "memory");
-}
-
-template <uint32_t N>
-__device__ __forceinline__ void wait_copies() {
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
-
-// Barrier for LDS hand-off: waits for this wave's LDS traffic, not for its
-// copies in flight (a full __syncthreads would drain those).
-__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Swizzle of the activation rows in LDS: a 16-row x 128-byte tile is stored
 // row-major with the 16-byte chunk c of row r at position c ^ row_swizzle(r),
