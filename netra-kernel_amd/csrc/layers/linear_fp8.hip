@@ -135,8 +135,9 @@ __device__ __forceinline__ void store_tile(uint8_t* tile, uint32_t lane, const u
 // Rows: x [rows, n] -> tiles of 16 rows x 128 columns, scales s[b, row] with
 // `sld` floats per block (sld = rows rounded up to 16 at least). One wave per tile; rows past
 // the end are zeros. Bound by memory: a tile's loads, 64 bytes a lane, are one wave's whole
-// work, so enough are under way. 8192 x 4096 bf16: 102 MB in and out, 20.7 us, 4.9 TB/s (a
-// large copy: 5.1); 1001 x 1111 fp32 4.9 us, 64 x 2048 bf16 2.5 us (a launch).
+// work, so enough are under way. 8192 x 4096 bf16: 102 MB in and out, 20.5 us, 5.0 TB/s (a
+// large copy: 5.1 to 5.2); 64 x 2048 bf16 2.9 us (a launch); 1001 x 1111 fp32 5.0 us, where a load
+// instruction's lanes touch 64 lines for 16 bytes each.
 template <typename X>
 __device__ __forceinline__ void quant_rows(const X* __restrict__ x, uint64_t stride, uint8_t* __restrict__ q,
                                            float* __restrict__ s, uint32_t rows, uint32_t n, uint32_t sld,
@@ -207,10 +208,12 @@ struct Product {
 // matrix core works on the next. (The scales differ per row of Q, so the sum over blocks
 // cannot stay in the matrix core.) Copies spread over the products: in a burst at the head of
 // a step they hold up the wave that issues them.
-// What bounds it: LDS traffic beside the products. 256x128 at T 4096, N 2048, K 4096: 41 us
-// (1.7 PFLOP/s; the library's product without block scales reaches 2.6 at 8192 x 8192 x
-// 4096); a step moves 176 KiB through LDS, 1408 cycles, for 1024 cycles of products, and takes
-// about 2600. 128x64 at T 1001, N 1500, K 1111: 7.6 us, nine steps and one round.
+// What bounds it: no unit alone, but that all waves of the one workgroup on a CU go in step.
+// 256x128 at T 2048, N 4096, K 4096: 35.9 us (1.9 PFLOP/s; the library's product without block
+// scales 2.4 to 2.6 at 8192 x 8192 x 4096). A step takes 2180 cycles for 1024 of products: by
+// counters the matrix cores are busy 47% of the waves' time, LDS 29%, and a wave spends 30% of it
+// at the barrier or behind copies and 33% waiting to issue. 128x64 at T 1001, N 1500, K 1111: 8.2
+// us, nine steps and one round.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 struct Tile {
   static constexpr uint32_t kWaves = WP * WQ;
@@ -421,14 +424,14 @@ __device__ __forceinline__ void product_tile(const Product& a, uint32_t group, u
 // of P by its own products, both a phase ago. Group 1 copies its own half of P, likewise.
 // Copies are waited for at the end of the products of the same block, a phase and a half
 // after they were issued, and needed by group 0 in the next phase (group 1: its own).
-// A step moves 256 KiB through LDS (64 in, 192 to registers: each tile of P feeds four
-// waves, each of Q two), 2048 cycles of it, as long as its products take: both compete.
-// T 8192, N 8192, K 4096 with the quantisation: 243 us (2.26 PFLOP/s; the library's product
-// without block scales and without the quantisation 212 us). All waves in step,
-// product_tile's way, take 4% longer, without whole-tile copies 2%, with the copies spread over
-// both groups' products 7%, with Q's operands straight from L2 to registers 18%. (256x128 in turns is
-// slower, 47.8 us against 41.5 at T 2048, N 4096, K 4096: its phases are 16 products long.) About 60 us go
-// with the copies (timed without them).
+// T 8192, N 8192, K 4096: 230 us (2.4 PFLOP/s; the library's product without block scales 212 to
+// 229 us), behind 20.5 of quantisation. A step takes 3320 cycles for 2048 of products: by counters
+// the matrix cores are busy 62% of the waves' time, LDS 28%, and a wave spends 30% of it at a
+// barrier or behind copies. All waves in step, product_tile's way, take 4% longer, without
+// whole-tile copies 2%, with the copies spread over both groups' products 7%, with Q's operands
+// straight from L2 to registers 18%. (256x128 in turns is slower, 47.8 us against 41.5 as calls at T
+// 2048, N 4096, K 4096: its phases are 16 products long.) About 60 us go with the copies (timed
+// without them).
 __device__ __forceinline__ void product_turns(const Product& a, uint32_t index, uint8_t* s_stage) {
   using L = Tile<2, 4, 8, 4, 2>;
   constexpr uint32_t kStage = L::kScaleAt + 1024u + 512u;  // Q's scales, then P's for either group
@@ -545,8 +548,8 @@ __device__ __forceinline__ void product_sum(const Product& a) {
 // lanes hold a tile of 16 rows x 128 values exactly as an operand wants it, and the
 // four lanes of a row find its scale with two exchanges. Else their tiles come from
 // a.q. Bound by the weights' way from memory, or by a launch's length where they are few:
-// T 1, N 28672, K 8192 (235 MB) 40.2 us, 5.8 TB/s; T 1, N 2048, K 2048 (4 MB, from the last
-// level cache) 4.4 us, T 64, N 4096, K 2048 4.4 us behind 2.5 of quantisation.
+// T 1, N 28672, K 8192 (235 MB) 40.4 us, 5.8 TB/s; T 1, N 2048, K 2048 (4 MB, from the last
+// level cache) 4.7 us, T 64, N 4096, K 2048 4.6 us behind 2.9 of quantisation.
 template <uint32_t NP, uint32_t NQ, bool kFused, typename X>
 __device__ __forceinline__ void product_stream(const Product& a, const X* __restrict__ x, uint64_t x_stride,
                                                uint32_t n) {
@@ -678,16 +681,18 @@ struct Outer {
 // tokens of one read then meet every bank twice, which is what 512 bytes need.
 // Workgroups, waves and the stage hand-over are product_tile's. Columns past the
 // matrix read the next row and make outputs that are not stored; tokens past the
-// end read zeros. 128x256 at T 4096, N 4096, K 2048: 61.5 us, 1.12 PFLOP/s (a library
-// product of the same size 79 us, a large one 1.42 PFLOP/s), the matrix cores busy 41% of
-// the cycles: 176 KiB per step through LDS, 1408 cycles, beside 1024 of products. Reading
-// less, by waves of 64 x 128 over one half of a step's tokens each and a sum of the halves
-// at the end (144 KiB per step), takes 62.5 us, and 9.0 us instead of 8.3 at T 333, N 1024, K
-// 2048: the longer wait for a step's first operands costs as much. Two groups of waves in
-// turn, product_turns' way, take 76 us, steps of 32 tokens in six stages 70, operands read two tiles ahead the same
-// 62. 256x256 at T 8192, N 4096, K 4096: 216 us (1.27 PFLOP/s), with its two stages' copies
-// spread over the whole step 230; about 30 are its stores, which nothing hides with one
-// workgroup per CU, and with all copies from lines the cache holds it takes 40 less.
+// end read zeros. 128x256 at T 4096, N 4096, K 2048: 61 us as a call of its own, 64 behind the
+// input gradient (1.1 PFLOP/s; a library product of the same size 79 us, a large one 1.42
+// PFLOP/s). A step takes 1950 cycles for 1024 of products: by counters the matrix cores are busy
+// 52% of the waves' time, LDS 26%, and a wave spends 28% of it at the barrier or behind copies and 36%
+// waiting to issue. Reading less from LDS, by waves of 64 x 128 over one half of a step's tokens each
+// and a sum of the halves at the end, takes 62.5 us against 61.5, and 9.0 instead of 8.3 at T 333, N
+// 1024, K 2048: the longer wait for a step's first operands costs as much. Two groups of waves in
+// turn, product_turns' way, take 76 us, steps of 32 tokens in six stages 70, operands read two tiles
+// ahead the same 62, non-temporal stores 64. 256x256 at T 8192, N 4096, K 4096: 206 us as a call (1.33
+// PFLOP/s; with non-temporal stores 209), with its two stages' copies spread over the whole step
+// 6% longer; about 30 are its stores, which nothing hides with one workgroup per CU, and with all
+// copies from lines the cache holds it takes 40 less.
 template <uint32_t WP, uint32_t WQ, uint32_t NP, uint32_t NQ, uint32_t S>
 constexpr uint32_t outer_lds() {
   return S * 64u * 32u * (WP * NP + WQ * NQ);
@@ -1029,8 +1034,8 @@ NETRA_OUTER_TILE(128, 256, 2, 4, 4, 4, 3)
 NETRA_OUTER_TILE(128, 128, 2, 4, 4, 2, 4)
 // Both products of a small backward pass in one launch, the weight gradient's
 // workgroups (the first `outer`, a multiple of 8) with their longer way first: neither
-// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 13.3 us, 10.0 of it this
-// kernel; in two launches 16.9).
+// fills the chip, and a launch is saved (T 333, N 1024, K 2048: a call 13.4 us, this kernel 9.6 at
+// best and 11.0 in the middle; in two launches 16.9).
 extern "C" __global__ __launch_bounds__(512) void netra_linear_backward_small_gfx950(nklin::Product a, nklin::Outer b,
                                                                                      uint32_t outer) {
   constexpr uint32_t kP = nklin::Tile<4, 2, 1, 2, 4>::kLds, kO = nklin::outer_lds<2, 4, 4, 2, 4>();

@@ -231,10 +231,12 @@ struct Balance {
 
 // Counts, then the tokens' rows, 64 / G per wave. With `parts` the counting was
 // shared out over the workgroups of the launch before; without, this launch is
-// one workgroup. Bound by memory at the largest sizes (32768 x 500 fp32: 131 MB, 26.2 us, 5.0
-// TB/s), else by the vector units (32768 x 256 bf16: 15.2 us for 34 MB) and by what every
-// workgroup does once: a chain of parts, barriers and the last sum (4096 x 256 bf16: 7.7 us for 4
-// MB; 16 x 16 in one workgroup 3.8).
+// one workgroup. Bound by memory at the largest sizes (32768 x 500 fp32: 131 MB, 25.7 us at best,
+// 28.3 in the middle). Else by the vector units and by what every workgroup does once, a chain of
+// parts, barriers and the last sum: 32768 x 256 bf16, 34 MB, takes 13.9 us at best and 16.9 in the
+// middle, the vector units busy 62% of it by counters (28 instructions a value, and 180 a wave
+// besides); 4096 x 256 bf16 7.6 and 9.5 us on 64 CUs, whose vector units are busy 54%; 16 x 16 in
+// one workgroup 3.9.
 template <typename X, uint32_t G, uint32_t NV>
 __device__ __forceinline__ void balance(const Balance& a) {
   __shared__ uint32_t s_count[kMaxExperts + 1u];

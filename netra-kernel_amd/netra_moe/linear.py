@@ -15,7 +15,8 @@ Training: BlockLinear(..., gradients=True) also keeps W^T, and
 
 gives the gradients with respect to the input (bf16; dy is quantised per 1x128)
 and the weight (fp32; a bf16 product over the tokens, fp32 inputs rounded to bf16).
-Nothing is recorded by autograd: the caller passes x again.
+Nothing is recorded by autograd (forward of an x that requires gradients returns a
+tensor without history): the caller passes x again and dx on.
 
 PyTorch provides device memory and the stream only. Outputs and scratch are
 allocated per call from torch's allocator on the current stream, so calls on
