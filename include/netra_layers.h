@@ -121,6 +121,39 @@ int netra_router_balance(const void* logits, uint32_t logits_type, uint64_t logi
                          void* grad, uint64_t grad_stride, void* workspace, uint64_t workspace_bytes,
                          hipStream_t stream);
 
+// Root-mean-square norm before a projection or the experts.
+//   r = x + residual, rounded to the residual's type and written to sum (residual and sum null: r = x)
+//   y = r / sqrt(mean(r^2) + eps) * (weight + offset)
+// and, for the FP8 products behind it, codes e4m3 of y with one scale per 1x128 by the rule at the
+// top (of y in fp32, not of its rounding to y_type). y (bf16 or fp32) or codes and scales may be
+// null. codes_layout:
+//   NETRA_CODES_ROWS   codes [rows, cols], scales [rows, ceil(cols/128)] (what the bridges take)
+//   NETRA_CODES_TILES  what netra_linear_forward_codes takes: tile16x128, scales [ceil(cols/128), rows up to 16];
+//                      codes 16-byte aligned
+// rows 0 .. 2^21, cols 1 .. 16384; weight [cols] bf16 or fp32. Statistics are fp32 (|r| below 1e18).
+// sum may be the residual or x, y may be x or the residual (same address, type and stride); any
+// other overlap is refused.
+enum { NETRA_CODES_ROWS = 1, NETRA_CODES_TILES = 2 };
+uint64_t netra_norm_code_bytes(uint32_t rows, uint32_t cols, uint32_t codes_layout);
+uint64_t netra_norm_scale_count(uint32_t rows, uint32_t cols, uint32_t codes_layout);
+int netra_norm_forward(const void* x, uint32_t x_type, uint64_t x_stride, const void* residual, uint32_t residual_type,
+                       uint64_t residual_stride, const void* weight, uint32_t weight_type, float offset, float eps,
+                       void* sum, uint64_t sum_stride, void* y, uint32_t y_type, uint64_t y_stride, uint8_t* codes,
+                       float* scales, uint32_t codes_layout, uint32_t rows, uint32_t cols, hipStream_t stream);
+
+// Its gradients. r is what was normalised (sum, or x), dy the gradient of y, flow what flows into r
+// besides (the residual stream's gradient, of r's type, or null). With g = dy (weight + offset),
+// xh = r / sqrt(mean(r^2) + eps):
+//   dr = (g - xh mean(g xh)) / sqrt(mean(r^2) + eps) + flow    (of r's type: x's and the residual's)
+//   dw = sum over the rows of dy xh                            (fp32 [cols]; accumulate != 0 adds to it)
+// dr may be dy, r or flow (same address, type and stride). rows may be 0: dw is then zeros or as it was.
+uint64_t netra_norm_gradients_workspace(uint32_t rows, uint32_t cols);
+int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* r, uint32_t r_type,
+                         uint64_t r_stride, const void* flow, uint64_t flow_stride, const void* weight,
+                         uint32_t weight_type, float offset, float eps, void* dr, uint64_t dr_stride, float* dw,
+                         uint32_t accumulate, uint32_t rows, uint32_t cols, void* workspace, uint64_t workspace_bytes,
+                         hipStream_t stream);
+
 const char* netra_layers_last_error(void);
 
 #ifdef __cplusplus

@@ -168,4 +168,29 @@ inline CountPlan balance_plan(uint32_t tokens, uint32_t experts) {
   return count_plan(tokens, few < 256u ? few : 256u, 64u);
 }
 
+// Norms: waves a row and eight columns a lane so many times, rows a workgroup takes at once, and
+// workgroups (they loop over the rows).
+struct NormPlan {
+  uint32_t waves, chunks, rows, threads, groups;
+};
+inline NormPlan norm_shape(uint32_t cols) {
+  if (cols <= 512u) return {1, 1, 4, 256, 0};
+  if (cols <= 1024u) return {1, 2, 4, 256, 0};
+  const uint32_t waves = cols <= 2048u ? 4u : cols <= 4096u ? 8u : 16u;
+  return {waves, cols <= 8192u ? 1u : 2u, 1, 64u * waves, 0};
+}
+inline NormPlan norm_plan(uint32_t rows, uint32_t cols) {
+  NormPlan p = norm_shape(cols);
+  const uint32_t groups = (rows + p.rows - 1u) / p.rows, most = 8192u * 64u / p.threads;
+  p.groups = groups < most ? groups : most;
+  return p;
+}
+// A workgroup leaves partial sums of dw for each row that it takes at once.
+inline NormPlan norm_gradients_plan(uint32_t rows, uint32_t cols) {
+  NormPlan p = norm_shape(cols);
+  const uint32_t groups = (rows + p.rows - 1u) / p.rows, most = 4096u * 64u / p.threads;
+  p.groups = groups < most ? groups : most;
+  return p;
+}
+
 }  // namespace nkplan
