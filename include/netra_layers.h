@@ -154,6 +154,36 @@ int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t dy_stride, c
                          uint32_t accumulate, uint32_t rows, uint32_t cols, void* workspace, uint64_t workspace_bytes,
                          hipStream_t stream);
 
+// Routing to experts. s = softmax(logits) over the experts or sigmoid(logits); c = s + bias (bias
+// fp32 [experts] or null: it moves the choice, not the weights). The experts are `groups` runs of
+// equal length; a group's score is its largest c (NETRA_GROUP_MAX) or the sum of its two largest
+// (NETRA_GROUP_TOP2), and the top_groups best groups are kept. ids[t, 0 .. k) are the k largest c of those in
+// falling order; ties go to the lower index, of groups as of experts. c is compared exactly: by the logits
+// where their order decides (no bias, no sums of two), else in 64 bits. A NaN ranks as -inf.
+//   weights[t, i] = scale * s_i, or scale * s_i / sum over the chosen of s (renormalise; 0 where the sum is 0,
+//   as where all of them are below 2^-126)
+// shared 1: logits has a column more, the shared expert's gate, and slot k is
+// (experts, sigmoid(logits[t, experts])), unscaled. Tokens whose mask byte is 0 get ids -1 and weights 0.
+// experts 1 .. 1024, k + shared 1 .. 16, groups 1 .. 16; ids and weights have row strides in elements.
+enum { NETRA_SOFTMAX = 0, NETRA_SIGMOID = 1 };
+enum { NETRA_GROUP_MAX = 0, NETRA_GROUP_TOP2 = 1 };
+int netra_router_select(const void* logits, uint32_t logits_type, uint64_t logits_stride, const float* bias,
+                        const uint8_t* mask, uint32_t tokens, uint32_t experts, uint32_t k, uint32_t shared,
+                        uint32_t scoring, uint32_t groups, uint32_t top_groups, uint32_t group_score, uint32_t renormalise,
+                        float scale, int32_t* ids, uint64_t ids_stride, float* weights, uint64_t weights_stride,
+                        hipStream_t stream);
+
+// The weights' gradient carried to the logits, for given choices: with dweights fp32 [tokens, k + shared],
+//   grad[t, e] = sum_i dweights[t, i] dweights_i / dlogits_e    (of the logits' type, [tokens, experts + shared])
+// ids as above; slots whose id is not an expert (a dropped route) have the weight 0 and no gradient, and
+// are left out of the sum that renormalises. An id that stands in several slots counts as often.
+// Tokens whose mask byte is 0 get zeros. accumulate != 0 adds to grad (the balance loss's gradient, say).
+int netra_router_select_gradient(const float* dweights, uint64_t dweights_stride, const void* logits,
+                                 uint32_t logits_type, uint64_t logits_stride, const int32_t* ids, uint64_t ids_stride,
+                                 const uint8_t* mask, uint32_t tokens, uint32_t experts, uint32_t k, uint32_t shared,
+                                 uint32_t scoring, uint32_t renormalise, float scale, void* grad, uint64_t grad_stride,
+                                 uint32_t accumulate, hipStream_t stream);
+
 const char* netra_layers_last_error(void);
 
 #ifdef __cplusplus

@@ -193,4 +193,10 @@ inline NormPlan norm_gradients_plan(uint32_t rows, uint32_t cols) {
   return p;
 }
 
+// Workgroups of the routing: each takes so many tokens at a time and loops past a whole chip's worth of waves.
+inline uint32_t select_groups(uint32_t tokens, uint32_t at_once) {
+  const uint32_t groups = (tokens - 1u) / at_once + 1u;
+  return groups < 4096u ? groups : 4096u;
+}
+
 }  // namespace nkplan

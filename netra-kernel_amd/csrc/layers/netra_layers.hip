@@ -522,3 +522,4 @@ extern "C" int netra_router_balance(const void* logits, uint32_t logits_type, ui
 extern "C" const char* netra_layers_last_error(void) { return g_error.c_str(); }
 
 #include "norm_call.h"
+#include "router_select_call.h"

@@ -1,0 +1,488 @@
+// Routing to experts: scores, the choice of the k best (of the best groups), their weights, and
+// the weights' gradient.
+//
+// A token's row is held by G lanes (16: a wave takes four tokens; 64), and lane i of each 16 holds
+// the token's i-th choice, so k is at most 16. What is compared is exact: where the choice goes by
+// the logits' own order (no bias, groups by their best expert) the logits are compared, else scores in
+// 64 bits.
+#pragma once
+#include <type_traits>
+
+#include "router_balance.hip"
+
+namespace nksel {
+
+constexpr uint32_t kMost = 16;  // choices of a token, and groups of experts
+
+enum Scoring { kSoftmax, kSigmoid };
+
+// exp(-|z|); NaN stays NaN.
+__device__ __forceinline__ float exp_minus(float z) { return nkbal::exp_nonpos(-fabsf(z)); }
+// sigmoid(z), to a few ulp at both ends.
+__device__ __forceinline__ float sigmoid(float z) {
+  const float e = exp_minus(z);
+  return (z < 0.0f ? e : 1.0f) / (1.0f + e);
+}
+// Its derivative; from e, as 1 - sigmoid has few bits left where the sigmoid is near one.
+__device__ __forceinline__ float slope(float z) {
+  const float e = exp_minus(z), d = 1.0f + e;
+  return e / (d * d);
+}
+
+struct Select {
+  const void* z;
+  uint64_t z_stride;
+  const float* bias;          // null: none
+  const uint8_t* mask;        // null: all tokens
+  uint32_t tokens, experts, k, shared;
+  uint32_t scoring, groups, each, top_groups, top2, renormalise;
+  float scale;
+  int32_t* ids;
+  uint64_t ids_stride;
+  float* weights;
+  uint64_t weights_stride;
+};
+
+// Order of logits; a NaN ranks as -inf. 0 is free for what cannot be chosen.
+__device__ __forceinline__ uint32_t order(float z) {
+  return nk::order_bits(z == z ? z : -__builtin_inff());
+}
+
+template <uint32_t G, bool kMax>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+  auto join = [](uint32_t a, uint32_t b) __attribute__((always_inline)) { return kMax ? max(a, b) : min(a, b); };
+#define NETRA_DPP(CTRL) (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false)
+  v = join(v, NETRA_DPP(0xB1));
+  v = join(v, NETRA_DPP(0x4E));
+  v = join(v, NETRA_DPP(0x141));
+  v = join(v, NETRA_DPP(0x140));
+#undef NETRA_DPP
+  if constexpr (G == 16u) return v;
+  const auto r16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = join((uint32_t)r16[0], (uint32_t)r16[1]);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return join((uint32_t)r32[0], (uint32_t)r32[1]);
+}
+
+// v of the lane n further on (mod 16) in the row of 16. (Every lane has to be active: never under a
+// condition that differs between lanes.)
+template <uint32_t N>
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + (int)(16u - N), 0xF, 0xF, false);
+}
+template <uint32_t N>
+__device__ __forceinline__ float turned(float v) {
+  return __uint_as_float(turned<N>(__float_as_uint(v)));
+}
+template <uint32_t N = 1, typename F>
+__device__ __forceinline__ void each_turn(F&& f) {
+  if constexpr (N < 16u) {
+    f(std::integral_constant<uint32_t, N>{});
+    each_turn<N + 1u>(f);
+  }
+}
+
+// The groups that are kept, one bit each: `score` is lane g's group's (g < groups), in an order of T.
+template <typename T, typename Turn>
+__device__ __forceinline__ bool kept(T score, uint32_t groups, uint32_t top, Turn&& turn) {
+  const uint32_t g = threadIdx.x & 15u;
+  uint32_t before = 0u;
+  each_turn([&](auto n) __attribute__((always_inline)) {
+    const uint32_t other = (g + n) & 15u;
+    const T s = turn(score, n);
+    before += other < groups && (s > score || (s == score && other < g)) ? 1u : 0u;
+  });
+  return g < groups && before < top;
+}
+
+// Weights of the choices, lane i of a row of 16 its token's i-th, from its logit z (the row's
+// largest logit and the sum of its exponentials where the softmax is over the whole row), and the
+// stores.
+template <typename X>
+__device__ __forceinline__ void finish(const Select& a, uint32_t t, uint32_t id, float top, float total, bool writes) {
+  const uint32_t i = threadIdx.x & 15u;
+  const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
+  const bool mine = i < a.k;
+  auto value = [&](uint32_t e) __attribute__((always_inline)) {
+    if constexpr (sizeof(X) == 4) return row[e];
+    else return nk::bf16_f32(row[e]);
+  };
+  const float z = value(mine ? id : 0u);
+  float s;
+  if (a.scoring == kSigmoid) {
+    s = sigmoid(z);
+  } else {
+    if (a.renormalise) {
+      top = nkbal::reduce<16, true>(mine ? z : -__builtin_inff());
+      if (top == -__builtin_inff()) top = 0.0f;
+    }
+    s = nkbal::exp_nonpos(z - top);
+  }
+  if (a.renormalise) total = nkbal::sum<16>(mine ? s : 0.0f);
+  float w = s;
+  if (a.renormalise || a.scoring == kSoftmax) w = total == 0.0f ? 0.0f : s / total;
+  w *= a.scale;
+  const bool live = !a.mask || a.mask[t];
+  if (!writes || i >= a.k + a.shared) return;
+  if (!mine) {
+    id = a.experts;
+    w = sigmoid(value(a.experts));
+  }
+  a.ids[(uint64_t)t * a.ids_stride + i] = live ? (int32_t)id : -1;
+  a.weights[(uint64_t)t * a.weights_stride + i] = live ? w : 0.0f;
+}
+
+// The choice by the logits' own order.
+template <typename X, uint32_t G, uint32_t NV>
+__device__ __forceinline__ void select_direct(const Select& a) {
+  constexpr uint32_t kTokens = 64u / G, kWaves = 4u;
+  __shared__ uint32_t s_key[kWaves][kTokens][G * NV];
+  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t batches = (a.tokens - 1u) / kTokens + 1u;
+  for (uint32_t b = blockIdx.x * kWaves + wave; b < batches; b += gridDim.x * kWaves) {
+    const uint32_t t0 = b * kTokens, rows = min(kTokens, a.tokens - t0), t = t0 + min(lane / G, rows - 1u);
+    nkbal::Rows<X, NV> raw;
+    nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
+    uint32_t key[NV];
+    float top = 0.0f, total = 0.0f;
+    {
+      float z[NV];
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        const uint32_t e = nkbal::expert<G>(lane, j);
+        z[j] = e < E ? nkbal::at(raw, j, e, E) : -__builtin_inff();
+        key[j] = e < E ? order(z[j]) : 0u;
+      }
+      if (a.scoring == kSoftmax && !a.renormalise) {
+        top = z[0];
+#pragma unroll
+        for (uint32_t j = 1; j < NV; ++j) top = fmaxf(top, z[j]);
+        top = nkbal::reduce<G, true>(top);
+        if (top == -__builtin_inff()) top = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j) total += nkbal::exp_nonpos(z[j] - top);
+        total = nkbal::sum<G>(total);
+      }
+    }
+    if (a.groups > 1u) {
+      uint32_t* s = s_key[wave][lane / G];
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) s[nkbal::expert<G>(lane, j)] = key[j];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      uint32_t best = 0u;
+      if (i < a.groups)
+        for (uint32_t m = 0; m < a.each; ++m) best = max(best, s[i * a.each + m]);
+      const bool keep = kept(best, a.groups, a.top_groups,
+                             [](uint32_t v, auto n) __attribute__((always_inline)) { return turned<decltype(n)::value>(v); });
+      const uint32_t bits = (uint32_t)(__ballot(keep) >> (lane & 48u)) & 0xffffu;
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j)
+        if (!(bits >> min(nkbal::expert<G>(lane, j) / a.each, 31u) & 1u)) key[j] = 0u;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    uint32_t id = 0u;
+    const uint32_t base = nkbal::expert<G>(lane, 0u);
+    for (uint32_t n = 0; n < a.k; ++n) {
+      uint32_t m = key[0];
+#pragma unroll
+      for (uint32_t j = 1; j < NV; ++j) m = max(m, key[j]);
+      m = across<G, true>(m);
+      uint32_t at = ~0u;
+#pragma unroll
+      for (uint32_t j = NV; j-- > 0u;)
+        if (key[j] == m) at = nkbal::expert<G>(lane, j);
+      at = across<G, false>(at);
+      if (i == n) id = at;
+      const uint32_t gone = at - base;
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j)
+        if (gone == nkbal::expert<G>(0u, j)) key[j] = 0u;
+    }
+    finish<X>(a, t, id, top, total, lane / G < rows && (G == 16u || lane < 16u));
+  }
+}
+
+__device__ __forceinline__ double sum64(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+  return v;
+}
+__device__ __forceinline__ float max64(float v) { return nkbal::reduce<64, true>(v); }
+
+// One token by a wave, its scores in 64 bits.
+template <typename X>
+__device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double* s) {
+  constexpr uint32_t NV = 16;
+  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts;
+  const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
+  float z[NV], top = -__builtin_inff(), total = 0.0f;
+  double c[NV];
+#pragma unroll
+  for (uint32_t j = 0; j < NV; ++j) {
+    const uint32_t e = lane + 64u * j;
+    z[j] = -__builtin_inff();
+    if (e < E) {
+      if constexpr (sizeof(X) == 4) z[j] = row[e];
+      else z[j] = nk::bf16_f32(row[e]);
+    }
+    top = fmaxf(top, z[j]);
+  }
+  if (a.scoring == kSoftmax) {
+    top = max64(top);
+    if (top == -__builtin_inff()) top = 0.0f;
+    double all = 0.0;
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) {
+      c[j] = exp((double)z[j] - (double)top);
+      all += c[j];
+    }
+    all = sum64(all);
+    total = (float)all;
+    const double inv = all == 0.0 ? 0.0 : 1.0 / all;
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) c[j] *= inv;
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) c[j] = 1.0 / (1.0 + exp(-(double)z[j]));
+  }
+  uint32_t taken = 0u;  // of the lane's values: what cannot be chosen
+#pragma unroll
+  for (uint32_t j = 0; j < NV; ++j) {
+    const uint32_t e = lane + 64u * j;
+    if (e >= E) taken |= 1u << j;
+    else if (a.bias) c[j] += (double)a.bias[e];
+    if (!(c[j] == c[j])) c[j] = -__builtin_inf();
+  }
+  if (a.groups > 1u) {
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j)
+      if (lane + 64u * j < E) s[lane + 64u * j] = c[j];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    double best = -__builtin_inf(), second = -__builtin_inf();
+    if (i < a.groups)
+      for (uint32_t m = 0; m < a.each; ++m) {
+        const double v = s[i * a.each + m];
+        second = fmax(second, fmin(best, v));
+        best = fmax(best, v);
+      }
+    if (a.top2) best += second;
+    const bool keep = kept(best, a.groups, a.top_groups, [](double v, auto n) __attribute__((always_inline)) {
+      const uint64_t u = (uint64_t)__double_as_longlong(v);
+      return __longlong_as_double((long long)((uint64_t)turned<decltype(n)::value>((uint32_t)(u >> 32)) << 32 | turned<decltype(n)::value>((uint32_t)u)));
+    });
+    const uint32_t bits = (uint32_t)__ballot(keep) & 0xffffu;
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j)
+      if (!(bits >> min((lane + 64u * j) / a.each, 31u) & 1u)) taken |= 1u << j;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  uint32_t id = 0u;
+  for (uint32_t n = 0; n < a.k; ++n) {
+    double m = -__builtin_inf();
+    uint32_t at = ~0u;
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j)
+      if (!(taken >> j & 1u) && (at == ~0u || c[j] > m)) {
+        m = c[j];
+        at = lane + 64u * j;
+      }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const double om = __shfl_xor(m, d);
+      const uint32_t oa = (uint32_t)__shfl_xor((int)at, d);
+      if (oa != ~0u && (at == ~0u || om > m || (om == m && oa < at))) {
+        m = om;
+        at = oa;
+      }
+    }
+    if (i == n) id = at;
+    if ((at & 63u) == lane) taken |= 1u << (at / 64u);
+  }
+  finish<X>(a, t, id, top, total, lane < 16u);
+}
+
+template <typename X>
+__device__ __forceinline__ void select_scored(const Select& a) {
+  __shared__ double s[4][1024];
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  for (uint32_t t = blockIdx.x * 4u + wave; t < a.tokens; t += gridDim.x * 4u) select_exact<X>(a, t, s[wave]);
+}
+
+struct SelectGradient {
+  const float* dw;
+  uint64_t dw_stride;
+  const void* z;
+  uint64_t z_stride;
+  const int32_t* ids;
+  uint64_t ids_stride;
+  const uint8_t* mask;
+  uint32_t tokens, experts, k, shared, scoring, renormalise;
+  float scale;
+  void* grad;                 // of z's type
+  uint64_t grad_stride;
+  uint32_t accumulate;
+};
+
+// The gradient of the logits. Lane i of a row of 16 has the token's i-th choice. Differences of the
+// weights' gradients are taken before they are weighted (sum_j s_j (v_i - v_j), not v_i S - sum_j s_j v_j):
+// nothing cancels where one expert has almost all. The row goes through LDS.
+template <typename X, uint32_t G, uint32_t NV>
+__device__ __forceinline__ void gradient(const SelectGradient& a) {
+  constexpr uint32_t kTokens = 64u / G, kWaves = 4u;
+  __shared__ float s_row[kWaves][kTokens][G * NV];
+  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t batches = (a.tokens - 1u) / kTokens + 1u;
+  const bool whole = a.scoring == kSoftmax && !a.renormalise;
+  float* s = s_row[wave][lane / G];
+  // bits of an expert that was not chosen: a NaN that no arithmetic gives
+  const float none = __uint_as_float(0xffc0ffeeu);
+  auto hit = [&](float v) __attribute__((always_inline)) { return __float_as_uint(v) != 0xffc0ffeeu; };
+#pragma unroll
+  for (uint32_t j = 0; j < NV; ++j) s[nkbal::expert<G>(lane, j)] = none;
+  for (uint32_t b = blockIdx.x * kWaves + wave; b < batches; b += gridDim.x * kWaves) {
+    const uint32_t t0 = b * kTokens, rows = min(kTokens, a.tokens - t0), t = t0 + min(lane / G, rows - 1u);
+    const bool live = !a.mask || a.mask[t];
+    const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
+    auto value = [&](uint32_t e) __attribute__((always_inline)) {
+      if constexpr (sizeof(X) == 4) return row[e];
+      else return nk::bf16_f32(row[e]);
+    };
+    nkbal::Rows<X, NV> raw;
+    if (whole) nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
+    const bool slot = i < a.k;
+    const uint32_t id = slot ? (uint32_t)a.ids[(uint64_t)t * a.ids_stride + i] : ~0u;
+    const bool chosen = id < E && live;
+    const float d = i < a.k + a.shared ? a.dw[(uint64_t)t * a.dw_stride + i] : 0.0f;
+    const float z = chosen ? value(id) : 0.0f;
+    float v = chosen ? d * a.scale : 0.0f, out[NV];
+    // The first slot of an expert speaks for all slots that name it: v becomes their sum where the
+    // score is one of the whole row.
+    bool first = chosen;
+    float together = v;
+    each_turn([&](auto n) __attribute__((always_inline)) {
+      const uint32_t other = (i + n) & 15u;
+      const bool again = turned<decltype(n)::value>(id) == id && chosen;
+      const float ov = turned<decltype(n)::value>(v);
+      if (again) {
+        together += ov;
+        if (other < i) first = false;
+      }
+    });
+    float mine = 0.0f;  // the choice's gradient
+    float inv = 0.0f, q = 0.0f, top = 0.0f;
+    if (whole) {
+      top = -__builtin_inff();
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        const uint32_t e = nkbal::expert<G>(lane, j);
+        out[j] = e < E ? nkbal::at(raw, j, e, E) : -__builtin_inff();
+        top = fmaxf(top, out[j]);
+      }
+      top = nkbal::reduce<G, true>(top);
+      if (top == -__builtin_inff()) top = 0.0f;
+      if (first) s[id] = 1.0f;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      float others = 0.0f, total = 0.0f;
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        out[j] = nkbal::exp_nonpos(out[j] - top);
+        total += out[j];
+        if (!hit(s[nkbal::expert<G>(lane, j)])) others += out[j];
+      }
+      total = nkbal::sum<G>(total);
+      others = nkbal::sum<G>(others);
+      inv = total == 0.0f ? 0.0f : 1.0f / total;
+      const float p = first ? nkbal::exp_nonpos(z - top) * inv : 0.0f;
+      v = first ? together : 0.0f;
+      q = nkbal::sum<16>(p * v);
+      float diff = v * (others * inv);
+      each_turn([&](auto n) __attribute__((always_inline)) { diff = fmaf(turned<decltype(n)::value>(p), v - turned<decltype(n)::value>(v), diff); });
+      mine = p * diff;
+    } else {
+      float p;
+      if (a.scoring == kSigmoid) {
+        p = chosen ? sigmoid(z) : 0.0f;
+      } else {
+        float m = nkbal::reduce<16, true>(chosen ? z : -__builtin_inff());
+        if (m == -__builtin_inff()) m = 0.0f;
+        p = chosen ? nkbal::exp_nonpos(z - m) : 0.0f;
+      }
+      if (a.renormalise) {
+        const float total = nkbal::sum<16>(p);
+        const float r = total == 0.0f ? 0.0f : 1.0f / total;
+        float diff = 0.0f;
+        each_turn([&](auto n) __attribute__((always_inline)) { diff = fmaf(turned<decltype(n)::value>(p), v - turned<decltype(n)::value>(v), diff); });
+        v = a.scoring == kSigmoid ? diff * r * r : diff * r * (p * r);
+      }
+      if (a.scoring == kSigmoid) v *= slope(z);
+      if (!chosen) v = 0.0f;
+      mine = v;
+      each_turn([&](auto n) __attribute__((always_inline)) {
+        const float ov = turned<decltype(n)::value>(v);
+        mine += turned<decltype(n)::value>(id) == id && chosen ? ov : 0.0f;
+      });
+    }
+    if (first) s[id] = mine;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (whole) {
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) out[j] = live ? -(out[j] * inv) * q : 0.0f;
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) out[j] = 0.0f;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) {
+      const float at = s[nkbal::expert<G>(lane, j)];
+      if (hit(at)) out[j] = at;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (first) s[id] = none;
+    const bool writes = lane / G < rows;
+    X* to = static_cast<X*>(a.grad) + (uint64_t)t * a.grad_stride;
+    if (a.accumulate) {
+      nkbal::Rows<X, NV> old;
+      nkbal::load_rows<X, G, NV>(a.grad, a.grad_stride, t0, rows, E, old);
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        const uint32_t e = nkbal::expert<G>(lane, j);
+        out[j] += e < E ? nkbal::at(old, j, e, E) : 0.0f;
+      }
+    }
+    nkbal::store_rows<X, G, NV>(a.grad, a.grad_stride, t0, rows, E, out);
+    if (a.shared && i == a.k && writes && (G == 16u || lane < 16u)) {
+      float gate = live ? d * slope(value(E)) : 0.0f;
+      if constexpr (sizeof(X) == 4) {
+        to[E] = a.accumulate ? to[E] + gate : gate;
+      } else {
+        if (a.accumulate) gate += nk::bf16_f32(to[E]);
+        to[E] = (uint16_t)nk::bf16x2_hw(gate, 0.0f);
+      }
+    }
+  }
+}
+
+}  // namespace nksel
+
+#define NETRA_SELECT(NAME, X, G, NV)                                                                        \
+  extern "C" __global__ __launch_bounds__(256) void netra_router_select_##NAME##_##G##x##NV##_gfx950(       \
+      nksel::Select a) {                                                                                    \
+    nksel::select_direct<X, G, NV>(a);                                                                      \
+  }                                                                                                         \
+  extern "C" __global__                                                                                     \
+      __launch_bounds__(256) void netra_router_select_gradient_##NAME##_##G##x##NV##_gfx950(nksel::SelectGradient a) { \
+    nksel::gradient<X, G, NV>(a);                                                                           \
+  }
+#define NETRA_SELECTS(NAME, X)                                                                              \
+  NETRA_SELECT(NAME, X, 16, 4)                                                                              \
+  NETRA_SELECT(NAME, X, 16, 8)                                                                              \
+  NETRA_SELECT(NAME, X, 16, 16)                                                                             \
+  NETRA_SELECT(NAME, X, 16, 32)                                                                             \
+  NETRA_SELECT(NAME, X, 64, 16)                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void netra_router_select_scored_##NAME##_gfx950(nksel::Select a) { \
+    nksel::select_scored<X>(a);                                                                             \
+  }
+NETRA_SELECTS(bf16, uint16_t)
+NETRA_SELECTS(f32, float)

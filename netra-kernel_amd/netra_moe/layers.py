@@ -31,6 +31,8 @@ SIGNATURES = {
     "netra_norm_forward": (ctypes.c_int, [P, U32, U64, P, U32, U64, P, U32, F32, F32, P, U64, P, U32, U64, P, P, U32, U32, U32, P]),
     "netra_norm_gradients_workspace": (U64, [U32] * 2),
     "netra_norm_gradients": (ctypes.c_int, [P, U32, U64, P, U32, U64, P, U64, P, U32, F32, F32, P, U64, P, U32, U32, U32, P, U64, P]),
+    "netra_router_select": (ctypes.c_int, [P, U32, U64, P, P] + [U32] * 9 + [F32, P, U64, P, U64, P]),
+    "netra_router_select_gradient": (ctypes.c_int, [P, U64, P, U32, U64, P, U64, P] + [U32] * 6 + [F32, P, U64, U32, P]),
     "netra_layers_last_error": (ctypes.c_char_p, []),
 }
 TYPES = {torch.bfloat16: 0, torch.float32: 1}  # NETRA_BF16, NETRA_F32
