@@ -184,6 +184,30 @@ int netra_router_select_gradient(const float* dweights, uint64_t dweights_stride
                                  uint32_t scoring, uint32_t renormalise, float scale, void* grad, uint64_t grad_stride,
                                  uint32_t accumulate, hipStream_t stream);
 
+// Low-rank adapters of many requests beside a shared projection: for every token t with the adapter l,
+//   out[t] = y[t] + scale[l] B_l (A_l x[t]),  A_l [rank, k], B_l [n, rank] bf16 (fp32 is rounded when packed)
+// and out[t] = y[t] for tokens without one. x bf16 or fp32 [tokens, k] (fp32 is rounded to bf16), y
+// and out bf16 [tokens, n], scale fp32 [adapters]. A_l x and all sums are fp32, A_l x enters the
+// second product with 16 bits, and the sum with y is rounded once. adapters 1 .. 1024, rank 1 .. 128.
+//
+// Weights are laid out once: a [adapters, rank, k], b [adapters, n, rank], both of `type`. which:
+// 0 packed_a, 1 packed_b; both 16-byte aligned.
+uint64_t netra_adapters_packed_bytes(uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k, uint32_t which);
+int netra_adapters_pack(const void* a, const void* b, uint32_t type, void* packed_a, void* packed_b, uint32_t adapters,
+                        uint32_t rank, uint32_t n, uint32_t k, hipStream_t stream);
+// A batch's plan, for every call with the same ids (all layers of a step): ids i32 [tokens], outside 0 .. adapters - 1
+// for none. plan 16-byte aligned; calls that read it may overlap. A call whose tokens or
+// adapters are not the plan's writes nothing.
+uint64_t netra_adapters_plan_bytes(uint32_t tokens, uint32_t adapters);
+int netra_adapters_plan(const int32_t* ids, uint32_t tokens, uint32_t adapters, void* plan, uint64_t plan_bytes,
+                        hipStream_t stream);
+// out may be y (same address and stride); any other overlap is refused. tokens 0 .. 2^21.
+uint64_t netra_adapters_add_workspace(uint32_t tokens, uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k);
+int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_stride, const void* packed_a, const void* packed_b,
+                       const float* scale, const void* plan, const uint16_t* y, uint64_t y_stride, uint16_t* out,
+                       uint64_t out_stride, uint32_t tokens, uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k,
+                       void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+
 const char* netra_layers_last_error(void);
 
 #ifdef __cplusplus

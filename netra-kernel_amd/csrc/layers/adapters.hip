@@ -1,0 +1,388 @@
+// Low-rank adapters of many requests beside a shared projection: out = y + s_l B_l (A_l x) for each
+// token with its adapter l.
+//
+// A plan sorts the batch's tokens by adapter into tiles of one adapter each; every layer of a step
+// uses the same one. Then two products: u = A x (contraction k, the ranks of a tile's tokens as
+// fp32) and out = y + s B u (contraction of the rank). Operands are packed once so that a lane's
+// operand bytes lie together:
+//   A  [adapter][128-block of k][16 ranks][4][64 lanes][8]: lane l's operand j is rank l % 16,
+//      columns 32 (l / 16) + 8 j .. + 7 of the block (the sum runs over k in any order, so a lane
+//      reads 64 neighbouring bytes of a row of x)
+//   B  [adapter][64 columns][16 ranks][64 lanes][4][4]: lane l's operand j is column
+//      16 (l % 16 / 4) + 4 j + l % 4, ranks 4 (l / 16) .. + 3 (a lane's results of the four j are
+//      16 neighbouring columns of a token)
+// u goes into the second product as the sum of two bf16 values (the rounded value and what the
+// rounding left), in one matrix instruction with B's operand twice: 16 bits instead of 8 for no
+// more instructions than its contraction of 32 has room for.
+#pragma once
+#include "linear_fp8.hip"
+
+namespace nkada {
+
+using nk::u32x2;
+using nk::u32x4;
+using nk::v4f;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kMaxAdapters = 1024, kMaxRank = 128;
+
+// Plan words: tiles, tokens, adapters, 0; the tokens by adapter (those without one last, as
+// adapter `adapters`); the tiles {adapter, first, tokens, 0}.
+constexpr uint32_t kPlanHead = 4;
+__device__ __forceinline__ const uint4* plan_tiles(const uint32_t* plan, uint32_t tokens) {
+  return reinterpret_cast<const uint4*>(plan + kPlanHead + (tokens + 3u) / 4u * 4u);
+}
+
+// The plan by one workgroup: 16 waves count a run of the tokens each, then place them in order.
+// Within 64 tokens a lane's place is the number of lanes before it with the same adapter, found one
+// adapter at a time.
+__device__ __forceinline__ void make_plan(const int32_t* __restrict__ ids, uint32_t tokens, uint32_t adapters,
+                                          uint32_t tile, uint32_t* plan) {
+  __shared__ uint32_t count[16][kMaxAdapters + 1];
+  __shared__ uint32_t scan[2][16], carry[2];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, parts = adapters + 1u;
+  for (uint32_t i = threadIdx.x; i < 16u * (kMaxAdapters + 1u); i += 1024u) count[i / (kMaxAdapters + 1u)][i % (kMaxAdapters + 1u)] = 0u;
+  if (threadIdx.x < 2u) carry[threadIdx.x] = 0u;
+  __syncthreads();
+  const uint32_t each = ((tokens + 15u) / 16u + 63u) / 64u * 64u, t0 = wave * each, t1 = min(tokens, t0 + each);
+  auto adapter = [&](uint32_t t) __attribute__((always_inline)) { return min((uint32_t)ids[t], adapters); };
+  for (uint32_t t = t0 + lane; t < t1; t += 64u) atomicAdd(&count[wave][adapter(t)], 1u);
+  __syncthreads();
+  // an adapter's tokens and tiles before it, 1024 adapters at a time
+  uint4* tiles = const_cast<uint4*>(plan_tiles(plan, tokens));
+  for (uint32_t first = 0; first < parts; first += 1024u) {
+    const uint32_t l = first + threadIdx.x;
+    uint32_t n = 0u;
+    if (l < parts)
+      for (uint32_t w = 0; w < 16u; ++w) n += count[w][l];
+    uint32_t own[2] = {n, (n + tile - 1u) / tile}, before[2];
+#pragma unroll
+    for (uint32_t s = 0; s < 2u; ++s) {
+      uint32_t v = own[s];
+      for (uint32_t d = 1; d < 64u; d *= 2u) {
+        const uint32_t o = (uint32_t)__shfl_up((int)v, d);
+        if (lane >= d) v += o;
+      }
+      if (lane == 63u) scan[s][wave] = v;
+      before[s] = v - own[s];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t s = 0; s < 2u; ++s) {
+      before[s] += carry[s];
+      for (uint32_t w = 0; w < wave; ++w) before[s] += scan[s][w];
+    }
+    __syncthreads();
+    if (threadIdx.x == 1023u) {
+      carry[0] = before[0] + own[0];
+      carry[1] = before[1] + own[1];
+    }
+    if (l < parts) {
+      uint32_t at = before[0];
+      for (uint32_t w = 0; w < 16u; ++w) {
+        const uint32_t c = count[w][l];
+        count[w][l] = at;
+        at += c;
+      }
+      for (uint32_t i = 0; i < own[1]; ++i)
+        tiles[before[1] + i] = make_uint4(l, before[0] + i * tile, min(tile, n - i * tile), 0u);
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0u) {
+    plan[0] = carry[1];
+    plan[1] = tokens;
+    plan[2] = adapters;
+    plan[3] = 0u;
+  }
+  for (uint32_t b = t0; b < t1; b += 64u) {
+    const uint32_t t = b + lane;
+    const bool there = t < t1;
+    const uint32_t l = there ? adapter(t) : 0u;
+    uint64_t left = __ballot(there);
+    while (left) {
+      const uint32_t who = (uint32_t)__builtin_amdgcn_readlane((int)l, __ffsll((unsigned long long)left) - 1);
+      const uint64_t with = __ballot(there && l == who);
+      const uint32_t at = count[wave][who];
+      if (there && l == who) plan[kPlanHead + at + __popcll(with & ((1ull << lane) - 1ull))] = t;
+      if (lane == 0u) count[wave][who] = at + __popcll(with);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      left &= ~with;
+    }
+  }
+}
+
+// Packing: a thread per 8 values of A, 4 of B; zeros outside the matrices. Weights bf16 or fp32.
+template <typename X>
+__device__ __forceinline__ uint32_t bf16_at(const X* m, uint64_t i, bool there) {
+  if (!there) return 0u;
+  if constexpr (sizeof(X) == 2) return m[i];
+  else return nk::bf16_rne(m[i]);
+}
+template <typename X>
+__device__ __forceinline__ void pack_a(const X* __restrict__ a, uint4* __restrict__ out, uint32_t adapters, uint32_t rank,
+                                       uint32_t k, uint32_t nr) {
+  const uint32_t kb = (k + 127u) / 128u;
+  const uint64_t all = (uint64_t)adapters * kb * nr * 256u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
+    const uint32_t lane = (uint32_t)(i & 63u), j = (uint32_t)(i >> 6) & 3u;
+    const uint64_t rest = i >> 8, block = rest / nr;
+    const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane & 15u), c = (uint32_t)(block % kb) * 128u + (lane >> 4) * 32u + j * 8u;
+    const uint64_t row = ((block / kb) * rank + r) * (uint64_t)k;
+    uint32_t w[4];
+#pragma unroll
+    for (uint32_t h = 0; h < 4u; ++h)
+      w[h] = bf16_at(a, row + c + 2u * h, r < rank && c + 2u * h < k) |
+             bf16_at(a, row + c + 2u * h + 1u, r < rank && c + 2u * h + 1u < k) << 16;
+    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <typename X>
+__device__ __forceinline__ void pack_b(const X* __restrict__ b, uint2* __restrict__ out, uint32_t adapters, uint32_t rank,
+                                       uint32_t n, uint32_t nr) {
+  const uint32_t nb = (n + 63u) / 64u;
+  const uint64_t all = (uint64_t)adapters * nb * nr * 256u;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
+    const uint32_t j = (uint32_t)i & 3u, lane = (uint32_t)(i >> 2) & 63u;
+    const uint64_t rest = i >> 8, block = rest / nr;
+    const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane >> 4) * 4u;
+    const uint32_t c = (uint32_t)(block % nb) * 64u + 16u * ((lane & 15u) >> 2) + 4u * j + (lane & 3u);
+    const uint64_t row = ((block / nb) * n + c) * (uint64_t)rank;
+    uint32_t w[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; ++h)
+      w[h] = bf16_at(b, row + r + 2u * h, c < n && r + 2u * h < rank) |
+             bf16_at(b, row + r + 2u * h + 1u, c < n && r + 2u * h + 1u < rank) << 16;
+    out[i] = make_uint2(w[0], w[1]);
+  }
+}
+
+struct Adapters {
+  const void* x;
+  uint64_t x_stride;
+  const uint8_t* a;
+  const uint8_t* b;
+  const float* scale;
+  const uint32_t* plan;
+  float* u;                   // [splits][tokens by the plan's order][16 nr]
+  uint32_t splits, split_blocks;  // of k's 128-blocks
+  const uint16_t* y;
+  uint64_t y_stride;
+  uint16_t* out;
+  uint64_t out_stride;
+  uint32_t tokens, adapters, rank, n, k, in_place, wide, chunks;  // wide: 64-column groups a wave takes; chunks: workgroups across the columns
+};
+
+__device__ __forceinline__ bool tile_of(const Adapters& a, uint32_t at, uint4& tile) {
+  if (a.plan[1] != a.tokens || a.plan[2] != a.adapters || at >= a.plan[0]) return false;
+  tile = plan_tiles(a.plan, a.tokens)[at];
+  return true;
+}
+
+// u of a tile: TT times 16 tokens by 16 NR ranks. The eight waves of a workgroup share k's blocks
+// out among them and join their sums through LDS, in the order of the waves.
+template <typename X, uint32_t TT, uint32_t NR>
+__device__ __forceinline__ void shrink(const Adapters& a) {
+  constexpr uint32_t W = 8u;
+  __shared__ v4f part[W][TT * NR][64];
+  uint4 tile;
+  if (!tile_of(a, blockIdx.x, tile) || tile.x >= a.adapters) return;
+  const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t kb = (a.k + 127u) / 128u, b1 = min(kb, (blockIdx.y + 1u) * a.split_blocks);
+  const X* row[TT];
+#pragma unroll
+  for (uint32_t t = 0; t < TT; ++t) {
+    const uint32_t at = min(t * 16u + (lane & 15u), tile.z - 1u);  // (past the tile its last token again)
+    row[t] = static_cast<const X*>(a.x) + (uint64_t)a.plan[kPlanHead + tile.y + at] * a.x_stride;
+  }
+  v4f acc[TT][NR];
+#pragma unroll
+  for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+    for (uint32_t r = 0; r < NR; ++r) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t b = blockIdx.y * a.split_blocks + wave; b < b1; b += W) {
+    const uint4* ab = reinterpret_cast<const uint4*>(a.a) + ((uint64_t)tile.x * kb + b) * (NR * 256u) + lane;
+    nklin::Raw<X> raw[TT];
+#pragma unroll
+    for (uint32_t t = 0; t < TT; ++t) {
+      raw[t] = {};
+      if (b * 128u + (lane >> 4) * 32u < a.k) nklin::load32(row[t], b * 128u + (lane >> 4) * 32u, a.k, raw[t]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) {
+      bf16x8 x[TT];
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t) {
+        u32x4 w;
+#pragma unroll
+        for (uint32_t h = 0; h < 4u; ++h) {
+          if constexpr (sizeof(X) == 2) w[h] = raw[t].w[4u * j + h];
+          else w[h] = nk::bf16x2_hw(raw[t].w[8u * j + 2u * h], raw[t].w[8u * j + 2u * h + 1u]);
+        }
+        x[t] = __builtin_bit_cast(bf16x8, w);
+      }
+#pragma unroll
+      for (uint32_t r = 0; r < NR; ++r) {
+        const bf16x8 w = __builtin_bit_cast(bf16x8, ab[(r * 4u + j) * 64u]);
+#pragma unroll
+        for (uint32_t t = 0; t < TT; ++t) acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[t], acc[t][r], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+    for (uint32_t r = 0; r < NR; ++r) part[wave][t * NR + r][lane] = acc[t][r];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < TT * NR * 64u; i += 512u) {
+    const uint32_t l = i & 63u, tr = i >> 6, at = tr / NR * 16u + (l & 15u);
+    v4f v = part[0][tr][l];
+#pragma unroll
+    for (uint32_t w = 1; w < W; ++w) v += part[w][tr][l];
+    if (at < tile.z)
+      *reinterpret_cast<v4f*>(a.u + ((uint64_t)blockIdx.y * a.tokens + tile.y + at) * (16u * NR) + tr % NR * 16u + (l >> 4) * 4u) = v;
+  }
+}
+
+struct __attribute__((packed, aligned(2))) Unaligned32 {
+  uint32_t w[8];
+};
+
+// 16 neighbouring columns of a row from c on (nothing at or past n).
+__device__ __forceinline__ Unaligned32 load16(const uint16_t* row, uint32_t c, uint32_t n) {
+  if (c + 16u <= n) return *reinterpret_cast<const Unaligned32*>(row + c);
+  Unaligned32 v = {};
+#pragma unroll
+  for (uint32_t i = 0; i < 16u; ++i)
+    if (c + i < n) v.w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i & 1u));
+  return v;
+}
+__device__ __forceinline__ void store16(uint16_t* row, uint32_t c, uint32_t n, const Unaligned32& v) {
+  if (c + 16u <= n) {
+    *reinterpret_cast<Unaligned32*>(row + c) = v;
+    return;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 16u; ++i)
+    if (c + i < n) row[c + i] = (uint16_t)(v.w[i / 2u] >> (16u * (i & 1u)));
+}
+
+// out of a tile, `wide` times 64 columns a wave.
+template <uint32_t TT, uint32_t NR>
+__device__ __forceinline__ void expand(const Adapters& a) {
+  uint4 tile;
+  const uint32_t at_tile = blockIdx.x / a.chunks, chunk = blockIdx.x - at_tile * a.chunks;
+  if (!tile_of(a, at_tile, tile)) return;
+  const bool none = tile.x >= a.adapters;
+  if (none && a.in_place) return;
+  const uint32_t lane = threadIdx.x & 63u, q = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t nb = (a.n + 63u) / 64u, s0 = (chunk * 4u + wave) * a.wide, s1 = min(nb, s0 + a.wide);
+  const uint16_t* from[TT];
+  uint16_t* to[TT];
+  bool there[TT];
+  bf16x8 u[TT][NR];
+  const float scale = none ? 0.0f : a.scale[tile.x];
+#pragma unroll
+  for (uint32_t t = 0; t < TT; ++t) {
+    const uint32_t i = t * 16u + (lane & 15u), at = tile.y + min(i, tile.z - 1u);
+    there[t] = i < tile.z;
+    const uint32_t token = a.plan[kPlanHead + at];
+    from[t] = a.y + (uint64_t)token * a.y_stride;
+    to[t] = a.out + (uint64_t)token * a.out_stride;
+#pragma unroll
+    for (uint32_t r = 0; r < NR; ++r) {
+      v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (!none)
+        for (uint32_t s = 0; s < a.splits; ++s)
+          v += *reinterpret_cast<const v4f*>(a.u + ((uint64_t)s * a.tokens + at) * (16u * NR) + r * 16u + q * 4u);
+      float hi[4], lo[4];
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e) {
+        // ranks past the last are zeros times what x holds: not 0 where that is an infinity
+        const float f = r * 16u + q * 4u + e < a.rank ? v[e] * scale : 0.0f;
+        hi[e] = nk::bf16_round_hw(f);
+        lo[e] = fabsf(hi[e]) < __builtin_inff() ? f - hi[e] : 0.0f;
+      }
+      const u32x4 w = {nk::bf16x2_hw(hi[0], hi[1]), nk::bf16x2_hw(hi[2], hi[3]), nk::bf16x2_hw(lo[0], lo[1]),
+                       nk::bf16x2_hw(lo[2], lo[3])};
+      u[t][r] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+  for (uint32_t s = s0; s < s1; ++s) {
+    const uint32_t c = s * 64u + q * 16u;
+    Unaligned32 y[TT];
+#pragma unroll
+    for (uint32_t t = 0; t < TT; ++t) y[t] = load16(from[t], c, a.n);
+    if (!none) {
+      v4f acc[TT][4];
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) acc[t][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      const uint4* bb = reinterpret_cast<const uint4*>(a.b) + (((uint64_t)tile.x * nb + s) * NR * 64u + lane) * 2u;
+#pragma unroll
+      for (uint32_t r = 0; r < NR; ++r) {
+        const uint4 lo = bb[r * 128u], hi = bb[r * 128u + 1u];
+        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) {
+          const u32x4 twice = {w[2u * j], w[2u * j + 1u], w[2u * j], w[2u * j + 1u]};
+          const bf16x8 b = __builtin_bit_cast(bf16x8, twice);
+#pragma unroll
+          for (uint32_t t = 0; t < TT; ++t)
+            acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, u[t][r], acc[t][j], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i)
+          y[t].w[i] = nk::bf16x2_hw(nk::bf16_lo(y[t].w[i]) + acc[t][i / 2u][2u * (i & 1u)],
+                                    nk::bf16_hi(y[t].w[i]) + acc[t][i / 2u][2u * (i & 1u) + 1u]);
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < TT; ++t)
+      if (there[t]) store16(to[t], c, a.n, y[t]);
+  }
+}
+
+}  // namespace nkada
+
+extern "C" __global__ __launch_bounds__(1024) void netra_adapters_plan_gfx950(const int32_t* ids, uint32_t tokens,
+                                                                              uint32_t adapters, uint32_t tile,
+                                                                              uint32_t* plan) {
+  nkada::make_plan(ids, tokens, adapters, tile, plan);
+}
+#define NETRA_ADAPTERS_PACK(NAME, X)                                                                            \
+  extern "C" __global__ __launch_bounds__(256) void netra_adapters_pack_a_##NAME##_gfx950(                      \
+      const X* a, uint4* out, uint32_t adapters, uint32_t rank, uint32_t k, uint32_t nr) {                      \
+    nkada::pack_a(a, out, adapters, rank, k, nr);                                                               \
+  }                                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void netra_adapters_pack_b_##NAME##_gfx950(                      \
+      const X* b, uint2* out, uint32_t adapters, uint32_t rank, uint32_t n, uint32_t nr) {                      \
+    nkada::pack_b(b, out, adapters, rank, n, nr);                                                               \
+  }
+NETRA_ADAPTERS_PACK(bf16, uint16_t)
+NETRA_ADAPTERS_PACK(f32, float)
+// t: 16-token parts of a tile, r: 16-rank parts
+#define NETRA_ADAPTERS(TT, NR)                                                                                  \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_bf16_t##TT##r##NR##_gfx950(           \
+      nkada::Adapters a) {                                                                                      \
+    nkada::shrink<uint16_t, TT, NR>(a);                                                                         \
+  }                                                                                                             \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_f32_t##TT##r##NR##_gfx950(            \
+      nkada::Adapters a) {                                                                                      \
+    nkada::shrink<float, TT, NR>(a);                                                                            \
+  }                                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void netra_adapters_expand_t##TT##r##NR##_gfx950(nkada::Adapters a) { \
+    nkada::expand<TT, NR>(a);                                                                                   \
+  }
+NETRA_ADAPTERS(1, 1)
+NETRA_ADAPTERS(1, 2)
+NETRA_ADAPTERS(1, 4)
+NETRA_ADAPTERS(1, 8)
+NETRA_ADAPTERS(2, 1)
+NETRA_ADAPTERS(2, 2)
+NETRA_ADAPTERS(2, 4)
+NETRA_ADAPTERS(2, 8)

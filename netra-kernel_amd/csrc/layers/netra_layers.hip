@@ -523,3 +523,4 @@ extern "C" const char* netra_layers_last_error(void) { return g_error.c_str(); }
 
 #include "norm_call.h"
 #include "router_select_call.h"
+#include "adapters_call.h"

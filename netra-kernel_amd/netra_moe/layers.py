@@ -33,6 +33,12 @@ SIGNATURES = {
     "netra_norm_gradients": (ctypes.c_int, [P, U32, U64, P, U32, U64, P, U64, P, U32, F32, F32, P, U64, P, U32, U32, U32, P, U64, P]),
     "netra_router_select": (ctypes.c_int, [P, U32, U64, P, P] + [U32] * 9 + [F32, P, U64, P, U64, P]),
     "netra_router_select_gradient": (ctypes.c_int, [P, U64, P, U32, U64, P, U64, P] + [U32] * 6 + [F32, P, U64, U32, P]),
+    "netra_adapters_packed_bytes": (U64, [U32] * 5),
+    "netra_adapters_pack": (ctypes.c_int, [P, P, U32, P, P] + [U32] * 4 + [P]),
+    "netra_adapters_plan_bytes": (U64, [U32] * 2),
+    "netra_adapters_plan": (ctypes.c_int, [P, U32, U32, P, U64, P]),
+    "netra_adapters_add_workspace": (U64, [U32] * 5),
+    "netra_adapters_add": (ctypes.c_int, [P, U32, U64, P, P, P, P, P, U64, P, U64] + [U32] * 5 + [P, U64, P]),
     "netra_layers_last_error": (ctypes.c_char_p, []),
 }
 TYPES = {torch.bfloat16: 0, torch.float32: 1}  # NETRA_BF16, NETRA_F32

@@ -30,6 +30,7 @@ import torch
 
 from . import prep
 from . import weights as W
+from .adapters import AdapterPlan, LowRankAdapters
 from .layers import TYPES, check_rows, entry, launch, workspace
 
 
@@ -105,9 +106,16 @@ class BlockLinear:
                out.data_ptr(), out_stride, rows, self.N, self.K, ws_ptr, need)
         return out
 
-    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        """x bf16 or fp32 [T, K] -> x W^T, bf16 [T, N]."""
-        return self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
+    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, *, adapters: LowRankAdapters | None = None,
+                plan: AdapterPlan | None = None) -> torch.Tensor:
+        """x bf16 or fp32 [T, K] -> x W^T, bf16 [T, N]. adapters and plan: the tokens' low-rank
+        adapters are added (adapters.py)."""
+        if adapters is None:
+            return self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
+        if plan is None or (adapters.N, adapters.K) != (self.N, self.K):
+            raise ValueError(f"adapters: need a plan and adapters of N {self.N}, K {self.K}")
+        y = self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
+        return adapters.add(y, x, plan, y)
 
     __call__ = forward
 
