@@ -2,9 +2,15 @@
 // the weights' gradient.
 //
 // A token's row is held by G lanes (16: a wave takes four tokens; 64), and lane i of each 16 holds
-// the token's i-th choice, so k is at most 16. What is compared is exact: where the choice goes by
-// the logits' own order (no bias, groups by their best expert) the logits are compared, else scores in
-// 64 bits.
+// the token's i-th choice, so k is at most 16.
+//
+// What is compared is exact: logits where their own order decides (no bias, groups by their best
+// expert), else scores in 64 bits. All of it in 64 bits took 229 us for 32768 tokens of 256 experts.
+// So an expert is first a 32-bit key, its score in 22 bits and its index behind it (the
+// order of equal ones), which is sorted with one minimum and one maximum an exchange. Only where two neighbours in that
+// order that the choice hangs on are nearer than the key's error, and not the same score by the same
+// operands, the token is done again in 64 bits, by the whole wave. Keys of bf16 logits hold all of them and are never
+// done again.
 #pragma once
 #include <type_traits>
 
@@ -36,16 +42,18 @@ struct Select {
   const uint8_t* mask;        // null: all tokens
   uint32_t tokens, experts, k, shared;
   uint32_t scoring, groups, each, top_groups, top2, renormalise;
-  float scale;
+  uint32_t by_logits;         // the choice goes by the logits' order
+  float scale, inv_each;
   int32_t* ids;
   uint64_t ids_stride;
   float* weights;
   uint64_t weights_stride;
 };
 
-// Order of logits; a NaN ranks as -inf. 0 is free for what cannot be chosen.
+// Order of logits: the bits of -0 as of 0, of a NaN as of -inf, negative numbers' turned round.
 __device__ __forceinline__ uint32_t order(float z) {
-  return nk::order_bits(z == z ? z : -__builtin_inff());
+  const uint32_t u = __float_as_uint(fmaxf(z + 0.0f, -__builtin_inff()));
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 
 template <uint32_t G, bool kMax>
@@ -82,7 +90,7 @@ __device__ __forceinline__ void each_turn(F&& f) {
   }
 }
 
-// The groups that are kept, one bit each: `score` is lane g's group's (g < groups), in an order of T.
+// Whether lane g's group of 16 (g < groups) is among the `top` best by `score`, in an order of T; ties to the lower.
 template <typename T, typename Turn>
 __device__ __forceinline__ bool kept(T score, uint32_t groups, uint32_t top, Turn&& turn) {
   const uint32_t g = threadIdx.x & 15u;
@@ -132,77 +140,6 @@ __device__ __forceinline__ void finish(const Select& a, uint32_t t, uint32_t id,
   a.weights[(uint64_t)t * a.weights_stride + i] = live ? w : 0.0f;
 }
 
-// The choice by the logits' own order.
-template <typename X, uint32_t G, uint32_t NV>
-__device__ __forceinline__ void select_direct(const Select& a) {
-  constexpr uint32_t kTokens = 64u / G, kWaves = 4u;
-  __shared__ uint32_t s_key[kWaves][kTokens][G * NV];
-  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts;
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t batches = (a.tokens - 1u) / kTokens + 1u;
-  for (uint32_t b = blockIdx.x * kWaves + wave; b < batches; b += gridDim.x * kWaves) {
-    const uint32_t t0 = b * kTokens, rows = min(kTokens, a.tokens - t0), t = t0 + min(lane / G, rows - 1u);
-    nkbal::Rows<X, NV> raw;
-    nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
-    uint32_t key[NV];
-    float top = 0.0f, total = 0.0f;
-    {
-      float z[NV];
-#pragma unroll
-      for (uint32_t j = 0; j < NV; ++j) {
-        const uint32_t e = nkbal::expert<G>(lane, j);
-        z[j] = e < E ? nkbal::at(raw, j, e, E) : -__builtin_inff();
-        key[j] = e < E ? order(z[j]) : 0u;
-      }
-      if (a.scoring == kSoftmax && !a.renormalise) {
-        top = z[0];
-#pragma unroll
-        for (uint32_t j = 1; j < NV; ++j) top = fmaxf(top, z[j]);
-        top = nkbal::reduce<G, true>(top);
-        if (top == -__builtin_inff()) top = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < NV; ++j) total += nkbal::exp_nonpos(z[j] - top);
-        total = nkbal::sum<G>(total);
-      }
-    }
-    if (a.groups > 1u) {
-      uint32_t* s = s_key[wave][lane / G];
-#pragma unroll
-      for (uint32_t j = 0; j < NV; ++j) s[nkbal::expert<G>(lane, j)] = key[j];
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      uint32_t best = 0u;
-      if (i < a.groups)
-        for (uint32_t m = 0; m < a.each; ++m) best = max(best, s[i * a.each + m]);
-      const bool keep = kept(best, a.groups, a.top_groups,
-                             [](uint32_t v, auto n) __attribute__((always_inline)) { return turned<decltype(n)::value>(v); });
-      const uint32_t bits = (uint32_t)(__ballot(keep) >> (lane & 48u)) & 0xffffu;
-#pragma unroll
-      for (uint32_t j = 0; j < NV; ++j)
-        if (!(bits >> min(nkbal::expert<G>(lane, j) / a.each, 31u) & 1u)) key[j] = 0u;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    uint32_t id = 0u;
-    const uint32_t base = nkbal::expert<G>(lane, 0u);
-    for (uint32_t n = 0; n < a.k; ++n) {
-      uint32_t m = key[0];
-#pragma unroll
-      for (uint32_t j = 1; j < NV; ++j) m = max(m, key[j]);
-      m = across<G, true>(m);
-      uint32_t at = ~0u;
-#pragma unroll
-      for (uint32_t j = NV; j-- > 0u;)
-        if (key[j] == m) at = nkbal::expert<G>(lane, j);
-      at = across<G, false>(at);
-      if (i == n) id = at;
-      const uint32_t gone = at - base;
-#pragma unroll
-      for (uint32_t j = 0; j < NV; ++j)
-        if (gone == nkbal::expert<G>(0u, j)) key[j] = 0u;
-    }
-    finish<X>(a, t, id, top, total, lane / G < rows && (G == 16u || lane < 16u));
-  }
-}
-
 __device__ __forceinline__ double sum64(double v) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
@@ -210,10 +147,9 @@ __device__ __forceinline__ double sum64(double v) {
 }
 __device__ __forceinline__ float max64(float v) { return nkbal::reduce<64, true>(v); }
 
-// One token by a wave, its scores in 64 bits.
-template <typename X>
+// One token by a wave, its scores in 64 bits. s: 64 NV values.
+template <typename X, uint32_t NV>
 __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double* s) {
-  constexpr uint32_t NV = 16;
   const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts;
   const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
   float z[NV], top = -__builtin_inff(), total = 0.0f;
@@ -242,9 +178,13 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
     const double inv = all == 0.0 ? 0.0 : 1.0 / all;
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) c[j] *= inv;
-  } else {
+  } else if (!a.by_logits) {
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) c[j] = 1.0 / (1.0 + exp(-(double)z[j]));
+  }
+  if (a.by_logits) {
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) c[j] = (double)z[j];
   }
   uint32_t taken = 0u;  // of the lane's values: what cannot be chosen
 #pragma unroll
@@ -302,11 +242,230 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
   finish<X>(a, t, id, top, total, lane < 16u);
 }
 
-template <typename X>
-__device__ __forceinline__ void select_scored(const Select& a) {
-  __shared__ double s[4][1024];
+// What a key is made of: the whole logit (bf16), the distance to the row's largest logit (fp32), or
+// the score and the bias.
+enum Kind { kWhole, kDistance, kScore };
+
+// a >= b after.
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b) {
+  const uint32_t m = min(a, b);
+  a = max(a, b);
+  b = m;
+}
+// Falling order, by merging odd and even places of sorted halves (Batcher's network).
+template <uint32_t LO, uint32_t N, uint32_t R, uint32_t NV>
+__device__ __forceinline__ void merge(uint32_t (&v)[NV]) {
+  constexpr uint32_t S = R * 2u;
+  if constexpr (S < N) {
+    merge<LO, N, S>(v);
+    merge<LO + R, N, S>(v);
+#pragma unroll
+    for (uint32_t i = LO + R; i + R < LO + N; i += S) exchange(v[i], v[i + R]);
+  } else {
+    exchange(v[LO], v[LO + R]);
+  }
+}
+template <uint32_t LO, uint32_t N, uint32_t NV>
+__device__ __forceinline__ void sort(uint32_t (&v)[NV]) {
+  if constexpr (N > 1u) {
+    sort<LO, N / 2u>(v);
+    sort<LO + N / 2u, N / 2u>(v);
+    merge<LO, N, 1u>(v);
+  }
+}
+
+// Each wave takes 64 / G tokens at a time.
+template <typename X, uint32_t G, uint32_t NV, Kind K>
+__device__ __forceinline__ void select(const Select& a) {
+  constexpr uint32_t kTokens = 64u / G, kWaves = 4u, kMax = G * NV;
+  __shared__ double s_memory[kWaves][kMax > kTokens * kMax / 2u ? kMax : kTokens * kMax / 2u];
+  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u;
+  uint32_t E = a.experts;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  for (uint32_t t = blockIdx.x * 4u + wave; t < a.tokens; t += gridDim.x * 4u) select_exact<X>(a, t, s[wave]);
+  const uint32_t batches = (a.tokens - 1u) / kTokens + 1u;
+  constexpr float kUnits = 4194302.0f;  // of a key's upper 22 bits, from 1 on
+  // Scores: lo .. hi over 0 and the finite biases, and a score's 0 .. 1, are the units' range. A sigmoid is
+  // off by 5e-7 by the hardware's exponential and reciprocal, a softmax by its sum too; then the sum with the bias.
+  float bias[NV], lo = 0.0f, units = 0.0f;
+  uint32_t near = K == kWhole ? 0u : 4u;  // keys that are apart by no more are not told apart
+  if constexpr (K == kScore) {
+    const __amdgpu_buffer_rsrc_t r = nk::buffer_rsrc(a.bias, a.bias ? E * 4u : 0u);  // (no bias: zeros)
+    float hi = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < NV; j += 4u) {
+      const nk::u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(nkbal::expert<G>(lane, j) * 4u), 0, 0);
+#pragma unroll
+      for (uint32_t n = 0; n < 4u; ++n) bias[j + n] = __uint_as_float(v[n]);
+    }
+    asm volatile("" : "+s"(E));  // (as below)
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) {
+      const float f = fabsf(bias[j]) < __builtin_inff() ? bias[j] : 0.0f;
+      lo = fminf(lo, f);
+      hi = fmaxf(hi, f);
+    }
+    lo = -nkbal::reduce<G, true>(-lo);
+    hi = nkbal::reduce<G, true>(hi);
+    units = kUnits / (hi - lo + 1.0f);
+    const float off = (a.scoring == kSigmoid ? 6e-7f : 2.5e-6f) + 2.4e-7f * (1.0f + fmaxf(fabsf(lo), fabsf(hi)));
+    near = 3u + (uint32_t)fminf(2.0f * off * units, 8e6f);
+    // lanes' places past the last expert: the least key, behind every expert's that has it too
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) bias[j] = nkbal::expert<G>(lane, j) < E ? bias[j] : -__builtin_inff();
+  }
+  for (uint32_t b = blockIdx.x * kWaves + wave; b < batches; b += gridDim.x * kWaves) {
+    const uint32_t t0 = b * kTokens, rows = min(kTokens, a.tokens - t0), t = t0 + min(lane / G, rows - 1u);
+    nkbal::Rows<X, NV> raw;
+    nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
+    uint32_t key[NV];
+    float top = 0.0f, total = 0.0f;
+    // Each round compares with its own E: hoisted, the comparisons' masks would not fit the scalar registers.
+    asm volatile("" : "+s"(E));
+    {
+      float z[NV];
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        const uint32_t e = nkbal::expert<G>(lane, j);
+        z[j] = e < E ? nkbal::at(raw, j, e, E) : -__builtin_inff();
+      }
+      if (K == kDistance || a.scoring == kSoftmax) {
+        top = z[0];
+#pragma unroll
+        for (uint32_t j = 1; j < NV; ++j) top = fmaxf(top, z[j]);
+        top = nkbal::reduce<G, true>(top);
+      }
+      if constexpr (K != kScore) {
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j) {
+          const uint32_t e = nkbal::expert<G>(lane, j);
+          if constexpr (K == kWhole) {
+            key[j] = (order(z[j]) & 0xffff0000u) | (0xffffu - e);
+          } else {
+            // 32 and more below the largest: the least key
+            const float x = fmaxf(z[j], -__builtin_inff());
+            const float d = x == top ? 0.0f : fminf((top - x) * 0.03125f, 1.0f);
+            key[j] = (1u + (uint32_t)(kUnits * (1.0f - d))) << 10 | (1023u - e);
+          }
+        }
+      }
+      if (a.scoring == kSoftmax) {
+        if (top == -__builtin_inff()) top = 0.0f;
+        if (K == kScore || !a.renormalise) {
+#pragma unroll
+          for (uint32_t j = 0; j < NV; ++j) {
+            z[j] = nkbal::exp_nonpos(z[j] - top);
+            total += z[j];
+          }
+          total = nkbal::sum<G>(total);
+        }
+      }
+      if constexpr (K == kScore) {
+        if (a.scoring == kSigmoid) {
+#pragma unroll
+          for (uint32_t j = 0; j < NV; ++j)
+            z[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[j] * -1.44269504088896341f));
+        } else {
+          const float inv = total == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(total);
+#pragma unroll
+          for (uint32_t j = 0; j < NV; ++j) z[j] *= inv;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j) {
+          const uint32_t e = nkbal::expert<G>(lane, j);
+          const float c = (z[j] + bias[j] - lo) * units;
+          key[j] = (1u + (uint32_t)fminf(fmaxf(c, 0.0f), kUnits)) << 10 | (1023u - e);
+        }
+      }
+    }
+    bool again = false;
+    if (a.groups > 1u) {
+      uint32_t* s = reinterpret_cast<uint32_t*>(s_memory[wave]) + lane / G * kMax;
+#pragma unroll
+      for (uint32_t j = 0; j < NV; j += 4u)
+        *reinterpret_cast<uint4*>(s + nkbal::expert<G>(lane, j)) = make_uint4(key[j], key[j + 1u], key[j + 2u], key[j + 3u]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      uint32_t best = 0u, second = 0u;
+      auto take = [&](uint32_t v) __attribute__((always_inline)) {
+        second = max(second, min(best, v));
+        best = max(best, v);
+      };
+      if (i < a.groups) {
+        const uint32_t* from = s + i * a.each;
+        if (a.each % 4u == 0u) {
+          for (uint32_t m = 0; m < a.each; m += 4u) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from + m);
+            take(v.x);
+            take(v.y);
+            take(v.z);
+            take(v.w);
+          }
+        } else {
+          for (uint32_t m = 0; m < a.each; ++m) take(from[m]);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // (the best expert's key orders the groups itself, as lower groups have lower experts)
+      const uint32_t shift = a.top2 ? 4u : 10u;
+      const uint32_t score = i >= a.groups ? 0u : a.top2 ? ((best >> 10) + (second >> 10)) << 4 | (15u - i) : best;
+      uint32_t before = 0u;
+      each_turn([&](auto n) __attribute__((always_inline)) {
+        before += turned<decltype(n)::value>(score) > score ? 1u : 0u;
+      });
+      const bool keep = before < a.top_groups;
+      if constexpr (K != kWhole) {
+        const uint32_t least = across<16, false>(keep ? score : ~0u) >> shift;
+        const uint32_t most = across<16, true>(keep ? 0u : score) >> shift;
+        again = least - most <= (a.top2 ? 2u * near : near);
+      }
+      const uint32_t bits = (uint32_t)(__ballot(keep) >> (lane & 48u)) & 0xffffu;
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        const uint32_t g = (uint32_t)(((float)nkbal::expert<G>(lane, j) + 0.5f) * a.inv_each);
+        key[j] &= (uint32_t)__builtin_amdgcn_sbfe((int)bits, min(g, 31u), 1u);
+      }
+    }
+    sort<0u, NV>(key);
+    // two more than k, to see whether the k-th and the next one are apart
+    uint32_t mine = 0u;
+    const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
+    for (uint32_t n = 0; n < draws; ++n) {
+      const uint32_t m = across<G, true>(key[0]);
+      if (i == n) mine = m;
+      // by bits: of a choice between two places the compiler makes a place chosen at run time
+      const uint32_t gone = key[0] == m ? ~0u : 0u;
+#pragma unroll
+      for (uint32_t j = 0; j + 1u < NV; ++j) key[j] = (key[j] & ~gone) | (key[j + 1u] & gone);
+      key[NV - 1u] &= ~gone;
+    }
+    const uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
+    if constexpr (K != kWhole) {
+      // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
+      const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
+      uint32_t zb, bb = 0u;
+      if constexpr (sizeof(X) == 4) zb = __float_as_uint(row[id]);
+      else zb = row[id];
+      if (K == kScore && a.bias) bb = __float_as_uint(a.bias[id]);
+      const uint32_t next = turned<1>(mine), nz = turned<1>(zb), nb = turned<1>(bb);
+      const bool close = next != 0u && (mine >> 10) - (next >> 10) <= near;
+      const bool same = zb == nz && bb == nb;
+      const bool next_close = turned<1>(close ? 1u : 0u) != 0u;
+      bool bad = i < a.k && close && !same;
+      if (i + 1u == a.k) bad = close && (!same || a.k + 2u > kMost || next_close);
+      if (a.k == kMost && i + 1u == a.k) bad = true;  // no lane holds the next one
+      again |= bad;
+      const bool live = !a.mask || a.mask[t];
+      uint64_t todo = __ballot(again && live && lane / G < rows);
+      const bool done = G == 64u ? todo == 0u : (todo >> (lane & 48u) & 0xffffu) == 0u;
+      finish<X>(a, t, id, top, total, done && lane / G < rows && (G == 16u || lane < 16u));
+      while (todo) {
+        const uint32_t at = ((uint32_t)__ffsll((unsigned long long)todo) - 1u) / G;
+        select_exact<X, kMax / 64u>(a, t0 + at, s_memory[wave]);
+        todo &= G == 64u ? 0ull : ~(0xffffull << (at * 16u));
+      }
+    } else {
+      finish<X>(a, t, id, top, total, lane / G < rows && (G == 16u || lane < 16u));
+    }
+  }
 }
 
 struct SelectGradient {
@@ -466,23 +625,24 @@ __device__ __forceinline__ void gradient(const SelectGradient& a) {
 
 }  // namespace nksel
 
-#define NETRA_SELECT(NAME, X, G, NV)                                                                        \
+#define NETRA_SELECT(NAME, X, KIND, G, NV)                                                                  \
   extern "C" __global__ __launch_bounds__(256) void netra_router_select_##NAME##_##G##x##NV##_gfx950(       \
       nksel::Select a) {                                                                                    \
-    nksel::select_direct<X, G, NV>(a);                                                                      \
+    nksel::select<X, G, NV, nksel::KIND>(a);                                                                \
+  }                                                                                                         \
+  extern "C" __global__ __launch_bounds__(256) void netra_router_select_scored_##NAME##_##G##x##NV##_gfx950( \
+      nksel::Select a) {                                                                                    \
+    nksel::select<X, G, NV, nksel::kScore>(a);                                                              \
   }                                                                                                         \
   extern "C" __global__                                                                                     \
       __launch_bounds__(256) void netra_router_select_gradient_##NAME##_##G##x##NV##_gfx950(nksel::SelectGradient a) { \
     nksel::gradient<X, G, NV>(a);                                                                           \
   }
-#define NETRA_SELECTS(NAME, X)                                                                              \
-  NETRA_SELECT(NAME, X, 16, 4)                                                                              \
-  NETRA_SELECT(NAME, X, 16, 8)                                                                              \
-  NETRA_SELECT(NAME, X, 16, 16)                                                                             \
-  NETRA_SELECT(NAME, X, 16, 32)                                                                             \
-  NETRA_SELECT(NAME, X, 64, 16)                                                                             \
-  extern "C" __global__ __launch_bounds__(256) void netra_router_select_scored_##NAME##_gfx950(nksel::Select a) { \
-    nksel::select_scored<X>(a);                                                                             \
-  }
-NETRA_SELECTS(bf16, uint16_t)
-NETRA_SELECTS(f32, float)
+#define NETRA_SELECTS(NAME, X, KIND)                                                                        \
+  NETRA_SELECT(NAME, X, KIND, 16, 4)                                                                        \
+  NETRA_SELECT(NAME, X, KIND, 16, 8)                                                                        \
+  NETRA_SELECT(NAME, X, KIND, 16, 16)                                                                       \
+  NETRA_SELECT(NAME, X, KIND, 16, 32)                                                                       \
+  NETRA_SELECT(NAME, X, KIND, 64, 16)
+NETRA_SELECTS(bf16, uint16_t, kWhole)
+NETRA_SELECTS(f32, float, kDistance)

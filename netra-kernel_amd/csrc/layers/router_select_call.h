@@ -14,12 +14,14 @@ bool bad_choice(uint32_t tokens, uint32_t experts, uint32_t k, uint32_t shared, 
 // Rows of 32-bit values with a stride in elements.
 bool bad_words(const void* p, uint64_t stride, uint32_t cols) { return !p || !aligned(p, 4) || stride < cols; }
 
-#define NETRA_SELECT_SHAPES(KERNEL)                                 \
-  if (experts <= 64u) launch(KERNEL##_16x4_gfx950, grid, block, a); \
-  else if (experts <= 128u) launch(KERNEL##_16x8_gfx950, grid, block, a); \
-  else if (experts <= 256u) launch(KERNEL##_16x16_gfx950, grid, block, a); \
-  else if (experts <= 512u) launch(KERNEL##_16x32_gfx950, grid, block, a); \
-  else launch(KERNEL##_64x16_gfx950, grid, block, a)
+#define NETRA_SELECT_SHAPES(KERNEL)                                         \
+  do {                                                                      \
+    if (experts <= 64u) launch(KERNEL##_16x4_gfx950, grid, block, a);       \
+    else if (experts <= 128u) launch(KERNEL##_16x8_gfx950, grid, block, a); \
+    else if (experts <= 256u) launch(KERNEL##_16x16_gfx950, grid, block, a); \
+    else if (experts <= 512u) launch(KERNEL##_16x32_gfx950, grid, block, a); \
+    else launch(KERNEL##_64x16_gfx950, grid, block, a);                     \
+  } while (0)
 
 }  // namespace
 
@@ -71,19 +73,16 @@ extern "C" int netra_router_select(const void* logits, uint32_t logits_type, uin
   a.ids_stride = ids_stride;
   a.weights = weights;
   a.weights_stride = weights_stride;
+  a.inv_each = 1.0f / static_cast<float>(a.each);
+  a.by_logits = !bias && (a.groups == 1u || !a.top2);
   Launcher launch(stream);
-  const dim3 block(256);
-  if (bias || (a.groups > 1u && a.top2)) {
-    const dim3 grid(select_groups(tokens, 4u));
-    if (logits_type == NETRA_BF16) launch(netra_router_select_scored_bf16_gfx950, grid, block, a);
-    else launch(netra_router_select_scored_f32_gfx950, grid, block, a);
-    return launch.result(name);
-  }
-  const dim3 grid(select_groups(tokens, experts <= 512u ? 16u : 4u));
+  const dim3 grid(select_groups(tokens, experts <= 512u ? 16u : 4u)), block(256);
   if (logits_type == NETRA_BF16) {
-    NETRA_SELECT_SHAPES(netra_router_select_bf16);
+    if (a.by_logits) NETRA_SELECT_SHAPES(netra_router_select_bf16);
+    else NETRA_SELECT_SHAPES(netra_router_select_scored_bf16);
   } else {
-    NETRA_SELECT_SHAPES(netra_router_select_f32);
+    if (a.by_logits) NETRA_SELECT_SHAPES(netra_router_select_f32);
+    else NETRA_SELECT_SHAPES(netra_router_select_scored_f32);
   }
   return launch.result(name);
 }
