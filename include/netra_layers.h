@@ -164,7 +164,8 @@ int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t dy_stride, c
 //   as where all of them are below 2^-126)
 // shared 1: logits has a column more, the shared expert's gate, and slot k is
 // (experts, sigmoid(logits[t, experts])), unscaled. Tokens whose mask byte is 0 get ids -1 and weights 0.
-// experts 1 .. 1024, k + shared 1 .. 16, groups 1 .. 16; ids and weights have row strides in elements.
+// tokens 0 .. 2^25, experts 1 .. 1024, k + shared 1 .. 16, groups 1 .. 16; ids and weights have row strides in
+// elements.
 enum { NETRA_SOFTMAX = 0, NETRA_SIGMOID = 1 };
 enum { NETRA_GROUP_MAX = 0, NETRA_GROUP_TOP2 = 1 };
 int netra_router_select(const void* logits, uint32_t logits_type, uint64_t logits_stride, const float* bias,

@@ -193,7 +193,9 @@ inline NormPlan norm_gradients_plan(uint32_t rows, uint32_t cols) {
   return p;
 }
 
-// Workgroups of the routing: each takes so many tokens at a time and loops past a whole chip's worth of waves.
+// Tokens of the routing: with four a workgroup the launch's threads still fit their 32 bits.
+constexpr uint32_t kMaxRouted = 1u << 25;
+// Workgroups of the routing's gradient: each takes so many tokens at a time and loops past a whole chip's worth of waves.
 inline uint32_t select_groups(uint32_t tokens, uint32_t at_once) {
   const uint32_t groups = (tokens - 1u) / at_once + 1u;
   return groups < 4096u ? groups : 4096u;

@@ -43,7 +43,7 @@ struct Select {
   uint32_t tokens, experts, k, shared;
   uint32_t scoring, groups, each, top_groups, top2, renormalise;
   uint32_t by_logits;         // the choice goes by the logits' order
-  float scale, inv_each;
+  float scale;
   int32_t* ids;
   uint64_t ids_stride;
   float* weights;
@@ -107,7 +107,7 @@ __device__ __forceinline__ bool kept(T score, uint32_t groups, uint32_t top, Tur
 // largest logit and the sum of its exponentials where the softmax is over the whole row), and the
 // stores.
 template <typename X>
-__device__ __forceinline__ void finish(const Select& a, uint32_t t, uint32_t id, float top, float total, bool writes) {
+__device__ __forceinline__ void finish(const Select& a, uint32_t t, uint32_t id, float top, float total, bool live, bool writes) {
   const uint32_t i = threadIdx.x & 15u;
   const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
   const bool mine = i < a.k;
@@ -130,7 +130,6 @@ __device__ __forceinline__ void finish(const Select& a, uint32_t t, uint32_t id,
   float w = s;
   if (a.renormalise || a.scoring == kSoftmax) w = total == 0.0f ? 0.0f : s / total;
   w *= a.scale;
-  const bool live = !a.mask || a.mask[t];
   if (!writes || i >= a.k + a.shared) return;
   if (!mine) {
     id = a.experts;
@@ -150,7 +149,7 @@ __device__ __forceinline__ float max64(float v) { return nkbal::reduce<64, true>
 // One token by a wave, its scores in 64 bits. s: 64 NV values.
 template <typename X, uint32_t NV>
 __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double* s) {
-  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts;
+  const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, E = a.experts, each = a.each;
   const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
   float z[NV], top = -__builtin_inff(), total = 0.0f;
   double c[NV];
@@ -201,8 +200,8 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     double best = -__builtin_inf(), second = -__builtin_inf();
     if (i < a.groups)
-      for (uint32_t m = 0; m < a.each; ++m) {
-        const double v = s[i * a.each + m];
+      for (uint32_t m = 0; m < each; ++m) {
+        const double v = s[i * each + m];
         second = fmax(second, fmin(best, v));
         best = fmax(best, v);
       }
@@ -214,7 +213,7 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
     const uint32_t bits = (uint32_t)__ballot(keep) & 0xffffu;
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j)
-      if (!(bits >> min((lane + 64u * j) / a.each, 31u) & 1u)) taken |= 1u << j;
+      if (!(bits >> min((lane + 64u * j) / each, 31u) & 1u)) taken |= 1u << j;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   uint32_t id = 0u;
@@ -239,7 +238,7 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
     if (i == n) id = at;
     if ((at & 63u) == lane) taken |= 1u << (at / 64u);
   }
-  finish<X>(a, t, id, top, total, lane < 16u);
+  finish<X>(a, t, id, top, total, true, lane < 16u);
 }
 
 // What a key is made of: the whole logit (bf16), the distance to the row's largest logit (fp32), or
@@ -274,15 +273,38 @@ __device__ __forceinline__ void sort(uint32_t (&v)[NV]) {
   }
 }
 
-// Each wave takes 64 / G tokens at a time.
+// The n largest of the keys that a token's G lanes have in falling order; lane i gets the i-th. Of a lane's own
+// only the first M (n at most) can be among them.
+template <uint32_t G, uint32_t M, uint32_t NV>
+__device__ __forceinline__ uint32_t draw(const uint32_t (&v)[NV], uint32_t n) {
+  constexpr uint32_t L = M < NV ? M : NV;
+  const uint32_t i = threadIdx.x & 15u;
+  uint32_t key[L], mine = 0u;
+#pragma unroll
+  for (uint32_t j = 0; j < L; ++j) key[j] = v[j];
+  for (uint32_t at = 0; at < n; ++at) {
+    const uint32_t m = across<G, true>(key[0]);
+    if (i == at) mine = m;
+    // by bits: of a choice between two places the compiler makes a place chosen at run time
+    const uint32_t gone = key[0] == m ? ~0u : 0u;
+#pragma unroll
+    for (uint32_t j = 0; j + 1u < L; ++j) key[j] = (key[j] & ~gone) | (key[j + 1u] & gone);
+    key[L - 1u] &= ~gone;
+  }
+  return mine;
+}
+
+// Each wave takes 64 / G tokens, and no more than those: in a loop over more the compiler works out beforehand
+// all that the seldom 64-bit part can use, half as many instructions again.
 template <typename X, uint32_t G, uint32_t NV, Kind K>
 __device__ __forceinline__ void select(const Select& a) {
   constexpr uint32_t kTokens = 64u / G, kWaves = 4u, kMax = G * NV;
   __shared__ double s_memory[kWaves][kMax > kTokens * kMax / 2u ? kMax : kTokens * kMax / 2u];
   const uint32_t lane = threadIdx.x & 63u, i = lane & 15u;
-  uint32_t E = a.experts;
+  const uint32_t E = a.experts;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t batches = (a.tokens - 1u) / kTokens + 1u;
+  const uint32_t b = blockIdx.x * kWaves + wave;
+  if (b > (a.tokens - 1u) / kTokens) return;
   constexpr float kUnits = 4194302.0f;  // of a key's upper 22 bits, from 1 on
   // Scores: lo .. hi over 0 and the finite biases, and a score's 0 .. 1, are the units' range. A sigmoid is
   // off by 5e-7 by the hardware's exponential and reciprocal, a softmax by its sum too; then the sum with the bias.
@@ -297,7 +319,6 @@ __device__ __forceinline__ void select(const Select& a) {
 #pragma unroll
       for (uint32_t n = 0; n < 4u; ++n) bias[j + n] = __uint_as_float(v[n]);
     }
-    asm volatile("" : "+s"(E));  // (as below)
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) {
       const float f = fabsf(bias[j]) < __builtin_inff() ? bias[j] : 0.0f;
@@ -310,161 +331,166 @@ __device__ __forceinline__ void select(const Select& a) {
     const float off = (a.scoring == kSigmoid ? 6e-7f : 2.5e-6f) + 2.4e-7f * (1.0f + fmaxf(fabsf(lo), fabsf(hi)));
     near = 3u + (uint32_t)fminf(2.0f * off * units, 8e6f);
     // lanes' places past the last expert: the least key, behind every expert's that has it too
+    if (E < kMax) {
 #pragma unroll
-    for (uint32_t j = 0; j < NV; ++j) bias[j] = nkbal::expert<G>(lane, j) < E ? bias[j] : -__builtin_inff();
+      for (uint32_t j = 0; j < NV; ++j) bias[j] = nkbal::expert<G>(lane, j) < E ? bias[j] : -__builtin_inff();
+    }
   }
-  for (uint32_t b = blockIdx.x * kWaves + wave; b < batches; b += gridDim.x * kWaves) {
-    const uint32_t t0 = b * kTokens, rows = min(kTokens, a.tokens - t0), t = t0 + min(lane / G, rows - 1u);
-    nkbal::Rows<X, NV> raw;
-    nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
-    uint32_t key[NV];
-    float top = 0.0f, total = 0.0f;
-    // Each round compares with its own E: hoisted, the comparisons' masks would not fit the scalar registers.
-    asm volatile("" : "+s"(E));
-    {
-      float z[NV];
+  const uint32_t t0 = b * kTokens, rows = min(kTokens, a.tokens - t0), t = t0 + min(lane / G, rows - 1u);
+  nkbal::Rows<X, NV> raw;
+  nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
+  const bool live = !a.mask || a.mask[t];
+  uint32_t key[NV];
+  float top = 0.0f, total = 0.0f;
+  {
+    float z[NV];
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j) z[j] = nkbal::at(raw, j, 0u, 0u);
+    if (E < kMax || (E & 1u)) {
 #pragma unroll
       for (uint32_t j = 0; j < NV; ++j) {
         const uint32_t e = nkbal::expert<G>(lane, j);
         z[j] = e < E ? nkbal::at(raw, j, e, E) : -__builtin_inff();
       }
-      if (K == kDistance || a.scoring == kSoftmax) {
-        top = z[0];
-#pragma unroll
-        for (uint32_t j = 1; j < NV; ++j) top = fmaxf(top, z[j]);
-        top = nkbal::reduce<G, true>(top);
-      }
-      if constexpr (K != kScore) {
-#pragma unroll
-        for (uint32_t j = 0; j < NV; ++j) {
-          const uint32_t e = nkbal::expert<G>(lane, j);
-          if constexpr (K == kWhole) {
-            key[j] = (order(z[j]) & 0xffff0000u) | (0xffffu - e);
-          } else {
-            // 32 and more below the largest: the least key
-            const float x = fmaxf(z[j], -__builtin_inff());
-            const float d = x == top ? 0.0f : fminf((top - x) * 0.03125f, 1.0f);
-            key[j] = (1u + (uint32_t)(kUnits * (1.0f - d))) << 10 | (1023u - e);
-          }
-        }
-      }
-      if (a.scoring == kSoftmax) {
-        if (top == -__builtin_inff()) top = 0.0f;
-        if (K == kScore || !a.renormalise) {
-#pragma unroll
-          for (uint32_t j = 0; j < NV; ++j) {
-            z[j] = nkbal::exp_nonpos(z[j] - top);
-            total += z[j];
-          }
-          total = nkbal::sum<G>(total);
-        }
-      }
-      if constexpr (K == kScore) {
-        if (a.scoring == kSigmoid) {
-#pragma unroll
-          for (uint32_t j = 0; j < NV; ++j)
-            z[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[j] * -1.44269504088896341f));
-        } else {
-          const float inv = total == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(total);
-#pragma unroll
-          for (uint32_t j = 0; j < NV; ++j) z[j] *= inv;
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < NV; ++j) {
-          const uint32_t e = nkbal::expert<G>(lane, j);
-          const float c = (z[j] + bias[j] - lo) * units;
-          key[j] = (1u + (uint32_t)fminf(fmaxf(c, 0.0f), kUnits)) << 10 | (1023u - e);
-        }
-      }
     }
-    bool again = false;
-    if (a.groups > 1u) {
-      uint32_t* s = reinterpret_cast<uint32_t*>(s_memory[wave]) + lane / G * kMax;
+    if (K == kDistance || a.scoring == kSoftmax) {
+      top = z[0];
 #pragma unroll
-      for (uint32_t j = 0; j < NV; j += 4u)
-        *reinterpret_cast<uint4*>(s + nkbal::expert<G>(lane, j)) = make_uint4(key[j], key[j + 1u], key[j + 2u], key[j + 3u]);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      uint32_t best = 0u, second = 0u;
-      auto take = [&](uint32_t v) __attribute__((always_inline)) {
-        second = max(second, min(best, v));
-        best = max(best, v);
-      };
-      if (i < a.groups) {
-        const uint32_t* from = s + i * a.each;
-        if (a.each % 4u == 0u) {
-          for (uint32_t m = 0; m < a.each; m += 4u) {
-            const uint4 v = *reinterpret_cast<const uint4*>(from + m);
-            take(v.x);
-            take(v.y);
-            take(v.z);
-            take(v.w);
-          }
-        } else {
-          for (uint32_t m = 0; m < a.each; ++m) take(from[m]);
-        }
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      // (the best expert's key orders the groups itself, as lower groups have lower experts)
-      const uint32_t shift = a.top2 ? 4u : 10u;
-      const uint32_t score = i >= a.groups ? 0u : a.top2 ? ((best >> 10) + (second >> 10)) << 4 | (15u - i) : best;
-      uint32_t before = 0u;
-      each_turn([&](auto n) __attribute__((always_inline)) {
-        before += turned<decltype(n)::value>(score) > score ? 1u : 0u;
-      });
-      const bool keep = before < a.top_groups;
-      if constexpr (K != kWhole) {
-        const uint32_t least = across<16, false>(keep ? score : ~0u) >> shift;
-        const uint32_t most = across<16, true>(keep ? 0u : score) >> shift;
-        again = least - most <= (a.top2 ? 2u * near : near);
-      }
-      const uint32_t bits = (uint32_t)(__ballot(keep) >> (lane & 48u)) & 0xffffu;
+      for (uint32_t j = 1; j < NV; ++j) top = fmaxf(top, z[j]);
+      top = nkbal::reduce<G, true>(top);
+    }
+    if constexpr (K != kScore) {
 #pragma unroll
       for (uint32_t j = 0; j < NV; ++j) {
-        const uint32_t g = (uint32_t)(((float)nkbal::expert<G>(lane, j) + 0.5f) * a.inv_each);
-        key[j] &= (uint32_t)__builtin_amdgcn_sbfe((int)bits, min(g, 31u), 1u);
+        const uint32_t e = nkbal::expert<G>(lane, j);
+        if constexpr (K == kWhole) {
+          key[j] = (order(z[j]) & 0xffff0000u) | (0xffffu - e);
+        } else {
+          // 32 and more below the largest: the least key
+          const float x = fmaxf(z[j], -__builtin_inff());
+          const float d = x == top ? 0.0f : fminf((top - x) * 0.03125f, 1.0f);
+          key[j] = (1u + (uint32_t)(kUnits * (1.0f - d))) << 10 | (1023u - e);
+        }
       }
     }
-    sort<0u, NV>(key);
-    // two more than k, to see whether the k-th and the next one are apart
-    uint32_t mine = 0u;
-    const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
-    for (uint32_t n = 0; n < draws; ++n) {
-      const uint32_t m = across<G, true>(key[0]);
-      if (i == n) mine = m;
-      // by bits: of a choice between two places the compiler makes a place chosen at run time
-      const uint32_t gone = key[0] == m ? ~0u : 0u;
+    if (a.scoring == kSoftmax) {
+      if (top == -__builtin_inff()) top = 0.0f;
+      if (K == kScore || !a.renormalise) {
 #pragma unroll
-      for (uint32_t j = 0; j + 1u < NV; ++j) key[j] = (key[j] & ~gone) | (key[j + 1u] & gone);
-      key[NV - 1u] &= ~gone;
-    }
-    const uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
-    if constexpr (K != kWhole) {
-      // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
-      const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
-      uint32_t zb, bb = 0u;
-      if constexpr (sizeof(X) == 4) zb = __float_as_uint(row[id]);
-      else zb = row[id];
-      if (K == kScore && a.bias) bb = __float_as_uint(a.bias[id]);
-      const uint32_t next = turned<1>(mine), nz = turned<1>(zb), nb = turned<1>(bb);
-      const bool close = next != 0u && (mine >> 10) - (next >> 10) <= near;
-      const bool same = zb == nz && bb == nb;
-      const bool next_close = turned<1>(close ? 1u : 0u) != 0u;
-      bool bad = i < a.k && close && !same;
-      if (i + 1u == a.k) bad = close && (!same || a.k + 2u > kMost || next_close);
-      if (a.k == kMost && i + 1u == a.k) bad = true;  // no lane holds the next one
-      again |= bad;
-      const bool live = !a.mask || a.mask[t];
-      uint64_t todo = __ballot(again && live && lane / G < rows);
-      const bool done = G == 64u ? todo == 0u : (todo >> (lane & 48u) & 0xffffu) == 0u;
-      finish<X>(a, t, id, top, total, done && lane / G < rows && (G == 16u || lane < 16u));
-      while (todo) {
-        const uint32_t at = ((uint32_t)__ffsll((unsigned long long)todo) - 1u) / G;
-        select_exact<X, kMax / 64u>(a, t0 + at, s_memory[wave]);
-        todo &= G == 64u ? 0ull : ~(0xffffull << (at * 16u));
+        for (uint32_t j = 0; j < NV; ++j) {
+          z[j] = nkbal::exp_nonpos(z[j] - top);
+          total += z[j];
+        }
+        total = nkbal::sum<G>(total);
       }
-    } else {
-      finish<X>(a, t, id, top, total, lane / G < rows && (G == 16u || lane < 16u));
     }
+    if constexpr (K == kScore) {
+      if (a.scoring == kSigmoid) {
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j)
+          z[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[j] * -1.44269504088896341f));
+      } else {
+        const float inv = total == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(total);
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j) z[j] *= inv;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < NV; ++j) {
+        const uint32_t e = nkbal::expert<G>(lane, j);
+        const float c = (z[j] + bias[j] - lo) * units;
+        key[j] = (1u + (uint32_t)fminf(fmaxf(c, 0.0f), kUnits)) << 10 | (1023u - e);
+      }
+    }
+  }
+  bool again = false;
+  if (a.groups > 1u) {
+    uint32_t* s = reinterpret_cast<uint32_t*>(s_memory[wave]) + lane / G * kMax;
+#pragma unroll
+    for (uint32_t j = 0; j < NV; j += 4u)
+      *reinterpret_cast<uint4*>(s + nkbal::expert<G>(lane, j)) = make_uint4(key[j], key[j + 1u], key[j + 2u], key[j + 3u]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    uint32_t best = 0u, second = 0u;
+    auto take = [&](uint32_t v) __attribute__((always_inline)) {
+      second = max(second, min(best, v));
+      best = max(best, v);
+    };
+    if (i < a.groups) {
+      const uint32_t* from = s + i * a.each;
+      if (a.each % 4u == 0u) {
+        for (uint32_t m = 0; m < a.each; m += 4u) {
+          const uint4 v = *reinterpret_cast<const uint4*>(from + m);
+          take(v.x);
+          take(v.y);
+          take(v.z);
+          take(v.w);
+        }
+      } else {
+        for (uint32_t m = 0; m < a.each; ++m) take(from[m]);
+      }
+    }
+    // (the best expert's key orders the groups itself, as lower groups have lower experts)
+    const uint32_t shift = a.top2 ? 4u : 10u;
+    const uint32_t score = i >= a.groups ? 0u : a.top2 ? ((best >> 10) + (second >> 10)) << 4 | (15u - i) : best;
+    uint32_t before = 0u;
+    each_turn([&](auto n) __attribute__((always_inline)) {
+      before += turned<decltype(n)::value>(score) > score ? 1u : 0u;
+    });
+    const bool keep = before < a.top_groups;
+    if constexpr (K != kWhole) {
+      const uint32_t least = across<16, false>(keep ? score : ~0u) >> shift;
+      const uint32_t most = across<16, true>(keep ? 0u : score) >> shift;
+      again = least - most <= (a.top2 ? 2u * near : near);
+    }
+    // what is not kept leaves by zeros in LDS
+    if (i < a.groups && !keep) {
+      uint32_t* to = s + i * a.each;
+      if (a.each % 4u == 0u) {
+        for (uint32_t m = 0; m < a.each; m += 4u) *reinterpret_cast<uint4*>(to + m) = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        for (uint32_t m = 0; m < a.each; ++m) to[m] = 0u;
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (uint32_t j = 0; j < NV; j += 4u) {
+      const uint4 v = *reinterpret_cast<const uint4*>(s + nkbal::expert<G>(lane, j));
+      key[j] = v.x;
+      key[j + 1u] = v.y;
+      key[j + 2u] = v.z;
+      key[j + 3u] = v.w;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  sort<0u, NV>(key);
+  // two more than k, to see whether the k-th and the next one are apart
+  const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
+  uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws) : draw<G, 16u>(key, draws);
+  const uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
+  if constexpr (K != kWhole) {
+    // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
+    const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
+    uint32_t zb, bb = 0u;
+    if constexpr (sizeof(X) == 4) zb = __float_as_uint(row[id]);
+    else zb = row[id];
+    if (K == kScore && a.bias) bb = __float_as_uint(a.bias[id]);
+    const uint32_t next = turned<1>(mine), nz = turned<1>(zb), nb = turned<1>(bb);
+    const bool close = next != 0u && (mine >> 10) - (next >> 10) <= near;
+    const bool same = zb == nz && bb == nb;
+    const bool next_close = turned<1>(close ? 1u : 0u) != 0u;
+    bool bad = i < a.k && close && !same;
+    if (i + 1u == a.k) bad = close && (!same || a.k + 2u > kMost || next_close);
+    if (a.k == kMost && i + 1u == a.k) bad = true;  // no lane holds the next one
+    again |= bad;
+    uint64_t todo = __ballot(again && live && lane / G < rows);
+    const bool done = G == 64u ? todo == 0u : (todo >> (lane & 48u) & 0xffffu) == 0u;
+    finish<X>(a, t, id, top, total, live, done && lane / G < rows && (G == 16u || lane < 16u));
+    while (todo) {
+      const uint32_t at = ((uint32_t)__ffsll((unsigned long long)todo) - 1u) / G;
+      select_exact<X, kMax / 64u>(a, t0 + at, s_memory[wave]);
+      todo &= G == 64u ? 0ull : ~(0xffffull << (at * 16u));
+    }
+  } else {
+    finish<X>(a, t, id, top, total, live, lane / G < rows && (G == 16u || lane < 16u));
   }
 }
 

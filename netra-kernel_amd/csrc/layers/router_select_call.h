@@ -8,7 +8,7 @@
 namespace {
 
 bool bad_choice(uint32_t tokens, uint32_t experts, uint32_t k, uint32_t shared, uint32_t scoring, float scale) {
-  return tokens > 0x7fffffffu || experts == 0 || experts > nkbal::kMaxExperts || k == 0 || k > nksel::kMost || k > experts ||
+  return tokens > kMaxRouted || experts == 0 || experts > nkbal::kMaxExperts || k == 0 || k > nksel::kMost || k > experts ||
          shared > 1u || k + shared > nksel::kMost || scoring > NETRA_SIGMOID || !(scale == scale);
 }
 // Rows of 32-bit values with a stride in elements.
@@ -32,7 +32,7 @@ extern "C" int netra_router_select(const void* logits, uint32_t logits_type, uin
                                    uint64_t weights_stride, hipStream_t stream) {
   const char* name = "netra_router_select";
   if (bad_choice(tokens, experts, k, shared, scoring, scale))
-    return fail(-1, name, "experts 1 .. 1024, k (with the shared expert) 1 .. 16 and at most the experts, a known scoring");
+    return fail(-1, name, "tokens up to 2^25, experts 1 .. 1024, k (with the shared expert) 1 .. 16 and at most the experts, a known scoring");
   if (groups == 0 || groups > nksel::kMost || experts % groups || top_groups == 0 || top_groups > groups ||
       k > top_groups * (experts / groups) || group_score > NETRA_GROUP_TOP2 ||
       (groups > 1u && group_score == NETRA_GROUP_TOP2 && experts / groups < 2u))
@@ -73,10 +73,9 @@ extern "C" int netra_router_select(const void* logits, uint32_t logits_type, uin
   a.ids_stride = ids_stride;
   a.weights = weights;
   a.weights_stride = weights_stride;
-  a.inv_each = 1.0f / static_cast<float>(a.each);
   a.by_logits = !bias && (a.groups == 1u || !a.top2);
   Launcher launch(stream);
-  const dim3 grid(select_groups(tokens, experts <= 512u ? 16u : 4u)), block(256);
+  const dim3 grid((tokens - 1u) / (experts <= 512u ? 16u : 4u) + 1u), block(256);
   if (logits_type == NETRA_BF16) {
     if (a.by_logits) NETRA_SELECT_SHAPES(netra_router_select_bf16);
     else NETRA_SELECT_SHAPES(netra_router_select_scored_bf16);
@@ -95,7 +94,7 @@ extern "C" int netra_router_select_gradient(const float* dweights, uint64_t dwei
                                             hipStream_t stream) {
   const char* name = "netra_router_select_gradient";
   if (bad_choice(tokens, experts, k, shared, scoring, scale))
-    return fail(-1, name, "experts 1 .. 1024, k (with the shared expert) 1 .. 16 and at most the experts, a known scoring");
+    return fail(-1, name, "tokens up to 2^25, experts 1 .. 1024, k (with the shared expert) 1 .. 16 and at most the experts, a known scoring");
   if (tokens == 0) {
     g_error.clear();
     return 0;

@@ -13,7 +13,7 @@ F = ctypes.c_float
 
 
 @pytest.mark.parametrize("change", [
-    dict(z=0), dict(z=A + 1), dict(zt=2), dict(zs=31), dict(zs=1 << 27), dict(bias=D + 1), dict(T=1 << 31), dict(E=0), dict(E=1025, zs=2000),
+    dict(z=0), dict(z=A + 1), dict(zt=2), dict(zs=31), dict(zs=1 << 27), dict(bias=D + 1), dict(T=(1 << 25) + 1), dict(T=1 << 31), dict(E=0), dict(E=1025, zs=2000),
     dict(k=0), dict(k=17), dict(k=33), dict(shared=2), dict(shared=1, k=16, zs=40, s=20), dict(shared=1), dict(scoring=2), dict(G=0),
     dict(G=3), dict(G=17, E=34, zs=40), dict(G=4, top=0), dict(G=4, top=5), dict(G=4, top=1, k=9, s=9), dict(score=2),
     dict(G=16, E=16, top=16, score=1), dict(scale=float("nan")), dict(ids=0), dict(ids=B + 2), dict(s=7), dict(w=0), dict(w=D + 2),
