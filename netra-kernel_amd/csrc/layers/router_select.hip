@@ -200,10 +200,16 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     double best = -__builtin_inf(), second = -__builtin_inf();
     if (i < a.groups)
-      for (uint32_t m = 0; m < each; ++m) {
-        const double v = s[i * each + m];
-        second = fmax(second, fmin(best, v));
-        best = fmax(best, v);
+      for (uint32_t m = 0; m < each; m += 8u) {
+        double v[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) v[j] = s[i * each + min(m + j, each - 1u)];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) {
+          if (m + j >= each) v[j] = -__builtin_inf();
+          second = fmax(second, fmin(best, v[j]));
+          best = fmax(best, v[j]);
+        }
       }
     if (a.top2) best += second;
     const bool keep = kept(best, a.groups, a.top_groups, [](double v, auto n) __attribute__((always_inline)) {
@@ -216,27 +222,31 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
       if (!(bits >> min((lane + 64u * j) / each, 31u) & 1u)) taken |= 1u << j;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
+  // the bits in the numbers' order; 0 for what cannot be chosen
+  uint64_t key[NV];
+#pragma unroll
+  for (uint32_t j = 0; j < NV; ++j) {
+    const uint64_t u = (uint64_t)__double_as_longlong(c[j] + 0.0);
+    key[j] = taken >> j & 1u ? 0u : u ^ ((uint64_t)((int64_t)u >> 63) | 1ull << 63);
+  }
   uint32_t id = 0u;
   for (uint32_t n = 0; n < a.k; ++n) {
-    double m = -__builtin_inf();
-    uint32_t at = ~0u;
+    uint64_t m = key[0];
+    uint32_t at = lane;
 #pragma unroll
-    for (uint32_t j = 0; j < NV; ++j)
-      if (!(taken >> j & 1u) && (at == ~0u || c[j] > m)) {
-        m = c[j];
+    for (uint32_t j = 1; j < NV; ++j)
+      if (key[j] > m) {
+        m = key[j];
         at = lane + 64u * j;
       }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double om = __shfl_xor(m, d);
-      const uint32_t oa = (uint32_t)__shfl_xor((int)at, d);
-      if (oa != ~0u && (at == ~0u || om > m || (om == m && oa < at))) {
-        m = om;
-        at = oa;
-      }
-    }
+    const uint32_t hi = across<64, true>((uint32_t)(m >> 32));
+    const bool top_hi = (uint32_t)(m >> 32) == hi;
+    const uint32_t lo = across<64, true>(top_hi ? (uint32_t)m : 0u);
+    at = across<64, false>(top_hi && (uint32_t)m == lo ? at : ~0u);
     if (i == n) id = at;
-    if ((at & 63u) == lane) taken |= 1u << (at / 64u);
+#pragma unroll
+    for (uint32_t j = 0; j < NV; ++j)
+      if (at == lane + 64u * j) key[j] = 0u;
   }
   finish<X>(a, t, id, top, total, true, lane < 16u);
 }
