@@ -9,8 +9,8 @@
 //      columns 32 (l / 16) + 8 j .. + 7 of the block (the sum runs over k in any order, so a lane
 //      reads 64 neighbouring bytes of a row of x)
 //   B  [adapter][64 columns][16 ranks][64 lanes][4][4]: lane l's operand j is column
-//      16 (l % 16 / 4) + 4 j + l % 4, ranks 4 (l / 16) .. + 3 (a lane's results of the four j are
-//      16 neighbouring columns of a token)
+//      32 (j / 2) + 8 (l % 16 / 4) + 4 (j % 2) + l % 4, ranks 4 (l / 16) .. + 3 (a lane's results of two j
+//      are 8 neighbouring columns of a token, and four lanes' 64 bytes of it)
 // u goes into the second product as the sum of two bf16 values (the rounded value and what the
 // rounding left), in one matrix instruction with B's operand twice: 16 bits instead of 8 for no
 // more instructions than its contraction of 32 has room for.
@@ -146,7 +146,7 @@ __device__ __forceinline__ void pack_b(const X* __restrict__ b, uint2* __restric
     const uint32_t j = (uint32_t)i & 3u, lane = (uint32_t)(i >> 2) & 63u;
     const uint64_t rest = i >> 8, block = rest / nr;
     const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane >> 4) * 4u;
-    const uint32_t c = (uint32_t)(block % nb) * 64u + 16u * ((lane & 15u) >> 2) + 4u * j + (lane & 3u);
+    const uint32_t c = (uint32_t)(block % nb) * 64u + 32u * (j >> 1) + 8u * ((lane & 15u) >> 2) + 4u * (j & 1u) + (lane & 3u);
     const uint64_t row = ((block / nb) * n + c) * (uint64_t)rank;
     uint32_t w[2];
 #pragma unroll
@@ -200,14 +200,29 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t b = blockIdx.y * a.split_blocks + wave; b < b1; b += W) {
+  const uint32_t c = (lane >> 4) * 32u;
+  auto load = [&](uint32_t b, nklin::Raw<X> (&raw)[TT]) __attribute__((always_inline)) {
+    if (b >= b1) return;
+    if ((b + 1u) * 128u <= a.k) {
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t) nklin::load32(row[t], b * 128u + c, ~0u, raw[t]);
+    } else {
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t) {
+        raw[t] = {};
+        if (b * 128u + c < a.k) nklin::load32(row[t], b * 128u + c, a.k, raw[t]);
+      }
+    }
+  };
+  uint32_t b = blockIdx.y * a.split_blocks + wave;
+  nklin::Raw<X> ahead[TT];
+  load(b, ahead);
+  for (; b < b1; b += W) {
     const uint4* ab = reinterpret_cast<const uint4*>(a.a) + ((uint64_t)tile.x * kb + b) * (NR * 256u) + lane;
     nklin::Raw<X> raw[TT];
 #pragma unroll
-    for (uint32_t t = 0; t < TT; ++t) {
-      raw[t] = {};
-      if (b * 128u + (lane >> 4) * 32u < a.k) nklin::load32(row[t], b * 128u + (lane >> 4) * 32u, a.k, raw[t]);
-    }
+    for (uint32_t t = 0; t < TT; ++t) raw[t] = ahead[t];
+    load(b + W, ahead);
 #pragma unroll
     for (uint32_t j = 0; j < 4u; ++j) {
       bf16x8 x[TT];
@@ -244,30 +259,29 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   }
 }
 
-struct __attribute__((packed, aligned(2))) Unaligned32 {
-  uint32_t w[8];
-};
+using nklin::Unaligned16;
 
-// 16 neighbouring columns of a row from c on (nothing at or past n).
-__device__ __forceinline__ Unaligned32 load16(const uint16_t* row, uint32_t c, uint32_t n) {
-  if (c + 16u <= n) return *reinterpret_cast<const Unaligned32*>(row + c);
-  Unaligned32 v = {};
+// 8 neighbouring columns of a row from c on (nothing at or past n).
+__device__ __forceinline__ Unaligned16 load8(const uint16_t* row, uint32_t c, uint32_t n) {
+  if (c + 8u <= n) return *reinterpret_cast<const Unaligned16*>(row + c);
+  Unaligned16 v = {};
 #pragma unroll
-  for (uint32_t i = 0; i < 16u; ++i)
+  for (uint32_t i = 0; i < 8u; ++i)
     if (c + i < n) v.w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i & 1u));
   return v;
 }
-__device__ __forceinline__ void store16(uint16_t* row, uint32_t c, uint32_t n, const Unaligned32& v) {
-  if (c + 16u <= n) {
-    *reinterpret_cast<Unaligned32*>(row + c) = v;
+__device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, const Unaligned16& v) {
+  if (c + 8u <= n) {
+    *reinterpret_cast<Unaligned16*>(row + c) = v;
     return;
   }
 #pragma unroll
-  for (uint32_t i = 0; i < 16u; ++i)
+  for (uint32_t i = 0; i < 8u; ++i)
     if (c + i < n) row[c + i] = (uint16_t)(v.w[i / 2u] >> (16u * (i & 1u)));
 }
 
-// out of a tile, `wide` times 64 columns a wave.
+// out of a tile: the four waves of a workgroup take 256 neighbouring columns, `wide` times. The next ones' y is under
+// way during a turn.
 template <uint32_t TT, uint32_t NR>
 __device__ __forceinline__ void expand(const Adapters& a) {
   uint4 tile;
@@ -277,7 +291,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   if (none && a.in_place) return;
   const uint32_t lane = threadIdx.x & 63u, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t nb = (a.n + 63u) / 64u, s0 = (chunk * 4u + wave) * a.wide, s1 = min(nb, s0 + a.wide);
+  const uint32_t nb = (a.n + 63u) / 64u, s1 = min(nb, (chunk + 1u) * 4u * a.wide);
   const uint16_t* from[TT];
   uint16_t* to[TT];
   bool there[TT];
@@ -290,17 +304,22 @@ __device__ __forceinline__ void expand(const Adapters& a) {
     const uint32_t token = a.plan[kPlanHead + at];
     from[t] = a.y + (uint64_t)token * a.y_stride;
     to[t] = a.out + (uint64_t)token * a.out_stride;
+    v4f v[NR];
+#pragma unroll
+    for (uint32_t r = 0; r < NR; ++r) v[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!none)
+      for (uint32_t s = 0; s < a.splits; ++s) {
+        const v4f* from_u = reinterpret_cast<const v4f*>(a.u + ((uint64_t)s * a.tokens + at) * (16u * NR)) + q;
+#pragma unroll
+        for (uint32_t r = 0; r < NR; ++r) v[r] += from_u[r * 4u];
+      }
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) {
-      v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (!none)
-        for (uint32_t s = 0; s < a.splits; ++s)
-          v += *reinterpret_cast<const v4f*>(a.u + ((uint64_t)s * a.tokens + at) * (16u * NR) + r * 16u + q * 4u);
       float hi[4], lo[4];
 #pragma unroll
       for (uint32_t e = 0; e < 4u; ++e) {
         // ranks past the last are zeros times what x holds: not 0 where that is an infinity
-        const float f = r * 16u + q * 4u + e < a.rank ? v[e] * scale : 0.0f;
+        const float f = r * 16u + q * 4u + e < a.rank ? v[r][e] * scale : 0.0f;
         hi[e] = nk::bf16_round_hw(f);
         lo[e] = fabsf(hi[e]) < __builtin_inff() ? f - hi[e] : 0.0f;
       }
@@ -309,11 +328,27 @@ __device__ __forceinline__ void expand(const Adapters& a) {
       u[t][r] = __builtin_bit_cast(bf16x8, w);
     }
   }
-  for (uint32_t s = s0; s < s1; ++s) {
-    const uint32_t c = s * 64u + q * 16u;
-    Unaligned32 y[TT];
+  auto load = [&](uint32_t s, Unaligned16 (&y)[TT][2]) __attribute__((always_inline)) {
+    if (s >= s1) return;
+    const uint32_t n = (s + 1u) * 64u <= a.n ? ~0u : a.n;
 #pragma unroll
-    for (uint32_t t = 0; t < TT; ++t) y[t] = load16(from[t], c, a.n);
+    for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        if (n == ~0u) y[t][h] = *reinterpret_cast<const Unaligned16*>(from[t] + s * 64u + h * 32u + q * 8u);
+        else y[t][h] = load8(from[t], s * 64u + h * 32u + q * 8u, a.n);
+      }
+  };
+  uint32_t s = chunk * 4u * a.wide + wave;
+  Unaligned16 ahead[TT][2];
+  load(s, ahead);
+  for (; s < s1; s += 4u) {
+    Unaligned16 y[TT][2];
+#pragma unroll
+    for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) y[t][h] = ahead[t][h];
+    load(s + 4u, ahead);
     if (!none) {
       v4f acc[TT][4];
 #pragma unroll
@@ -337,13 +372,22 @@ __device__ __forceinline__ void expand(const Adapters& a) {
 #pragma unroll
       for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i)
-          y[t].w[i] = nk::bf16x2_hw(nk::bf16_lo(y[t].w[i]) + acc[t][i / 2u][2u * (i & 1u)],
-                                    nk::bf16_hi(y[t].w[i]) + acc[t][i / 2u][2u * (i & 1u) + 1u]);
+        for (uint32_t h = 0; h < 2u; ++h)
+#pragma unroll
+          for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t j = 2u * h + i / 2u, e = 2u * (i & 1u);
+            y[t][h].w[i] = nk::bf16x2_hw(nk::bf16_lo(y[t][h].w[i]) + acc[t][j][e], nk::bf16_hi(y[t][h].w[i]) + acc[t][j][e + 1u]);
+          }
     }
+    const bool whole = (s + 1u) * 64u <= a.n;
 #pragma unroll
     for (uint32_t t = 0; t < TT; ++t)
-      if (there[t]) store16(to[t], c, a.n, y[t]);
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        if (!there[t]) continue;
+        if (whole) *reinterpret_cast<Unaligned16*>(to[t] + s * 64u + h * 32u + q * 8u) = y[t][h];
+        else store8(to[t], s * 64u + h * 32u + q * 8u, a.n, y[t][h]);
+      }
   }
 }
 

@@ -185,10 +185,10 @@ inline NormPlan norm_plan(uint32_t rows, uint32_t cols) {
   p.groups = groups < most ? groups : most;
   return p;
 }
-// A workgroup leaves partial sums of dw for each row that it takes at once.
+// Each workgroup leaves a partial sum of dw.
 inline NormPlan norm_gradients_plan(uint32_t rows, uint32_t cols) {
   NormPlan p = norm_shape(cols);
-  const uint32_t groups = (rows + p.rows - 1u) / p.rows, most = 4096u * 64u / p.threads;
+  const uint32_t groups = (rows + p.rows - 1u) / p.rows, most = p.waves == 16u ? 256u : 512u;
   p.groups = groups < most ? groups : most;
   return p;
 }
@@ -220,7 +220,7 @@ inline AdapterPlan adapter_plan(uint32_t tokens, uint32_t adapters, uint32_t ran
   // a wave reads and packs its tile's u before its first columns: up to eight groups share that
   const uint64_t waves = static_cast<uint64_t>(p.tiles) * ((n + 63u) / 64u);
   while (p.wide < 8u && waves / (2u * p.wide) >= 4096u) p.wide *= 2u;
-  while (p.splits < 16u && p.tiles * p.splits * 2u <= 256u && blocks(k) / (p.splits * 2u) >= 8u) p.splits *= 2u;
+  while (p.splits < 16u && p.tiles * p.splits * 2u <= 640u && blocks(k) / (p.splits * 2u) >= 8u) p.splits *= 2u;
   p.split_blocks = (blocks(k) + p.splits - 1u) / p.splits;
   p.splits = (blocks(k) + p.split_blocks - 1u) / p.split_blocks;
   return p;

@@ -288,7 +288,7 @@ struct NormGradients {
   float offset, eps, inv_cols;
   void* dr;                   // of r's type
   uint64_t dr_stride;
-  float* partial;             // [groups * rows a group][cols]
+  float* partial;             // [groups][cols]
   uint32_t rows, cols;
 };
 
@@ -386,23 +386,46 @@ __device__ __forceinline__ void gradients(const NormGradients& a) {
       store8<X>(rd, at + k * step, a.cols, r[k]);
     }
   }
-  const __amdgpu_buffer_rsrc_t rp = nk::buffer_rsrc(a.partial + (uint64_t)first * a.cols, a.cols * 4u);
+  if constexpr (kRows > 1u) {  // the waves' rows together
+    __shared__ float s_dw[kRows][C * 512u];
+#pragma unroll
+    for (uint32_t k = 0; k < C; ++k)
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) s_dw[wave][(k * 8u + i) * 64u + (threadIdx.x & 63u)] = dw[k][i];
+    __syncthreads();
+    if (wave != 0u) return;
+#pragma unroll
+    for (uint32_t k = 0; k < C; ++k)
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i)
+#pragma unroll
+        for (uint32_t v = 1; v < kRows; ++v) dw[k][i] += s_dw[v][(k * 8u + i) * 64u + threadIdx.x];
+  }
+  const __amdgpu_buffer_rsrc_t rp = nk::buffer_rsrc(a.partial + (uint64_t)blockIdx.x * a.cols, a.cols * 4u);
 #pragma unroll
   for (uint32_t k = 0; k < C; ++k) store8<float>(rp, at + k * step, a.cols, dw[k]);
 }
 
-// dw = the sum of `parts` partial sums, in one order: 16 columns by 16 parts of them a workgroup.
+// dw = the sum of `parts` partial sums, in one order: a workgroup takes 64 columns, its 16 waves
+// every 16th part, eight loads at a time.
 __device__ __forceinline__ void sum_parts(const float* __restrict__ partial, uint32_t parts, uint32_t cols, float* dw,
                                           uint32_t accumulate) {
-  __shared__ float s[16][17];
-  const uint32_t i = threadIdx.x & 15u, k = threadIdx.x >> 4, c = blockIdx.x * 16u + i;
+  __shared__ float s[16][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = blockIdx.x * 64u + lane;
   float v = 0.0f;
   if (c < cols)
-    for (uint32_t p = k; p < parts; p += 16u) v += partial[(uint64_t)p * cols + c];
-  s[k][i] = v;
+    for (uint32_t p = wave; p < parts; p += 128u) {
+      float f[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) f[i] = partial[(uint64_t)min(p + 16u * i, parts - 1u) * cols + c];
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) v += p + 16u * i < parts ? f[i] : 0.0f;
+    }
+  s[wave][lane] = v;
   __syncthreads();
-  if (k != 0u || c >= cols) return;
-  for (uint32_t p = 1; p < 16u; ++p) v += s[p][i];
+  if (wave != 0u || c >= cols) return;
+#pragma unroll
+  for (uint32_t p = 1; p < 16u; ++p) v += s[p][lane];
   dw[c] = accumulate ? dw[c] + v : v;
 }
 
@@ -431,7 +454,7 @@ NETRA_NORMS(8, 1)
 NETRA_NORMS(16, 1)
 NETRA_NORMS(16, 2)
 
-extern "C" __global__ __launch_bounds__(256) void netra_norm_sum_gfx950(const float* partial, uint32_t parts,
+extern "C" __global__ __launch_bounds__(1024) void netra_norm_sum_gfx950(const float* partial, uint32_t parts,
                                                                         uint32_t cols, float* dw, uint32_t accumulate) {
   nknorm::sum_parts(partial, parts, cols, dw, accumulate);
 }

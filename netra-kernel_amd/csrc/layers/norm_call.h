@@ -109,7 +109,7 @@ extern "C" int netra_norm_forward(const void* x, uint32_t x_type, uint64_t x_str
 extern "C" uint64_t netra_norm_gradients_workspace(uint32_t rows, uint32_t cols) {
   if (rows == 0 || bad_norm(rows, cols)) return 0;
   const NormPlan plan = norm_gradients_plan(rows, cols);
-  return 4u * static_cast<uint64_t>(plan.groups) * plan.rows * cols;
+  return 4u * static_cast<uint64_t>(plan.groups) * cols;
 }
 
 extern "C" int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t dy_stride, const void* r, uint32_t r_type,
@@ -139,7 +139,7 @@ extern "C" int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t d
   uint32_t parts = 0;
   if (rows) {
     const NormPlan plan = norm_gradients_plan(rows, cols);
-    parts = plan.groups * plan.rows;
+    parts = plan.groups;
     nknorm::NormGradients a{};
     a.dy = dy;
     a.dy_stride = dy_stride;
@@ -162,7 +162,7 @@ extern "C" int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t d
     NETRA_NORM_SHAPES(netra_norm_gradients);
   }
   if (rows || !accumulate)
-    launch(netra_norm_sum_gfx950, dim3((cols + 15u) / 16u), dim3(256), static_cast<const float*>(workspace), parts, cols,
+    launch(netra_norm_sum_gfx950, dim3((cols + 63u) / 64u), dim3(1024), static_cast<const float*>(workspace), parts, cols,
            dw, accumulate ? 1u : 0u);
   return launch.result(name);
 }
