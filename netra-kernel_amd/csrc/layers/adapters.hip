@@ -6,11 +6,9 @@
 // fp32) and out = y + s B u (contraction of the rank). Operands are packed once so that a lane's
 // operand bytes lie together:
 //   A  [adapter][128-block of k][16 ranks][4][64 lanes][8]: lane l's operand j is rank l % 16,
-//      columns 32 (l / 16) + 8 j .. + 7 of the block (the sum runs over k in any order, so a lane
-//      reads 64 neighbouring bytes of a row of x)
+//      columns 32 j + 8 (l / 16) .. + 7 of the block
 //   B  [adapter][64 columns][16 ranks][64 lanes][4][4]: lane l's operand j is column
-//      32 (j / 2) + 8 (l % 16 / 4) + 4 (j % 2) + l % 4, ranks 4 (l / 16) .. + 3 (a lane's results of two j
-//      are 8 neighbouring columns of a token, and four lanes' 64 bytes of it)
+//      16 j + l % 16, ranks 4 (l / 16) .. + 3
 // u goes into the second product as the sum of two bf16 values (the rounded value and what the
 // rounding left), in one matrix instruction with B's operand twice: 16 bits instead of 8 for no
 // more instructions than its contraction of 32 has room for.
@@ -127,7 +125,7 @@ __device__ __forceinline__ void pack_a(const X* __restrict__ a, uint4* __restric
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
     const uint32_t lane = (uint32_t)(i & 63u), j = (uint32_t)(i >> 6) & 3u;
     const uint64_t rest = i >> 8, block = rest / nr;
-    const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane & 15u), c = (uint32_t)(block % kb) * 128u + (lane >> 4) * 32u + j * 8u;
+    const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane & 15u), c = (uint32_t)(block % kb) * 128u + j * 32u + (lane >> 4) * 8u;
     const uint64_t row = ((block / kb) * rank + r) * (uint64_t)k;
     uint32_t w[4];
 #pragma unroll
@@ -146,7 +144,7 @@ __device__ __forceinline__ void pack_b(const X* __restrict__ b, uint2* __restric
     const uint32_t j = (uint32_t)i & 3u, lane = (uint32_t)(i >> 2) & 63u;
     const uint64_t rest = i >> 8, block = rest / nr;
     const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane >> 4) * 4u;
-    const uint32_t c = (uint32_t)(block % nb) * 64u + 32u * (j >> 1) + 8u * ((lane & 15u) >> 2) + 4u * (j & 1u) + (lane & 3u);
+    const uint32_t c = (uint32_t)(block % nb) * 64u + 16u * j + (lane & 15u);
     const uint64_t row = ((block / nb) * n + c) * (uint64_t)rank;
     uint32_t w[2];
 #pragma unroll
@@ -170,7 +168,7 @@ struct Adapters {
   uint64_t y_stride;
   uint16_t* out;
   uint64_t out_stride;
-  uint32_t tokens, adapters, rank, n, k, in_place, wide, chunks;  // wide: 64-column groups a wave takes; chunks: workgroups across the columns
+  uint32_t tokens, adapters, rank, n, k, in_place, wide, chunks;  // wide: groups of 256 columns a workgroup takes; chunks: workgroups across the columns
 };
 
 __device__ __forceinline__ bool tile_of(const Adapters& a, uint32_t at, uint4& tile) {
@@ -179,8 +177,46 @@ __device__ __forceinline__ bool tile_of(const Adapters& a, uint32_t at, uint4& t
   return true;
 }
 
+using nklin::Unaligned16;
+
+// 8 neighbouring columns of a row as they lie in memory, from c on, and as bf16.
+template <typename X>
+struct Part {
+  Unaligned16 w[sizeof(X) / 2u];
+};
+template <typename X>
+__device__ __forceinline__ Part<X> part_whole(const X* row, uint32_t c) {
+  Part<X> v;
+#pragma unroll
+  for (uint32_t h = 0; h < sizeof(X) / 2u; ++h) v.w[h] = *reinterpret_cast<const Unaligned16*>(row + c + 4u * h);
+  return v;
+}
+template <typename X>
+__device__ __forceinline__ Part<X> part_to(const X* row, uint32_t c, uint32_t n) {  // zeros from column n on
+  if (c + 8u <= n) return part_whole(row, c);
+  Part<X> v = {};
+#pragma unroll
+  for (uint32_t i = 0; i < 8u; ++i)
+    if (c + i < n) {
+      if constexpr (sizeof(X) == 4) v.w[i / 4u].w[i & 3u] = __float_as_uint(row[c + i]);
+      else v.w[0].w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i & 1u));
+    }
+  return v;
+}
+template <typename X>
+__device__ __forceinline__ bf16x8 operand(const Part<X>& v) {
+  u32x4 w;
+#pragma unroll
+  for (uint32_t h = 0; h < 4u; ++h) {
+    if constexpr (sizeof(X) == 2) w[h] = v.w[0].w[h];
+    else w[h] = nk::bf16x2_hw(__uint_as_float(v.w[h / 2u].w[2u * (h & 1u)]), __uint_as_float(v.w[h / 2u].w[2u * (h & 1u) + 1u]));
+  }
+  return __builtin_bit_cast(bf16x8, w);
+}
+
 // u of a tile: TT times 16 tokens by 16 NR ranks. The eight waves of a workgroup share k's blocks
-// out among them and join their sums through LDS, in the order of the waves.
+// out among them and join their sums through LDS, in the order of the waves. The next block's x is under way
+// during a block's products.
 template <typename X, uint32_t TT, uint32_t NR>
 __device__ __forceinline__ void shrink(const Adapters& a) {
   constexpr uint32_t W = 8u;
@@ -188,7 +224,7 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   uint4 tile;
   if (!tile_of(a, blockIdx.x, tile) || tile.x >= a.adapters) return;
   const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t kb = (a.k + 127u) / 128u, b1 = min(kb, (blockIdx.y + 1u) * a.split_blocks);
+  const uint32_t kb = (a.k + 127u) / 128u, b1 = min(kb, (blockIdx.y + 1u) * a.split_blocks), c = (lane >> 4) * 8u;
   const X* row[TT];
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t) {
@@ -200,49 +236,46 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  const uint32_t c = (lane >> 4) * 32u;
-  auto load = [&](uint32_t b, nklin::Raw<X> (&raw)[TT]) __attribute__((always_inline)) {
-    if (b >= b1) return;
-    if ((b + 1u) * 128u <= a.k) {
+  const uint4* ab = reinterpret_cast<const uint4*>(a.a) + (uint64_t)tile.x * kb * (NR * 256u) + lane;
+  auto products = [&](uint32_t b, const Part<X> (&x)[TT][4]) __attribute__((always_inline)) {
 #pragma unroll
-      for (uint32_t t = 0; t < TT; ++t) nklin::load32(row[t], b * 128u + c, ~0u, raw[t]);
-    } else {
-#pragma unroll
-      for (uint32_t t = 0; t < TT; ++t) {
-        raw[t] = {};
-        if (b * 128u + c < a.k) nklin::load32(row[t], b * 128u + c, a.k, raw[t]);
-      }
-    }
-  };
-  uint32_t b = blockIdx.y * a.split_blocks + wave;
-  nklin::Raw<X> ahead[TT];
-  load(b, ahead);
-  for (; b < b1; b += W) {
-    const uint4* ab = reinterpret_cast<const uint4*>(a.a) + ((uint64_t)tile.x * kb + b) * (NR * 256u) + lane;
-    nklin::Raw<X> raw[TT];
-#pragma unroll
-    for (uint32_t t = 0; t < TT; ++t) raw[t] = ahead[t];
-    load(b + W, ahead);
-#pragma unroll
-    for (uint32_t j = 0; j < 4u; ++j) {
-      bf16x8 x[TT];
-#pragma unroll
-      for (uint32_t t = 0; t < TT; ++t) {
-        u32x4 w;
-#pragma unroll
-        for (uint32_t h = 0; h < 4u; ++h) {
-          if constexpr (sizeof(X) == 2) w[h] = raw[t].w[4u * j + h];
-          else w[h] = nk::bf16x2_hw(raw[t].w[8u * j + 2u * h], raw[t].w[8u * j + 2u * h + 1u]);
-        }
-        x[t] = __builtin_bit_cast(bf16x8, w);
-      }
+    for (uint32_t j = 0; j < 4u; ++j)
 #pragma unroll
       for (uint32_t r = 0; r < NR; ++r) {
-        const bf16x8 w = __builtin_bit_cast(bf16x8, ab[(r * 4u + j) * 64u]);
+        const bf16x8 w = __builtin_bit_cast(bf16x8, ab[(uint64_t)b * (NR * 256u) + (r * 4u + j) * 64u]);
 #pragma unroll
-        for (uint32_t t = 0; t < TT; ++t) acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[t], acc[t][r], 0, 0, 0);
+        for (uint32_t t = 0; t < TT; ++t)
+          acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, operand(x[t][j]), acc[t][r], 0, 0, 0);
       }
+  };
+  uint32_t b = blockIdx.y * a.split_blocks + wave;
+  const uint32_t whole = min(b1, a.k / 128u);  // blocks that end inside the rows
+  if (b < whole) {
+    Part<X> next[TT][4];
+    auto load = [&](uint32_t b) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j)
+#pragma unroll
+        for (uint32_t t = 0; t < TT; ++t) next[t][j] = part_whole(row[t], b * 128u + j * 32u + c);
+    };
+    load(b);
+    for (; b < whole; b += W) {
+      Part<X> x[TT][4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j)
+#pragma unroll
+        for (uint32_t t = 0; t < TT; ++t) x[t][j] = next[t][j];
+      load(b + W < whole ? b + W : b);  // (the last one's again, from the cache)
+      products(b, x);
     }
+  }
+  if (b < b1) {  // the last block, short
+    Part<X> x[TT][4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j)
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t) x[t][j] = part_to(row[t], b * 128u + j * 32u + c, a.k);
+    products(b, x);
   }
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t)
@@ -259,17 +292,6 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   }
 }
 
-using nklin::Unaligned16;
-
-// 8 neighbouring columns of a row from c on (nothing at or past n).
-__device__ __forceinline__ Unaligned16 load8(const uint16_t* row, uint32_t c, uint32_t n) {
-  if (c + 8u <= n) return *reinterpret_cast<const Unaligned16*>(row + c);
-  Unaligned16 v = {};
-#pragma unroll
-  for (uint32_t i = 0; i < 8u; ++i)
-    if (c + i < n) v.w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i & 1u));
-  return v;
-}
 __device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, const Unaligned16& v) {
   if (c + 8u <= n) {
     *reinterpret_cast<Unaligned16*>(row + c) = v;
@@ -280,10 +302,15 @@ __device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, co
     if (c + i < n) row[c + i] = (uint16_t)(v.w[i / 2u] >> (16u * (i & 1u)));
 }
 
-// out of a tile: the four waves of a workgroup take 256 neighbouring columns, `wide` times. The next ones' y is under
-// way during a turn.
+// out of a tile. The four waves of a workgroup multiply 64 columns each and hand the sums over through
+// LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together: as the
+// matrix core leaves them a lane has four columns, and rows of 64 bytes stored so took 60% of a copy's rate. `wide` times; the next
+// columns' y and B are under way during a turn.
 template <uint32_t TT, uint32_t NR>
 __device__ __forceinline__ void expand(const Adapters& a) {
+  constexpr uint32_t kPitch = 260u;  // spreads 16 tokens' rows over the banks
+  constexpr uint32_t kRows = 4u * TT, kLoads = kRows / 2u;  // rows of a wave; loads of a lane: two rows at a time
+  __shared__ float sums[TT * 16u][kPitch];
   uint4 tile;
   const uint32_t at_tile = blockIdx.x / a.chunks, chunk = blockIdx.x - at_tile * a.chunks;
   if (!tile_of(a, at_tile, tile)) return;
@@ -291,28 +318,41 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   if (none && a.in_place) return;
   const uint32_t lane = threadIdx.x & 63u, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t nb = (a.n + 63u) / 64u, s1 = min(nb, (chunk + 1u) * 4u * a.wide);
-  const uint16_t* from[TT];
-  uint16_t* to[TT];
-  bool there[TT];
+  const uint32_t nb = (a.n + 63u) / 64u;
+  const uint32_t g0 = chunk * a.wide, g1 = min((a.n + 255u) / 256u, g0 + a.wide);  // groups of 256 columns
+  // the wave's rows: lanes 0 .. 31 and 32 .. 63 have one each of every load's two
+  const uint16_t* from[kLoads];
+  uint16_t* to[kLoads];
+  bool there[kLoads];
+  const uint32_t c = (lane & 31u) * 8u, half = lane >> 5;
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; ++i) {
+    const uint32_t row = wave * kRows + 2u * i + half;
+    there[i] = row < tile.z;
+    const uint32_t token = a.plan[kPlanHead + tile.y + min(row, tile.z - 1u)];
+    from[i] = a.y + (uint64_t)token * a.y_stride;
+    to[i] = a.out + (uint64_t)token * a.out_stride;
+  }
+  if (none) {
+    for (uint32_t g = g0; g < g1; ++g)
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i)
+        if (there[i]) store8(to[i], g * 256u + c, a.n, part_to(from[i], g * 256u + c, a.n).w[0]);
+    return;
+  }
   bf16x8 u[TT][NR];
-  const float scale = none ? 0.0f : a.scale[tile.x];
+  const float scale = a.scale[tile.x];
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t) {
-    const uint32_t i = t * 16u + (lane & 15u), at = tile.y + min(i, tile.z - 1u);
-    there[t] = i < tile.z;
-    const uint32_t token = a.plan[kPlanHead + at];
-    from[t] = a.y + (uint64_t)token * a.y_stride;
-    to[t] = a.out + (uint64_t)token * a.out_stride;
+    const uint32_t at = tile.y + min(t * 16u + (lane & 15u), tile.z - 1u);
     v4f v[NR];
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) v[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (!none)
-      for (uint32_t s = 0; s < a.splits; ++s) {
-        const v4f* from_u = reinterpret_cast<const v4f*>(a.u + ((uint64_t)s * a.tokens + at) * (16u * NR)) + q;
+    for (uint32_t s = 0; s < a.splits; ++s) {
+      const v4f* from_u = reinterpret_cast<const v4f*>(a.u + ((uint64_t)s * a.tokens + at) * (16u * NR)) + q;
 #pragma unroll
-        for (uint32_t r = 0; r < NR; ++r) v[r] += from_u[r * 4u];
-      }
+      for (uint32_t r = 0; r < NR; ++r) v[r] += from_u[r * 4u];
+    }
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) {
       float hi[4], lo[4];
@@ -328,66 +368,70 @@ __device__ __forceinline__ void expand(const Adapters& a) {
       u[t][r] = __builtin_bit_cast(bf16x8, w);
     }
   }
-  auto load = [&](uint32_t s, Unaligned16 (&y)[TT][2]) __attribute__((always_inline)) {
-    if (s >= s1) return;
-    const uint32_t n = (s + 1u) * 64u <= a.n ? ~0u : a.n;
+  const uint4* b_at = reinterpret_cast<const uint4*>(a.b) + ((uint64_t)tile.x * nb * NR * 64u + lane) * 2u;
+  uint4 b_next[NR][2];
+  Unaligned16 y_next[kLoads];
+  const bool whole = tile.z == TT * 16u && a.n % 256u == 0u;
+  auto load = [&](uint32_t g) __attribute__((always_inline)) {
+    const uint32_t s = min(g * 4u + wave, nb - 1u);
 #pragma unroll
-    for (uint32_t t = 0; t < TT; ++t)
+    for (uint32_t r = 0; r < NR; ++r)
 #pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) {
-        if (n == ~0u) y[t][h] = *reinterpret_cast<const Unaligned16*>(from[t] + s * 64u + h * 32u + q * 8u);
-        else y[t][h] = load8(from[t], s * 64u + h * 32u + q * 8u, a.n);
-      }
-  };
-  uint32_t s = chunk * 4u * a.wide + wave;
-  Unaligned16 ahead[TT][2];
-  load(s, ahead);
-  for (; s < s1; s += 4u) {
-    Unaligned16 y[TT][2];
+      for (uint32_t h = 0; h < 2u; ++h) b_next[r][h] = b_at[(uint64_t)s * (NR * 128u) + r * 128u + h];
+    if (whole) {
 #pragma unroll
-    for (uint32_t t = 0; t < TT; ++t)
+      for (uint32_t i = 0; i < kLoads; ++i) y_next[i] = *reinterpret_cast<const Unaligned16*>(from[i] + g * 256u + c);
+    } else {
 #pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) y[t][h] = ahead[t][h];
-    load(s + 4u, ahead);
-    if (!none) {
-      v4f acc[TT][4];
-#pragma unroll
-      for (uint32_t t = 0; t < TT; ++t)
-#pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) acc[t][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      const uint4* bb = reinterpret_cast<const uint4*>(a.b) + (((uint64_t)tile.x * nb + s) * NR * 64u + lane) * 2u;
-#pragma unroll
-      for (uint32_t r = 0; r < NR; ++r) {
-        const uint4 lo = bb[r * 128u], hi = bb[r * 128u + 1u];
-        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) {
-          const u32x4 twice = {w[2u * j], w[2u * j + 1u], w[2u * j], w[2u * j + 1u]};
-          const bf16x8 b = __builtin_bit_cast(bf16x8, twice);
-#pragma unroll
-          for (uint32_t t = 0; t < TT; ++t)
-            acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, u[t][r], acc[t][j], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (uint32_t t = 0; t < TT; ++t)
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h)
-#pragma unroll
-          for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t j = 2u * h + i / 2u, e = 2u * (i & 1u);
-            y[t][h].w[i] = nk::bf16x2_hw(nk::bf16_lo(y[t][h].w[i]) + acc[t][j][e], nk::bf16_hi(y[t][h].w[i]) + acc[t][j][e + 1u]);
-          }
+      for (uint32_t i = 0; i < kLoads; ++i) y_next[i] = part_to(from[i], g * 256u + c, a.n).w[0];
     }
-    const bool whole = (s + 1u) * 64u <= a.n;
+  };
+  load(g0);
+  for (uint32_t g = g0; g < g1; ++g) {
+    uint4 b[NR][2];
+    Unaligned16 y[kLoads];
+#pragma unroll
+    for (uint32_t r = 0; r < NR; ++r)
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) b[r][h] = b_next[r][h];
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) y[i] = y_next[i];
+    load(g + 1u < g1 ? g + 1u : g);  // (the last turn's again, from the cache)
+    __builtin_amdgcn_sched_barrier(0);
+    v4f acc[TT][4];
 #pragma unroll
     for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) {
-        if (!there[t]) continue;
-        if (whole) *reinterpret_cast<Unaligned16*>(to[t] + s * 64u + h * 32u + q * 8u) = y[t][h];
-        else store8(to[t], s * 64u + h * 32u + q * 8u, a.n, y[t][h]);
+      for (uint32_t j = 0; j < 4u; ++j) acc[t][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t r = 0; r < NR; ++r) {
+      const uint32_t w[8] = {b[r][0].x, b[r][0].y, b[r][0].z, b[r][0].w, b[r][1].x, b[r][1].y, b[r][1].z, b[r][1].w};
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j) {
+        const u32x4 twice = {w[2u * j], w[2u * j + 1u], w[2u * j], w[2u * j + 1u]};
+#pragma unroll
+        for (uint32_t t = 0; t < TT; ++t)
+          acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, twice), u[t][r], acc[t][j], 0, 0, 0);
       }
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j)
+        *reinterpret_cast<v4f*>(&sums[t * 16u + (lane & 15u)][wave * 64u + j * 16u + q * 4u]) = acc[t][j];
+    nklds::barrier();
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const float* d = &sums[wave * kRows + 2u * i + half][c];
+      const v4f lo = *reinterpret_cast<const v4f*>(d), hi = *reinterpret_cast<const v4f*>(d + 4);
+      const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e)
+        y[i].w[e] = nk::bf16x2_hw(nk::bf16_lo(y[i].w[e]) + f[2u * e], nk::bf16_hi(y[i].w[e]) + f[2u * e + 1u]);
+      if (whole) *reinterpret_cast<Unaligned16*>(to[i] + g * 256u + c) = y[i];
+      else if (there[i]) store8(to[i], g * 256u + c, a.n, y[i]);
+    }
+    nklds::barrier();
   }
 }
 

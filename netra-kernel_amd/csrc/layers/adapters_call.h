@@ -125,7 +125,7 @@ extern "C" int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_str
   a.k = k;
   a.in_place = out == y;
   a.wide = p.wide;
-  a.chunks = ((n + 63u) / 64u + 4u * p.wide - 1u) / (4u * p.wide);
+  a.chunks = ((n + 255u) / 256u + p.wide - 1u) / p.wide;
   const uint64_t groups = static_cast<uint64_t>(a.chunks) * p.tiles;
   if (!launchable(groups, 256u)) return fail(-1, name, "more workgroups than one launch takes");
   const dim3 shrink(p.tiles, p.splits), expand(static_cast<uint32_t>(groups));

@@ -203,7 +203,7 @@ inline uint32_t select_groups(uint32_t tokens, uint32_t at_once) {
 
 // Adapters: 16-rank parts as the kernels have them; tokens a tile; tiles that a batch has at most (one
 // short one for each adapter in use and for the tokens without); splits of k's 128-blocks where the tiles are few, and
-// 64-column groups that a wave of the second product takes.
+// groups of 256 columns that a workgroup of the second product takes.
 inline uint32_t adapter_ranks(uint32_t rank) { return rank <= 16u ? 1u : rank <= 32u ? 2u : rank <= 64u ? 4u : 8u; }
 inline uint32_t adapter_tile(uint32_t tokens, uint32_t adapters) {
   return tokens > 1024u && tokens / 32u >= adapters ? 32u : 16u;
@@ -217,9 +217,9 @@ struct AdapterPlan {
 };
 inline AdapterPlan adapter_plan(uint32_t tokens, uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k) {
   AdapterPlan p{adapter_tiles(tokens, adapters), 1, blocks(k), 1};
-  // a wave reads and packs its tile's u before its first columns: up to eight groups share that
-  const uint64_t waves = static_cast<uint64_t>(p.tiles) * ((n + 63u) / 64u);
-  while (p.wide < 8u && waves / (2u * p.wide) >= 4096u) p.wide *= 2u;
+  // a workgroup reads and packs its tile's u before its first columns: up to eight groups share that
+  const uint64_t groups = static_cast<uint64_t>(p.tiles) * ((n + 255u) / 256u);
+  while (p.wide < 8u && groups / (2u * p.wide) >= 1024u) p.wide *= 2u;
   while (p.splits < 16u && p.tiles * p.splits * 2u <= 640u && blocks(k) / (p.splits * 2u) >= 8u) p.splits *= 2u;
   p.split_blocks = (blocks(k) + p.splits - 1u) / p.splits;
   p.splits = (blocks(k) + p.split_blocks - 1u) / p.split_blocks;
