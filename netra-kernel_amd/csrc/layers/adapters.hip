@@ -7,11 +7,12 @@
 // operand bytes lie together:
 //   A  [adapter][128-block of k][16 ranks][4][64 lanes][8]: lane l's operand j is rank l % 16,
 //      columns 32 j + 8 (l / 16) .. + 7 of the block
-//   B  [adapter][64 columns][16 ranks][64 lanes][4][4]: lane l's operand j is column
-//      16 j + l % 16, ranks 4 (l / 16) .. + 3
+//   B  [adapter][64 columns][32 ranks][4][64 lanes][8]: lane l's operand j is column 16 j + l % 16,
+//      ranks 8 (l / 16) .. + 7; of a rank up to 16
+//      [adapter][64 columns][2][64 lanes][2][4]: operands 2 h and 2 h + 1 of a lane, ranks 4 (l / 16) .. + 3
 // u goes into the second product as the sum of two bf16 values (the rounded value and what the
-// rounding left), in one matrix instruction with B's operand twice: 16 bits instead of 8 for no
-// more instructions than its contraction of 32 has room for.
+// rounding left), each in matrix instructions of its own: 16 bits instead of 8, at no cost where memory is the bound.
+// A rank up to 16 has both in one instruction, with B's operand twice.
 #pragma once
 #include "linear_fp8.hip"
 
@@ -141,9 +142,10 @@ __device__ __forceinline__ void pack_b(const X* __restrict__ b, uint2* __restric
   const uint32_t nb = (n + 63u) / 64u;
   const uint64_t all = (uint64_t)adapters * nb * nr * 256u;
   for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256u) {
-    const uint32_t j = (uint32_t)i & 3u, lane = (uint32_t)(i >> 2) & 63u;
-    const uint64_t rest = i >> 8, block = rest / nr;
-    const uint32_t r = (uint32_t)(rest % nr) * 16u + (lane >> 4) * 4u;
+    const uint32_t lane = (uint32_t)(i >> 1) & 63u, odd = (uint32_t)i & 1u;
+    const uint32_t j = nr == 1u ? ((uint32_t)(i >> 7) & 1u) * 2u + odd : (uint32_t)(i >> 7) & 3u;
+    const uint64_t rest = i / (nr == 1u ? 256u : 512u), parts = nr == 1u ? 1u : nr / 2u, block = rest / parts;
+    const uint32_t r = nr == 1u ? (lane >> 4) * 4u : (uint32_t)(rest % parts) * 32u + (lane >> 4) * 8u + odd * 4u;
     const uint32_t c = (uint32_t)(block % nb) * 64u + 16u * j + (lane & 15u);
     const uint64_t row = ((block / nb) * n + c) * (uint64_t)rank;
     uint32_t w[2];
@@ -162,13 +164,16 @@ struct Adapters {
   const uint8_t* b;
   const float* scale;
   const uint32_t* plan;
-  float* u;                   // [splits][tokens by the plan's order][16 nr]
+  // A x by the plan's order of tokens: of one split scaled, rounded and what that left, bf16 [2][tokens][16 nr]; of
+  // more fp32 [splits][tokens][16 nr]
+  void* u;
   uint32_t splits, split_blocks;  // of k's 128-blocks
   const uint16_t* y;
   uint64_t y_stride;
   uint16_t* out;
   uint64_t out_stride;
-  uint32_t tokens, adapters, rank, n, k, in_place, wide, chunks;  // wide: groups of 256 columns a workgroup takes; chunks: workgroups across the columns
+  uint32_t tokens, adapters, rank, ranks, n, k, in_place;  // ranks: 16-rank parts
+  uint32_t wide, chunks;      // wide: groups of 256 columns a workgroup takes; chunks: workgroups across the columns
 };
 
 __device__ __forceinline__ bool tile_of(const Adapters& a, uint32_t at, uint4& tile) {
@@ -214,17 +219,39 @@ __device__ __forceinline__ bf16x8 operand(const Part<X>& v) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// u of a tile: TT times 16 tokens by 16 NR ranks. The eight waves of a workgroup share k's blocks
-// out among them and join their sums through LDS, in the order of the waves. The next block's x is under way
-// during a block's products.
-template <typename X, uint32_t TT, uint32_t NR>
+// Four ranks of u from r on, scaled, as a rounded and a left-over bf16 value each. Ranks past the last are zeros times
+// what x holds, which is not 0 where that is an infinity.
+__device__ __forceinline__ void split(v4f v, float scale, uint32_t r, uint32_t rank, u32x2& hi, u32x2& lo) {
+  float h[4], l[4];
+#pragma unroll
+  for (uint32_t e = 0; e < 4u; ++e) {
+    const float f = r + e < rank ? v[e] * scale : 0.0f;
+    h[e] = nk::bf16_round_hw(f);
+    l[e] = fabsf(h[e]) < __builtin_inff() ? f - h[e] : 0.0f;
+  }
+  hi = u32x2{nk::bf16x2_hw(h[0], h[1]), nk::bf16x2_hw(h[2], h[3])};
+  lo = u32x2{nk::bf16x2_hw(l[0], l[1]), nk::bf16x2_hw(l[2], l[3])};
+}
+
+// u of the H-th part of a tile: TT times 16 tokens by 16 NR ranks (of the workgroup's place in y). The
+// eight waves of a workgroup share k's blocks out among them and join their sums through LDS, in the order of the waves.
+//
+// A wave's loads are counted in the order in which they are issued, so waiting for A (from the L2) waits for all of
+// x that was asked for before it (from memory). A block goes in two halves; each half's A is asked for a half ahead,
+// each half's x two halves ahead, and A before x:  A0(b) x1(b) | A1(b) x0(b+1) | A0(b+1) x1(b+1) | ...
+template <typename X, uint32_t TT, uint32_t H, uint32_t NR>
 __device__ __forceinline__ void shrink(const Adapters& a) {
   constexpr uint32_t W = 8u;
   __shared__ v4f part[W][TT * NR][64];
   uint4 tile;
-  if (!tile_of(a, blockIdx.x, tile) || tile.x >= a.adapters) return;
+  if (!tile_of(a, blockIdx.x / H, tile) || tile.x >= a.adapters) return;
+  const uint32_t before = blockIdx.x % H * (TT * 16u);  // this workgroup's part of the tile
+  if (before >= tile.z) return;
+  tile.y += before;
+  tile.z = min(tile.z - before, TT * 16u);
   const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t kb = (a.k + 127u) / 128u, b1 = min(kb, (blockIdx.y + 1u) * a.split_blocks), c = (lane >> 4) * 8u;
+  const uint32_t kb = (a.k + 127u) / 128u, split_at = blockIdx.y, r0 = blockIdx.z * NR;  // 16-rank parts before this one's
+  const uint32_t b1 = min(kb, (split_at + 1u) * a.split_blocks), c = (lane >> 4) * 8u;
   const X* row[TT];
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t) {
@@ -236,46 +263,75 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  const uint4* ab = reinterpret_cast<const uint4*>(a.a) + (uint64_t)tile.x * kb * (NR * 256u) + lane;
-  auto products = [&](uint32_t b, const Part<X> (&x)[TT][4]) __attribute__((always_inline)) {
+  const u32x4* ab = reinterpret_cast<const u32x4*>(a.a) + ((uint64_t)tile.x * kb * a.ranks + r0) * 256u + lane;
+  u32x4 wa[2][NR][2];  // A of each half
+  Part<X> x[2][TT][2], next[2][TT][2];
+  auto load_a = [&](uint32_t b, uint32_t h) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t j = 0; j < 4u; ++j)
+    for (uint32_t r = 0; r < NR; ++r)
 #pragma unroll
-      for (uint32_t r = 0; r < NR; ++r) {
-        const bf16x8 w = __builtin_bit_cast(bf16x8, ab[(uint64_t)b * (NR * 256u) + (r * 4u + j) * 64u]);
+      for (uint32_t j = 0; j < 2u; ++j) wa[h][r][j] = ab[((uint64_t)b * a.ranks + r) * 256u + (2u * h + j) * 64u];
+  };
+  auto load_x = [&](uint32_t b, uint32_t h, Part<X> (&to)[2][TT][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t j = 0; j < 2u; ++j)
+#pragma unroll
+      for (uint32_t t = 0; t < TT; ++t) to[h][t][j] = part_whole(row[t], b * 128u + (2u * h + j) * 32u + c);
+  };
+  auto products = [&](uint32_t h, const Part<X> (&from)[2][TT][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t j = 0; j < 2u; ++j)
+#pragma unroll
+      for (uint32_t r = 0; r < NR; ++r)
 #pragma unroll
         for (uint32_t t = 0; t < TT; ++t)
-          acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, operand(x[t][j]), acc[t][r], 0, 0, 0);
-      }
+          acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wa[h][r][j]), operand(from[h][t][j]),
+                                                              acc[t][r], 0, 0, 0);
   };
-  uint32_t b = blockIdx.y * a.split_blocks + wave;
+  // The wave's blocks: every 8th from b0 on. Each wave begins with another one, so that at any time the workgroups
+  // read all places of their rows: all in step they read one place, which is a part of the memory's channels where
+  // rows are a power of two apart (67 MB read alone: 18.0 us, so 12.1).
+  const uint32_t b0 = split_at * a.split_blocks + wave;
   const uint32_t whole = min(b1, a.k / 128u);  // blocks that end inside the rows
-  if (b < whole) {
-    Part<X> next[TT][4];
-    auto load = [&](uint32_t b) __attribute__((always_inline)) {
-#pragma unroll
-      for (uint32_t j = 0; j < 4u; ++j)
-#pragma unroll
-        for (uint32_t t = 0; t < TT; ++t) next[t][j] = part_whole(row[t], b * 128u + j * 32u + c);
+  const uint32_t count = b0 < whole ? (whole - b0 + W - 1u) / W : 0u;
+  if (count) {
+    uint32_t at = wave % count, b = b0 + at * W;
+    load_x(b, 0u, x);
+    load_a(b, 0u);
+    load_x(b, 1u, x);
+    auto block = [&](const Part<X> (&now)[2][TT][2], Part<X> (&then)[2][TT][2]) __attribute__((always_inline)) {
+      at = at + 1u == count ? 0u : at + 1u;  // (behind the last one the first again, from the cache)
+      const uint32_t b_next = b0 + at * W;
+      load_a(b, 1u);
+      load_x(b_next, 0u, then);
+      __builtin_amdgcn_sched_barrier(0);
+      products(0u, now);
+      __builtin_amdgcn_sched_barrier(0);
+      load_a(b_next, 0u);
+      load_x(b_next, 1u, then);
+      __builtin_amdgcn_sched_barrier(0);
+      products(1u, now);
+      __builtin_amdgcn_sched_barrier(0);
+      b = b_next;
     };
-    load(b);
-    for (; b < whole; b += W) {
-      Part<X> x[TT][4];
-#pragma unroll
-      for (uint32_t j = 0; j < 4u; ++j)
-#pragma unroll
-        for (uint32_t t = 0; t < TT; ++t) x[t][j] = next[t][j];
-      load(b + W < whole ? b + W : b);  // (the last one's again, from the cache)
-      products(b, x);
+    // (two in turn: x is not copied, which would wait for it)
+    for (uint32_t i = 0; i < count; i += 2u) {
+      block(x, next);
+      if (i + 1u == count) break;
+      block(next, x);
     }
   }
+  const uint32_t b = b0 + count * W;
   if (b < b1) {  // the last block, short
-    Part<X> x[TT][4];
 #pragma unroll
-    for (uint32_t j = 0; j < 4u; ++j)
+    for (uint32_t h = 0; h < 2u; ++h) {
 #pragma unroll
-      for (uint32_t t = 0; t < TT; ++t) x[t][j] = part_to(row[t], b * 128u + j * 32u + c, a.k);
-    products(b, x);
+      for (uint32_t j = 0; j < 2u; ++j)
+#pragma unroll
+        for (uint32_t t = 0; t < TT; ++t) x[h][t][j] = part_to(row[t], b * 128u + (2u * h + j) * 32u + c, a.k);
+      load_a(b, h);
+      products(h, x);
+    }
   }
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t)
@@ -283,12 +339,21 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
     for (uint32_t r = 0; r < NR; ++r) part[wave][t * NR + r][lane] = acc[t][r];
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < TT * NR * 64u; i += 512u) {
-    const uint32_t l = i & 63u, tr = i >> 6, at = tr / NR * 16u + (l & 15u);
+    const uint32_t l = i & 63u, tr = i >> 6, in = tr / NR * 16u + (l & 15u);
     v4f v = part[0][tr][l];
 #pragma unroll
     for (uint32_t w = 1; w < W; ++w) v += part[w][tr][l];
-    if (at < tile.z)
-      *reinterpret_cast<v4f*>(a.u + ((uint64_t)blockIdx.y * a.tokens + tile.y + at) * (16u * NR) + tr % NR * 16u + (l >> 4) * 4u) = v;
+    if (in >= tile.z) continue;
+    const uint32_t r = (r0 + tr % NR) * 16u + (l >> 4) * 4u, ranks = 16u * a.ranks;
+    if (a.splits > 1u) {
+      *reinterpret_cast<v4f*>(static_cast<float*>(a.u) + ((uint64_t)split_at * a.tokens + tile.y + in) * ranks + r) = v;
+    } else {
+      u32x2 hi, lo;
+      split(v, a.scale[tile.x], r, a.rank, hi, lo);
+      uint16_t* to = static_cast<uint16_t*>(a.u) + (uint64_t)(tile.y + in) * ranks + r;
+      *reinterpret_cast<u32x2*>(to) = hi;
+      *reinterpret_cast<u32x2*>(to + (uint64_t)a.tokens * ranks) = lo;
+    }
   }
 }
 
@@ -302,15 +367,15 @@ __device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, co
     if (c + i < n) row[c + i] = (uint16_t)(v.w[i / 2u] >> (16u * (i & 1u)));
 }
 
-// out of a tile. The four waves of a workgroup multiply 64 columns each and hand the sums over through
-// LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together: as the
+// out of a tile of H times TT times 16 tokens. The waves of a workgroup multiply 64 of 256 columns by TT times 16
+// tokens each and hand the sums over through LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together: as the
 // matrix core leaves them a lane has four columns, and rows of 64 bytes stored so took 60% of a copy's rate. `wide` times; the next
 // columns' y and B are under way during a turn.
-template <uint32_t TT, uint32_t NR>
+template <uint32_t TT, uint32_t H, uint32_t NR>
 __device__ __forceinline__ void expand(const Adapters& a) {
   constexpr uint32_t kPitch = 260u;  // spreads 16 tokens' rows over the banks
   constexpr uint32_t kRows = 4u * TT, kLoads = kRows / 2u;  // rows of a wave; loads of a lane: two rows at a time
-  __shared__ float sums[TT * 16u][kPitch];
+  __shared__ float sums[H * TT * 16u][kPitch];
   uint4 tile;
   const uint32_t at_tile = blockIdx.x / a.chunks, chunk = blockIdx.x - at_tile * a.chunks;
   if (!tile_of(a, at_tile, tile)) return;
@@ -318,7 +383,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   if (none && a.in_place) return;
   const uint32_t lane = threadIdx.x & 63u, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t nb = (a.n + 63u) / 64u;
+  const uint32_t nb = (a.n + 63u) / 64u, first = wave / 4u * (TT * 16u);  // the wave's first token
   const uint32_t g0 = chunk * a.wide, g1 = min((a.n + 255u) / 256u, g0 + a.wide);  // groups of 256 columns
   // the wave's rows: lanes 0 .. 31 and 32 .. 63 have one each of every load's two
   const uint16_t* from[kLoads];
@@ -340,85 +405,111 @@ __device__ __forceinline__ void expand(const Adapters& a) {
         if (there[i]) store8(to[i], g * 256u + c, a.n, part_to(from[i], g * 256u + c, a.n).w[0]);
     return;
   }
-  bf16x8 u[TT][NR];
-  const float scale = a.scale[tile.x];
+  // u's operands: of a rank up to 16 {rounded, left}, else the rounded ones, then the left ones
+  constexpr uint32_t kPairs = NR == 1u ? 1u : NR / 2u, kOperands = NR == 1u ? 1u : NR;
+  bf16x8 u[TT][kOperands];
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t) {
-    const uint32_t at = tile.y + min(t * 16u + (lane & 15u), tile.z - 1u);
-    v4f v[NR];
+    const uint32_t at = tile.y + min(first + t * 16u + (lane & 15u), tile.z - 1u);
+    u32x2 hi[NR], lo[NR];  // of four ranks from rank(i) on
+    auto rank = [&](uint32_t i) __attribute__((always_inline)) { return NR == 1u ? q * 4u : i / 2u * 32u + q * 8u + (i & 1u) * 4u; };
+    if (a.splits == 1u) {
+      const uint16_t* from_u = static_cast<const uint16_t*>(a.u) + (uint64_t)at * (16u * NR);
 #pragma unroll
-    for (uint32_t r = 0; r < NR; ++r) v[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-      const v4f* from_u = reinterpret_cast<const v4f*>(a.u + ((uint64_t)s * a.tokens + at) * (16u * NR)) + q;
-#pragma unroll
-      for (uint32_t r = 0; r < NR; ++r) v[r] += from_u[r * 4u];
-    }
-#pragma unroll
-    for (uint32_t r = 0; r < NR; ++r) {
-      float hi[4], lo[4];
-#pragma unroll
-      for (uint32_t e = 0; e < 4u; ++e) {
-        // ranks past the last are zeros times what x holds: not 0 where that is an infinity
-        const float f = r * 16u + q * 4u + e < a.rank ? v[r][e] * scale : 0.0f;
-        hi[e] = nk::bf16_round_hw(f);
-        lo[e] = fabsf(hi[e]) < __builtin_inff() ? f - hi[e] : 0.0f;
+      for (uint32_t i = 0; i < NR; ++i) {
+        hi[i] = *reinterpret_cast<const u32x2*>(from_u + rank(i));
+        lo[i] = *reinterpret_cast<const u32x2*>(from_u + (uint64_t)a.tokens * (16u * NR) + rank(i));
       }
-      const u32x4 w = {nk::bf16x2_hw(hi[0], hi[1]), nk::bf16x2_hw(hi[2], hi[3]), nk::bf16x2_hw(lo[0], lo[1]),
-                       nk::bf16x2_hw(lo[2], lo[3])};
-      u[t][r] = __builtin_bit_cast(bf16x8, w);
+    } else {
+      v4f v[NR];
+#pragma unroll
+      for (uint32_t i = 0; i < NR; ++i) v[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      for (uint32_t s = 0; s < a.splits; ++s) {
+        const float* from_u = static_cast<const float*>(a.u) + ((uint64_t)s * a.tokens + at) * (16u * NR);
+#pragma unroll
+        for (uint32_t i = 0; i < NR; ++i) v[i] += *reinterpret_cast<const v4f*>(from_u + rank(i));
+      }
+      const float scale = a.scale[tile.x];
+#pragma unroll
+      for (uint32_t i = 0; i < NR; ++i) split(v[i], scale, rank(i), a.rank, hi[i], lo[i]);
     }
-  }
-  const uint4* b_at = reinterpret_cast<const uint4*>(a.b) + ((uint64_t)tile.x * nb * NR * 64u + lane) * 2u;
-  uint4 b_next[NR][2];
-  Unaligned16 y_next[kLoads];
-  const bool whole = tile.z == TT * 16u && a.n % 256u == 0u;
-  auto load = [&](uint32_t g) __attribute__((always_inline)) {
-    const uint32_t s = min(g * 4u + wave, nb - 1u);
-#pragma unroll
-    for (uint32_t r = 0; r < NR; ++r)
-#pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) b_next[r][h] = b_at[(uint64_t)s * (NR * 128u) + r * 128u + h];
-    if (whole) {
-#pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) y_next[i] = *reinterpret_cast<const Unaligned16*>(from[i] + g * 256u + c);
+    if constexpr (NR == 1u) {
+      u[t][0] = __builtin_bit_cast(bf16x8, u32x4{hi[0][0], hi[0][1], lo[0][0], lo[0][1]});
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) y_next[i] = part_to(from[i], g * 256u + c, a.n).w[0];
+      for (uint32_t p = 0; p < kPairs; ++p) {
+        u[t][p] = __builtin_bit_cast(bf16x8, u32x4{hi[2u * p][0], hi[2u * p][1], hi[2u * p + 1u][0], hi[2u * p + 1u][1]});
+        u[t][kPairs + p] = __builtin_bit_cast(bf16x8, u32x4{lo[2u * p][0], lo[2u * p][1], lo[2u * p + 1u][0], lo[2u * p + 1u][1]});
+      }
+    }
+  }
+  const u32x4* b_at = reinterpret_cast<const u32x4*>(a.b) + (uint64_t)tile.x * nb * NR * 128u + lane;
+  // B of a group in two parts (of a rank up to 32 one): the second is asked for while the first is multiplied, the next
+  // group's first and y behind it, so that waiting for B never waits for y (loads are counted in order)
+  constexpr uint32_t kParts = NR >= 4u ? 2u : 1u, kPart = 2u * NR / kParts;
+  u32x4 b[kParts][kPart];
+  Unaligned16 y0[kLoads], y1[kLoads];
+  const bool whole = tile.z == H * TT * 16u && a.n % 256u == 0u;
+  auto load_b = [&](uint32_t g, uint32_t part) __attribute__((always_inline)) {
+    const uint32_t s = min(g * 4u + wave % 4u, nb - 1u);
+#pragma unroll
+    for (uint32_t i = 0; i < kPart; ++i) b[part][i] = b_at[(uint64_t)s * (NR * 128u) + (part * kPart + i) * 64u];
+  };
+  auto load_y = [&](uint32_t g, Unaligned16 (&y)[kLoads]) __attribute__((always_inline)) {
+    if (whole) {
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) y[i] = *reinterpret_cast<const Unaligned16*>(from[i] + g * 256u + c);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) y[i] = part_to(from[i], g * 256u + c, a.n).w[0];
     }
   };
-  load(g0);
-  for (uint32_t g = g0; g < g1; ++g) {
-    uint4 b[NR][2];
-    Unaligned16 y[kLoads];
-#pragma unroll
-    for (uint32_t r = 0; r < NR; ++r)
-#pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) b[r][h] = b_next[r][h];
-#pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i) y[i] = y_next[i];
-    load(g + 1u < g1 ? g + 1u : g);  // (the last turn's again, from the cache)
-    __builtin_amdgcn_sched_barrier(0);
+  const uint32_t turns = g1 - g0;
+  uint32_t g = g0 + at_tile % turns;  // (tiles begin with different columns, as above)
+  load_b(g, 0u);
+  load_y(g, y0);
+  auto group = [&](Unaligned16 (&y)[kLoads], Unaligned16 (&y_next)[kLoads]) __attribute__((always_inline)) {
+    const uint32_t at_g = g;
+    g = g + 1u == g1 ? g0 : g + 1u;  // (behind the last one the first again, from the cache)
     v4f acc[TT][4];
 #pragma unroll
     for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
       for (uint32_t j = 0; j < 4u; ++j) acc[t][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](uint32_t part) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t r = 0; r < NR; ++r) {
-      const uint32_t w[8] = {b[r][0].x, b[r][0].y, b[r][0].z, b[r][0].w, b[r][1].x, b[r][1].y, b[r][1].z, b[r][1].w};
+      for (uint32_t p = part * (kPairs / kParts); p < (part + 1u) * (kPairs / kParts); ++p)
 #pragma unroll
-      for (uint32_t j = 0; j < 4u; ++j) {
-        const u32x4 twice = {w[2u * j], w[2u * j + 1u], w[2u * j], w[2u * j + 1u]};
+        for (uint32_t j = 0; j < 4u; ++j) {
+          u32x4 w;
+          if constexpr (NR == 1u) {
+            const uint32_t k = 2u * (j & 1u);
+            w = u32x4{b[0][j / 2u][k], b[0][j / 2u][k + 1u], b[0][j / 2u][k], b[0][j / 2u][k + 1u]};
+          } else {
+            w = b[part][(p * 4u + j) % kPart];
+          }
 #pragma unroll
-        for (uint32_t t = 0; t < TT; ++t)
-          acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, twice), u[t][r], acc[t][j], 0, 0, 0);
-      }
+          for (uint32_t t = 0; t < TT; ++t)
+#pragma unroll
+            for (uint32_t o = p; o < kOperands; o += kPairs)
+              acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), u[t][o], acc[t][j], 0, 0, 0);
+        }
+    };
+    if constexpr (kParts == 2u) {
+      load_b(at_g, 1u);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    multiply(0u);
+    __builtin_amdgcn_sched_barrier(0);
+    load_b(g, 0u);
+    load_y(g, y_next);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kParts == 2u) multiply(1u);
 #pragma unroll
     for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
       for (uint32_t j = 0; j < 4u; ++j)
-        *reinterpret_cast<v4f*>(&sums[t * 16u + (lane & 15u)][wave * 64u + j * 16u + q * 4u]) = acc[t][j];
+        *reinterpret_cast<v4f*>(&sums[first + t * 16u + (lane & 15u)][wave % 4u * 64u + j * 16u + q * 4u]) = acc[t][j];
     nklds::barrier();
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; ++i) {
@@ -428,10 +519,15 @@ __device__ __forceinline__ void expand(const Adapters& a) {
 #pragma unroll
       for (uint32_t e = 0; e < 4u; ++e)
         y[i].w[e] = nk::bf16x2_hw(nk::bf16_lo(y[i].w[e]) + f[2u * e], nk::bf16_hi(y[i].w[e]) + f[2u * e + 1u]);
-      if (whole) *reinterpret_cast<Unaligned16*>(to[i] + g * 256u + c) = y[i];
-      else if (there[i]) store8(to[i], g * 256u + c, a.n, y[i]);
+      if (whole) *reinterpret_cast<Unaligned16*>(to[i] + at_g * 256u + c) = y[i];
+      else if (there[i]) store8(to[i], at_g * 256u + c, a.n, y[i]);
     }
     nklds::barrier();
+  };
+  for (uint32_t turn = 0; turn < turns; turn += 2u) {
+    group(y0, y1);
+    if (turn + 1u == turns) break;
+    group(y1, y0);
   }
 }
 
@@ -453,24 +549,32 @@ extern "C" __global__ __launch_bounds__(1024) void netra_adapters_plan_gfx950(co
   }
 NETRA_ADAPTERS_PACK(bf16, uint16_t)
 NETRA_ADAPTERS_PACK(f32, float)
-// t: 16-token parts of a tile, r: 16-rank parts
-#define NETRA_ADAPTERS(TT, NR)                                                                                  \
-  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_bf16_t##TT##r##NR##_gfx950(           \
+// t: 16-token parts of a wave's part of a tile, h: waves' parts of a tile, r: 16-rank parts
+#define NETRA_SHRINK(TT, H, NR)                                                                                 \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_bf16_t##TT##h##H##r##NR##_gfx950(     \
       nkada::Adapters a) {                                                                                      \
-    nkada::shrink<uint16_t, TT, NR>(a);                                                                         \
+    nkada::shrink<uint16_t, TT, H, NR>(a);                                                                      \
   }                                                                                                             \
-  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_f32_t##TT##r##NR##_gfx950(            \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_f32_t##TT##h##H##r##NR##_gfx950(      \
       nkada::Adapters a) {                                                                                      \
-    nkada::shrink<float, TT, NR>(a);                                                                            \
-  }                                                                                                             \
-  extern "C" __global__ __launch_bounds__(256) void netra_adapters_expand_t##TT##r##NR##_gfx950(nkada::Adapters a) { \
-    nkada::expand<TT, NR>(a);                                                                                   \
+    nkada::shrink<float, TT, H, NR>(a);                                                                         \
   }
-NETRA_ADAPTERS(1, 1)
-NETRA_ADAPTERS(1, 2)
-NETRA_ADAPTERS(1, 4)
-NETRA_ADAPTERS(1, 8)
-NETRA_ADAPTERS(2, 1)
-NETRA_ADAPTERS(2, 2)
-NETRA_ADAPTERS(2, 4)
-NETRA_ADAPTERS(2, 8)
+#define NETRA_EXPAND(TT, H, NR)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256 * H) void netra_adapters_expand_t##TT##h##H##r##NR##_gfx950(      \
+      nkada::Adapters a) {                                                                                      \
+    nkada::expand<TT, H, NR>(a);                                                                                \
+  }
+NETRA_SHRINK(1, 1, 1)
+NETRA_SHRINK(1, 1, 2)
+NETRA_SHRINK(1, 1, 4)
+NETRA_SHRINK(2, 2, 1)
+NETRA_SHRINK(2, 2, 2)
+NETRA_SHRINK(2, 2, 4)
+NETRA_EXPAND(1, 1, 1)
+NETRA_EXPAND(1, 1, 2)
+NETRA_EXPAND(1, 1, 4)
+NETRA_EXPAND(1, 1, 8)
+NETRA_EXPAND(2, 2, 1)
+NETRA_EXPAND(2, 2, 2)
+NETRA_EXPAND(2, 2, 4)
+NETRA_EXPAND(2, 2, 8)

@@ -64,7 +64,7 @@ def test_plan(T, L):
     of = torch.where((ids < 0) | (ids >= L), L, ids)
     assert words[:4].tolist()[1:] == [T, L, 0]
     assert torch.equal(words[4:4 + T].long(), torch.sort(of, stable=True).indices)
-    tile = 32 if T > 1024 and T // 32 >= L else 16
+    tile = 64 if T > 1024 and T // 64 >= L else 16
     start = 4 + -(-T // 4) * 4
     want, at = [], 0
     for l, n in enumerate(torch.bincount(of, minlength=L + 1).tolist()):
