@@ -233,25 +233,19 @@ __device__ __forceinline__ void split(v4f v, float scale, uint32_t r, uint32_t r
   lo = u32x2{nk::bf16x2_hw(l[0], l[1]), nk::bf16x2_hw(l[2], l[3])};
 }
 
-// u of the H-th part of a tile: TT times 16 tokens by 16 NR ranks (of the workgroup's place in y). The
-// eight waves of a workgroup share k's blocks out among them and join their sums through LDS, in the order of the waves.
+// The first product of a tile of TT times 16 tokens by 16 NR ranks from the 16-rank part r0 on: the eight waves of a
+// workgroup share k's blocks out among them and leave their sums in LDS, to be joined in the order of the waves.
 //
 // A wave's loads are counted in the order in which they are issued, so waiting for A (from the L2) waits for all of
-// x that was asked for before it (from memory). A block goes in two halves; each half's A is asked for a half ahead,
-// each half's x two halves ahead, and A before x:  A0(b) x1(b) | A1(b) x0(b+1) | A0(b+1) x1(b+1) | ...
-template <typename X, uint32_t TT, uint32_t H, uint32_t NR>
-__device__ __forceinline__ void shrink(const Adapters& a) {
+// x that was asked for before it (from memory). A block goes in two halves; a half's A is asked for before the next
+// half's x. (Both a half further ahead takes 170 registers instead of 122, one workgroup on a CU instead of two: 39.5 us
+// instead of 35.7 at T 8192, K 4096, rank 64.)
+template <typename X, uint32_t TT, uint32_t NR>
+__device__ __forceinline__ void first_product(const Adapters& a, const uint4& tile, uint32_t split_at, uint32_t r0,
+                                              v4f (&part)[8][TT * NR][64]) {
   constexpr uint32_t W = 8u;
-  __shared__ v4f part[W][TT * NR][64];
-  uint4 tile;
-  if (!tile_of(a, blockIdx.x / H, tile) || tile.x >= a.adapters) return;
-  const uint32_t before = blockIdx.x % H * (TT * 16u);  // this workgroup's part of the tile
-  if (before >= tile.z) return;
-  tile.y += before;
-  tile.z = min(tile.z - before, TT * 16u);
   const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t kb = (a.k + 127u) / 128u, split_at = blockIdx.y, r0 = blockIdx.z * NR;  // 16-rank parts before this one's
-  const uint32_t b1 = min(kb, (split_at + 1u) * a.split_blocks), c = (lane >> 4) * 8u;
+  const uint32_t kb = (a.k + 127u) / 128u, b1 = min(kb, (split_at + 1u) * a.split_blocks), c = (lane >> 4) * 8u;
   const X* row[TT];
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t) {
@@ -264,28 +258,28 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const u32x4* ab = reinterpret_cast<const u32x4*>(a.a) + ((uint64_t)tile.x * kb * a.ranks + r0) * 256u + lane;
-  u32x4 wa[2][NR][2];  // A of each half
-  Part<X> x[2][TT][2], next[2][TT][2];
+  u32x4 wa[NR][2];    // A of a half
+  Part<X> x[2][TT][2];  // x of both
   auto load_a = [&](uint32_t b, uint32_t h) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r)
 #pragma unroll
-      for (uint32_t j = 0; j < 2u; ++j) wa[h][r][j] = ab[((uint64_t)b * a.ranks + r) * 256u + (2u * h + j) * 64u];
+      for (uint32_t j = 0; j < 2u; ++j) wa[r][j] = ab[((uint64_t)b * a.ranks + r) * 256u + (2u * h + j) * 64u];
   };
-  auto load_x = [&](uint32_t b, uint32_t h, Part<X> (&to)[2][TT][2]) __attribute__((always_inline)) {
+  auto load_x = [&](uint32_t b, uint32_t h) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t j = 0; j < 2u; ++j)
 #pragma unroll
-      for (uint32_t t = 0; t < TT; ++t) to[h][t][j] = part_whole(row[t], b * 128u + (2u * h + j) * 32u + c);
+      for (uint32_t t = 0; t < TT; ++t) x[h][t][j] = part_whole(row[t], b * 128u + (2u * h + j) * 32u + c);
   };
-  auto products = [&](uint32_t h, const Part<X> (&from)[2][TT][2]) __attribute__((always_inline)) {
+  auto products = [&](uint32_t h) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t j = 0; j < 2u; ++j)
 #pragma unroll
       for (uint32_t r = 0; r < NR; ++r)
 #pragma unroll
         for (uint32_t t = 0; t < TT; ++t)
-          acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wa[h][r][j]), operand(from[h][t][j]),
+          acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wa[r][j]), operand(x[h][t][j]),
                                                               acc[t][r], 0, 0, 0);
   };
   // The wave's blocks: every 8th from b0 on. Each wave begins with another one, so that at any time the workgroups
@@ -296,29 +290,21 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   const uint32_t count = b0 < whole ? (whole - b0 + W - 1u) / W : 0u;
   if (count) {
     uint32_t at = wave % count, b = b0 + at * W;
-    load_x(b, 0u, x);
-    load_a(b, 0u);
-    load_x(b, 1u, x);
-    auto block = [&](const Part<X> (&now)[2][TT][2], Part<X> (&then)[2][TT][2]) __attribute__((always_inline)) {
+    load_x(b, 0u);
+    for (uint32_t i = 0; i < count; ++i) {
       at = at + 1u == count ? 0u : at + 1u;  // (behind the last one the first again, from the cache)
       const uint32_t b_next = b0 + at * W;
+      load_a(b, 0u);
+      load_x(b, 1u);
+      __builtin_amdgcn_sched_barrier(0);
+      products(0u);
+      __builtin_amdgcn_sched_barrier(0);
       load_a(b, 1u);
-      load_x(b_next, 0u, then);
+      load_x(b_next, 0u);
       __builtin_amdgcn_sched_barrier(0);
-      products(0u, now);
-      __builtin_amdgcn_sched_barrier(0);
-      load_a(b_next, 0u);
-      load_x(b_next, 1u, then);
-      __builtin_amdgcn_sched_barrier(0);
-      products(1u, now);
+      products(1u);
       __builtin_amdgcn_sched_barrier(0);
       b = b_next;
-    };
-    // (two in turn: x is not copied, which would wait for it)
-    for (uint32_t i = 0; i < count; i += 2u) {
-      block(x, next);
-      if (i + 1u == count) break;
-      block(next, x);
     }
   }
   const uint32_t b = b0 + count * W;
@@ -330,7 +316,7 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
 #pragma unroll
         for (uint32_t t = 0; t < TT; ++t) x[h][t][j] = part_to(row[t], b * 128u + (2u * h + j) * 32u + c, a.k);
       load_a(b, h);
-      products(h, x);
+      products(h);
     }
   }
 #pragma unroll
@@ -338,12 +324,32 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
 #pragma unroll
     for (uint32_t r = 0; r < NR; ++r) part[wave][t * NR + r][lane] = acc[t][r];
   __syncthreads();
+}
+// Four ranks of a token: place i of 64 TT NR.
+template <uint32_t N>
+__device__ __forceinline__ v4f joined(const v4f (&part)[8][N][64], uint32_t i) {
+  v4f v = part[0][i >> 6][i & 63u];
+#pragma unroll
+  for (uint32_t w = 1; w < 8u; ++w) v += part[w][i >> 6][i & 63u];
+  return v;
+}
+
+// u of the H-th part of a tile, of NR of its 16-rank parts (the workgroup's place in z), of one split.
+template <typename X, uint32_t TT, uint32_t H, uint32_t NR>
+__device__ __forceinline__ void shrink(const Adapters& a) {
+  __shared__ v4f part[8][TT * NR][64];
+  uint4 tile;
+  if (!tile_of(a, blockIdx.x / H, tile) || tile.x >= a.adapters) return;
+  const uint32_t before = blockIdx.x % H * (TT * 16u);  // this workgroup's part of the tile
+  if (before >= tile.z) return;
+  tile.y += before;
+  tile.z = min(tile.z - before, TT * 16u);
+  const uint32_t split_at = blockIdx.y, r0 = blockIdx.z * NR;
+  first_product<X, TT, NR>(a, tile, split_at, r0, part);
   for (uint32_t i = threadIdx.x; i < TT * NR * 64u; i += 512u) {
     const uint32_t l = i & 63u, tr = i >> 6, in = tr / NR * 16u + (l & 15u);
-    v4f v = part[0][tr][l];
-#pragma unroll
-    for (uint32_t w = 1; w < W; ++w) v += part[w][tr][l];
     if (in >= tile.z) continue;
+    const v4f v = joined(part, i);
     const uint32_t r = (r0 + tr % NR) * 16u + (l >> 4) * 4u, ranks = 16u * a.ranks;
     if (a.splits > 1u) {
       *reinterpret_cast<v4f*>(static_cast<float*>(a.u) + ((uint64_t)split_at * a.tokens + tile.y + in) * ranks + r) = v;
@@ -531,6 +537,95 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   }
 }
 
+// Both products of a tile of 16 tokens and 512 columns in one launch: each workgroup works the tile's u out for itself.
+template <typename X, uint32_t NR>
+__device__ __forceinline__ void fused(const Adapters& a) {
+  constexpr uint32_t kPitch = 516u;  // spreads 16 tokens' rows over the banks
+  constexpr uint32_t kPairs = NR == 1u ? 1u : NR / 2u, kOperands = NR == 1u ? 1u : NR;
+  constexpr uint32_t kSums = 16u * kPitch * 4u, kParts = 8u * NR * 1024u;
+  __shared__ __attribute__((aligned(16))) uint8_t memory[kSums > kParts ? kSums : kParts];
+  __shared__ u32x2 s_u[2][16][4u * NR + 1u];  // [rounded, left][token][four ranks]
+  auto& part = *reinterpret_cast<v4f (*)[8][NR][64]>(memory);
+  auto& sums = *reinterpret_cast<float (*)[16][kPitch]>(memory);
+  uint4 tile;
+  const uint32_t at_tile = blockIdx.x / a.chunks, chunk = blockIdx.x - at_tile * a.chunks;
+  if (!tile_of(a, at_tile, tile)) return;
+  const bool none = tile.x >= a.adapters;
+  if (none && a.in_place) return;
+  const uint32_t lane = threadIdx.x & 63u, q = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t c = chunk * 512u + lane * 8u, nb = (a.n + 63u) / 64u;
+  const uint16_t* from[2];
+  uint16_t* to[2];
+  Unaligned16 y[2];
+#pragma unroll
+  for (uint32_t i = 0; i < 2u; ++i) {
+    const uint32_t token = a.plan[kPlanHead + tile.y + min(wave * 2u + i, tile.z - 1u)];
+    from[i] = a.y + (uint64_t)token * a.y_stride;
+    to[i] = a.out + (uint64_t)token * a.out_stride;
+    y[i] = part_to(from[i], c, a.n).w[0];
+  }
+  if (!none) {
+    const u32x4* b_at = reinterpret_cast<const u32x4*>(a.b) +
+                        ((uint64_t)tile.x * nb + min(chunk * 8u + wave, nb - 1u)) * (NR * 128u) + lane;
+    u32x4 b[2u * NR];
+#pragma unroll
+    for (uint32_t i = 0; i < 2u * NR; ++i) b[i] = b_at[i * 64u];
+    first_product<X, 1u, NR>(a, tile, 0u, 0u, part);
+    if (threadIdx.x < NR * 64u) {
+      const uint32_t r = (threadIdx.x >> 6) * 16u + (lane >> 4) * 4u;
+      u32x2 hi, lo;
+      split(joined(part, threadIdx.x), a.scale[tile.x], r, a.rank, hi, lo);
+      s_u[0][lane & 15u][r / 4u] = hi;
+      s_u[1][lane & 15u][r / 4u] = lo;
+    }
+    __syncthreads();
+    auto four = [&](uint32_t which, uint32_t r4) __attribute__((always_inline)) { return s_u[which][lane & 15u][r4]; };
+    bf16x8 u[kOperands];
+    if constexpr (NR == 1u) {
+      const u32x2 hi = four(0u, q), lo = four(1u, q);
+      u[0] = __builtin_bit_cast(bf16x8, u32x4{hi[0], hi[1], lo[0], lo[1]});
+    } else {
+#pragma unroll
+      for (uint32_t o = 0; o < kOperands; ++o) {
+        const u32x2 first = four(o / kPairs, o % kPairs * 8u + q * 2u), second = four(o / kPairs, o % kPairs * 8u + q * 2u + 1u);
+        u[o] = __builtin_bit_cast(bf16x8, u32x4{first[0], first[1], second[0], second[1]});
+      }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; ++j) {
+      v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (uint32_t p = 0; p < kPairs; ++p) {
+        u32x4 w;
+        if constexpr (NR == 1u) {
+          const uint32_t k = 2u * (j & 1u);
+          w = u32x4{b[j / 2u][k], b[j / 2u][k + 1u], b[j / 2u][k], b[j / 2u][k + 1u]};
+        } else {
+          w = b[p * 4u + j];
+        }
+#pragma unroll
+        for (uint32_t o = p; o < kOperands; o += kPairs)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), u[o], acc, 0, 0, 0);
+      }
+      *reinterpret_cast<v4f*>(&sums[lane & 15u][wave * 64u + j * 16u + q * 4u]) = acc;  // (part has been read: the barrier above)
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; ++i) {
+      const float* d = &sums[wave * 2u + i][lane * 8u];
+      const v4f lo = *reinterpret_cast<const v4f*>(d), hi = *reinterpret_cast<const v4f*>(d + 4);
+      const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e)
+        y[i].w[e] = nk::bf16x2_hw(nk::bf16_lo(y[i].w[e]) + f[2u * e], nk::bf16_hi(y[i].w[e]) + f[2u * e + 1u]);
+    }
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 2u; ++i)
+    if (wave * 2u + i < tile.z) store8(to[i], c, a.n, y[i]);
+}
+
 }  // namespace nkada
 
 extern "C" __global__ __launch_bounds__(1024) void netra_adapters_plan_gfx950(const int32_t* ids, uint32_t tokens,
@@ -570,6 +665,17 @@ NETRA_SHRINK(1, 1, 4)
 NETRA_SHRINK(2, 2, 1)
 NETRA_SHRINK(2, 2, 2)
 NETRA_SHRINK(2, 2, 4)
+#define NETRA_FUSED(NR)                                                                                         \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_fused_bf16_r##NR##_gfx950(nkada::Adapters a) { \
+    nkada::fused<uint16_t, NR>(a);                                                                              \
+  }                                                                                                             \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_fused_f32_r##NR##_gfx950(nkada::Adapters a) { \
+    nkada::fused<float, NR>(a);                                                                                 \
+  }
+NETRA_FUSED(1)
+NETRA_FUSED(2)
+NETRA_FUSED(4)
+NETRA_FUSED(8)
 NETRA_EXPAND(1, 1, 1)
 NETRA_EXPAND(1, 1, 2)
 NETRA_EXPAND(1, 1, 4)

@@ -12,7 +12,7 @@ bool bad_adapters(uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k) {
          n > kMaxSize || k > kMaxSize;
 }
 uint64_t u_bytes(const AdapterPlan& plan, uint32_t tokens, uint32_t rank) {
-  return 64ull * adapter_ranks(rank) * plan.splits * tokens;
+  return plan.fused ? 0 : 64ull * adapter_ranks(rank) * plan.splits * tokens;
 }
 
 }  // namespace
@@ -126,12 +126,28 @@ extern "C" int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_str
   a.k = k;
   a.in_place = out == y;
   a.wide = p.wide;
-  a.chunks = ((n + 255u) / 256u + p.wide - 1u) / p.wide;
+  const uint32_t width = p.fused ? 512u : 256u * p.wide;  // columns of a workgroup
+  a.chunks = (n + width - 1u) / width;
   const uint64_t groups = static_cast<uint64_t>(a.chunks) * p.tiles;
   if (!launchable(groups, 512u)) return fail(-1, name, "more workgroups than one launch takes");
+  Launcher launch(stream);
+  if (p.fused) {
+    const dim3 grid(static_cast<uint32_t>(groups)), block(512);
+    if (x_type == NETRA_BF16) {
+      if (a.ranks == 1u) launch(netra_adapters_fused_bf16_r1_gfx950, grid, block, a);
+      else if (a.ranks == 2u) launch(netra_adapters_fused_bf16_r2_gfx950, grid, block, a);
+      else if (a.ranks == 4u) launch(netra_adapters_fused_bf16_r4_gfx950, grid, block, a);
+      else launch(netra_adapters_fused_bf16_r8_gfx950, grid, block, a);
+    } else {
+      if (a.ranks == 1u) launch(netra_adapters_fused_f32_r1_gfx950, grid, block, a);
+      else if (a.ranks == 2u) launch(netra_adapters_fused_f32_r2_gfx950, grid, block, a);
+      else if (a.ranks == 4u) launch(netra_adapters_fused_f32_r4_gfx950, grid, block, a);
+      else launch(netra_adapters_fused_f32_r8_gfx950, grid, block, a);
+    }
+    return launch.result(name);
+  }
   const uint32_t parts = adapter_tile(tokens, adapters) == 16u ? 1u : 2u;  // of a tile
   const dim3 shrink(p.tiles * parts, p.splits, a.ranks == 8u ? 2u : 1u), expand(static_cast<uint32_t>(groups));
-  Launcher launch(stream);
 // (a rank over 64 in two parts of the first product: of one the operands do not fit the registers)
 #define NETRA_RUN(TT, H, NR, EXPAND_NR)                                                                   \
   do {                                                                                                    \

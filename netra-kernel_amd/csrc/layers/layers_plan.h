@@ -214,9 +214,22 @@ inline uint32_t adapter_tiles(uint32_t tokens, uint32_t adapters) {
 }
 struct AdapterPlan {
   uint32_t tiles, splits, split_blocks, wide;
+  bool fused;
 };
 inline AdapterPlan adapter_plan(uint32_t tokens, uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k) {
-  AdapterPlan p{adapter_tiles(tokens, adapters), 1, blocks(k), 1};
+  AdapterPlan p{adapter_tiles(tokens, adapters), 1, blocks(k), 1, false};
+  // One launch, in which each workgroup of 512 columns works u out for itself, where the workgroups find a CU
+  // each and A is short (us, in one launch / in two; a launch takes the host 3.5 besides):
+  //   A  64 KB  T 64, 32 adapters, N 2048: 144 workgroups 4.7 / 6.7    T 1000, 30, 2048: 372, 11.3 / 8.3
+  //   A 128 KB  T 16, 16, N 4096: 136, 5.6 / 7.1    T 64, 16, 4096: 160, 5.6 / 7.2    T 256, 32, 4096: 384, 11.7 / 8.2
+  //   A 256 KB  T 64, 16, N 4096: 160, 9.2 / 8.2
+  const uint64_t a_bytes = 32ull * adapter_ranks(rank) * up(k, 128u);  // of one adapter
+  if (adapter_tile(tokens, adapters) == 16u && a_bytes <= 131072u &&
+      static_cast<uint64_t>(p.tiles) * ((n + 511u) / 512u) <= 256u) {
+    p.fused = true;
+    p.split_blocks = blocks(k);
+    return p;
+  }
   // a workgroup reads and packs its tile's u before its first columns: up to eight groups share that
   const uint64_t groups = static_cast<uint64_t>(p.tiles) * ((n + 255u) / 256u);
   while (p.wide < 8u && groups / (2u * p.wide) >= 1024u) p.wide *= 2u;

@@ -10,14 +10,14 @@ pytestmark = pytest.mark.skipif(not paths.layers_library().is_file(), reason="li
 
 
 @pytest.mark.parametrize("change", [
-    dict(x=0), dict(x=A + 1), dict(xt=2), dict(xs=255), dict(pa=0), dict(pa=B + 8), dict(pb=0), dict(pb=D + 4), dict(scale=0),
+    dict(x=0), dict(x=A + 1), dict(xt=2), dict(xs=8191), dict(pa=0), dict(pa=B + 8), dict(pb=0), dict(pb=D + 4), dict(scale=0),
     dict(scale=4 * A + 2), dict(plan=0), dict(plan=5 * A + 8), dict(y=0), dict(y=6 * A + 1), dict(ys=127), dict(o=0), dict(o=7 * A + 1),
     dict(os=127), dict(o=A), dict(o=6 * A + 2), dict(os=200, o=6 * A), dict(T=(1 << 21) + 1), dict(L=0), dict(L=1025), dict(r=0),
-    dict(r=129), dict(n=0), dict(k=0), dict(n=(1 << 21) + 1, ys=1 << 22, os=1 << 22), dict(ws=0), dict(ws=8 * A + 8), dict(short=1)])
+    dict(r=129), dict(n=0), dict(k=0), dict(n=(1 << 21) + 1, ys=1 << 22, os=1 << 22), dict(ws=0), dict(ws=8 * A + 8), dict(short=1)])  # (of two launches)
 def test_add_refusals(change):
-    a = dict(x=A, xt=0, xs=256, pa=B, pb=D, scale=4 * A, plan=5 * A, y=6 * A, ys=128, o=7 * A, os=128, T=40, L=3, r=8, n=128,
-             k=256, ws=8 * A, short=0)
-    need = layers.library().netra_adapters_add_workspace(40, 3, 8, 128, 256)
+    a = dict(x=A, xt=0, xs=8192, pa=B, pb=D, scale=4 * A, plan=5 * A, y=6 * A, ys=128, o=7 * A, os=128, T=40, L=3, r=100, n=128,
+             k=8192, ws=8 * A, short=0)
+    need = layers.library().netra_adapters_add_workspace(40, 3, 100, 128, 8192)
     a.update(change)
     refused("netra_adapters_add", a["x"], a["xt"], a["xs"], a["pa"], a["pb"], a["scale"], a["plan"], a["y"], a["ys"], a["o"],
             a["os"], a["T"], a["L"], a["r"], a["n"], a["k"], a["ws"], need - a["short"], None)

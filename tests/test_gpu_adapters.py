@@ -30,7 +30,8 @@ def ids_of(T, L, chunk, seed):
 SIZES = [(1, 1, 1, 1, 1, 1), (1, 4, 8, 2048, 2048, 1), (2, 2, 16, 64, 64, 1), (3, 1, 17, 100, 70, 3), (16, 5, 4, 128, 63, 1),
          (17, 1, 16, 129, 65, 17), (64, 32, 16, 512, 500, 1), (50, 7, 33, 1111, 130, 9), (203, 3, 12, 257, 300, 41),
          (100, 1000, 6, 96, 80, 1), (300, 2, 128, 333, 777, 150), (1025, 4, 64, 200, 129, 100), (2000, 9, 100, 130, 257, 33),
-         (1500, 1, 32, 64, 2050, 1500), (40, 3, 20, 8192, 40, 5), (5000, 1024, 5, 40, 33, 2)]
+         (1500, 1, 32, 64, 2050, 1500), (40, 3, 20, 8192, 40, 5), (7, 2, 50, 130, 600, 1), (33, 3, 100, 300, 1030, 4), (5, 2, 128, 512, 512, 1),
+         (600, 3, 40, 640, 520, 7), (1100, 2, 90, 1030, 1500, 13), (5000, 1024, 5, 40, 33, 2)]
 
 
 @pytest.mark.parametrize("T,L,r,K,N,chunk", SIZES)
