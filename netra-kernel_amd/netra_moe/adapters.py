@@ -91,7 +91,7 @@ class LowRankAdapters:
         x_stride = check_rows("x", x, (tokens, self.K), self.device)
         y_stride = check_rows("y", y, (tokens, self.N), self.device, (torch.bfloat16,))
         if out is None:
-            out, out_stride = torch.empty((tokens, self.N), dtype=torch.bfloat16, device=self.device), self.N
+            out, out_stride = torch.empty_like(y), self.N
         else:
             out_stride = check_rows("out", out, (tokens, self.N), self.device, (torch.bfloat16,))
         need = self._need(tokens, adapters, self.rank, self.N, self.K)

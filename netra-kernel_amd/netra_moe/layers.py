@@ -3,6 +3,7 @@ libnetra_layers.so), and what their Python forms share."""
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -60,6 +61,7 @@ def library() -> ctypes.CDLL:
     return _lib
 
 
+@functools.lru_cache(maxsize=None)
 def entry(name: str):
     """An entry point as a plain callable, looked up once."""
     return getattr(library(), name)

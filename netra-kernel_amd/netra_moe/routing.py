@@ -69,8 +69,8 @@ def route(logits: torch.Tensor, k: int, *, scoring: str = "softmax", selection_b
                 or not selection_bias.is_contiguous():
             raise ValueError(f"selection_bias: need contiguous torch.float32 ({experts},) on {device}")
         bias = selection_bias.data_ptr()
-    ids = torch.empty((tokens, slots), dtype=torch.int32, device=device)
-    weights = torch.empty((tokens, slots), dtype=torch.float32, device=device)
+    ids = logits.new_empty((tokens, slots), dtype=torch.int32)
+    weights = torch.empty_like(ids, dtype=torch.float32)
     launch(entry("netra_router_select"), "netra_router_select", device, logits.data_ptr(), TYPES[logits.dtype], stride, bias,
            m, tokens, experts, k, int(shared), _number("scoring", scoring, SCORING), groups, top_groups,
            _number("group_score", group_score, GROUP_SCORE), int(renormalise), scale, ids.data_ptr(), slots,
@@ -97,7 +97,7 @@ def route_gradient(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tens
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out, o_stride = logits.new_empty((tokens, experts + shared)), experts + shared
+        out, o_stride = torch.empty_like(logits), experts + shared
     else:
         o_stride = check_rows("out", out, (tokens, experts + shared), device, (logits.dtype,))
     launch(entry("netra_router_select_gradient"), "netra_router_select_gradient", device, dweights.data_ptr(), d_stride,
