@@ -168,6 +168,9 @@ inline CountPlan balance_plan(uint32_t tokens, uint32_t experts) {
   return count_plan(tokens, few < 256u ? few : 256u, 64u);
 }
 
+// Bytes that the cache behind the L2s holds: what moves more than these finds nothing of it there.
+constexpr uint64_t kInfinityCache = 256ull << 20;
+
 // Norms: waves a row and eight columns a lane so many times, rows a workgroup takes at once, and
 // workgroups (they loop over the rows).
 struct NormPlan {

@@ -42,14 +42,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* m, uint64
                          there ? cols * (uint32_t)sizeof(X) : 0u);
 }
 
-template <typename X>
+// kOnce: non-temporal loads and stores.
+template <typename X, bool kOnce = false>
 __device__ __forceinline__ Eight<X> load8(__amdgpu_buffer_rsrc_t r, uint32_t c, uint32_t cols) {
+  constexpr int kAux = kOnce ? 2 : 0;
   Eight<X> v;
   if constexpr (sizeof(X) == 4) {
-    v.lo = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(c * 4u), 0, 0);
-    v.hi = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(c * 4u + 16u), 0, 0);
+    v.lo = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(c * 4u), 0, kAux);
+    v.hi = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(c * 4u + 16u), 0, kAux);
   } else {
-    v.w = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(c * 2u), 0, 0);
+    v.w = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(c * 2u), 0, kAux);
     const bool mine = (cols & 1u) && c < cols && c + 8u > cols;
     v.last = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, mine ? (int)((cols - 1u) * 2u) : kNowhere, 0, 0);
   }
@@ -73,8 +75,9 @@ __device__ __forceinline__ void values(const Eight<X>& v, uint32_t c, uint32_t c
   }
 }
 
-template <typename X>
+template <typename X, bool kOnce = false>
 __device__ __forceinline__ void store8(__amdgpu_buffer_rsrc_t r, uint32_t c, uint32_t cols, const float (&f)[8]) {
+  constexpr int kAux = kOnce ? 2 : 0;
   if constexpr (sizeof(X) == 4) {
     u32x4 lo, hi;
 #pragma unroll
@@ -82,13 +85,13 @@ __device__ __forceinline__ void store8(__amdgpu_buffer_rsrc_t r, uint32_t c, uin
       lo[i] = __float_as_uint(f[i]);
       hi[i] = __float_as_uint(f[4u + i]);
     }
-    __builtin_amdgcn_raw_buffer_store_b128(lo, r, (int)(c * 4u), 0, 0);
-    __builtin_amdgcn_raw_buffer_store_b128(hi, r, (int)(c * 4u + 16u), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(lo, r, (int)(c * 4u), 0, kAux);
+    __builtin_amdgcn_raw_buffer_store_b128(hi, r, (int)(c * 4u + 16u), 0, kAux);
   } else {
     u32x4 w;
 #pragma unroll
     for (uint32_t i = 0; i < 4u; ++i) w[i] = nk::bf16x2_hw(f[2u * i], f[2u * i + 1u]);
-    __builtin_amdgcn_raw_buffer_store_b128(w, r, (int)(c * 2u), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(w, r, (int)(c * 2u), 0, kAux);
     if (cols & 1u) {
       const uint32_t i = (cols - 1u - c) / 2u;  // the dword that the row's last value begins
 #pragma unroll
@@ -160,6 +163,7 @@ struct Norm {
 };
 
 // Codes of eight columns, and their group's scale by its first lane.
+template <bool kOnce>
 __device__ __forceinline__ void quantise8(const Norm& a, uint32_t row, uint32_t c, const float (&y)[8]) {
   uint32_t m = 0u;
 #pragma unroll
@@ -183,7 +187,7 @@ __device__ __forceinline__ void quantise8(const Norm& a, uint32_t row, uint32_t 
     return;
   }
   const __amdgpu_buffer_rsrc_t r = nk::buffer_rsrc(a.codes + (uint64_t)row * a.cols, a.cols & ~3u);
-  __builtin_amdgcn_raw_buffer_store_b64(q, r, (int)c, 0, 0);
+  __builtin_amdgcn_raw_buffer_store_b64(q, r, (int)c, 0, kOnce ? 2 : 0);
   if (a.cols & 3u) {
     const uint32_t from = a.cols & ~3u;  // the last one to three columns, by the lane that has them
     if (from / 8u * 8u == c) {
@@ -203,7 +207,10 @@ struct Shape {
   static constexpr uint32_t kRows = W == 1u ? 4u : 1u, kThreads = W == 1u ? 256u : 64u * W;
 };
 
-template <typename X, typename R, uint32_t W, uint32_t C>
+// kOnce, where all that goes in and out is more than the 256 MiB behind the L2s hold: x and the residual are
+// not kept there, nor the outputs. T 16384, H 4096 with residual and codes (604 MB): 117.3 us, with loads alone
+// non-temporal 112.9, stores alone 113.9, both 110.3 (5.5 TB/s; a large copy 5.1); T 4096 (151 MB) 27.1, both 31.0.
+template <typename X, typename R, uint32_t W, uint32_t C, bool kOnce>
 __device__ __forceinline__ void forward(const Norm& a) {
   __shared__ float part[2u * W];
   constexpr uint32_t kRows = Shape<W>::kRows;
@@ -216,8 +223,8 @@ __device__ __forceinline__ void forward(const Norm& a) {
         row_rsrc<R>(a.residual, a.residual_stride, row, a.cols, row < a.rows && a.residual != nullptr);
 #pragma unroll
     for (uint32_t k = 0; k < C; ++k) {
-      x[k] = load8<X>(rx, at + k * step, a.cols);
-      res[k] = load8<R>(rr, at + k * step, a.cols);
+      x[k] = load8<X, kOnce>(rx, at + k * step, a.cols);
+      res[k] = load8<R, kOnce>(rr, at + k * step, a.cols);
     }
   };
   uint32_t row = blockIdx.x * kRows + (W == 1u ? wave : 0u), turn = 0u;
@@ -252,7 +259,7 @@ __device__ __forceinline__ void forward(const Norm& a) {
     if (a.residual && there) {
       const __amdgpu_buffer_rsrc_t rs = row_rsrc<R>(a.sum, a.sum_stride, row, a.cols, true);
 #pragma unroll
-      for (uint32_t k = 0; k < C; ++k) store8<R>(rs, at + k * step, a.cols, r[k]);
+      for (uint32_t k = 0; k < C; ++k) store8<R, kOnce>(rs, at + k * step, a.cols, r[k]);
     }
 #pragma unroll
     for (uint32_t k = 0; k < C; ++k)
@@ -262,16 +269,16 @@ __device__ __forceinline__ void forward(const Norm& a) {
       if (a.y_bf16) {
         const __amdgpu_buffer_rsrc_t ry = row_rsrc<uint16_t>(a.y, a.y_stride, row, a.cols, true);
 #pragma unroll
-        for (uint32_t k = 0; k < C; ++k) store8<uint16_t>(ry, at + k * step, a.cols, r[k]);
+        for (uint32_t k = 0; k < C; ++k) store8<uint16_t, kOnce>(ry, at + k * step, a.cols, r[k]);
       } else {
         const __amdgpu_buffer_rsrc_t ry = row_rsrc<float>(a.y, a.y_stride, row, a.cols, true);
 #pragma unroll
-        for (uint32_t k = 0; k < C; ++k) store8<float>(ry, at + k * step, a.cols, r[k]);
+        for (uint32_t k = 0; k < C; ++k) store8<float, kOnce>(ry, at + k * step, a.cols, r[k]);
       }
     }
     if (a.layout != kNone) {
 #pragma unroll
-      for (uint32_t k = 0; k < C; ++k) quantise8(a, row, at + k * step, r[k]);
+      for (uint32_t k = 0; k < C; ++k) quantise8<kOnce>(a, row, at + k * step, r[k]);
     }
   }
 }
@@ -292,7 +299,9 @@ struct NormGradients {
   uint32_t rows, cols;
 };
 
-template <typename G, typename X, uint32_t W, uint32_t C>
+// kOnce as above, of the loads alone: T 16384, H 4096 (537 MB) 107.6 us, so 91.5 (5.9 TB/s), with stores too 98.5; T 4096
+// (134 MB) 29.4 and 29.9.
+template <typename G, typename X, uint32_t W, uint32_t C, bool kOnce>
 __device__ __forceinline__ void gradients(const NormGradients& a) {
   __shared__ float part[4u * W];
   constexpr uint32_t kRows = Shape<W>::kRows;
@@ -305,15 +314,15 @@ __device__ __forceinline__ void gradients(const NormGradients& a) {
     const __amdgpu_buffer_rsrc_t rg = row_rsrc<G>(a.dy, a.dy_stride, row, a.cols, row < a.rows);
 #pragma unroll
     for (uint32_t k = 0; k < C; ++k) {
-      x[k] = load8<X>(rx, at + k * step, a.cols);
-      g[k] = load8<G>(rg, at + k * step, a.cols);
+      x[k] = load8<X, kOnce>(rx, at + k * step, a.cols);
+      g[k] = load8<G, kOnce>(rg, at + k * step, a.cols);
     }
   };
   auto load_flow = [&](uint32_t row, Eight<X> (&flow)[C]) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t rf =
         row_rsrc<X>(a.flow, a.flow_stride, row, a.cols, row < a.rows && a.flow != nullptr);
 #pragma unroll
-    for (uint32_t k = 0; k < C; ++k) flow[k] = load8<X>(rf, at + k * step, a.cols);
+    for (uint32_t k = 0; k < C; ++k) flow[k] = load8<X, kOnce>(rf, at + k * step, a.cols);
   };
   const uint32_t first = blockIdx.x * kRows + (W == 1u ? wave : 0u);
   uint32_t row = first, turn = 0u;
@@ -432,21 +441,24 @@ __device__ __forceinline__ void sum_parts(const float* __restrict__ partial, uin
 }  // namespace nknorm
 
 // <type of x>_<type of the residual>, W waves a row, C times eight columns a lane
-#define NETRA_NORM(X, R, XT, RT, W, C)                                                                                \
-  extern "C" __global__ __launch_bounds__(nknorm::Shape<W>::kThreads) void netra_norm_##X##_##R##_w##W##c##C##_gfx950( \
-      nknorm::Norm a) {                                                                                               \
-    nknorm::forward<XT, RT, W, C>(a);                                                                                 \
-  }                                                                                                                   \
-  extern "C" __global__                                                                                               \
-      __launch_bounds__(nknorm::Shape<W>::kThreads) void netra_norm_gradients_##X##_##R##_w##W##c##C##_gfx950(        \
-          nknorm::NormGradients a) {                                                                                  \
-    nknorm::gradients<XT, RT, W, C>(a);                                                                               \
+#define NETRA_NORM(X, R, XT, RT, W, C, NAME, ONCE)                                                             \
+  extern "C" __global__                                                                                        \
+      __launch_bounds__(nknorm::Shape<W>::kThreads) void netra_norm_##X##_##R##_w##W##c##C##NAME##_gfx950(nknorm::Norm a) { \
+    nknorm::forward<XT, RT, W, C, ONCE>(a);                                                                    \
+  }                                                                                                            \
+  extern "C" __global__                                                                                        \
+      __launch_bounds__(nknorm::Shape<W>::kThreads) void netra_norm_gradients_##X##_##R##_w##W##c##C##NAME##_gfx950( \
+          nknorm::NormGradients a) {                                                                           \
+    nknorm::gradients<XT, RT, W, C, ONCE>(a);                                                                  \
   }
-#define NETRA_NORMS(W, C)                      \
-  NETRA_NORM(bf16, bf16, uint16_t, uint16_t, W, C) \
-  NETRA_NORM(bf16, f32, uint16_t, float, W, C) \
-  NETRA_NORM(f32, bf16, float, uint16_t, W, C) \
-  NETRA_NORM(f32, f32, float, float, W, C)
+#define NETRA_NORM_BOTH(X, R, XT, RT, W, C) \
+  NETRA_NORM(X, R, XT, RT, W, C, , false)   \
+  NETRA_NORM(X, R, XT, RT, W, C, _once, true)
+#define NETRA_NORMS(W, C)                               \
+  NETRA_NORM_BOTH(bf16, bf16, uint16_t, uint16_t, W, C) \
+  NETRA_NORM_BOTH(bf16, f32, uint16_t, float, W, C)     \
+  NETRA_NORM_BOTH(f32, bf16, float, uint16_t, W, C)     \
+  NETRA_NORM_BOTH(f32, f32, float, float, W, C)
 NETRA_NORMS(1, 1)
 NETRA_NORMS(1, 2)
 NETRA_NORMS(4, 1)

@@ -17,19 +17,24 @@ bool bad_norm(uint32_t rows, uint32_t cols) { return rows > kMaxSize || cols == 
 bool bad_weight(const void* w, uint32_t type) { return !w || bad_type(type) || !aligned(w, elem(type)); }
 
 // The launch of one of the kernels by the types and the row's length.
+#define NETRA_NORM_ONE(KERNEL, X, R, W, C)                                          \
+  do {                                                                              \
+    if (once) launch(KERNEL##_##X##_##R##_w##W##c##C##_once_gfx950, grid, block, a); \
+    else launch(KERNEL##_##X##_##R##_w##W##c##C##_gfx950, grid, block, a);          \
+  } while (0)
 #define NETRA_NORM_TYPES(KERNEL, W, C)                                                               \
   do {                                                                                               \
-    if (first == NETRA_BF16 && second == NETRA_BF16) launch(KERNEL##_bf16_bf16_w##W##c##C##_gfx950, grid, block, a); \
-    else if (first == NETRA_BF16) launch(KERNEL##_bf16_f32_w##W##c##C##_gfx950, grid, block, a);     \
-    else if (second == NETRA_BF16) launch(KERNEL##_f32_bf16_w##W##c##C##_gfx950, grid, block, a);    \
-    else launch(KERNEL##_f32_f32_w##W##c##C##_gfx950, grid, block, a);                               \
+    if (first == NETRA_BF16 && second == NETRA_BF16) NETRA_NORM_ONE(KERNEL, bf16, bf16, W, C);       \
+    else if (first == NETRA_BF16) NETRA_NORM_ONE(KERNEL, bf16, f32, W, C);                           \
+    else if (second == NETRA_BF16) NETRA_NORM_ONE(KERNEL, f32, bf16, W, C);                          \
+    else NETRA_NORM_ONE(KERNEL, f32, f32, W, C);                                                     \
   } while (0)
-#define NETRA_NORM_SHAPES(KERNEL)                                        \
+#define NETRA_NORM_SHAPES(KERNEL)                                            \
   if (plan.waves == 1u && plan.chunks == 1u) NETRA_NORM_TYPES(KERNEL, 1, 1); \
-  else if (plan.waves == 1u) NETRA_NORM_TYPES(KERNEL, 1, 2);             \
-  else if (plan.waves == 4u) NETRA_NORM_TYPES(KERNEL, 4, 1);             \
-  else if (plan.waves == 8u) NETRA_NORM_TYPES(KERNEL, 8, 1);             \
-  else if (plan.chunks == 1u) NETRA_NORM_TYPES(KERNEL, 16, 1);           \
+  else if (plan.waves == 1u) NETRA_NORM_TYPES(KERNEL, 1, 2);                 \
+  else if (plan.waves == 4u) NETRA_NORM_TYPES(KERNEL, 4, 1);                 \
+  else if (plan.waves == 8u) NETRA_NORM_TYPES(KERNEL, 8, 1);                 \
+  else if (plan.chunks == 1u) NETRA_NORM_TYPES(KERNEL, 16, 1);               \
   else NETRA_NORM_TYPES(KERNEL, 16, 2)
 
 }  // namespace
@@ -100,6 +105,9 @@ extern "C" int netra_norm_forward(const void* x, uint32_t x_type, uint64_t x_str
   a.all_rows = a.layout == nknorm::kTiles ? up(rows, 16u) : rows;
   const NormPlan plan = norm_plan(a.all_rows, cols);
   const uint32_t first = x_type, second = residual ? residual_type : x_type;
+  const uint64_t row = row_bytes(cols, x_type) + (residual ? 2u * row_bytes(cols, residual_type) : 0u) +
+                       (y ? row_bytes(cols, y_type) : 0u) + (codes ? cols : 0u);
+  const bool once = row * rows > kInfinityCache;
   const dim3 grid(plan.groups), block(plan.threads);
   Launcher launch(stream);
   NETRA_NORM_SHAPES(netra_norm);
@@ -158,6 +166,7 @@ extern "C" int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t d
     a.rows = rows;
     a.cols = cols;
     const uint32_t first = dy_type, second = r_type;
+    const bool once = (row_bytes(cols, dy_type) + (flow ? 3u : 2u) * row_bytes(cols, r_type)) * rows > kInfinityCache;
     const dim3 grid(plan.groups), block(plan.threads);
     NETRA_NORM_SHAPES(netra_norm_gradients);
   }
@@ -168,3 +177,4 @@ extern "C" int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t d
 }
 #undef NETRA_NORM_SHAPES
 #undef NETRA_NORM_TYPES
+#undef NETRA_NORM_ONE

@@ -13,7 +13,7 @@ DEV = "cuda:0"
 # one value, odd ends, each number of waves a row and its borders, more rows than workgroups
 SIZES = [(1, 1), (1, 7), (2, 8), (3, 128), (5, 130), (4, 511), (6, 512), (5, 513), (7, 1023), (17, 1024), (3, 1025), (9, 1111),
          (1, 2048), (33, 2048), (3, 2049), (2, 4095), (5, 4096), (2, 4097), (3, 8192), (2, 8193), (2, 11111), (3, 16384),
-         (9001, 65), (2500, 1030)]
+         (9001, 65), (2500, 1030), (70000, 520)]
 
 
 def tensors(T, H, seed, *dtypes, std=1.0):
