@@ -9,8 +9,9 @@
 // So an expert is first a 32-bit key, its score in 22 bits and its index behind it (the
 // order of equal ones), which is sorted with one minimum and one maximum an exchange. Only where two neighbours in that
 // order that the choice hangs on are nearer than the key's error, and not the same score by the same
-// operands, the token is done again in 64 bits, by the whole wave. Keys of bf16 logits hold all of them and are never
-// done again.
+// operands, the few experts (or groups) drawn are put in order by their scores in 64 bits; and only where that does not
+// settle it, or the scores are a softmax's, the token is done again in 64 bits, by the whole wave: 6 us of one wave's
+// time, however few the tokens. Keys of bf16 logits hold all of them and are never done again.
 #pragma once
 #include <type_traits>
 
@@ -146,6 +147,34 @@ __device__ __forceinline__ double sum64(double v) {
 }
 __device__ __forceinline__ float max64(float v) { return nkbal::reduce<64, true>(v); }
 
+// A 64-bit score's place in the order of scores; a NaN ranks as -inf.
+__device__ __forceinline__ uint64_t order(double c) {
+  const uint64_t u = (uint64_t)__double_as_longlong((c == c ? c : -__builtin_inf()) + 0.0);
+  return u ^ ((uint64_t)((int64_t)u >> 63) | 1ull << 63);
+}
+template <uint32_t N>
+__device__ __forceinline__ uint64_t turned(uint64_t v) {
+  return (uint64_t)turned<N>((uint32_t)(v >> 32)) << 32 | turned<N>((uint32_t)v);
+}
+// An expert's score in 64 bits (of a softmax by its logits).
+template <typename X>
+__device__ __forceinline__ uint64_t exact_score(const Select& a, const X* row, uint32_t e) {
+  float z;
+  if constexpr (sizeof(X) == 4) z = row[e];
+  else z = nk::bf16_f32(row[e]);
+  double c = (double)z;
+  if (!a.by_logits) {
+    c = 1.0 / (1.0 + exp(-c));
+    if (a.bias) c += (double)a.bias[e];
+  }
+  return order(c);
+}
+// The sum of two of them, as a place in the order again.
+__device__ __forceinline__ double score_of(uint64_t key) {
+  const uint64_t u = key >> 63 ? key & ~(1ull << 63) : ~key;
+  return __longlong_as_double((long long)u);
+}
+
 // One token by a wave, its scores in 64 bits. s: 64 NV values.
 template <typename X, uint32_t NV>
 __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double* s) {
@@ -226,8 +255,7 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
   uint64_t key[NV];
 #pragma unroll
   for (uint32_t j = 0; j < NV; ++j) {
-    const uint64_t u = (uint64_t)__double_as_longlong(c[j] + 0.0);
-    key[j] = taken >> j & 1u ? 0u : u ^ ((uint64_t)((int64_t)u >> 63) | 1ull << 63);
+    key[j] = taken >> j & 1u ? 0u : order(c[j]);
   }
   uint32_t id = 0u;
   for (uint32_t n = 0; n < a.k; ++n) {
@@ -350,6 +378,8 @@ __device__ __forceinline__ void select(const Select& a) {
   nkbal::Rows<X, NV> raw;
   nkbal::load_rows<X, G, NV>(a.z, a.z_stride, t0, rows, E, raw);
   const bool live = !a.mask || a.mask[t];
+  const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
+  const bool exact_near = K == kDistance || a.scoring == kSigmoid;  // (a softmax's sum in 64 bits takes the whole row)
   uint32_t key[NV];
   float top = 0.0f, total = 0.0f;
   {
@@ -445,11 +475,31 @@ __device__ __forceinline__ void select(const Select& a) {
     each_turn([&](auto n) __attribute__((always_inline)) {
       before += turned<decltype(n)::value>(score) > score ? 1u : 0u;
     });
-    const bool keep = before < a.top_groups;
+    bool keep = before < a.top_groups;
     if constexpr (K != kWhole) {
       const uint32_t least = across<16, false>(keep ? score : ~0u) >> shift;
       const uint32_t most = across<16, true>(keep ? 0u : score) >> shift;
       again = least - most <= (a.top2 ? 2u * near : near);
+      // Groups too near: their best experts' scores in 64 bits, if it is certain which experts those are.
+      if (exact_near && __ballot(again && live)) {
+        uint32_t v[3] = {0u, 0u, 0u};
+        if (i < a.groups)
+          for (uint32_t m = 0; m < a.each; ++m) {
+            const uint32_t x = s[i * a.each + m];
+            v[2] = max(v[2], min(v[1], x));
+            v[1] = max(v[1], min(v[0], x));
+            v[0] = max(v[0], x);
+          }
+        const uint32_t of = a.top2 ? 1u : 0u;
+        const bool certain = i >= a.groups || v[of + 1u] == 0u || (v[of] >> 10) - (v[of + 1u] >> 10) > near;
+        uint64_t exact = 0u;
+        if (i < a.groups) {
+          exact = exact_score(a, row, 1023u - (v[0] & 1023u));
+          if (a.top2) exact = order(score_of(exact) + score_of(exact_score(a, row, 1023u - (v[1] & 1023u))));
+        }
+        keep = kept(exact, a.groups, a.top_groups, [](uint64_t u, auto n) __attribute__((always_inline)) { return turned<decltype(n)::value>(u); });
+        again = across<16, false>(certain ? 1u : 0u) == 0u;
+      }
     }
     // what is not kept leaves by zeros in LDS
     if (i < a.groups && !keep) {
@@ -474,11 +524,10 @@ __device__ __forceinline__ void select(const Select& a) {
   sort<0u, NV>(key);
   // two more than k, to see whether the k-th and the next one are apart
   const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
-  uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws) : draw<G, 16u>(key, draws);
-  const uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
+  const uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws) : draw<G, 16u>(key, draws);
+  uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
   if constexpr (K != kWhole) {
     // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
-    const X* row = static_cast<const X*>(a.z) + (uint64_t)t * a.z_stride;
     uint32_t zb, bb = 0u;
     if constexpr (sizeof(X) == 4) zb = __float_as_uint(row[id]);
     else zb = row[id];
@@ -490,6 +539,28 @@ __device__ __forceinline__ void select(const Select& a) {
     bool bad = i < a.k && close && !same;
     if (i + 1u == a.k) bad = close && (!same || a.k + 2u > kMost || next_close);
     if (a.k == kMost && i + 1u == a.k) bad = true;  // no lane holds the next one
+    // Choices too near: the order of those drawn by their scores in 64 bits, if what was not drawn is certainly behind
+    // the k-th then.
+    if (exact_near && __ballot(bad && live)) {
+      const bool drawn = i < draws && mine != 0u;
+      const uint64_t exact = drawn ? exact_score(a, row, id) : 0u;
+      uint32_t before = 0u;
+      each_turn([&](auto n) __attribute__((always_inline)) {
+        const uint64_t other = turned<decltype(n)::value>(exact);
+        const uint32_t other_id = turned<decltype(n)::value>(id);
+        before += other > exact || (other == exact && other_id < id) ? 1u : 0u;
+      });
+      const bool chosen = drawn && before < a.k;
+      const uint32_t least = across<16, false>(chosen ? mine >> 10 : ~0u);
+      const uint32_t last = across<16, false>(i < draws ? mine >> 10 : ~0u);  // 0: there are no others
+      bad = last != 0u && least - last <= near;
+      const uint32_t place = drawn ? before : ~0u, old = id;
+      id = place == i ? old : 0u;
+      each_turn([&](auto n) __attribute__((always_inline)) {
+        const uint32_t other_place = turned<decltype(n)::value>(place), other_id = turned<decltype(n)::value>(old);
+        id = other_place == i ? other_id : id;
+      });
+    }
     again |= bad;
     uint64_t todo = __ballot(again && live && lane / G < rows);
     const bool done = G == 64u ? todo == 0u : (todo >> (lane & 48u) & 0xffffu) == 0u;
