@@ -70,6 +70,13 @@ int netra_linear_forward(const void* x, uint32_t x_type, uint64_t x_stride, cons
                          const float* scale, uint16_t* y, uint64_t y_stride, uint32_t rows, uint32_t n,
                          uint32_t k, void* workspace, uint64_t workspace_bytes, hipStream_t stream);
 
+// The same for rows that are quantised already: codes and scales as netra_norm_forward leaves them with
+// NETRA_CODES_TILES.
+uint64_t netra_linear_forward_codes_workspace(uint32_t rows, uint32_t n, uint32_t k);
+int netra_linear_forward_codes(const uint8_t* codes, const float* scales, const uint8_t* packed, const float* scale,
+                               uint16_t* y, uint64_t y_stride, uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                               uint64_t workspace_bytes, hipStream_t stream);
+
 // dy [rows, n] -> dx bf16 [rows, k]; packed_t from netra_linear_pack(transpose = 1),
 // scale the same grid as forward's.
 int netra_linear_input_gradient(const void* dy, uint32_t dy_type, uint64_t dy_stride, const uint8_t* packed_t,

@@ -83,6 +83,12 @@ inline ProductPlan product_plan(uint32_t rows, uint32_t ni, uint32_t nc, bool bf
   return {kStream, wide, 4, 1, 0};
 }
 
+// The same for rows that are quantised already: nothing to do on the way.
+inline ProductPlan codes_plan(uint32_t rows, uint32_t ni, uint32_t nc) {
+  if (rows > 64u) return product_tiles(rows, ni, nc);
+  return {kStream, (ni + 15u) / 16u >= 512u ? 2u : 1u, 4, 1, 0};
+}
+
 // Tile and split of the weight gradient, chosen as product_tiles' (steps of 64 tokens: 256x256
 // 1.55 us, 128x256 0.93, 128x128 0.48, one workgroup per CU each). As whole calls, best and
 // next: T 333, N 1024, K 2048 128x128 8.3 us, 128x256 11.8; T 4096, N 4096, K 2048 128x256 64,

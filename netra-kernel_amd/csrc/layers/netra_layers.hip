@@ -230,6 +230,43 @@ extern "C" int netra_linear_input_gradient(const void* dy, uint32_t dy_type, uin
                        workspace, workspace_bytes, stream);
 }
 
+// Rows that come quantised (netra_norm_forward with NETRA_CODES_TILES).
+extern "C" uint64_t netra_linear_forward_codes_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  if (rows == 0) return 0;
+  const ProductPlan plan = codes_plan(rows, n, k);
+  return plan.splits > 1u ? 4u * static_cast<uint64_t>(plan.splits) * rows * up(n, 4u) : 0u;
+}
+extern "C" int netra_linear_forward_codes(const uint8_t* codes, const float* scales, const uint8_t* packed,
+                                          const float* scale, uint16_t* y, uint64_t y_stride, uint32_t rows, uint32_t n,
+                                          uint32_t k, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  const char* name = "netra_linear_forward_codes";
+  if (bad_sizes(rows, n, k)) return fail(-1, name, "sizes have to be 1 .. 2^21 (rows may be 0)");
+  if (rows == 0) {
+    g_error.clear();
+    return 0;
+  }
+  if (!codes || !aligned(codes, 16) || !scales || !aligned(scales, 4) || !packed || !aligned(packed, 16) || !scale ||
+      !aligned(scale, 4) || bad_matrix(y, NETRA_BF16, y_stride, n))
+    return fail(-1, name, "null or misaligned pointer, or row stride below the row");
+  const uint64_t bytes = code_bytes(rows, k), scale_bytes = 4ull * up(rows, 16u) * blocks(k);
+  const Span out{y, y_stride * 2u, static_cast<uint64_t>(n) * 2u, rows};
+  if (share(out, {codes, bytes, bytes, 1}) || share(out, {scales, scale_bytes, scale_bytes, 1}))
+    return fail(-1, name, "the output shares memory with the codes or their scales");
+  if (bad_workspace(workspace, workspace_bytes, netra_linear_forward_codes_workspace(rows, n, k)))
+    return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  const ProductCall c{name, codes, NETRA_BF16, k, packed, scale, blocks(k), 1u, y, y_stride, rows, n, k};
+  const ProductPlan plan = codes_plan(rows, n, k);
+  if (check_grid(c, plan) != 0) return -1;
+  nklin::Product a{};
+  set_up(c, plan, static_cast<uint8_t*>(workspace), a);
+  a.q = codes;
+  a.sq = scales;
+  a.partial = static_cast<float*>(workspace);
+  Launcher launch(stream);
+  run(c, a, plan, launch);
+  return launch.result(name);
+}
+
 // One call of the weight gradient.
 struct OuterCall {
   const char* name;

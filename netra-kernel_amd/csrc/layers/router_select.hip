@@ -685,10 +685,11 @@ __device__ __forceinline__ void gradient(const SelectGradient& a) {
       if (a.scoring == kSigmoid) v *= slope(z);
       if (!chosen) v = 0.0f;
       mine = v;
-      each_turn([&](auto n) __attribute__((always_inline)) {
-        const float ov = turned<decltype(n)::value>(v);
-        mine += turned<decltype(n)::value>(id) == id && chosen ? ov : 0.0f;
-      });
+      if (__ballot(chosen && !first))  // an expert in several slots
+        each_turn([&](auto n) __attribute__((always_inline)) {
+          const float ov = turned<decltype(n)::value>(v);
+          mine += turned<decltype(n)::value>(id) == id && chosen ? ov : 0.0f;
+        });
     }
     if (first) s[id] = mine;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -19,6 +19,8 @@ SIGNATURES = {
     "netra_linear_input_gradient_workspace": (U64, [U32] * 4),
     "netra_linear_weight_gradient_workspace": (U64, [U32] * 4),
     "netra_linear_forward": (ctypes.c_int, [P, U32, U64, P, P, P, U64, U32, U32, U32, P, U64, P]),
+    "netra_linear_forward_codes_workspace": (U64, [U32] * 3),
+    "netra_linear_forward_codes": (ctypes.c_int, [P, P, P, P, P, U64, U32, U32, U32, P, U64, P]),
     "netra_linear_input_gradient": (ctypes.c_int, [P, U32, U64, P, P, P, U64, U32, U32, U32, P, U64, P]),
     "netra_linear_weight_gradient": (ctypes.c_int, [P, U32, U64, P, U32, U64, P, U32, U32, U32, U32, P, U64, P]),
     "netra_linear_backward_workspace": (U64, [U32] * 5),

@@ -119,6 +119,25 @@ class BlockLinear:
 
     __call__ = forward
 
+    def forward_codes(self, codes: torch.Tensor, scale: torch.Tensor, rows: int, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The same for `rows` rows that rms_norm has quantised (codes="tiles"): bf16 [rows, N]."""
+        blocks, padded = -(-self.K // 128), -(-rows // 16) * 16
+        for name, t, dtype, shape in (("codes", codes, torch.uint8, (padded * blocks * 128,)),
+                                      ("scale", scale, torch.float32, (blocks, padded))):
+            if t.shape != shape or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"{name}: need contiguous {dtype} {shape} on {self.device} for {rows} rows of {self.K}, got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if out is None:
+            out, out_stride = torch.empty((rows, self.N), dtype=torch.bfloat16, device=self.device), self.N
+        else:
+            out_stride = check_rows("out", out, (rows, self.N), self.device, (torch.bfloat16,))
+        which = "netra_linear_forward_codes"
+        need = entry(which + "_workspace")(rows, self.N, self.K)
+        ws, ws_ptr = workspace(need, self.device)
+        launch(entry(which), which, self.device, codes.data_ptr(), scale.data_ptr(), self.packed.data_ptr(), self._scale_ptr,
+               out.data_ptr(), out_stride, rows, self.N, self.K, ws_ptr, need)
+        return out
+
     def input_gradient(self, dy: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """dy bf16 or fp32 [T, N] -> dy W, bf16 [T, K]."""
         if self.packed_t is None:

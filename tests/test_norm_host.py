@@ -90,3 +90,15 @@ def test_untile_inverts_the_layout():
             codes[((row // 16) * 3 + b) * 2048 + (i % 32) // 16 * 1024 + ((row % 16) + 16 * (i // 32)) * 16 + i % 16] = want[row, c]
     got, _ = N.untile(codes, torch.zeros(3, 48), rows, cols)
     assert torch.equal(got, want.view(torch.float8_e4m3fn).double()[:rows, :cols])
+
+
+@pytest.mark.parametrize("change", [dict(c=0), dict(c=A + 8), dict(s=0), dict(s=B + 2), dict(p=0), dict(p=D + 8), dict(w=0), dict(w=E + 2),
+                                    dict(y=0), dict(y=5 * A + 1), dict(ys=127), dict(n=0), dict(k=0), dict(rows=(1 << 21) + 1), dict(y=A), dict(y=B),
+                                    dict(k=8192, ws=0), dict(k=8192, ws=6 * A + 4), dict(k=8192, short=1)])
+def test_codes_product_refusals(change):
+    a = dict(c=A, s=B, p=D, w=E, y=5 * A, ys=128, rows=300, n=128, k=256, ws=6 * A, short=0)
+    a.update(change)
+    need = layers.library().netra_linear_forward_codes_workspace(300, 128, a["k"])
+    assert bool(need) == (a["k"] == 8192)
+    refused("netra_linear_forward_codes", a["c"], a["s"], a["p"], a["w"], a["y"], a["ys"], a["rows"], a["n"], a["k"], a["ws"],
+            need - a["short"], None)
