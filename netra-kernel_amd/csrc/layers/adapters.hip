@@ -196,16 +196,42 @@ __device__ __forceinline__ Part<X> part_whole(const X* row, uint32_t c) {
   for (uint32_t h = 0; h < sizeof(X) / 2u; ++h) v.w[h] = *reinterpret_cast<const Unaligned16*>(row + c + 4u * h);
   return v;
 }
+// The same with zeros from column n on, of which nothing is read: the row's last eight, moved down. (Value by value, the
+// lanes at a row's end hold up their whole wave for eight loads.)
 template <typename X>
-__device__ __forceinline__ Part<X> part_to(const X* row, uint32_t c, uint32_t n) {  // zeros from column n on
-  if (c + 8u <= n) return part_whole(row, c);
+__device__ __forceinline__ Part<X> part_to(const X* row, uint32_t c, uint32_t n) {
   Part<X> v = {};
+  if (n < 8u) {
 #pragma unroll
-  for (uint32_t i = 0; i < 8u; ++i)
-    if (c + i < n) {
-      if constexpr (sizeof(X) == 4) v.w[i / 4u].w[i & 3u] = __float_as_uint(row[c + i]);
-      else v.w[0].w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i & 1u));
-    }
+    for (uint32_t i = 0; i < 7u; ++i)
+      if (c + i < n) {
+        if constexpr (sizeof(X) == 4) v.w[i / 4u].w[i & 3u] = __float_as_uint(row[c + i]);
+        else v.w[0].w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i & 1u));
+      }
+    return v;
+  }
+  const uint32_t at = min(c, n - 8u), by = min(c - at, 8u);
+  v = part_whole(row, at);
+  if constexpr (sizeof(X) == 4) {
+    uint32_t w[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) w[i] = v.w[i / 4u].w[i & 3u];
+#pragma unroll
+    for (uint32_t d = 1; d < 8u; d *= 2u)
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) w[i] = by & d ? (i + d < 8u ? w[i + d] : 0u) : w[i];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) v.w[i / 4u].w[i & 3u] = by < 8u ? w[i] : 0u;
+  } else {
+    const uint64_t lo = (uint64_t)v.w[0].w[1] << 32 | v.w[0].w[0], hi = (uint64_t)v.w[0].w[3] << 32 | v.w[0].w[2];
+    const uint32_t bits = 16u * (by & 3u);
+    const uint64_t up = hi >> bits, down = lo >> bits | (bits ? hi << (64u - bits) : 0u);
+    const uint64_t first = by < 4u ? down : by < 8u ? up : 0u, second = by < 4u ? up : 0u;
+    v.w[0].w[0] = (uint32_t)first;
+    v.w[0].w[1] = (uint32_t)(first >> 32);
+    v.w[0].w[2] = (uint32_t)second;
+    v.w[0].w[3] = (uint32_t)(second >> 32);
+  }
   return v;
 }
 template <typename X>
@@ -455,14 +481,14 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   constexpr uint32_t kParts = NR >= 4u ? 2u : 1u, kPart = 2u * NR / kParts;
   u32x4 b[kParts][kPart];
   Unaligned16 y0[kLoads], y1[kLoads];
-  const bool whole = tile.z == H * TT * 16u && a.n % 256u == 0u;
+  auto whole = [&](uint32_t g) __attribute__((always_inline)) { return (g + 1u) * 256u <= a.n; };
   auto load_b = [&](uint32_t g, uint32_t part) __attribute__((always_inline)) {
     const uint32_t s = min(g * 4u + wave % 4u, nb - 1u);
 #pragma unroll
     for (uint32_t i = 0; i < kPart; ++i) b[part][i] = b_at[(uint64_t)s * (NR * 128u) + (part * kPart + i) * 64u];
   };
   auto load_y = [&](uint32_t g, Unaligned16 (&y)[kLoads]) __attribute__((always_inline)) {
-    if (whole) {
+    if (whole(g)) {
 #pragma unroll
       for (uint32_t i = 0; i < kLoads; ++i) y[i] = *reinterpret_cast<const Unaligned16*>(from[i] + g * 256u + c);
     } else {
@@ -525,8 +551,9 @@ __device__ __forceinline__ void expand(const Adapters& a) {
 #pragma unroll
       for (uint32_t e = 0; e < 4u; ++e)
         y[i].w[e] = nk::bf16x2_hw(nk::bf16_lo(y[i].w[e]) + f[2u * e], nk::bf16_hi(y[i].w[e]) + f[2u * e + 1u]);
-      if (whole) *reinterpret_cast<Unaligned16*>(to[i] + at_g * 256u + c) = y[i];
-      else if (there[i]) store8(to[i], at_g * 256u + c, a.n, y[i]);
+      if (!there[i]) continue;
+      if (whole(at_g)) *reinterpret_cast<Unaligned16*>(to[i] + at_g * 256u + c) = y[i];
+      else store8(to[i], at_g * 256u + c, a.n, y[i]);
     }
     nklds::barrier();
   };

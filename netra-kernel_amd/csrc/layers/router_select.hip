@@ -465,7 +465,13 @@ __device__ __forceinline__ void select(const Select& a) {
           take(v.w);
         }
       } else {
-        for (uint32_t m = 0; m < a.each; ++m) take(from[m]);
+        for (uint32_t m = 0; m < a.each; m += 8u) {
+          uint32_t v[8];
+#pragma unroll
+          for (uint32_t n = 0; n < 8u; ++n) v[n] = from[min(m + n, a.each - 1u)];
+#pragma unroll
+          for (uint32_t n = 0; n < 8u; ++n) take(m + n < a.each ? v[n] : 0u);
+        }
       }
     }
     // (the best expert's key orders the groups itself, as lower groups have lower experts)
