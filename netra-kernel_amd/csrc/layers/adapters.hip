@@ -360,16 +360,12 @@ __device__ __forceinline__ v4f joined(const v4f (&part)[8][N][64], uint32_t i) {
   return v;
 }
 
-// u of the H-th part of a tile, of NR of its 16-rank parts (the workgroup's place in z), of one split.
-template <typename X, uint32_t TT, uint32_t H, uint32_t NR>
+// u of a tile, of NR of its 16-rank parts (the workgroup's place in z), of one split.
+template <typename X, uint32_t TT, uint32_t NR>
 __device__ __forceinline__ void shrink(const Adapters& a) {
   __shared__ v4f part[8][TT * NR][64];
   uint4 tile;
-  if (!tile_of(a, blockIdx.x / H, tile) || tile.x >= a.adapters) return;
-  const uint32_t before = blockIdx.x % H * (TT * 16u);  // this workgroup's part of the tile
-  if (before >= tile.z) return;
-  tile.y += before;
-  tile.z = min(tile.z - before, TT * 16u);
+  if (!tile_of(a, blockIdx.x, tile) || tile.x >= a.adapters) return;
   const uint32_t split_at = blockIdx.y, r0 = blockIdx.z * NR;
   first_product<X, TT, NR>(a, tile, split_at, r0, part);
   for (uint32_t i = threadIdx.x; i < TT * NR * 64u; i += 512u) {
@@ -399,15 +395,14 @@ __device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, co
     if (c + i < n) row[c + i] = (uint16_t)(v.w[i / 2u] >> (16u * (i & 1u)));
 }
 
-// out of a tile of H times TT times 16 tokens. The waves of a workgroup multiply 64 of 256 columns by TT times 16
-// tokens each and hand the sums over through LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together: as the
+// out of a tile of TT times 16 tokens. The four waves of a workgroup multiply 64 of 256 columns each and hand the sums over through LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together: as the
 // matrix core leaves them a lane has four columns, and rows of 64 bytes stored so took 60% of a copy's rate. `wide` times; the next
 // columns' y and B are under way during a turn.
-template <uint32_t TT, uint32_t H, uint32_t NR>
+template <uint32_t TT, uint32_t NR>
 __device__ __forceinline__ void expand(const Adapters& a) {
   constexpr uint32_t kPitch = 260u;  // spreads 16 tokens' rows over the banks
   constexpr uint32_t kRows = 4u * TT, kLoads = kRows / 2u;  // rows of a wave; loads of a lane: two rows at a time
-  __shared__ float sums[H * TT * 16u][kPitch];
+  __shared__ float sums[TT * 16u][kPitch];
   uint4 tile;
   const uint32_t at_tile = blockIdx.x / a.chunks, chunk = blockIdx.x - at_tile * a.chunks;
   if (!tile_of(a, at_tile, tile)) return;
@@ -415,7 +410,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   if (none && a.in_place) return;
   const uint32_t lane = threadIdx.x & 63u, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t nb = (a.n + 63u) / 64u, first = wave / 4u * (TT * 16u);  // the wave's first token
+  const uint32_t nb = (a.n + 63u) / 64u;
   const uint32_t g0 = chunk * a.wide, g1 = min((a.n + 255u) / 256u, g0 + a.wide);  // groups of 256 columns
   // the wave's rows: lanes 0 .. 31 and 32 .. 63 have one each of every load's two
   const uint16_t* from[kLoads];
@@ -442,7 +437,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   bf16x8 u[TT][kOperands];
 #pragma unroll
   for (uint32_t t = 0; t < TT; ++t) {
-    const uint32_t at = tile.y + min(first + t * 16u + (lane & 15u), tile.z - 1u);
+    const uint32_t at = tile.y + min(t * 16u + (lane & 15u), tile.z - 1u);
     u32x2 hi[NR], lo[NR];  // of four ranks from rank(i) on
     auto rank = [&](uint32_t i) __attribute__((always_inline)) { return NR == 1u ? q * 4u : i / 2u * 32u + q * 8u + (i & 1u) * 4u; };
     if (a.splits == 1u) {
@@ -483,7 +478,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   Unaligned16 y0[kLoads], y1[kLoads];
   auto whole = [&](uint32_t g) __attribute__((always_inline)) { return (g + 1u) * 256u <= a.n; };
   auto load_b = [&](uint32_t g, uint32_t part) __attribute__((always_inline)) {
-    const uint32_t s = min(g * 4u + wave % 4u, nb - 1u);
+    const uint32_t s = min(g * 4u + wave, nb - 1u);
 #pragma unroll
     for (uint32_t i = 0; i < kPart; ++i) b[part][i] = b_at[(uint64_t)s * (NR * 128u) + (part * kPart + i) * 64u];
   };
@@ -541,7 +536,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
     for (uint32_t t = 0; t < TT; ++t)
 #pragma unroll
       for (uint32_t j = 0; j < 4u; ++j)
-        *reinterpret_cast<v4f*>(&sums[first + t * 16u + (lane & 15u)][wave % 4u * 64u + j * 16u + q * 4u]) = acc[t][j];
+        *reinterpret_cast<v4f*>(&sums[t * 16u + (lane & 15u)][wave * 64u + j * 16u + q * 4u]) = acc[t][j];
     nklds::barrier();
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; ++i) {
@@ -671,27 +666,20 @@ extern "C" __global__ __launch_bounds__(1024) void netra_adapters_plan_gfx950(co
   }
 NETRA_ADAPTERS_PACK(bf16, uint16_t)
 NETRA_ADAPTERS_PACK(f32, float)
-// t: 16-token parts of a wave's part of a tile, h: waves' parts of a tile, r: 16-rank parts
-#define NETRA_SHRINK(TT, H, NR)                                                                                 \
-  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_bf16_t##TT##h##H##r##NR##_gfx950(     \
+// t: 16-token parts of a tile, r: 16-rank parts
+#define NETRA_SHRINK(TT, NR)                                                                                    \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_bf16_t##TT##r##NR##_gfx950(           \
       nkada::Adapters a) {                                                                                      \
-    nkada::shrink<uint16_t, TT, H, NR>(a);                                                                      \
+    nkada::shrink<uint16_t, TT, NR>(a);                                                                         \
   }                                                                                                             \
-  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_f32_t##TT##h##H##r##NR##_gfx950(      \
+  extern "C" __global__ __launch_bounds__(512) void netra_adapters_shrink_f32_t##TT##r##NR##_gfx950(            \
       nkada::Adapters a) {                                                                                      \
-    nkada::shrink<float, TT, H, NR>(a);                                                                         \
+    nkada::shrink<float, TT, NR>(a);                                                                            \
   }
-#define NETRA_EXPAND(TT, H, NR)                                                                                 \
-  extern "C" __global__ __launch_bounds__(256 * H) void netra_adapters_expand_t##TT##h##H##r##NR##_gfx950(      \
-      nkada::Adapters a) {                                                                                      \
-    nkada::expand<TT, H, NR>(a);                                                                                \
+#define NETRA_EXPAND(TT, NR)                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void netra_adapters_expand_t##TT##r##NR##_gfx950(nkada::Adapters a) { \
+    nkada::expand<TT, NR>(a);                                                                                   \
   }
-NETRA_SHRINK(1, 1, 1)
-NETRA_SHRINK(1, 1, 2)
-NETRA_SHRINK(1, 1, 4)
-NETRA_SHRINK(2, 2, 1)
-NETRA_SHRINK(2, 2, 2)
-NETRA_SHRINK(2, 2, 4)
 #define NETRA_FUSED(NR)                                                                                         \
   extern "C" __global__ __launch_bounds__(512) void netra_adapters_fused_bf16_r##NR##_gfx950(nkada::Adapters a) { \
     nkada::fused<uint16_t, NR>(a);                                                                              \
@@ -699,15 +687,21 @@ NETRA_SHRINK(2, 2, 4)
   extern "C" __global__ __launch_bounds__(512) void netra_adapters_fused_f32_r##NR##_gfx950(nkada::Adapters a) { \
     nkada::fused<float, NR>(a);                                                                                 \
   }
+NETRA_SHRINK(1, 1)
+NETRA_SHRINK(1, 2)
+NETRA_SHRINK(1, 4)
+NETRA_SHRINK(2, 1)
+NETRA_SHRINK(2, 2)
+NETRA_SHRINK(2, 4)
+NETRA_EXPAND(1, 1)
+NETRA_EXPAND(1, 2)
+NETRA_EXPAND(1, 4)
+NETRA_EXPAND(1, 8)
+NETRA_EXPAND(2, 1)
+NETRA_EXPAND(2, 2)
+NETRA_EXPAND(2, 4)
+NETRA_EXPAND(2, 8)
 NETRA_FUSED(1)
 NETRA_FUSED(2)
 NETRA_FUSED(4)
 NETRA_FUSED(8)
-NETRA_EXPAND(1, 1, 1)
-NETRA_EXPAND(1, 1, 2)
-NETRA_EXPAND(1, 1, 4)
-NETRA_EXPAND(1, 1, 8)
-NETRA_EXPAND(2, 2, 1)
-NETRA_EXPAND(2, 2, 2)
-NETRA_EXPAND(2, 2, 4)
-NETRA_EXPAND(2, 2, 8)

@@ -146,24 +146,23 @@ extern "C" int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_str
     }
     return launch.result(name);
   }
-  const uint32_t parts = adapter_tile(tokens, adapters) == 16u ? 1u : 2u;  // of a tile
-  const dim3 shrink(p.tiles * parts, p.splits, a.ranks == 8u ? 2u : 1u), expand(static_cast<uint32_t>(groups));
-// (a rank over 64 in two parts of the first product: of one the operands do not fit the registers)
-#define NETRA_RUN(TT, H, NR, EXPAND_NR)                                                                   \
-  do {                                                                                                    \
-    if (x_type == NETRA_BF16) launch(netra_adapters_shrink_bf16_t##TT##h##H##r##NR##_gfx950, shrink, dim3(512), a); \
-    else launch(netra_adapters_shrink_f32_t##TT##h##H##r##NR##_gfx950, shrink, dim3(512), a);             \
-    launch(netra_adapters_expand_t##TT##h##H##r##EXPAND_NR##_gfx950, expand, dim3(256 * H), a);           \
+  // (a rank over 64 in two parts of the first product: of one the operands do not fit the registers)
+  const dim3 shrink(p.tiles, p.splits, a.ranks == 8u ? 2u : 1u), expand(static_cast<uint32_t>(groups));
+#define NETRA_RUN(TT, NR, EXPAND_NR)                                                                        \
+  do {                                                                                                      \
+    if (x_type == NETRA_BF16) launch(netra_adapters_shrink_bf16_t##TT##r##NR##_gfx950, shrink, dim3(512), a); \
+    else launch(netra_adapters_shrink_f32_t##TT##r##NR##_gfx950, shrink, dim3(512), a);                     \
+    launch(netra_adapters_expand_t##TT##r##EXPAND_NR##_gfx950, expand, dim3(256), a);                       \
   } while (0)
-#define NETRA_RANKS(TT, H)                     \
-  if (a.ranks == 1u) NETRA_RUN(TT, H, 1, 1);   \
-  else if (a.ranks == 2u) NETRA_RUN(TT, H, 2, 2); \
-  else if (a.ranks == 4u) NETRA_RUN(TT, H, 4, 4); \
-  else NETRA_RUN(TT, H, 4, 8)
-  if (parts == 1u) {
-    NETRA_RANKS(1, 1);
+#define NETRA_RANKS(TT)                        \
+  if (a.ranks == 1u) NETRA_RUN(TT, 1, 1);      \
+  else if (a.ranks == 2u) NETRA_RUN(TT, 2, 2); \
+  else if (a.ranks == 4u) NETRA_RUN(TT, 4, 4); \
+  else NETRA_RUN(TT, 4, 8)
+  if (adapter_tile(tokens, adapters) == 16u) {
+    NETRA_RANKS(1);
   } else {
-    NETRA_RANKS(2, 2);
+    NETRA_RANKS(2);
   }
 #undef NETRA_RANKS
 #undef NETRA_RUN

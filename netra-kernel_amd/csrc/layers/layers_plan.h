@@ -214,8 +214,12 @@ inline uint32_t select_groups(uint32_t tokens, uint32_t at_once) {
 // short one for each adapter in use and for the tokens without); splits of k's 128-blocks where the tiles are few, and
 // groups of 256 columns that a workgroup of the second product takes.
 inline uint32_t adapter_ranks(uint32_t rank) { return rank <= 16u ? 1u : rank <= 32u ? 2u : rank <= 64u ? 4u : 8u; }
+// (Tiles of 32 share what is read of A and B and fill fewer CUs: us, of 16 / of 32,
+//   K 4096   T 4096, N 4096, rank 64  40 / 48    T 8192, N 8192, rank 16  79 / 85, 64  111 / 104, 128  152 / 132
+//   K 3008   T 3333, N 5440, rank 48  36 / 45    T 8192, N 4096, 60 adapters of rank 64  110 / 90
+// The plan does not know the rank.)
 inline uint32_t adapter_tile(uint32_t tokens, uint32_t adapters) {
-  return tokens > 1024u && tokens / 64u >= adapters ? 64u : 16u;
+  return tokens >= 8192u && tokens / 64u >= adapters ? 32u : 16u;
 }
 inline uint32_t adapter_tiles(uint32_t tokens, uint32_t adapters) {
   const uint32_t tile = adapter_tile(tokens, adapters), parts = adapters + 1u;
@@ -242,8 +246,7 @@ inline AdapterPlan adapter_plan(uint32_t tokens, uint32_t adapters, uint32_t ran
   // a workgroup reads and packs its tile's u before its first columns: up to eight groups share that
   const uint64_t groups = static_cast<uint64_t>(p.tiles) * ((n + 255u) / 256u);
   while (p.wide < 8u && groups / (2u * p.wide) >= 1024u) p.wide *= 2u;
-  const uint32_t parts = p.tiles * (adapter_tile(tokens, adapters) == 16u ? 1u : 2u);
-  while (p.splits < 16u && parts * p.splits * 2u <= 512u && blocks(k) / (p.splits * 2u) >= 8u) p.splits *= 2u;
+  while (p.splits < 16u && p.tiles * p.splits * 2u <= 512u && blocks(k) / (p.splits * 2u) >= 8u) p.splits *= 2u;
   p.split_blocks = (blocks(k) + p.splits - 1u) / p.splits;
   p.splits = (blocks(k) + p.split_blocks - 1u) / p.split_blocks;
   return p;

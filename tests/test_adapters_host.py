@@ -54,8 +54,8 @@ def test_sizes_and_no_tokens():
 def test_most_tiles_of_a_batch():
     """The plan holds the most tiles that any split of the tokens over the adapters (and none) gives."""
     lib = layers.library()
-    for T, L in [(1, 1), (2, 5), (40, 3), (63, 64), (1025, 8), (2000, 50), (2000, 63)]:
-        tile = 64 if T > 1024 and T // 64 >= L else 16
+    for T, L in [(1, 1), (2, 5), (40, 3), (63, 64), (1025, 8), (2000, 50), (2000, 63), (8192, 8), (8200, 128), (8200, 129)]:
+        tile = 32 if T >= 8192 and T // 64 >= L else 16
         parts = min(L + 1, T)
         most = parts + (T - parts) // tile  # one token each, the rest in one
         assert lib.netra_adapters_plan_bytes(T, L) >= 16 + 4 * T + 16 * most

@@ -31,7 +31,7 @@ SIZES = [(1, 1, 1, 1, 1, 1), (1, 4, 8, 2048, 2048, 1), (2, 2, 16, 64, 64, 1), (3
          (17, 1, 16, 129, 65, 17), (64, 32, 16, 512, 500, 1), (50, 7, 33, 1111, 130, 9), (203, 3, 12, 257, 300, 41),
          (100, 1000, 6, 96, 80, 1), (300, 2, 128, 333, 777, 150), (1025, 4, 64, 200, 129, 100), (2000, 9, 100, 130, 257, 33),
          (1500, 1, 32, 64, 2050, 1500), (40, 3, 20, 8192, 40, 5), (7, 2, 50, 130, 600, 1), (33, 3, 100, 300, 1030, 4), (5, 2, 128, 512, 512, 1),
-         (600, 3, 40, 640, 520, 7), (1100, 2, 90, 1030, 1500, 13), (5000, 1024, 5, 40, 33, 2)]
+         (600, 3, 40, 640, 520, 7), (1100, 2, 90, 1030, 1500, 13), (5000, 1024, 5, 40, 33, 2), (8200, 3, 100, 330, 300, 700), (8192, 9, 24, 130, 600, 11), (9000, 2, 64, 256, 129, 1), (8500, 120, 16, 70, 512, 5)]
 
 
 @pytest.mark.parametrize("T,L,r,K,N,chunk", SIZES)
@@ -55,7 +55,7 @@ def test_add(T, L, r, K, N, chunk, dtype):
     assert torch.equal(yd, got)
 
 
-@pytest.mark.parametrize("T,L", [(1, 1), (63, 3), (64, 64), (1000, 1), (1024, 1024), (1025, 32), (5000, 7), (70000, 500)])
+@pytest.mark.parametrize("T,L", [(1, 1), (63, 3), (64, 64), (1000, 1), (1024, 1024), (1025, 32), (5000, 7), (9000, 5), (70000, 500)])
 def test_plan(T, L):
     """Every token once, by adapter and within one in the batch's order, in tiles of one adapter."""
     g = torch.Generator().manual_seed(T)
@@ -65,7 +65,7 @@ def test_plan(T, L):
     of = torch.where((ids < 0) | (ids >= L), L, ids)
     assert words[:4].tolist()[1:] == [T, L, 0]
     assert torch.equal(words[4:4 + T].long(), torch.sort(of, stable=True).indices)
-    tile = 64 if T > 1024 and T // 64 >= L else 16
+    tile = 32 if T >= 8192 and T // 64 >= L else 16
     start = 4 + -(-T // 4) * 4
     want, at = [], 0
     for l, n in enumerate(torch.bincount(of, minlength=L + 1).tolist()):
