@@ -385,6 +385,16 @@ __device__ __forceinline__ void shrink(const Adapters& a) {
   }
 }
 
+// Eight columns past the caches.
+typedef uint32_t Once16 __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ Unaligned16 load_once(const uint16_t* from) {
+  const Once16 v = __builtin_nontemporal_load(reinterpret_cast<const Once16*>(from));
+  return {{v[0], v[1], v[2], v[3]}};
+}
+__device__ __forceinline__ void store_once(uint16_t* to, const Unaligned16& v) {
+  __builtin_nontemporal_store(Once16{v.w[0], v.w[1], v.w[2], v.w[3]}, reinterpret_cast<Once16*>(to));
+}
+
 __device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, const Unaligned16& v) {
   if (c + 8u <= n) {
     *reinterpret_cast<Unaligned16*>(row + c) = v;
@@ -395,10 +405,13 @@ __device__ __forceinline__ void store8(uint16_t* row, uint32_t c, uint32_t n, co
     if (c + i < n) row[c + i] = (uint16_t)(v.w[i / 2u] >> (16u * (i & 1u)));
 }
 
-// out of a tile of TT times 16 tokens. The four waves of a workgroup multiply 64 of 256 columns each and hand the sums over through LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together: as the
-// matrix core leaves them a lane has four columns, and rows of 64 bytes stored so took 60% of a copy's rate. `wide` times; the next
-// columns' y and B are under way during a turn.
-template <uint32_t TT, uint32_t NR>
+// out of a tile of TT times 16 tokens. The four waves of a workgroup multiply 64 of 256 columns each and hand the
+// sums over through LDS, from where a wave adds and stores whole rows of 256 columns, 512 bytes that lie together:
+// as the matrix core leaves them a lane has four columns, and rows of 64 bytes stored so took 60% of a copy's rate.
+// `wide` times; the next columns' y and B are under way during a turn.
+//
+// kOnce: y and out non-temporal, where they are more than the caches keep and would push B out of the L2 (adapter_once).
+template <uint32_t TT, uint32_t NR, bool kOnce>
 __device__ __forceinline__ void expand(const Adapters& a) {
   constexpr uint32_t kPitch = 260u;  // spreads 16 tokens' rows over the banks
   constexpr uint32_t kRows = 4u * TT, kLoads = kRows / 2u;  // rows of a wave; loads of a lane: two rows at a time
@@ -485,7 +498,10 @@ __device__ __forceinline__ void expand(const Adapters& a) {
   auto load_y = [&](uint32_t g, Unaligned16 (&y)[kLoads]) __attribute__((always_inline)) {
     if (whole(g)) {
 #pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) y[i] = *reinterpret_cast<const Unaligned16*>(from[i] + g * 256u + c);
+      for (uint32_t i = 0; i < kLoads; ++i) {
+        const uint16_t* at = from[i] + g * 256u + c;
+        y[i] = kOnce ? load_once(at) : *reinterpret_cast<const Unaligned16*>(at);
+      }
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < kLoads; ++i) y[i] = part_to(from[i], g * 256u + c, a.n).w[0];
@@ -547,7 +563,7 @@ __device__ __forceinline__ void expand(const Adapters& a) {
       for (uint32_t e = 0; e < 4u; ++e)
         y[i].w[e] = nk::bf16x2_hw(nk::bf16_lo(y[i].w[e]) + f[2u * e], nk::bf16_hi(y[i].w[e]) + f[2u * e + 1u]);
       if (!there[i]) continue;
-      if (whole(at_g)) *reinterpret_cast<Unaligned16*>(to[i] + at_g * 256u + c) = y[i];
+      if (kOnce && whole(at_g)) store_once(to[i] + at_g * 256u + c, y[i]);
       else store8(to[i], at_g * 256u + c, a.n, y[i]);
     }
     nklds::barrier();
@@ -678,7 +694,11 @@ NETRA_ADAPTERS_PACK(f32, float)
   }
 #define NETRA_EXPAND(TT, NR)                                                                                    \
   extern "C" __global__ __launch_bounds__(256) void netra_adapters_expand_t##TT##r##NR##_gfx950(nkada::Adapters a) { \
-    nkada::expand<TT, NR>(a);                                                                                   \
+    nkada::expand<TT, NR, false>(a);                                                                            \
+  }                                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void netra_adapters_expand_t##TT##r##NR##_once_gfx950(           \
+      nkada::Adapters a) {                                                                                      \
+    nkada::expand<TT, NR, true>(a);                                                                             \
   }
 #define NETRA_FUSED(NR)                                                                                         \
   extern "C" __global__ __launch_bounds__(512) void netra_adapters_fused_bf16_r##NR##_gfx950(nkada::Adapters a) { \

@@ -148,11 +148,13 @@ extern "C" int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_str
   }
   // (a rank over 64 in two parts of the first product: of one the operands do not fit the registers)
   const dim3 shrink(p.tiles, p.splits, a.ranks == 8u ? 2u : 1u), expand(static_cast<uint32_t>(groups));
+  const bool once = adapter_once(tokens, adapters, rank, n);
 #define NETRA_RUN(TT, NR, EXPAND_NR)                                                                        \
   do {                                                                                                      \
     if (x_type == NETRA_BF16) launch(netra_adapters_shrink_bf16_t##TT##r##NR##_gfx950, shrink, dim3(512), a); \
     else launch(netra_adapters_shrink_f32_t##TT##r##NR##_gfx950, shrink, dim3(512), a);                     \
-    launch(netra_adapters_expand_t##TT##r##EXPAND_NR##_gfx950, expand, dim3(256), a);                       \
+    if (once) launch(netra_adapters_expand_t##TT##r##EXPAND_NR##_once_gfx950, expand, dim3(256), a);        \
+    else launch(netra_adapters_expand_t##TT##r##EXPAND_NR##_gfx950, expand, dim3(256), a);                  \
   } while (0)
 #define NETRA_RANKS(TT)                        \
   if (a.ranks == 1u) NETRA_RUN(TT, 1, 1);      \

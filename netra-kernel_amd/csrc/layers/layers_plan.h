@@ -176,6 +176,7 @@ inline CountPlan balance_plan(uint32_t tokens, uint32_t experts) {
 
 // Bytes that the cache behind the L2s holds: what moves more than these finds nothing of it there.
 constexpr uint64_t kInfinityCache = 256ull << 20;
+constexpr uint64_t kL2 = 4ull << 20;  // of one of the eight XCDs
 
 // Norms: waves a row and eight columns a lane so many times, rows a workgroup takes at once, and
 // workgroups (they loop over the rows).
@@ -243,13 +244,25 @@ inline AdapterPlan adapter_plan(uint32_t tokens, uint32_t adapters, uint32_t ran
     p.split_blocks = blocks(k);
     return p;
   }
-  // a workgroup reads and packs its tile's u before its first columns: up to eight groups share that
+  // A workgroup reads and packs its tile's u before its first columns: up to eight groups of columns share that, the fewer
+  // the less there is of u, as more workgroups end more evenly. us at N 4096, K 4096, T 8192, of 1024 / 2048 / 4096 workgroups
+  // or more: rank 16 56 / 53 / 52, 32 61 / 57 / 60, 64 74 / 74 / 82, 128 94 / 97 / 112.
   const uint64_t groups = static_cast<uint64_t>(p.tiles) * ((n + 255u) / 256u);
-  while (p.wide < 8u && groups / (2u * p.wide) >= 1024u) p.wide *= 2u;
+  const uint32_t ranks = adapter_ranks(rank), least = ranks <= 4u ? 4096u / ranks : 1024u;
+  while (p.wide < 8u && groups / (2u * p.wide) >= least) p.wide *= 2u;
   while (p.splits < 16u && p.tiles * p.splits * 2u <= 512u && blocks(k) / (p.splits * 2u) >= 8u) p.splits *= 2u;
   p.split_blocks = (blocks(k) + p.splits - 1u) / p.splits;
   p.splits = (blocks(k) + p.split_blocks - 1u) / p.split_blocks;
   return p;
+}
+// Whether y and out go past the caches: together they are more than the one behind the L2s holds, or than all L2s hold while
+// B would fill one (4 MB). us without / with, of 8 adapters and K 4096:
+//   268 MB  T 8192, N 8192, rank 16  82 / 81    32 87 / 80    64 103 / 92    128 130 / 122
+//   134 MB  T 4096, N 8192: B of 2 MB 42.7 / 43.6    4 50.1 / 47.5    8 66.0 / 59.2    16 85.8 / 84.4
+//           T 8192, N 4096: B of 1 MB 51.3 / 55.6    2 57.3 / 56.5    4 72.9 / 66.7     8 94.0 / 90.7
+inline bool adapter_once(uint32_t tokens, uint32_t adapters, uint32_t rank, uint32_t n) {
+  const uint64_t moved = 4ull * tokens * n, b = 32ull * adapter_ranks(rank) * n * adapters;
+  return moved > kInfinityCache || (moved > 8u * kL2 && b >= kL2);
 }
 
 }  // namespace nkplan

@@ -15,6 +15,8 @@ int main() {
       const nkplan::AdapterPlan p = nkplan::adapter_plan(a, b, c, d, e);
       std::printf("%u %u %u %u %u %u %u\n", nkplan::adapter_tile(a, b), nkplan::adapter_ranks(c), p.tiles, p.splits,
                   p.split_blocks, p.wide, p.fused ? 1u : 0u);
+    } else if (!std::strcmp(what, "once") && std::scanf("%u %u %u %u", &a, &b, &c, &d) == 4) {
+      std::printf("%u\n", nkplan::adapter_once(a, b, c, d) ? 1u : 0u);
     } else if (!std::strcmp(what, "codes") && std::scanf("%u %u %u", &a, &b, &c) == 3) {
       const nkplan::ProductPlan p = nkplan::codes_plan(a, b, c);
       std::printf("%u %u %u\n", static_cast<unsigned>(p.form), p.p, p.q);

@@ -153,3 +153,27 @@ def test_views_of_one_row_and_one_column():
     n = rms_norm(column, w[:1], out_type=F)
     assert torch.equal(n.y, rms_norm(column.contiguous(), w[:1], out_type=F).y)
     assert torch.equal(route(column, 1).weights, torch.ones(300, 1, device=DEV))
+
+
+# T, adapters, rank, K, N: y and out of more than 256 MiB, of each tile and rank
+ONCE = [(7000, 3, 16, 128, 10001), (7000, 9, 20, 128, 9999), (7001, 3, 64, 200, 10240), (7000, 60, 100, 200, 10000),
+        (9000, 3, 16, 128, 10001), (9001, 9, 20, 128, 9999), (8192, 3, 64, 200, 10240), (9000, 60, 100, 200, 10000)]
+
+
+@pytest.mark.parametrize("T,L,r,K,N", ONCE)
+def test_adapters_of_more_than_the_caches_hold(T, L, r, K, N):
+    """A row does not depend on the others; the first and last rows by the formula."""
+    a, b, s = A.adapters(L, r, K, N, r)
+    lora = LowRankAdapters(a.to(DEV), b.to(DEV), s.to(DEV))
+    gen = torch.Generator(device=DEV).manual_seed(T)
+    x, y = (torch.randn(T, n, generator=gen, device=DEV).to(BF) for n in (K, N))
+    ids = torch.randint(-1, L, (T,), generator=gen, device=DEV, dtype=torch.int32)
+    got = lora.add(y, x, lora.plan(ids))
+    for rows in (slice(0, 50), slice(T - 50, T)):
+        want, bound = A.add(y[rows].cpu(), x[rows].cpu(), a, b, s, ids[rows].cpu())
+        assert_within(got[rows], want, bound)
+    order = torch.randperm(T, generator=gen, device=DEV)
+    again = lora.add(y[order], x[order], lora.plan(ids[order]))
+    assert torch.equal(again, got[order])
+    assert torch.equal(got[ids < 0], y[ids < 0])
+    assert lora.add(y, x, lora.plan(ids), y) is y and torch.equal(y, got)

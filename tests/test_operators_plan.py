@@ -8,6 +8,7 @@ import pytest
 
 import test_gpu_adapters
 import test_gpu_norm
+import test_gpu_operator_calls
 from conftest import REPO
 
 LAYERS = REPO / "netra-kernel_amd" / "csrc" / "layers"
@@ -61,6 +62,15 @@ def test_adapters_sizes_reach_every_kernel(plan):
     got = plan([("adapters", T, L, r, N, K) for T, L, r, K, N, _ in test_gpu_adapters.SIZES])
     assert {(g[0], g[1], g[6]) for g in got} == {(16, r, f) for r in (1, 2, 4, 8) for f in (0, 1)} | {(32, r, 0) for r in (1, 2, 4, 8)}
     assert any(g[3] > 1 for g in got)
+
+
+def test_adapters_sizes_reach_every_kernel_past_the_caches(plan):
+    sizes = test_gpu_operator_calls.ONCE
+    once = plan([("once", T, L, r, N) for T, L, r, _, N in sizes])
+    got = plan([("adapters", T, L, r, N, K) for T, L, r, K, N in sizes])
+    assert all(o == [1] for o in once) and {(g[0], g[1], g[6]) for g in got} == {(t, r, 0) for t in (16, 32) for r in (1, 2, 4, 8)}
+    # little B beside as much
+    assert plan([("once", 4096, 8, 16, 8192), ("once", 4096, 16, 16, 8192), ("once", 64, 64, 128, 8192)]) == [[0], [1], [0]]
 
 
 def test_products_of_codes(plan):
