@@ -12,6 +12,9 @@
 // operands, the few experts (or groups) drawn are put in order by their scores in 64 bits; and only where that does not
 // settle it, or the scores are a softmax's, the token is done again in 64 bits, by the whole wave: 6 us of one wave's
 // time, however few the tokens. Keys of bf16 logits hold all of them and are never done again.
+//
+// T 32768, 256 experts by sigmoid, bias and groups: 17 us, bound by its instructions (the vector units are
+// busy 91% of the time; the 19 MB alone would take 4). T 64: 3.3 us, a launch.
 #pragma once
 #include <type_traits>
 
@@ -91,17 +94,19 @@ __device__ __forceinline__ void each_turn(F&& f) {
   }
 }
 
-// Whether lane g's group of 16 (g < groups) is among the `top` best by `score`, in an order of T; ties to the lower.
+// Whether a group (its score is lane g * each_lane's of a row of 16) is among the `top` best by `score`, in an order
+// of T; ties to the lower. False in other lanes.
 template <typename T, typename Turn>
-__device__ __forceinline__ bool kept(T score, uint32_t groups, uint32_t top, Turn&& turn) {
+__device__ __forceinline__ bool kept(T score, uint32_t groups, uint32_t top, uint32_t each_lane, Turn&& turn) {
   const uint32_t g = threadIdx.x & 15u;
+  auto leads = [&](uint32_t lane) __attribute__((always_inline)) { return (lane & (each_lane - 1u)) == 0u && lane < groups * each_lane; };
   uint32_t before = 0u;
   each_turn([&](auto n) __attribute__((always_inline)) {
     const uint32_t other = (g + n) & 15u;
     const T s = turn(score, n);
-    before += other < groups && (s > score || (s == score && other < g)) ? 1u : 0u;
+    before += leads(other) && (s > score || (s == score && other < g)) ? 1u : 0u;
   });
-  return g < groups && before < top;
+  return leads(g) && before < top;
 }
 
 // Weights of the choices, lane i of a row of 16 its token's i-th, from its logit z (the row's
@@ -241,7 +246,7 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
         }
       }
     if (a.top2) best += second;
-    const bool keep = kept(best, a.groups, a.top_groups, [](double v, auto n) __attribute__((always_inline)) {
+    const bool keep = kept(best, a.groups, a.top_groups, 1u, [](double v, auto n) __attribute__((always_inline)) {
       const uint64_t u = (uint64_t)__double_as_longlong(v);
       return __longlong_as_double((long long)((uint64_t)turned<decltype(n)::value>((uint32_t)(u >> 32)) << 32 | turned<decltype(n)::value>((uint32_t)u)));
     });
@@ -449,34 +454,49 @@ __device__ __forceinline__ void select(const Select& a) {
     for (uint32_t j = 0; j < NV; j += 4u)
       *reinterpret_cast<uint4*>(s + nkbal::expert<G>(lane, j)) = make_uint4(key[j], key[j + 1u], key[j + 2u], key[j + 3u]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // A group's experts go to as many neighbouring lanes (a power of two) as the groups leave; they join theirs after.
+    const uint32_t each_lane = a.groups <= 2u ? 8u : a.groups <= 4u ? 4u : a.groups <= 8u ? 2u : 1u;
+    const uint32_t group = i / each_lane, in = i & (each_lane - 1u);
+    const uint32_t share = ((a.each + 3u) / 4u + each_lane - 1u) / each_lane * 4u;
+    const uint32_t m0 = group < a.groups ? min(in * share, a.each) : 0u, m1 = group < a.groups ? min(m0 + share, a.each) : 0u;
+    const uint32_t* from = s + group * a.each;
+    auto joined = [&](auto&& take_other) __attribute__((always_inline)) {
+      if (each_lane >= 2u) take_other(std::integral_constant<int, 0xB1>{});
+      if (each_lane >= 4u) take_other(std::integral_constant<int, 0x4E>{});
+      if (each_lane >= 8u) take_other(std::integral_constant<int, 0x141>{});
+    };
     uint32_t best = 0u, second = 0u;
     auto take = [&](uint32_t v) __attribute__((always_inline)) {
       second = max(second, min(best, v));
       best = max(best, v);
     };
-    if (i < a.groups) {
-      const uint32_t* from = s + i * a.each;
-      if (a.each % 4u == 0u) {
-        for (uint32_t m = 0; m < a.each; m += 4u) {
-          const uint4 v = *reinterpret_cast<const uint4*>(from + m);
-          take(v.x);
-          take(v.y);
-          take(v.z);
-          take(v.w);
-        }
-      } else {
-        for (uint32_t m = 0; m < a.each; m += 8u) {
-          uint32_t v[8];
+    if (a.each % 4u == 0u) {
+      for (uint32_t m = m0; m < m1; m += 4u) {
+        const uint4 v = *reinterpret_cast<const uint4*>(from + m);
+        take(v.x);
+        take(v.y);
+        take(v.z);
+        take(v.w);
+      }
+    } else {
+      for (uint32_t m = m0; m < m1; m += 8u) {
+        uint32_t v[8];
 #pragma unroll
-          for (uint32_t n = 0; n < 8u; ++n) v[n] = from[min(m + n, a.each - 1u)];
+        for (uint32_t n = 0; n < 8u; ++n) v[n] = from[min(m + n, m1 - 1u)];
 #pragma unroll
-          for (uint32_t n = 0; n < 8u; ++n) take(m + n < a.each ? v[n] : 0u);
-        }
+        for (uint32_t n = 0; n < 8u; ++n) take(m + n < m1 ? v[n] : 0u);
       }
     }
+    joined([&](auto ctrl) __attribute__((always_inline)) {
+      const uint32_t b0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)best, decltype(ctrl)::value, 0xF, 0xF, false);
+      const uint32_t b1 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)second, decltype(ctrl)::value, 0xF, 0xF, false);
+      take(b0);
+      take(b1);
+    });
+    const bool leads = in == 0u && group < a.groups;  // its score stands for the group
     // (the best expert's key orders the groups itself, as lower groups have lower experts)
     const uint32_t shift = a.top2 ? 4u : 10u;
-    const uint32_t score = i >= a.groups ? 0u : a.top2 ? ((best >> 10) + (second >> 10)) << 4 | (15u - i) : best;
+    const uint32_t score = !leads ? 0u : a.top2 ? ((best >> 10) + (second >> 10)) << 4 | (15u - i) : best;
     uint32_t before = 0u;
     each_turn([&](auto n) __attribute__((always_inline)) {
       before += turned<decltype(n)::value>(score) > score ? 1u : 0u;
@@ -489,31 +509,38 @@ __device__ __forceinline__ void select(const Select& a) {
       // Groups too near: their best experts' scores in 64 bits, if it is certain which experts those are.
       if (exact_near && __ballot(again && live)) {
         uint32_t v[3] = {0u, 0u, 0u};
-        if (i < a.groups)
-          for (uint32_t m = 0; m < a.each; ++m) {
-            const uint32_t x = s[i * a.each + m];
-            v[2] = max(v[2], min(v[1], x));
-            v[1] = max(v[1], min(v[0], x));
-            v[0] = max(v[0], x);
-          }
+        auto take3 = [&](uint32_t x) __attribute__((always_inline)) {
+          v[2] = max(v[2], min(v[1], x));
+          v[1] = max(v[1], min(v[0], x));
+          v[0] = max(v[0], x);
+        };
+        for (uint32_t m = m0; m < m1; ++m) take3(from[m]);
+        joined([&](auto ctrl) __attribute__((always_inline)) {
+          uint32_t x[3];
+#pragma unroll
+          for (uint32_t n = 0; n < 3u; ++n) x[n] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[n], decltype(ctrl)::value, 0xF, 0xF, false);
+#pragma unroll
+          for (uint32_t n = 0; n < 3u; ++n) take3(x[n]);
+        });
         const uint32_t of = a.top2 ? 1u : 0u;
-        const bool certain = i >= a.groups || v[of + 1u] == 0u || (v[of] >> 10) - (v[of + 1u] >> 10) > near;
+        const bool certain = !leads || v[of + 1u] == 0u || (v[of] >> 10) - (v[of + 1u] >> 10) > near;
         uint64_t exact = 0u;
-        if (i < a.groups) {
+        if (leads) {
           exact = exact_score(a, row, 1023u - (v[0] & 1023u));
           if (a.top2) exact = order(score_of(exact) + score_of(exact_score(a, row, 1023u - (v[1] & 1023u))));
         }
-        keep = kept(exact, a.groups, a.top_groups, [](uint64_t u, auto n) __attribute__((always_inline)) { return turned<decltype(n)::value>(u); });
+        keep = kept(exact, a.groups, a.top_groups, each_lane, [](uint64_t u, auto n) __attribute__((always_inline)) { return turned<decltype(n)::value>(u); });
         again = across<16, false>(certain ? 1u : 0u) == 0u;
       }
     }
     // what is not kept leaves by zeros in LDS
-    if (i < a.groups && !keep) {
-      uint32_t* to = s + i * a.each;
+    const uint32_t of_row = (uint32_t)(__ballot(keep) >> (lane & 48u)) & 0xffffu;
+    if (!(of_row >> (group * each_lane) & 1u)) {
+      uint32_t* to = s + group * a.each;
       if (a.each % 4u == 0u) {
-        for (uint32_t m = 0; m < a.each; m += 4u) *reinterpret_cast<uint4*>(to + m) = make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t m = m0; m < m1; m += 4u) *reinterpret_cast<uint4*>(to + m) = make_uint4(0u, 0u, 0u, 0u);
       } else {
-        for (uint32_t m = 0; m < a.each; ++m) to[m] = 0u;
+        for (uint32_t m = m0; m < m1; ++m) to[m] = 0u;
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -598,7 +625,9 @@ struct SelectGradient {
 
 // The gradient of the logits. Lane i of a row of 16 has the token's i-th choice. Differences of the
 // weights' gradients are taken before they are weighted (sum_j s_j (v_i - v_j), not v_i S - sum_j s_j v_j):
-// nothing cancels where one expert has almost all. The row goes through LDS.
+// nothing cancels where one expert has almost all. The row goes through LDS. T 32768, 500 experts in fp32,
+// every logit with a gradient: 30 us (133 MB, 4.4 TB/s; the vector units are busy 75% of the time); T 4096, 256 experts by
+// sigmoid 4.8.
 template <typename X, uint32_t G, uint32_t NV>
 __device__ __forceinline__ void gradient(const SelectGradient& a) {
   constexpr uint32_t kTokens = 64u / G, kWaves = 4u;
