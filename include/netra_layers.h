@@ -1,6 +1,8 @@
 // Operators next to the routed-MoE layer (libnetra_layers.so): the block-FP8
-// linear layer y = x W^T with its gradients, per-expert route counts, and the
-// router's balance loss with its gradient.
+// linear layer y = x W^T with its gradients, the root-mean-square norm before it
+// (output in 8 bits too) with its gradients, the routing to experts with its gradient, per-expert
+// route counts, the router's balance loss with its gradient, and low-rank
+// adapters beside a projection.
 //
 // Block-FP8 linear layer. W [n, k] is e4m3 with one fp32 scale per 128x128
 // block (scale grid [ceil(n/128), ceil(k/128)], row-major), as a block-FP8

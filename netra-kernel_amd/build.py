@@ -5,7 +5,8 @@ Outputs (git-ignored, shipped with the source tree to the GPU host):
   netra-kernel_amd/lib/libnetra_engine.so      C-ABI engine runtime
   netra-kernel_amd/lib/libnetra_moe.so         direct entry points (weight prep, no-alloc prefill)
   netra-kernel_amd/lib/libnetra_bridges.so     the reference's per-operation bridge ABIs
-  netra-kernel_amd/lib/libnetra_layers.so      block-FP8 linear layer, expert counts, balance loss
+  netra-kernel_amd/lib/libnetra_layers.so      operators beside the layer: block-FP8 linear layer, norm,
+                                               routing, expert counts, balance loss, low-rank adapters
 
 Run: python netra-kernel_amd/build.py  (or __graft_entry__.build()).
 """

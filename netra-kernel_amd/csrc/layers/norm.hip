@@ -7,7 +7,9 @@
 //
 // A row is held in registers by W waves (eight neighbouring columns a lane, C times), so it is
 // read once; sums are fp32. y is quantised as it stands in fp32, not after its rounding to bf16:
-// one rounding instead of two.
+// one rounding instead of two. Memory bounds both: T 16384, H 4096 with residual and codes 110 us
+// (606 MB, 5.5 TB/s), its gradients 87 and 4.8 for dw's sum (537 MB); a large copy runs at 5.1. Few rows are a launch: T 1,
+// H 2048 2.2 us, T 333 4.4 and 3.5.
 #pragma once
 #include "linear_fp8.hip"
 #include "router_balance.hip"
@@ -416,7 +418,8 @@ __device__ __forceinline__ void gradients(const NormGradients& a) {
 }
 
 // dw = the sum of `parts` partial sums, in one order: a workgroup takes 64 columns, its 16 waves
-// every 16th part, eight loads at a time.
+// every 16th part, eight loads at a time. (At most 512 parts: more of them, summed one load at
+// a time, took 88 us where the gradients and their sum now take 10, at T 4943, H 538.)
 __device__ __forceinline__ void sum_parts(const float* __restrict__ partial, uint32_t parts, uint32_t cols, float* dw,
                                           uint32_t accumulate) {
   __shared__ float s[16][64];
