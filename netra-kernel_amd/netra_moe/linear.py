@@ -112,8 +112,11 @@ class BlockLinear:
         adapters are added (adapters.py)."""
         if adapters is None:
             return self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
-        if plan is None or (adapters.N, adapters.K) != (self.N, self.K):
-            raise ValueError(f"adapters: need a plan and adapters of N {self.N}, K {self.K}")
+        if plan is None or (adapters.N, adapters.K, adapters.device) != (self.N, self.K, self.device):
+            raise ValueError(f"adapters: need a plan and adapters of N {self.N}, K {self.K} on {self.device}")
+        if x.dim() != 2 or (plan.tokens, plan.adapters, plan.data.device) != (x.shape[0], adapters.count, self.device):
+            raise ValueError(f"plan: need one of x's tokens for {adapters.count} adapters on {self.device}, got {plan.tokens} tokens for "
+                             f"{plan.adapters} on {plan.data.device}")  # (before y is written)
         y = self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
         return adapters.add(y, x, plan, y)
 

@@ -177,3 +177,14 @@ def test_adapters_of_more_than_the_caches_hold(T, L, r, K, N):
     assert torch.equal(again, got[order])
     assert torch.equal(got[ids < 0], y[ids < 0])
     assert lora.add(y, x, lora.plan(ids), y) is y and torch.equal(y, got)
+
+
+def test_a_projection_refuses_another_batchs_plan_before_it_writes():
+    step = Step(40)
+    out = torch.zeros(40, 512, dtype=BF, device=DEV)
+    for plan in (make_plan(step.ids[:39].contiguous(), Step.L), make_plan(step.ids, Step.L + 1), None):
+        with pytest.raises(ValueError):
+            step.proj.forward(step.x, out, adapters=step.adapters, plan=plan)
+    torch.cuda.synchronize()
+    assert not out.any()
+    assert step.proj.forward(step.x, out, adapters=step.adapters, plan=make_plan(step.ids, Step.L)) is out and out.any()
