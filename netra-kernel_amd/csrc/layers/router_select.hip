@@ -316,10 +316,10 @@ __device__ __forceinline__ void sort(uint32_t (&v)[NV]) {
   }
 }
 
-// The n largest of the keys that a token's G lanes have in falling order; lane i gets the i-th. Of a lane's own
-// only the first M (n at most) can be among them.
+// The n largest of the keys that a token's G lanes have in falling order; lane i gets the i-th, all get the next
+// one (rest; 0: none). Of a lane's own only the first M (n + 1 at most, n without rest) can be among them.
 template <uint32_t G, uint32_t M, uint32_t NV>
-__device__ __forceinline__ uint32_t draw(const uint32_t (&v)[NV], uint32_t n) {
+__device__ __forceinline__ uint32_t draw(const uint32_t (&v)[NV], uint32_t n, uint32_t& rest) {
   constexpr uint32_t L = M < NV ? M : NV;
   const uint32_t i = threadIdx.x & 15u;
   uint32_t key[L], mine = 0u;
@@ -334,6 +334,7 @@ __device__ __forceinline__ uint32_t draw(const uint32_t (&v)[NV], uint32_t n) {
     for (uint32_t j = 0; j + 1u < L; ++j) key[j] = (key[j] & ~gone) | (key[j + 1u] & gone);
     key[L - 1u] &= ~gone;
   }
+  rest = across<G, true>(key[0]);
   return mine;
 }
 
@@ -557,7 +558,9 @@ __device__ __forceinline__ void select(const Select& a) {
   sort<0u, NV>(key);
   // two more than k, to see whether the k-th and the next one are apart
   const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
-  const uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws) : draw<G, 16u>(key, draws);
+  uint32_t rest;
+  constexpr uint32_t kRest = K == kWhole ? 0u : 1u;
+  const uint32_t mine = draws <= 10u ? draw<G, 10u + kRest>(key, draws, rest) : draw<G, 16u + kRest>(key, draws, rest);
   uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
   if constexpr (K != kWhole) {
     // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
@@ -571,7 +574,7 @@ __device__ __forceinline__ void select(const Select& a) {
     const bool next_close = turned<1>(close ? 1u : 0u) != 0u;
     bool bad = i < a.k && close && !same;
     if (i + 1u == a.k) bad = close && (!same || a.k + 2u > kMost || next_close);
-    if (a.k == kMost && i + 1u == a.k) bad = true;  // no lane holds the next one
+    if (a.k == kMost && i + 1u == a.k) bad = rest != 0u && (mine >> 10) - (rest >> 10) <= near;  // no lane holds the next one
     // Choices too near: the order of those drawn by their scores in 64 bits, if what was not drawn is certainly behind
     // the k-th then.
     if (exact_near && __ballot(bad && live)) {
@@ -585,8 +588,7 @@ __device__ __forceinline__ void select(const Select& a) {
       });
       const bool chosen = drawn && before < a.k;
       const uint32_t least = across<16, false>(chosen ? mine >> 10 : ~0u);
-      const uint32_t last = across<16, false>(i < draws ? mine >> 10 : ~0u);  // 0: there are no others
-      bad = last != 0u && least - last <= near;
+      bad = rest != 0u && least - (rest >> 10) <= near;
       const uint32_t place = drawn ? before : ~0u, old = id;
       id = place == i ? old : 0u;
       each_turn([&](auto n) __attribute__((always_inline)) {

@@ -248,3 +248,26 @@ def test_gradient_refusals():
                      ((dw, z, ids), dict(out=torch.zeros(4, 8, device=DEV, dtype=BF)))]:
         with pytest.raises((ValueError, RuntimeError)):
             route_gradient(*args, **kw)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E", [20, 128, 300, 700])
+@pytest.mark.parametrize("k", [8, 13, 14, 15, 16])
+def test_near_scores_on_both_sides_of_the_last_choice(scoring, E, k):
+    """The k-th and the next few experts are equal, or apart by less than fp32 tells or by a little more; in some tokens
+    one lane has most of them."""
+    T = 240
+    g = torch.Generator().manual_seed(E + k)
+    z = torch.randn(T, E, generator=g) * 0.1
+    for t in range(T):
+        order = torch.arange(E) if t % 3 == 0 else torch.randperm(E, generator=g)
+        z[t, order[:k - 2]] += 3.0
+        step = (0.0, 2.0 ** -23, 2.0 ** -21, 2.0 ** -19)[t % 4]
+        near = order[k - 2:k + 2]
+        z[t, near] = 2.0 + step * torch.randint(0, 3, (len(near),), generator=g)
+    check_route(z, k, scoring=scoring)
+    check_route(z, k, scoring=scoring, bias=torch.zeros(E))
+    check_route(z, k, scoring=scoring, bias=(torch.rand(E, generator=g) * 2.0 ** -18))
+    check_route(z.to(BF), k, scoring=scoring, bias=torch.zeros(E))
+    if E % 4 == 0:
+        check_route(z, k, scoring=scoring, groups=4, top_groups=4 if E == 20 else 3, group_score="top2")
