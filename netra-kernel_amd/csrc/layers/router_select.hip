@@ -316,8 +316,8 @@ __device__ __forceinline__ void sort(uint32_t (&v)[NV]) {
   }
 }
 
-// The n largest of the keys that a token's G lanes have in falling order; lane i gets the i-th, all get the next
-// one (rest; 0: none). Of a lane's own only the first M (n + 1 at most, n without rest) can be among them.
+// The n largest of the keys that a token's G lanes have in falling order; lane i gets the i-th. Of a lane's own
+// only the first M (n at most) can be among them; with M above 16 all lanes get the next one too (rest; 0: none).
 template <uint32_t G, uint32_t M, uint32_t NV>
 __device__ __forceinline__ uint32_t draw(const uint32_t (&v)[NV], uint32_t n, uint32_t& rest) {
   constexpr uint32_t L = M < NV ? M : NV;
@@ -334,7 +334,7 @@ __device__ __forceinline__ uint32_t draw(const uint32_t (&v)[NV], uint32_t n, ui
     for (uint32_t j = 0; j + 1u < L; ++j) key[j] = (key[j] & ~gone) | (key[j + 1u] & gone);
     key[L - 1u] &= ~gone;
   }
-  rest = across<G, true>(key[0]);
+  if constexpr (M > kMost) rest = across<G, true>(key[0]);
   return mine;
 }
 
@@ -351,9 +351,15 @@ __device__ __forceinline__ void select(const Select& a) {
   if (b > (a.tokens - 1u) / kTokens) return;
   constexpr float kUnits = 4194302.0f;  // of a key's upper 22 bits, from 1 on
   // Scores: lo .. hi over 0 and the finite biases, and a score's 0 .. 1, are the units' range. A sigmoid is
-  // off by 5e-7 by the hardware's exponential and reciprocal, a softmax by its sum too; then the sum with the bias.
+  // off by 5e-7 by the hardware's exponential and reciprocal, a softmax by its sum too, of the largest (mostly far below
+  // one: T 32768, 256 experts with a bias 20 us, held against one 26); then the sum with the bias.
   float bias[NV], lo = 0.0f, units = 0.0f;
+  float widest = 0.0f;                    // of the biases
   uint32_t near = K == kWhole ? 0u : 4u;  // keys that are apart by no more are not told apart
+  // (by scores that are off by `off` of the largest, and their sum with the bias)
+  auto apart = [&](float off, float largest) __attribute__((always_inline)) {
+    return 3u + (uint32_t)fminf(2.0f * (off * largest + 2.4e-7f * (largest + widest)) * units, 8e6f);
+  };
   if constexpr (K == kScore) {
     const __amdgpu_buffer_rsrc_t r = nk::buffer_rsrc(a.bias, a.bias ? E * 4u : 0u);  // (no bias: zeros)
     float hi = 0.0f;
@@ -372,8 +378,8 @@ __device__ __forceinline__ void select(const Select& a) {
     lo = -nkbal::reduce<G, true>(-lo);
     hi = nkbal::reduce<G, true>(hi);
     units = kUnits / (hi - lo + 1.0f);
-    const float off = (a.scoring == kSigmoid ? 6e-7f : 2.5e-6f) + 2.4e-7f * (1.0f + fmaxf(fabsf(lo), fabsf(hi)));
-    near = 3u + (uint32_t)fminf(2.0f * off * units, 8e6f);
+    widest = fmaxf(-lo, hi);
+    if (a.scoring == kSigmoid) near = apart(6e-7f, 1.0f);
     // lanes' places past the last expert: the least key, behind every expert's that has it too
     if (E < kMax) {
 #pragma unroll
@@ -437,6 +443,7 @@ __device__ __forceinline__ void select(const Select& a) {
           z[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[j] * -1.44269504088896341f));
       } else {
         const float inv = total == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(total);
+        near = apart(2.5e-6f, inv);  // the largest is exp(0) / total (a NaN: all are near)
 #pragma unroll
         for (uint32_t j = 0; j < NV; ++j) z[j] *= inv;
       }
@@ -558,9 +565,8 @@ __device__ __forceinline__ void select(const Select& a) {
   sort<0u, NV>(key);
   // two more than k, to see whether the k-th and the next one are apart
   const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
-  uint32_t rest;
-  constexpr uint32_t kRest = K == kWhole ? 0u : 1u;
-  const uint32_t mine = draws <= 10u ? draw<G, 10u + kRest>(key, draws, rest) : draw<G, 16u + kRest>(key, draws, rest);
+  uint32_t rest = 0u;
+  const uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws, rest) : draw<G, K == kWhole ? 16u : 17u>(key, draws, rest);
   uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
   if constexpr (K != kWhole) {
     // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
@@ -588,6 +594,8 @@ __device__ __forceinline__ void select(const Select& a) {
       });
       const bool chosen = drawn && before < a.k;
       const uint32_t least = across<16, false>(chosen ? mine >> 10 : ~0u);
+      // (up to ten draws have no next one, which would cost every wave 3%; the last one drawn is no less)
+      if (draws <= 10u) rest = across<16, false>(i < draws ? mine : ~0u);
       bad = rest != 0u && least - (rest >> 10) <= near;
       const uint32_t place = drawn ? before : ~0u, old = id;
       id = place == i ? old : 0u;
