@@ -566,7 +566,14 @@ __device__ __forceinline__ void select(const Select& a) {
   // two more than k, to see whether the k-th and the next one are apart
   const uint32_t draws = K == kWhole ? a.k : min(a.k + 2u, kMost);
   uint32_t rest = 0u;
-  const uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws, rest) : draw<G, K == kWhole ? 16u : 17u>(key, draws, rest);
+  uint32_t mine = draws <= 10u ? draw<G, 10u>(key, draws, rest) : draw<G, K == kWhole ? 16u : 17u>(key, draws, rest);
+  if constexpr (K != kWhole) {
+    // Places past the last expert are no choice: where the kept groups have fewer experts than are drawn, such places, whose
+    // keys are behind all of theirs, are drawn after them. (Of bf16 logits k are drawn and no more, which the groups have.)
+    auto expert_or_none = [&](uint32_t v) __attribute__((always_inline)) { return 1023u - (v & 1023u) < E ? v : 0u; };
+    mine = expert_or_none(mine);
+    rest = expert_or_none(rest);
+  }
   uint32_t id = min(K == kWhole ? 0xffffu - (mine & 0xffffu) : 1023u - (mine & 1023u), E - 1u);
   if constexpr (K != kWhole) {
     // lane i: its choice and the next one. Equal logits and biases are told apart by the index.
