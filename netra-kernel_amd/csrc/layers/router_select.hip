@@ -349,7 +349,10 @@ __device__ __forceinline__ void select(const Select& a) {
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t b = blockIdx.x * kWaves + wave;
   if (b > (a.tokens - 1u) / kTokens) return;
-  constexpr float kUnits = 4194302.0f;  // of a key's upper 22 bits, from 1 on
+  // Of a key's upper 22 bits, from 1 on: the units of finite values; of scores 1 is -inf's (and a NaN's), kInf is +inf's, and
+  // what finite scores are off by, 3e-6 of the range, does not reach it.
+  constexpr float kUnits = 4194237.0f;
+  constexpr uint32_t kInf = 4194303u;
   // Scores: lo .. hi over 0 and the finite biases, and a score's 0 .. 1, are the units' range. A sigmoid is
   // off by 5e-7 by the hardware's exponential and reciprocal, a softmax by its sum too, of the largest (mostly far below
   // one: T 32768, 256 experts with a bias 20 us, held against one 26); then the sum with the bias.
@@ -451,7 +454,7 @@ __device__ __forceinline__ void select(const Select& a) {
       for (uint32_t j = 0; j < NV; ++j) {
         const uint32_t e = nkbal::expert<G>(lane, j);
         const float c = (z[j] + bias[j] - lo) * units;
-        key[j] = (1u + (uint32_t)fminf(fmaxf(c, 0.0f), kUnits)) << 10 | (1023u - e);
+        key[j] = (2u + (uint32_t)(int32_t)fminf(fmaxf(c, -1.0f), (float)(kInf - 2u))) << 10 | (1023u - e);
       }
     }
   }
@@ -504,7 +507,9 @@ __device__ __forceinline__ void select(const Select& a) {
     const bool leads = in == 0u && group < a.groups;  // its score stands for the group
     // (the best expert's key orders the groups itself, as lower groups have lower experts)
     const uint32_t shift = a.top2 ? 4u : 10u;
-    const uint32_t score = !leads ? 0u : a.top2 ? ((best >> 10) + (second >> 10)) << 4 | (15u - i) : best;
+    // Sums of two: with -inf (as of a NaN, or of both infinities) behind all others, with +inf before all.
+    const uint32_t b0 = best >> 10, b1 = second >> 10, sum = b1 == 1u ? 0u : b0 == kInf ? 2u * kInf : b0 + b1;
+    const uint32_t score = !leads ? 0u : a.top2 ? sum << 4 | (15u - i) : best;
     uint32_t before = 0u;
     each_turn([&](auto n) __attribute__((always_inline)) {
       before += turned<decltype(n)::value>(score) > score ? 1u : 0u;

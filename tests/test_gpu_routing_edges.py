@@ -1,12 +1,16 @@
-"""netra_moe.routing where the kept groups hold hardly more experts than are chosen (forms and bounds of routing_case.py)."""
+"""netra_moe.routing where the kept groups hold hardly more experts than are chosen, and where biases and logits are
+infinite or NaN (forms and bounds of routing_case.py)."""
 import pytest
 import torch
 
+import routing_case as R
 from conftest import gpu_available
+from netra_moe.routing import route
 from test_gpu_routing import check_route
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a GPU")]
 BF, F = torch.bfloat16, torch.float32
+DEV = "cuda:0"
 
 
 def near_pairs(T, E, seed, every):
@@ -50,3 +54,55 @@ def test_places_behind_the_last_expert_are_not_chosen(E, G, top, k, scoring):
                     check_route(v, k, renormalise=False, bias=b, group_score="top2", **kw)
             if G > 1 and E // G > 1:
                 check_route(v, k, renormalise=False, group_score="top2", **kw)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("E,G,top,k", [(8, 4, 2, 3), (63, 7, 3, 5), (128, 8, 4, 8), (256, 16, 5, 12), (500, 4, 2, 16), (700, 10, 4, 6)])
+def test_infinite_biases(E, G, top, k, scoring, dtype):
+    """Groups with no, one or two experts that a bias of -inf leaves, and experts that a bias of +inf or NaN stands at."""
+    each = E // G
+    g = torch.Generator().manual_seed(E)
+    finite = (torch.rand(E, generator=g) - 0.5) * 0.2
+    biases = []
+    for left in (0, 1, 2):
+        b = finite.clone().view(G, each)
+        b[1, left:] = -torch.inf
+        b[G - 1, :max(0, each - left)] = -torch.inf
+        biases.append(b.flatten())
+        b = b.clone()
+        b[0, 1:] = torch.nan
+        biases.append(b.flatten())
+    for n in (1, 2):
+        b = finite.clone()
+        b[E - n:] = torch.inf
+        biases.append(b)
+    biases += [torch.full((E,), -torch.inf), torch.full((E,), torch.inf),
+               torch.where(torch.arange(E) % each == 0, finite, -torch.inf), torch.where(torch.arange(E) % each < 2, finite, -torch.inf),
+               torch.where(torch.arange(E) % 5 == 1, 3e38, -3e38), torch.where(torch.arange(E) % 5 == 1, torch.inf, finite * 1e38)]
+    for T, every in ((1, 1), (203, 203), (203, 4), (203, 1)):
+        z = near_pairs(T, E, T + every, every).to(dtype)
+        for b in biases:
+            for group_score in ("top2", "max"):
+                check_route(z, k, scoring=scoring, bias=b, renormalise=False, groups=G, top_groups=top, group_score=group_score)
+            check_route(z, k, scoring=scoring, bias=b, renormalise=False)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("E,G,top,k", [(8, 4, 2, 3), (63, 7, 3, 5), (128, 8, 4, 8), (700, 10, 4, 6)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_groups_with_nan_logits(E, G, top, k, biased, dtype):
+    """NaN logits that leave a group no, one or two experts; a NaN ranks as -inf."""
+    T, each = 203, E // G
+    for every in (T, 4, 1):
+        z = near_pairs(T, E, every, every).to(dtype)
+        for t in range(T):
+            group = z[t, (t % G) * each:(t % G + 1) * each]
+            group[t // G % 3:] = torch.nan
+            if t % 5 == 0:
+                z[t, 0] = torch.inf if t % 2 else -torch.inf
+        bias = (torch.rand(E, generator=torch.Generator().manual_seed(E)) - 0.5) * 0.2 if biased else None
+        for group_score in ("top2", "max"):
+            kw = dict(scoring="sigmoid", groups=G, top_groups=top, group_score=group_score)
+            r = route(z.to(DEV), k, selection_bias=None if bias is None else bias.to(DEV), **kw)
+            assert torch.equal(r.ids.cpu().long(), R.choose(z, k, "sigmoid", bias, G, top, group_score))
