@@ -246,10 +246,8 @@ __device__ __forceinline__ void select_exact(const Select& a, uint32_t t, double
         }
       }
     if (a.top2) best += second;
-    const bool keep = kept(best, a.groups, a.top_groups, 1u, [](double v, auto n) __attribute__((always_inline)) {
-      const uint64_t u = (uint64_t)__double_as_longlong(v);
-      return __longlong_as_double((long long)((uint64_t)turned<decltype(n)::value>((uint32_t)(u >> 32)) << 32 | turned<decltype(n)::value>((uint32_t)u)));
-    });
+    // (by their places in the order: +inf and -inf together are a NaN, which ranks as -inf and not before all)
+    const bool keep = kept(order(best), a.groups, a.top_groups, 1u, [](uint64_t u, auto n) __attribute__((always_inline)) { return turned<decltype(n)::value>(u); });
     const uint32_t bits = (uint32_t)__ballot(keep) & 0xffffu;
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j)
