@@ -57,7 +57,6 @@ def test_places_behind_the_last_expert_are_not_chosen(E, G, top, k, scoring):
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
-@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("E,G,top,k", [(8, 4, 2, 3), (63, 7, 3, 5), (128, 8, 4, 8), (256, 16, 5, 12), (700, 10, 4, 6)])
 def test_sums_of_both_infinities(E, G, top, k, scoring):
     """+inf beside nothing but -inf in a group: their sum is not a number and ranks as -inf."""
@@ -72,6 +71,7 @@ def test_sums_of_both_infinities(E, G, top, k, scoring):
             check_route(z, k, scoring=scoring, bias=bias, renormalise=False, groups=G, top_groups=top, group_score="top2")
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("dtype", [BF, F])
 @pytest.mark.parametrize("E,G,top,k", [(8, 4, 2, 3), (63, 7, 3, 5), (128, 8, 4, 8), (256, 16, 5, 12), (500, 4, 2, 16), (700, 10, 4, 6)])
 def test_infinite_biases(E, G, top, k, scoring, dtype):
