@@ -730,14 +730,18 @@ __device__ __forceinline__ void gradient(const SelectGradient& a) {
         if (m == -__builtin_inff()) m = 0.0f;
         p = chosen ? nkbal::exp_nonpos(z - m) : 0.0f;
       }
+      float steep = a.scoring == kSigmoid ? slope(z) : p;
       if (a.renormalise) {
+        // (each factor by the sum by itself: of small sigmoids 1 / sum^2 is past the range of fp32)
         const float total = nkbal::sum<16>(p);
         const float r = total == 0.0f ? 0.0f : 1.0f / total;
         float diff = 0.0f;
+        p *= r;
+        steep *= r;
         each_turn([&](auto n) __attribute__((always_inline)) { diff = fmaf(turned<decltype(n)::value>(p), v - turned<decltype(n)::value>(v), diff); });
-        v = a.scoring == kSigmoid ? diff * r * r : diff * r * (p * r);
+        v = diff;
       }
-      if (a.scoring == kSigmoid) v *= slope(z);
+      v *= steep;
       if (!chosen) v = 0.0f;
       mine = v;
       if (__ballot(chosen && !first))  // an expert in several slots

@@ -1,11 +1,12 @@
-"""netra_moe.routing where the kept groups hold hardly more experts than are chosen, and where biases and logits are
-infinite or NaN (forms and bounds of routing_case.py)."""
+"""netra_moe.routing where the kept groups hold hardly more experts than are chosen, where biases and
+logits are infinite or NaN, and where gradients of small scores are large (forms and bounds of routing_case.py)."""
 import pytest
 import torch
 
 import routing_case as R
 from conftest import gpu_available
-from netra_moe.routing import route
+from layers_case import assert_within
+from netra_moe.routing import route, route_gradient
 from test_gpu_routing import check_route
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a GPU")]
@@ -121,3 +122,18 @@ def test_groups_with_nan_logits(E, G, top, k, biased, dtype):
             kw = dict(scoring="sigmoid", groups=G, top_groups=top, group_score=group_score)
             r = route(z.to(DEV), k, selection_bias=None if bias is None else bias.to(DEV), **kw)
             assert torch.equal(r.ids.cpu().long(), R.choose(z, k, "sigmoid", bias, G, top, group_score))
+
+
+@pytest.mark.parametrize("E", [40, 600])
+def test_gradient_of_small_sigmoids(E):
+    """Renormalised weights do not depend on how small their sum is, nor does what 1/sum is multiplied with."""
+    T, k = 50, 6
+    g = torch.Generator().manual_seed(E)
+    for low in (-86.0, -70.0, -50.0):
+        z = low + torch.rand(T, E, generator=g)
+        ids = R.choose(z, k)
+        for size in (1e-3, 1.0, 3e4):
+            dw = torch.randn(T, k, generator=g) * size
+            want, bound = R.gradient(dw, z, ids, "sigmoid")
+            got = route_gradient(dw.to(DEV), z.to(DEV), ids.to(DEV, torch.int32), scoring="sigmoid")
+            assert_within(got, want, bound, f"low {low}, size {size}")
