@@ -211,7 +211,8 @@ int netra_adapters_pack(const void* a, const void* b, uint32_t type, void* packe
 uint64_t netra_adapters_plan_bytes(uint32_t tokens, uint32_t adapters);
 int netra_adapters_plan(const int32_t* ids, uint32_t tokens, uint32_t adapters, void* plan, uint64_t plan_bytes,
                         hipStream_t stream);
-// out may be y (same address and stride); any other overlap is refused. tokens 0 .. 2^21.
+// out may be y (same address and stride); any other overlap of out or the workspace with what the call reads, or of the two,
+// is refused. tokens 0 .. 2^21.
 uint64_t netra_adapters_add_workspace(uint32_t tokens, uint32_t adapters, uint32_t rank, uint32_t n, uint32_t k);
 int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_stride, const void* packed_a, const void* packed_b,
                        const float* scale, const void* plan, const uint16_t* y, uint64_t y_stride, uint16_t* out,

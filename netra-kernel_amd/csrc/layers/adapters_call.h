@@ -99,11 +99,21 @@ extern "C" int netra_adapters_add(const void* x, uint32_t x_type, uint64_t x_str
       !aligned(plan, 16))
     return fail(-1, name, "null or misaligned pointer, unknown type, or row stride below the row");
   const Span to = rows_span(out, NETRA_BF16, out_stride, tokens, n), from = rows_span(y, NETRA_BF16, y_stride, tokens, n);
-  if (share(to, rows_span(x, x_type, x_stride, tokens, k)) || (share(to, from) && !same(to, from)))
-    return fail(-1, name, "out shares memory with x, or with y and is not in its place");
   const AdapterPlan p = adapter_plan(tokens, adapters, rank, n, k);
-  if (bad_workspace(workspace, workspace_bytes, u_bytes(p, tokens, rank)))
+  const uint64_t need = u_bytes(p, tokens, rank);
+  if (bad_workspace(workspace, workspace_bytes, need))
     return fail(-1, name, "workspace too small, null or not 16-byte aligned");
+  const auto bytes = [](const void* at, uint64_t size) { return Span{at, size, size, size ? 1u : 0u}; };
+  const Span scratch = bytes(workspace, need);
+  const Span read[] = {rows_span(x, x_type, x_stride, tokens, k),
+                       bytes(packed_a, netra_adapters_packed_bytes(adapters, rank, n, k, 0)),
+                       bytes(packed_b, netra_adapters_packed_bytes(adapters, rank, n, k, 1)), bytes(scale, 4ull * adapters),
+                       bytes(plan, netra_adapters_plan_bytes(tokens, adapters))};
+  for (const Span& r : read)
+    if (share(to, r) || share(scratch, r))
+      return fail(-1, name, "out or the workspace shares memory with x, the weights, the scales or the plan");
+  if ((share(to, from) && !same(to, from)) || share(scratch, from) || share(scratch, to))
+    return fail(-1, name, "out shares memory with y and is not in its place, or the workspace shares memory with one of them");
   nkada::Adapters a{};
   a.x = x;
   a.x_stride = x_stride;
