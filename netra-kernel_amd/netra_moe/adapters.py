@@ -75,6 +75,9 @@ class LowRankAdapters:
         """Adapters (a [r, K], b [N, r]) of different ranks, filled with zeros to the largest."""
         if not pairs:
             raise ValueError("from_pairs needs an adapter")
+        for i, (a, b) in enumerate(pairs):
+            if a.dim() != 2 or b.dim() != 2 or b.shape[1] != a.shape[0]:
+                raise ValueError(f"pairs[{i}]: need a [r, K] and b [N, r], got {tuple(a.shape)} and {tuple(b.shape)}")
         rank = max(a.shape[0] for a, _ in pairs)
         fill = torch.nn.functional.pad
         return cls(torch.stack([fill(a, (0, 0, 0, rank - a.shape[0])) for a, _ in pairs]),
