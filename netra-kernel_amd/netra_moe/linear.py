@@ -111,6 +111,8 @@ class BlockLinear:
         """x bf16 or fp32 [T, K] -> x W^T, bf16 [T, N]. adapters and plan: the tokens' low-rank
         adapters are added (adapters.py)."""
         if adapters is None:
+            if plan is not None:
+                raise ValueError("plan: needs the adapters that it is for")
             return self._times("netra_linear_forward", "x", x, self.K, out, self.N, self.packed)
         if plan is None or (adapters.N, adapters.K, adapters.device) != (self.N, self.K, self.device):
             raise ValueError(f"adapters: need a plan and adapters of N {self.N}, K {self.K} on {self.device}")
