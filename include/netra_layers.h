@@ -139,7 +139,8 @@ int netra_router_balance(const void* logits, uint32_t logits_type, uint64_t logi
 //   NETRA_CODES_ROWS   codes [rows, cols], scales [rows, ceil(cols/128)] (what the bridges take)
 //   NETRA_CODES_TILES  what netra_linear_forward_codes takes: tile16x128, scales [ceil(cols/128), rows up to 16];
 //                      codes 16-byte aligned
-// rows 0 .. 2^21, cols 1 .. 16384; weight [cols] bf16 or fp32. Statistics are fp32 (|r| below 1e18).
+// rows 0 .. 2^21, cols 1 .. 16384; weight [cols] bf16 or fp32. Statistics are fp32: |r| below 1e17, so that a row's sum of
+// squares is finite at any length (a row whose sum is not has y 0), and mean(r^2) + eps not below 2^-126.
 // sum may be the residual or x, y may be x or the residual (same address, type and stride); any
 // other overlap is refused.
 enum { NETRA_CODES_ROWS = 1, NETRA_CODES_TILES = 2 };
