@@ -169,7 +169,8 @@ int netra_norm_gradients(const void* dy, uint32_t dy_type, uint64_t dy_stride, c
 // equal length; a group's score is its largest c (NETRA_GROUP_MAX) or the sum of its two largest
 // (NETRA_GROUP_TOP2), and the top_groups best groups are kept. ids[t, 0 .. k) are the k largest c of those in
 // falling order; ties go to the lower index, of groups as of experts. c is compared exactly: by the logits
-// where their order decides (no bias, no sums of two), else in 64 bits. A NaN ranks as -inf.
+// where their order decides (no bias, no sums of two), else in 64 bits. A NaN ranks as -inf, also one that is the sum of two.
+// (-inf in bias takes an expert out at no cost; a large finite number does so too, but most tokens then need 64 bits throughout.)
 //   weights[t, i] = scale * s_i, or scale * s_i / sum over the chosen of s (renormalise; 0 where the sum is 0,
 //   as where all of them are below 2^-126)
 // shared 1: logits has a column more, the shared expert's gate, and slot k is

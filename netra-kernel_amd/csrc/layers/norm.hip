@@ -210,7 +210,7 @@ struct Shape {
 };
 
 // kOnce, where all that goes in and out is more than the 256 MiB behind the L2s hold: x and the residual are
-// not kept there, nor the outputs. T 16384, H 4096 with residual and codes (604 MB): 117.3 us, with loads alone
+// not kept there, nor the outputs. T 16384, H 4096 with residual and codes (606 MB): 117.3 us, with loads alone
 // non-temporal 112.9, stores alone 113.9, both 110.3 (5.5 TB/s; a large copy 5.1); T 4096 (151 MB) 27.1, both 31.0.
 template <typename X, typename R, uint32_t W, uint32_t C, bool kOnce>
 __device__ __forceinline__ void forward(const Norm& a) {

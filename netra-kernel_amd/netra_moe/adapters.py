@@ -72,7 +72,8 @@ class LowRankAdapters:
 
     @classmethod
     def from_pairs(cls, pairs: Sequence[tuple[torch.Tensor, torch.Tensor]], scale: torch.Tensor | None = None) -> "LowRankAdapters":
-        """Adapters (a [r, K], b [N, r]) of different ranks, filled with zeros to the largest."""
+        """Adapters (a [r, K], b [N, r]) of different ranks, filled with zeros to the largest (with which a row of x that
+        holds an infinity or NaN gives NaN)."""
         if not pairs:
             raise ValueError("from_pairs needs an adapter")
         for i, (a, b) in enumerate(pairs):
@@ -87,7 +88,7 @@ class LowRankAdapters:
         return make_plan(ids, self.count)
 
     def add(self, y: torch.Tensor, x: torch.Tensor, plan: AdapterPlan, out: torch.Tensor | None = None) -> torch.Tensor:
-        """y bf16 [T, N] + the adapters of x bf16 or fp32 [T, K], bf16 [T, N]; out may be y."""
+        """y bf16 [T, N] + the adapters of x bf16 or fp32 (rounded to bf16) [T, K], bf16 [T, N]; out may be y."""
         data, tokens, adapters = plan
         if adapters != self.count or data.device != self.device:
             raise ValueError(f"plan: need one of {self.count} adapters on {self.device}, got {adapters} on {data.device}")

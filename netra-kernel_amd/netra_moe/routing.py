@@ -8,7 +8,8 @@
     r.ids, r.weights                                        # int32 and fp32 [T, 8 (+ 1)]
 
 ids feed expert_counts, balance_loss and the bridges. selection_bias moves the choice and not
-the weights (MoELayer's router_bias is added to the logits instead: give logits + bias for that).
+the weights (MoELayer's router_bias is added to the logits instead: give logits + bias for that). A bias of -inf takes an
+expert out at no cost; a large finite one (-1e9) does so too and makes the call several times as long.
 
     g = route_gradient(dweights, logits, r.ids)             # of the logits' type and shape
     route_gradient(dweights, logits, r.ids, out=b.grad, accumulate=True)   # adds to the balance loss's
